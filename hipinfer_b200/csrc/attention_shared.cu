@@ -1,0 +1,367 @@
+// Attention of a step's rows over a paged cache in which groups of requests share the pages of a long prefix, computed once for all rows of a
+// group (csrc/shared_plan.cu makes the items).
+//
+//   over a range A of keys: m_A = max s_j, l_A = sum 2^(s_j - m_A), o_A = sum 2^(s_j - m_A) v_j, s_j = log2(e) scale q . k_j, all in 32 bits;
+//   ranges are joined as o = sum_A 2^(m_A - m) o_A / sum_A 2^(m_A - m) l_A, m = max m_A.
+//
+// shared_items_kernel leaves (m, l) and o of every item's rows in the workspace; any head size up to 256, page size and group, both element
+// types: 16 or 64 rows a block by 64 keys a tile, products on the FMA pipe, everything widened to 32 bits in shared memory. bfloat16 heads of
+// 64 and 128 go to the tensor cores instead (attention_shared_tc.cu).
+// shared_join_kernel, a warp per row and head, adds the keys of the step's own rows (a row sees those up to itself, so that the items need no mask) and
+// joins the parts in a fixed order: the same plan and inputs give the same bits.
+#include "common.cuh"
+#include "shared_plan.h"
+
+namespace {
+
+constexpr int SI_KEYS = 64, SI_THREADS = 256;
+
+__device__ __forceinline__ float exp2_of(float x) { return exp2f(x); }
+
+// Four elements of a row of D from column c on, zeros behind its end.
+template <typename T> __device__ __forceinline__ float4 row4(const T* row, int c, int D, bool vec) {
+  if (vec && c + 4 <= D) return hb_load4(row + c);
+  float4 v;
+  v.x = c < D ? hb_to_float(row[c]) : 0.f;
+  v.y = c + 1 < D ? hb_to_float(row[c + 1]) : 0.f;
+  v.z = c + 2 < D ? hb_to_float(row[c + 2]) : 0.f;
+  v.w = c + 3 < D ? hb_to_float(row[c + 3]) : 0.f;
+  return v;
+}
+
+template <int RM, int NC> constexpr int items_smem() {
+  return (16 * RM * (64 * NC + 4) + 2 * SI_KEYS * (64 * NC + 4) + 16 * RM * (SI_KEYS + 4)) * 4;
+}
+
+// A thread has RM rows (ty RM ..) by four keys (tx, tx + 16, ..) of the scores, and RM rows by 4 NC columns of the output.
+template <typename T, int RM, int NC>
+__global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
+                                                                  const int* plan, float* part_o, float2* part_ml, int Hq, int Hkv, int D,
+                                                                  int page_size, float scale_log2, int vec) {
+  constexpr int R = 16 * RM, DP = 64 * NC, LD = DP + 4, LP = SI_KEYS + 4;
+  extern __shared__ __align__(16) float sh[];
+  float *sQ = sh, *sK = sQ + R * LD, *sV = sK + SI_KEYS * LD, *sP = sV + SI_KEYS * LD;
+  hb_pdl_wait();
+  hb_pdl_launch();
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = Hq / Hkv;
+  const SharedItem* items = (const SharedItem*)(plan + plan[SP_OFF_ITEMS]);
+  const int* ctas = plan + plan[SP_OFF_CTAS];
+  for (int it = ctas[blockIdx.x]; it < ctas[blockIdx.x + 1]; it++) {
+    const SharedItem e = items[it];
+    const int rows = e.tokens * G;
+    for (int r0 = blockIdx.y * R; r0 < rows; r0 += gridDim.y * R) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < R * (DP / 4); i += SI_THREADS) {
+        const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r0 + r < rows) v = row4(q + (size_t)(e.token + (r0 + r) / G) * ldq + (size_t)(e.head * G + (r0 + r) % G) * D, c, D, vec);
+        *(float4*)(sQ + r * LD + c) = v;
+      }
+      float m[RM], l[RM], acc[RM][4 * NC];
+      int last[RM];                                     // the last key that the row sees
+#pragma unroll
+      for (int i = 0; i < RM; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+        last[i] = e.pos == SP_NO_MASK ? SP_NO_MASK : e.pos + (r0 + ty * RM + i) / G;
+#pragma unroll
+        for (int c = 0; c < 4 * NC; c++) acc[i][c] = 0.f;
+      }
+      for (int k0 = e.lo; k0 < e.hi; k0 += SI_KEYS) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < SI_KEYS * (DP / 4); i += SI_THREADS) {
+          const int j = i / (DP / 4), c = 4 * (i % (DP / 4)), p = k0 + j;
+          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+          if (p < e.hi) {
+            const size_t row = ((size_t)bt[(size_t)e.table * bt_stride + p / page_size] * Hkv + e.head) * page_size + p % page_size;
+            k = row4(kc + row * D, c, D, vec);
+            v = row4(vc + row * D, c, D, vec);
+          }
+          *(float4*)(sK + j * LD + c) = k;
+          *(float4*)(sV + j * LD + c) = v;
+        }
+        __syncthreads();
+        float s[RM][4] = {};
+#pragma unroll 4
+        for (int c = 0; c < DP; c += 4) {
+          float4 a[RM], b[4];
+#pragma unroll
+          for (int i = 0; i < RM; i++) a[i] = *(const float4*)(sQ + (ty * RM + i) * LD + c);
+#pragma unroll
+          for (int j = 0; j < 4; j++) b[j] = *(const float4*)(sK + (tx + 16 * j) * LD + c);
+#pragma unroll
+          for (int i = 0; i < RM; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+        }
+        float corr[RM];
+#pragma unroll
+        for (int i = 0; i < RM; i++) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int p = k0 + tx + 16 * j;
+            s[i][j] = p < e.hi && p <= last[i] ? s[i][j] * scale_log2 : -INFINITY;
+            mx = fmaxf(mx, s[i][j]);
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const float mn = fmaxf(m[i], mx), sub = mn == -INFINITY ? 0.f : mn;
+          corr[i] = exp2_of(m[i] - sub);
+          m[i] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float p = exp2_of(s[i][j] - sub);
+            sum += p;
+            sP[(ty * RM + i) * LP + tx + 16 * j] = p;
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          l[i] = l[i] * corr[i] + sum;
+        }
+        __syncwarp();               // the 16 lanes that share a row of P are of one warp
+#pragma unroll
+        for (int i = 0; i < RM; i++)
+#pragma unroll
+          for (int c = 0; c < 4 * NC; c++) acc[i][c] *= corr[i];
+#pragma unroll 4
+        for (int j = 0; j < SI_KEYS; j += 4) {
+          float pr[RM][4];
+#pragma unroll
+          for (int i = 0; i < RM; i++) *(float4*)pr[i] = *(const float4*)(sP + (ty * RM + i) * LP + j);
+#pragma unroll
+          for (int jj = 0; jj < 4; jj++)
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+              const float4 v = *(const float4*)(sV + (j + jj) * LD + 64 * n + 4 * tx);
+#pragma unroll
+              for (int i = 0; i < RM; i++) {
+                // a value behind the row is not multiplied by 0: it may be an infinity or NaN
+                const float p = pr[i][jj];
+                if (p != 0.f) {
+                  acc[i][4 * n] = fmaf(p, v.x, acc[i][4 * n]);
+                  acc[i][4 * n + 1] = fmaf(p, v.y, acc[i][4 * n + 1]);
+                  acc[i][4 * n + 2] = fmaf(p, v.z, acc[i][4 * n + 2]);
+                  acc[i][4 * n + 3] = fmaf(p, v.w, acc[i][4 * n + 3]);
+                }
+              }
+            }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RM; i++) {
+        const int r = r0 + ty * RM + i;
+        if (r >= rows) continue;
+        const size_t row = (size_t)e.part + r;
+        if (tx == 0) part_ml[row] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+            if (64 * n + 4 * tx + c < D) part_o[row * D + 64 * n + 4 * tx + c] = acc[i][4 * n + c];
+      }
+    }
+  }
+}
+
+// E elements of a row of D from column c on as floats.
+template <int E, typename T> __device__ __forceinline__ void load_elements(const T* row, int c, int D, bool vec, float* x) {
+  if constexpr (E >= 4) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const float4 v = row4(row, c + i, D, vec);
+      x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    }
+  } else {
+    if (vec && c + 2 <= D) {
+      if constexpr (sizeof(T) == 4) {
+        const float2 v = *(const float2*)(row + c);
+        x[0] = v.x; x[1] = v.y;
+      } else {
+        const float2 v = __bfloat1622float2(*(const __nv_bfloat162*)(row + c));
+        x[0] = v.x; x[1] = v.y;
+      }
+    } else {
+      x[0] = c < D ? hb_to_float(row[c]) : 0.f;
+      x[1] = c + 1 < D ? hb_to_float(row[c + 1]) : 0.f;
+    }
+  }
+}
+
+constexpr int SJ_WARPS = 4;
+
+// A warp per row of q and head; a lane has E columns.
+template <typename T, int E>
+__global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
+                                                                    const int* plan, const float* part_o, const float2* part_ml, T* out, int Hq,
+                                                                    int Hkv, int D, int page_size, float scale_log2, int vec) {
+  hb_pdl_wait();
+  hb_pdl_launch();
+  const int lane = threadIdx.x & 31, c = lane * E, G = Hq / Hkv;
+  const int u = blockIdx.x * SJ_WARPS + (threadIdx.x >> 5), T_rows = plan[SP_TOKENS];
+  if (u >= T_rows * Hq) return;
+  const int t = u / Hq, head = u % Hq, h = head / G, g = head % G;
+  const SharedToken e = ((const SharedToken*)(plan + plan[SP_OFF_TOKENS]))[t];
+  float m = -INFINITY, l = 0.f, acc[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) acc[i] = 0.f;
+
+  // the keys of the step's own rows
+  if (e.fresh > 0) {
+    float x[E];
+    load_elements<E>(q + (size_t)t * ldq + (size_t)head * D, c, D, vec, x);
+    for (int j0 = 0; j0 < e.fresh; j0 += 4) {
+      float k[4][E], v[4][E];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int p = e.first + min(j0 + j, e.fresh - 1);
+        const size_t row = ((size_t)bt[(size_t)e.table * bt_stride + p / page_size] * Hkv + h) * page_size + p % page_size;
+        load_elements<E>(kc + row * D, c, D, vec, k[j]);
+        load_elements<E>(vc + row * D, c, D, vec, v[j]);
+      }
+      float s[4], mx = m;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; i++) a = fmaf(x[i], k[j][i], a);
+        s[j] = j0 + j < e.fresh ? hb_warp_sum(a) * scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[j]);
+      }
+      const float sub = mx == -INFINITY ? 0.f : mx, corr = exp2_of(m - sub);
+      m = mx;
+      l *= corr;
+#pragma unroll
+      for (int i = 0; i < E; i++) acc[i] *= corr;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (j0 + j < e.fresh) {
+          const float p = exp2_of(s[j] - sub);
+          l += p;
+#pragma unroll
+          for (int i = 0; i < E; i++) acc[i] = fmaf(p, v[j][i], acc[i]);
+        }
+    }
+  }
+
+  // the parts, 32 at a time: a lane holds one's maximum and sum
+  const int n = e.pre_n + e.own_n;
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    const int k = k0 + lane;
+    const int row = k < e.pre_n ? e.pre_base + (h * e.pre_n + k) * e.pre_rows + g : e.own_base + (h * e.own_n + k - e.pre_n) * e.own_rows + g;
+    const float2 ml = k < n ? part_ml[row] : make_float2(-INFINITY, 0.f);
+    const float mx = hb_warp_max(fmaxf(ml.x, m)), sub = mx == -INFINITY ? 0.f : mx, corr = exp2_of(m - sub);
+    // a part without a visible key has sum 0 and no output; one whose sum is NaN makes the row NaN
+    const float w = ml.y == 0.f ? 0.f : ml.y != ml.y ? ml.y : exp2_of(ml.x - sub);
+    m = mx;
+    l = l * corr + hb_warp_sum(w == 0.f ? 0.f : w * ml.y);
+#pragma unroll
+    for (int i = 0; i < E; i++) acc[i] *= corr;
+    const int in = min(32, n - k0);
+    for (int j0 = 0; j0 < in; j0 += 4) {
+      float o[4][E], wj[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int from = __shfl_sync(0xffffffffu, row, min(j0 + j, in - 1));
+        wj[j] = __shfl_sync(0xffffffffu, w, min(j0 + j, in - 1));
+        if (j0 + j >= in) wj[j] = 0.f;
+        if (wj[j] != 0.f) load_elements<E>(part_o + (size_t)from * D, c, D, vec, o[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (wj[j] != 0.f) {
+#pragma unroll
+          for (int i = 0; i < E; i++) acc[i] = fmaf(wj[j], o[j][i], acc[i]);
+        }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;       // a row that sees nothing is 0
+  T* dst = out + ((size_t)t * Hq + head) * D;
+#pragma unroll
+  for (int i = 0; i < E; i++) acc[i] *= inv;
+  if (vec && E >= 4) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4)
+      if (c + i < D) hb_store4(dst + c + i, make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++)
+      if (c + i < D) dst[c + i] = hb_from_float<T>(acc[i]);
+  }
+}
+
+template <typename T, int RM, int NC>
+int launch_items(const void* q, long ldq, const void* kc, const void* vc, const int* bt, int bt_stride, const int* plan, int ctas, int max_rows,
+                 float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
+  constexpr int smem = items_smem<RM, NC>();
+  auto kern = shared_items_kernel<T, RM, NC>;
+  static bool configured = false;
+  if (!configured) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
+    configured = true;
+  }
+  const int blocks = (max_rows + 16 * RM - 1) / (16 * RM);
+  const cudaError_t e = hb_launch(kern, dim3(ctas, blocks < 65535 ? blocks : 65535), SI_THREADS, smem, s, (const T*)q, ldq, (const T*)kc, (const T*)vc, bt,
+                                  bt_stride, plan, part_o, part_ml, Hq, Hkv, D, page_size, scale_log2, vec);
+  if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+int check_sizes(const char* who, int Hq, int Hkv, int D, int page_size) {
+  if (Hkv < 1 || Hq < Hkv || Hq % Hkv) HB_FAIL("%s: %d heads are not a multiple of %d kv heads", who, Hq, Hkv);
+  if (D < 1 || D > 256) HB_FAIL("%s: heads of %d (1 to 256 are supported)", who, D);
+  if (page_size < 1) HB_FAIL("%s: pages of %d", who, page_size);
+  return 0;
+}
+
+}  // namespace
+
+// Rows that an item of the plain kernel should have at most, per kv head: a block's 64, or whole tokens beyond.
+HB_EXPORT int hb_shared_items_rows() { return 64; }
+
+// q [T, ldq] (heads of D side by side), caches [page, Hkv, page_size, D], bt [R, bt_stride], plan on the device (see shared_plan.cu) and its
+// n_ctas and max_rows; part_o [parts][D], part_ml [parts] (16-byte aligned). vec: all rows start on 16 bytes.
+HB_EXPORT int hb_shared_items(const void* q, long ldq, const void* kc, const void* vc, int dt, const int* bt, int bt_stride, const int* plan, int ctas,
+                              int max_rows, float* part_o, void* part_ml, int Hq, int Hkv, int D, int page_size, float scale, int vec,
+                              cudaStream_t s) {
+  if (check_sizes("hb_shared_items", Hq, Hkv, D, page_size)) return -1;
+  if (ctas <= 0 || max_rows <= 0) return 0;
+  const float sl2 = scale * 1.4426950408889634f;
+  int r = -1;
+#define SI_LAUNCH(RM, NC) \
+  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, plan, ctas, max_rows, part_o, (float2*)part_ml, Hq, Hkv, D, page_size, sl2, vec, s)
+  HB_DISPATCH_1(dt, "hb_shared_items", {
+    if (max_rows <= 16) {
+      if (D <= 64) SI_LAUNCH(1, 1); else if (D <= 128) SI_LAUNCH(1, 2); else SI_LAUNCH(1, 4);
+    } else {
+      if (D <= 64) SI_LAUNCH(4, 1); else if (D <= 128) SI_LAUNCH(4, 2); else SI_LAUNCH(4, 4);
+    }
+  });
+#undef SI_LAUNCH
+  if (r) return r;
+  HB_CHECK_LAUNCH("hb_shared_items");
+  return 0;
+}
+
+// out [T, Hq, D] from the parts and the keys of the step's own rows. T as in the plan.
+HB_EXPORT int hb_shared_join(const void* q, long ldq, const void* kc, const void* vc, int dt, const int* bt, int bt_stride, const int* plan, int T,
+                             const float* part_o, const void* part_ml, void* out, int Hq, int Hkv, int D, int page_size, float scale, int vec,
+                             cudaStream_t s) {
+  if (check_sizes("hb_shared_join", Hq, Hkv, D, page_size)) return -1;
+  if (T <= 0) return 0;
+  const long warps = (long)T * Hq;
+  if (warps > (1l << 30)) HB_FAIL("hb_shared_join: %d rows of %d heads are beyond the grid limit", T, Hq);
+  const float sl2 = scale * 1.4426950408889634f;
+  cudaError_t e = cudaSuccess;
+#define SJ_LAUNCH(E)                                                                                                                     \
+  e = hb_launch(shared_join_kernel<TA, E>, dim3((unsigned)((warps + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq,   \
+                (const TA*)kc, (const TA*)vc, bt, bt_stride, plan, part_o, (const float2*)part_ml, (TA*)out, Hq, Hkv, D, page_size, sl2, vec)
+  HB_DISPATCH_1(dt, "hb_shared_join", { if (D <= 64) SJ_LAUNCH(2); else if (D <= 128) SJ_LAUNCH(4); else SJ_LAUNCH(8); });
+#undef SJ_LAUNCH
+  if (e != cudaSuccess) HB_FAIL("hb_shared_join: %s", cudaGetErrorString(e));
+  HB_CHECK_LAUNCH("hb_shared_join");
+  return 0;
+}

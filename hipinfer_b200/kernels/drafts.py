@@ -1,0 +1,178 @@
+"""Operators of a step that samples many continuations behind shared pages, with drafted tokens: attention over a paged cache in which
+groups of requests share a long prefix (computed once for all of a group's rows), and the verification of drafted tokens against the
+target's logits. Reached as `ops.SharedPlan`, `ops.attention_shared` and `ops.verify_drafts` (csrc/shared_plan.cu, attention_shared.cu, verify_drafts.cu).
+
+The reference has neither: its batch slots hold a copy of the prompt each (src/api.cu:1409-1411), and its `verify_step` (2029-2060) returns
+logits and leaves the choice to the caller."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import library, ops
+
+_p, _i, _l, _f = C.c_void_p, C.c_int, C.c_long, C.c_float
+ops._SIGS["drafts"] = {
+    "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i],
+    "hb_shared_items": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _i, _p, _p, _i, _i, _i, _i, _f, _i, _p],
+    "hb_shared_join": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _p, _p, _p, _i, _i, _i, _i, _f, _i, _p],
+    "hb_verify_drafts": [_p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _l, _p, _i, _l, _l, _p, _p, _p, _p, _p],
+}
+MAX_DRAFTS = 63
+
+# the header of a plan (csrc/shared_plan.h)
+_ITEMS, _CTAS, _PARTS, _TOKENS, _MAX_ROWS, _OFF_ITEMS, _OFF_CTAS, _OFF_TOKENS, _INTS = range(9)
+_HEADER = 16
+
+
+def plan_numbers(q_lens, ctx_lens, groups, n_heads: int, n_kv_heads: int, tile_tokens: int, narrow_tokens: int, key_tile: int, n_ctas: int,
+                 item_cost: float, part_cost: float) -> np.ndarray:
+    """The plan as int32 numbers (csrc/shared_plan.cu, which runs on the host); raises KernelError for lengths that make none."""
+    q, c = (np.ascontiguousarray(x, dtype=np.int32) for x in (q_lens, ctx_lens))
+    g = np.ascontiguousarray(groups, dtype=np.int32).reshape(-1, 3)
+    if q.ndim != 1 or q.shape != c.shape:
+        raise ops.KernelError(f"a plan needs one number of rows and one length a request, got {q.shape} and {c.shape}")
+    fn = ops._fn("drafts", "hb_shared_plan")
+    cap = 4096 + 16 * int(q.clip(0).sum())
+    while True:
+        out = np.empty(cap, dtype=np.int32)
+        n = fn(q.ctypes.data, c.ctypes.data, len(q), g.ctypes.data, len(g), n_heads, n_kv_heads, tile_tokens, narrow_tokens, key_tile, n_ctas,
+               item_cost, part_cost, out.ctypes.data, cap)
+        if n > 0:
+            return out[:n]
+        if n == 0:
+            raise ops.KernelError(library.load("drafts").hb_last_error().decode())
+        cap = -n
+
+
+class SharedPlan:
+    """How a step's rows attend to a paged cache whose requests share prefixes; made from the lengths alone, once a step, and used by every
+    layer of that step whose heads and pages are these.
+
+    q_lens[r] rows of request r (its rows are consecutive, requests one after the other) stand at positions ctx_lens[r], ...; a row sees the
+    keys up to its own. groups: (first request, requests, shared tokens): the block tables of these requests name the same pages for the
+    positions below `shared tokens` (which need not be a multiple of the page size). Requests of no group, and groups of which fewer than two
+    bring rows, attend on their own."""
+
+    def __init__(self, q_lens: Sequence[int], ctx_lens: Sequence[int], groups: Sequence[Tuple[int, int, int]], n_heads: int, n_kv_heads: int,
+                 head_dim: int, page_size: int, dtype: torch.dtype, device="cuda:0"):
+        if n_kv_heads < 1 or n_heads < n_kv_heads or n_heads % n_kv_heads:
+            raise ops.KernelError(f"attention_shared: {n_heads} heads are not a multiple of {n_kv_heads} kv heads")
+        if not 1 <= head_dim <= 256 or page_size < 1 or dtype not in ops._DT:
+            raise ops.KernelError(f"attention_shared: heads of {head_dim}, pages of {page_size}, {dtype} are not supported")
+        self.n_heads, self.n_kv_heads, self.head_dim, self.page_size, self.dtype = n_heads, n_kv_heads, head_dim, page_size, dtype
+        self.device = torch.device(device)
+        self.n_requests = len(q_lens)
+        group = n_heads // n_kv_heads
+        tile, narrow, key_tile, ctas, item_cost, part_cost = max(1, 64 // group), 0, 64, 2 * _sms(self.device), 1.0, head_dim * 2e-6
+        numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, tile, narrow, key_tile, ctas, item_cost, part_cost)
+        self.rows, self.parts = int(numbers[_TOKENS]), int(numbers[_PARTS])
+        self.ctas, self.max_rows = int(numbers[_CTAS]), int(numbers[_MAX_ROWS])
+        self.most_keys = max((int(c) + int(n) for c, n in zip(ctx_lens, q_lens) if n), default=0)
+        host = torch.from_numpy(numbers)
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        self.numbers = host.to(self.device, non_blocking=True)
+        self._host = host                     # until the copy is over
+
+
+def _sms(device) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count if device.type == "cuda" else 148
+
+
+def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, plan: SharedPlan,
+                     out: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of the plan's rows over their requests' pages. q [T, Hq D] (rows may be part of wider ones); caches [page, Hkv, page_size, D]
+    of the same type; block_table int32 [R, pages]; out [T, Hq D]; scale 1 / sqrt(D) by default. Scores, softmax and sums are 32-bit; the
+    keys' cut, and with it a result's last bits, is a matter of the plan."""
+    ops._need_cuda(q, k_cache, v_cache, block_table, out)
+    Hq, Hkv, D, ps, T = plan.n_heads, plan.n_kv_heads, plan.head_dim, plan.page_size, plan.rows
+    if q.dim() != 2 or q.shape != (T, Hq * D) or q.stride(1) != 1 or q.dtype != plan.dtype:
+        raise ops.KernelError(f"attention_shared: q {tuple(q.shape)} {q.dtype}, strides {q.stride()}; the plan has {T} rows of {Hq} heads of {D}, {plan.dtype}")
+    for name, x in (("keys", k_cache), ("values", v_cache)):
+        if x.dim() != 4 or x.shape[1:] != (Hkv, ps, D) or not x.is_contiguous() or x.dtype != plan.dtype:
+            raise ops.KernelError(f"attention_shared: {name} {tuple(x.shape)} {x.dtype} are no pages of {Hkv} heads x {ps} tokens x {D}, {plan.dtype}")
+    if k_cache.shape[0] != v_cache.shape[0]:
+        raise ops.KernelError(f"attention_shared: {k_cache.shape[0]} pages of keys, {v_cache.shape[0]} of values")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1 or block_table.shape[0] != plan.n_requests \
+            or block_table.shape[1] * ps < plan.most_keys:
+        raise ops.KernelError(f"attention_shared: block table {tuple(block_table.shape)} {block_table.dtype}; the plan has {plan.n_requests} requests of up "
+                              f"to {plan.most_keys} tokens in pages of {ps}")
+    if out is None:
+        out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
+    elif out.shape != (T, Hq * D) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ops.KernelError(f"attention_shared: out {tuple(out.shape)} {out.dtype}, strides {out.stride()}")
+    if not T:
+        return out
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    dt, st, bts = ops._DT[q.dtype], library.current_stream(), block_table.stride(0)
+    ws = torch.empty(plan.parts * (D + 2) + 4, dtype=torch.float32, device=q.device) if plan.parts else None
+    part_o = None if ws is None else ws.data_ptr()
+    part_ml = None if ws is None else part_o + 4 * (plan.parts * D + (-plan.parts * D) % 4)
+    size = q.element_size()
+    vec = int(D % 4 == 0 and (q.stride(0) * size) % 16 == 0 and not any(x.data_ptr() % 16 for x in (q, k_cache, v_cache, out)))
+    if plan.ctas:
+        ops._call("drafts", "hb_shared_items", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), dt, block_table.data_ptr(), bts,
+                  plan.numbers.data_ptr(), plan.ctas, plan.max_rows, part_o, part_ml, Hq, Hkv, D, ps, scale, vec, st)
+    ops._call("drafts", "hb_shared_join", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), dt, block_table.data_ptr(), bts,
+              plan.numbers.data_ptr(), T, part_o, part_ml, out.data_ptr(), Hq, Hkv, D, ps, scale, vec, st)
+    return out
+
+
+def _vector(x, dtype, n, what):
+    if x.dtype != dtype or x.numel() != n or not x.is_contiguous():
+        raise ops.KernelError(f"verify_drafts: {what} {tuple(x.shape)} {x.dtype}, {n} of {dtype} side by side are expected")
+
+
+def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Tensor, drafts: torch.Tensor, temperature: torch.Tensor,
+                  uniform: torch.Tensor, noise: torch.Tensor, draft_probs: Optional[torch.Tensor] = None):
+    """Accepts or refuses drafted tokens so that what is produced is distributed as if the target alone had drawn it.
+
+    Request r has n_drafts[r] drafts in row r of `drafts` (int32 [R, K]) and n_drafts[r] + 1 rows of logits ([T, V], float32 or bfloat16) from row
+    start[r] on; p_i is the softmax of the i-th over `temperature[r]` (float32 [R]; 0: greedy, a point mass on the lowest index of the largest
+    logit, which is also what a row without a finite largest logit is; NaN counts as above all). Draft i is accepted iff all before it are and
+    uniform[r, i] * q_i(draft) < p_i(draft), with q_i = draft_probs[r, i] ([R, K, V], float32 or bfloat16), or 1 where no distributions are given (drafts
+    that were looked up). The token behind the accepted ones is the arg max of w / noise[r] (float32 [R, V], exponential variates; ties: the lowest
+    index), w = max(p_i - q_i, 0) at the first draft refused (p_i where that is 0 everywhere), p_{n+1} if none was.
+
+    Returns (tokens int32 [R, K + 1]: accepted drafts, the token behind them, -1; counts int32 [R]: how many tokens; logprobs float32 [R, K + 1]:
+    log p_i of each, at temperature 1 for a greedy request, 0 for a row without a finite largest logit and behind the last). A request whose
+    rows lie outside the logits gets no token."""
+    ops._need_cuda(logits, start, n_drafts, drafts, temperature, uniform, noise, draft_probs)
+    ops._rows_contiguous(logits, "verify_drafts logits")
+    if drafts.dim() != 2 or drafts.dtype != torch.int32 or not drafts.is_contiguous():
+        raise ops.KernelError(f"verify_drafts: drafts {tuple(drafts.shape)} {drafts.dtype}, strides {drafts.stride()}; int32 [R, K] is expected")
+    (T, V), (R, K) = logits.shape, drafts.shape
+    if K > MAX_DRAFTS:
+        raise ops.KernelError(f"verify_drafts: {K} drafts a request, at most {MAX_DRAFTS}")
+    _vector(start, torch.int32, R, "start")
+    _vector(n_drafts, torch.int32, R, "n_drafts")
+    _vector(temperature, torch.float32, R, "temperature")
+    _vector(uniform, torch.float32, R * K, "uniform")
+    if noise.shape != (R, V) or noise.dtype != torch.float32 or (V > 1 and noise.stride(1) != 1):
+        raise ops.KernelError(f"verify_drafts: noise {tuple(noise.shape)} {noise.dtype}, strides {noise.stride()}; float32 [{R}, {V}] is expected")
+    if draft_probs is not None and (draft_probs.shape != (R, K, V) or draft_probs.dtype not in ops._DT or (V > 1 and draft_probs.stride(2) != 1)):
+        raise ops.KernelError(f"verify_drafts: draft_probs {tuple(draft_probs.shape)} {draft_probs.dtype}, strides {draft_probs.stride()}; [{R}, {K}, {V}] is "
+                              f"expected")
+    dt = ops._dt(logits)
+    numbers = torch.empty(R * (K + 2), dtype=torch.int32, device=logits.device)
+    tokens, counts = numbers[:R * (K + 1)].view(R, K + 1), numbers[R * (K + 1):]
+    logprobs = torch.empty(R, K + 1, dtype=torch.float32, device=logits.device)
+    if not R:
+        return tokens, counts, logprobs
+    if not V:
+        raise ops.KernelError("verify_drafts: empty vocabulary")
+    lib = library.load("drafts")
+    lib.hb_verify_drafts_workspace.restype = C.c_long
+    ws = torch.empty(lib.hb_verify_drafts_workspace(R, K, V, dt), dtype=torch.uint8, device=logits.device)
+    probs = draft_probs if K else None
+    library.launches[0] += 1
+    ops._call("drafts", "hb_verify_drafts", logits.data_ptr(), dt, logits.stride(0), T, V, start.data_ptr(), n_drafts.data_ptr(), drafts.data_ptr(), R, K,
+              temperature.data_ptr(), uniform.data_ptr(), noise.data_ptr(), noise.stride(0), ops._ptr(probs), 0 if probs is None else ops._dt(probs),
+              0 if probs is None else probs.stride(0), 0 if probs is None else probs.stride(1), ws.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
+              logprobs.data_ptr(), library.current_stream())
+    return tokens, counts, logprobs

@@ -1741,3 +1741,7 @@ def output_norm(x: torch.Tensor, y, weight: torch.Tensor, bias: Optional[torch.T
           1 if center else 0, x.data_ptr(), _ptr(rounded), _dt(rounded) if rounded is not None else 0, _ptr(keep_in), _ptr(keep), _ptr(states),
           states.stride(0) if states is not None else 0, _ptr(coef), n, T, W, _stream())
     return x
+
+
+# Attention over shared prefixes and the verification of drafted tokens (kernels/drafts.py)
+from .drafts import SharedPlan, attention_shared, verify_drafts  # noqa: E402,F401
