@@ -36,8 +36,8 @@ template <int RM, int NC> constexpr int items_smem() {
 // A thread has RM rows (ty RM ..) by four keys (tx, tx + 16, ..) of the scores, and RM rows by 4 NC columns of the output.
 template <typename T, int RM, int NC>
 __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
-                                                                  const int* plan, float* part_o, float2* part_ml, int Hq, int Hkv, int D,
-                                                                  int page_size, float scale_log2, int vec) {
+                                                                  const int* plan, int narrow, float* part_o, float2* part_ml, int Hq, int Hkv,
+                                                                  int D, int page_size, float scale_log2, int vec) {
   constexpr int R = 16 * RM, DP = 64 * NC, LD = DP + 4, LP = SI_KEYS + 4;
   extern __shared__ __align__(16) float sh[];
   float *sQ = sh, *sK = sQ + R * LD, *sV = sK + SI_KEYS * LD, *sP = sV + SI_KEYS * LD;
@@ -155,7 +155,11 @@ __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, lo
         const int r = r0 + ty * RM + i;
         if (r >= rows) continue;
         const size_t row = (size_t)e.part + r;
-        if (tx == 0) part_ml[row] = make_float2(m[i], l[i]);
+        if (tx == 0) {
+          part_ml[row] = make_float2(m[i], l[i]);
+          // a plan that was made for the tensor cores has a second part here (rows of q that TMA cannot address)
+          if (e.tokens <= narrow) part_ml[row + rows] = make_float2(-INFINITY, 0.f);
+        }
 #pragma unroll
         for (int n = 0; n < NC; n++)
 #pragma unroll
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
 
 template <typename T, int RM, int NC>
 int launch_items(const void* q, long ldq, const void* kc, const void* vc, const int* bt, int bt_stride, const int* plan, int ctas, int max_rows,
-                 float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
+                 int narrow, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
   constexpr int smem = items_smem<RM, NC>();
   auto kern = shared_items_kernel<T, RM, NC>;
   static bool configured = false;
@@ -305,7 +309,7 @@ int launch_items(const void* q, long ldq, const void* kc, const void* vc, const 
   }
   const int blocks = (max_rows + 16 * RM - 1) / (16 * RM);
   const cudaError_t e = hb_launch(kern, dim3(ctas, blocks < 65535 ? blocks : 65535), SI_THREADS, smem, s, (const T*)q, ldq, (const T*)kc, (const T*)vc, bt,
-                                  bt_stride, plan, part_o, part_ml, Hq, Hkv, D, page_size, scale_log2, vec);
+                                  bt_stride, plan, narrow, part_o, part_ml, Hq, Hkv, D, page_size, scale_log2, vec);
   if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
   return 0;
 }
@@ -319,20 +323,17 @@ int check_sizes(const char* who, int Hq, int Hkv, int D, int page_size) {
 
 }  // namespace
 
-// Rows that an item of the plain kernel should have at most, per kv head: a block's 64, or whole tokens beyond.
-HB_EXPORT int hb_shared_items_rows() { return 64; }
-
 // q [T, ldq] (heads of D side by side), caches [page, Hkv, page_size, D], bt [R, bt_stride], plan on the device (see shared_plan.cu) and its
-// n_ctas and max_rows; part_o [parts][D], part_ml [parts] (16-byte aligned). vec: all rows start on 16 bytes.
+// n_ctas, max_rows and narrow_tokens; part_o [parts][D], part_ml [parts] (16-byte aligned). vec: all rows start on 16 bytes.
 HB_EXPORT int hb_shared_items(const void* q, long ldq, const void* kc, const void* vc, int dt, const int* bt, int bt_stride, const int* plan, int ctas,
-                              int max_rows, float* part_o, void* part_ml, int Hq, int Hkv, int D, int page_size, float scale, int vec,
+                              int max_rows, int narrow, float* part_o, void* part_ml, int Hq, int Hkv, int D, int page_size, float scale, int vec,
                               cudaStream_t s) {
   if (check_sizes("hb_shared_items", Hq, Hkv, D, page_size)) return -1;
   if (ctas <= 0 || max_rows <= 0) return 0;
   const float sl2 = scale * 1.4426950408889634f;
   int r = -1;
 #define SI_LAUNCH(RM, NC) \
-  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, plan, ctas, max_rows, part_o, (float2*)part_ml, Hq, Hkv, D, page_size, sl2, vec, s)
+  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, plan, ctas, max_rows, narrow, part_o, (float2*)part_ml, Hq, Hkv, D, page_size, sl2, vec, s)
   HB_DISPATCH_1(dt, "hb_shared_items", {
     if (max_rows <= 16) {
       if (D <= 64) SI_LAUNCH(1, 1); else if (D <= 128) SI_LAUNCH(1, 2); else SI_LAUNCH(1, 4);

@@ -1,0 +1,487 @@
+// The items of the shared-prefix attention (shared_plan.cu, attention_shared.cu) on the 5th-generation tensor cores: bfloat16, heads of 64 or 128.
+//
+// Persistent CTAs, one an SM, walk the items that the plan gives them. An item is up to 2 x 128 query rows (consecutive tokens times the heads
+// of a kv head) against a range of keys, in tiles of 128 absolute positions. Two CHAINS, a softmax warpgroup, a score tile, an accumulator
+// and running maxima and sums each, work in turn: where an item has more rows than 128 a chain has half of them and every key tile, and
+// a tile of K and V that was loaded once serves both; where it has fewer, both chains have the same rows and take the key tiles in turn, and
+// leave a part of the result each. Either way the exponentials of one chain run beside the products of the other.
+//   softmax warps   a thread owns a query row: reads its row of S from tensor memory, masks it where the tile reaches over the item's
+//                   range or the row's position, exponentiates in 32 bits, and writes P as bfloat16 over S in tensor memory, from where the second
+//                   product reads it as its A operand (shared memory then feeds K and V alone);
+//   K and V loaders TMA, a page and 64 columns a box, a lane holds a page's number; Q comes with K, one box of (64 columns, heads, tokens);
+//   two MMA warps   S = Q K^T of the next units, and O += P V of those whose P is written.
+// A score tile and its P are the same tensor memory: the next scores wait until the product behind them is done, so when they arrive the
+// accumulator is complete and may be rescaled (only when a row's maximum grew by more than 2^8: any reference value gives the same quotient).
+// V rows outside of the item's range, which may hold anything, are set to zero in shared memory by the softmax threads that mask them: P
+// is 0 there, and 0 times an infinity is no 0. Every wait is bounded.
+#include "shared_plan.h"
+#include "tc_common.cuh"
+
+namespace {
+
+constexpr int ST_ROWS = 128, ST_KEYS = 128, ST_THREADS = 384;
+constexpr float ST_SLACK = 8.f;
+
+template <int D> struct StSizes {
+  static constexpr int TILE = 128 * 64 * 2;                 // [128][64] bfloat16; an operand of D columns is D / 64 of them
+  static constexpr int OPND = D / 64 * TILE;
+  static constexpr int NK = D == 128 ? 2 : 5, NV = D == 128 ? 3 : 6;
+};
+template <int D> struct StBars {
+  uint64_t q_full[2], q_free[2], k_full[StSizes<D>::NK], k_free[StSizes<D>::NK], v_full[StSizes<D>::NV], v_free[StSizes<D>::NV];
+  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+template <int D> constexpr int st_smem() { return (2 + StSizes<D>::NK + StSizes<D>::NV) * StSizes<D>::OPND + (int)sizeof(StBars<D>); }
+static_assert(st_smem<128>() <= 227 * 1024 && st_smem<64>() <= 227 * 1024, "shared memory of a block");
+
+// MN-major operand with the 128-byte swizzle (V as it lies in its pages): 64 contiguous elements of the head a row, eight keys per 1,024-byte
+// group; the next 64 columns lie a tile further.
+__device__ __forceinline__ uint64_t desc_mn128(uint32_t smem_addr, int next) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D[tensor memory] (+)= A[tensor memory: a lane a row, two bfloat16 a column] B[shared memory]; one thread.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 columns of this thread's lane, not waited for, and back.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(taddr));
+}
+__device__ __forceinline__ void ld32_fence(uint32_t* r) { asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory"); }
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {   // two fmaf, each rounded by itself
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(hb_smem_u32(dst)), "l"((uint64_t)m), "r"(hb_smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+struct Work {      // an item as the roles go through it
+  SharedItem e;
+  int kt0, tiles;  // its key tiles
+  bool wide;       // a chain has half of the rows (else half of the tiles)
+  __device__ __forceinline__ int units() const { return wide ? 2 * tiles : tiles; }
+};
+__device__ __forceinline__ Work work_of(const SharedItem* items, int it, int last, int tokens_a_chain) {
+  Work w;
+  const int4* src = (const int4*)(items + (it < last ? it : last - 1));
+  *(int4*)&w.e = src[0];
+  *((int4*)&w.e + 1) = src[1];
+  w.kt0 = w.e.lo / ST_KEYS;
+  w.tiles = (w.e.hi - 1) / ST_KEYS - w.kt0 + 1;
+  w.wide = w.e.tokens > tokens_a_chain;
+  return w;
+}
+
+template <int D>
+__global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                        const __grid_constant__ CUtensorMap map_v, const int* bt, int bt_stride,
+                                                                        const int* plan, float* part_o, float2* part_ml, int Hkv, int G, int page_size,
+                                                                        float scale_log2, int* status) {
+  using S = StSizes<D>;
+  constexpr int NH = D / 64, TILE = S::TILE, OPND = S::OPND, NK = S::NK, NV = S::NV;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *sQ = smem, *sK = sQ + 2 * OPND, *sV = sK + NK * OPND;
+  StBars<D>* bar = (StBars<D>*)(sV + NV * OPND);
+  volatile int* abort_flag = &bar->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (hb_smem_u32(smem) & 1023) {   // never seen; the tiles would not be where the tensor core expects them
+    hb_pdl_wait();
+    hb_pdl_launch();
+    if (threadIdx.x == 0) atomicExch(status, 1);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < 2; b++) {
+      hb_mbar_init(&bar->q_full[b], 1); hb_mbar_init(&bar->q_free[b], 1);
+      hb_mbar_init(&bar->s_full[b], 1); hb_mbar_init(&bar->p_full[b], 4); hb_mbar_init(&bar->pv_done[b], 1);
+    }
+    for (int b = 0; b < NK; b++) { hb_mbar_init(&bar->k_full[b], 1); hb_mbar_init(&bar->k_free[b], 1); }
+    for (int b = 0; b < NV; b++) { hb_mbar_init(&bar->v_full[b], 1); hb_mbar_init(&bar->v_free[b], 1); }
+    bar->abort_flag = 0;
+    hb_fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) { hb_tma_prefetch_desc(&map_q); hb_tma_prefetch_desc(&map_k); hb_tma_prefetch_desc(&map_v); }
+  if (warp == 10) {
+    hb_tmem_alloc(&bar->tmem_slot, 512);
+    hb_tmem_relinquish();
+  }
+  hb_tc_fence_before();
+  __syncthreads();
+  hb_tc_fence_after();
+  const uint32_t tmem = bar->tmem_slot;   // S and P of chain c at c * 128, its O at 256 + c * 128
+  hb_pdl_wait();
+  hb_pdl_launch();
+  const SharedItem* items = (const SharedItem*)(plan + plan[SP_OFF_ITEMS]);
+  const int* ctas = plan + plan[SP_OFF_CTAS];
+  const int it0 = ctas[blockIdx.x], it1 = ctas[blockIdx.x + 1], RT = ST_ROWS / G;
+
+  // Units (a chain's work on a key tile) are numbered through all items, chain = unit & 1; wide: units 2 i and 2 i + 1 are tile i, else unit i is.
+  // The next item begins with chain 0 again, so a chain counts its own units.
+  // Q buffers: a wide item has both, a narrow one the one that the item before did not have.
+  // Registers: 3 x 128 threads were launched with 168; a softmax thread holds a row of scores and takes 208, the other warps keep 88 (2 x 208 + 88 = 3 x 168).
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp < 10) {  // ---------------- TMA
+    const bool is_k = warp == 8;
+    const CUtensorMap* map = is_k ? &map_k : &map_v;
+    uint64_t *full = is_k ? bar->k_full : bar->v_full, *free = is_k ? bar->k_free : bar->v_free;
+    uint8_t* ring = is_k ? sK : sV;
+    const uint32_t stages = is_k ? NK : NV;
+    const int places = ST_KEYS / page_size;
+    uint32_t stage = 0, use = 0, q_use[2] = {0, 0}, qb = 0;
+    bool ok = true;
+    Work ahead = work_of(items, it0, it1, RT);
+    for (int it = it0; it < it1 && ok; it++) {
+      const Work w = ahead;
+      ahead = work_of(items, it + 1, it1, RT);
+      const int* table = bt + (size_t)w.e.table * bt_stride;
+      if (is_k) {
+        for (int c = 0; c < (w.wide ? 2 : 1) && ok; c++) {
+          const uint32_t b = w.wide ? (uint32_t)c : qb;
+          ok = __all_sync(0xffffffffu, hb_mbar_wait(&bar->q_free[b], (q_use[b] & 1) ^ 1, abort_flag));
+          if (!ok) break;
+          q_use[b]++;
+          if (hb_elect()) {
+            hb_mbar_expect_tx(&bar->q_full[b], (uint32_t)(RT * G * D * 2));
+#pragma unroll
+            for (int hf = 0; hf < NH; hf++)
+              tma_load_3d(sQ + b * OPND + hf * TILE, &map_q, &bar->q_full[b], hf * 64, w.e.head * G, w.e.token + c * RT);
+          }
+          __syncwarp();
+        }
+        if (!w.wide) qb ^= 1;
+      }
+      auto page = [&](int t) {
+        const int pg = (w.kt0 + t) * places + lane;
+        return lane < places && pg * page_size < w.e.hi && (pg + 1) * page_size > w.e.lo ? table[pg] : -1;
+      };
+      int next = page(0);
+      for (int t = 0; t < w.tiles && ok; t++) {
+        const uint32_t boxes = __ballot_sync(0xffffffffu, next >= 0);
+        const int row = (next * Hkv + w.e.head) * page_size;
+        next = t + 1 < w.tiles ? page(t + 1) : -1;
+        ok = __all_sync(0xffffffffu, hb_mbar_wait(&free[stage], (use & 1) ^ 1, abort_flag));
+        if (!ok) break;
+        if (hb_elect()) hb_mbar_expect_tx(&full[stage], (uint32_t)__popc(boxes) * page_size * D * 2);
+        __syncwarp();
+        for (int p = 0; p < places; p += 4) {       // four boxes an election
+          int from[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) from[j] = __shfl_sync(0xffffffffu, row, (p + j) & 31);
+          if (hb_elect()) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              if (p + j < places && (boxes >> (p + j) & 1)) {
+                uint8_t* dst = ring + stage * OPND + (p + j) * page_size * 128;            // rows of 128 bytes in each 64-column tile
+#pragma unroll
+                for (int hf = 0; hf < NH; hf++) hb_tma_load_2d(dst + hf * TILE, map, &full[stage], hf * 64, from[j]);
+              }
+          }
+          __syncwarp();
+        }
+        if (++stage == stages) { stage = 0; use++; }
+      }
+    }
+  } else if (warp == 10) {  // ---------------- tensor cores: S = Q K^T
+    if (hb_elect()) {
+      constexpr uint32_t idesc = hb_umma_idesc_bf16(ST_ROWS, ST_KEYS);
+      uint32_t stage = 0, use = 0, q_use[2] = {0, 0}, qb = 0, n[2] = {0, 0};
+      bool ok = true;
+      Work ahead = work_of(items, it0, it1, RT);
+      for (int it = it0; it < it1 && ok; it++) {
+        const Work w = ahead;
+        ahead = work_of(items, it + 1, it1, RT);
+        const int units = w.units();
+        for (int u = 0; u < units && ok; u++) {
+          const uint32_t c = u & 1, b = w.wide ? c : qb;
+          if (u == 0 || (w.wide && u == 1)) {
+            ok = hb_mbar_wait(&bar->q_full[b], q_use[b] & 1, abort_flag);
+            q_use[b]++;
+          }
+          // the product behind the chain's unit before has read its P
+          ok = ok && hb_mbar_wait(&bar->k_full[stage], use & 1, abort_flag) && (n[c] == 0 || hb_mbar_wait(&bar->pv_done[c], (n[c] - 1) & 1, abort_flag));
+          if (!ok) break;
+          hb_tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk++) {   // 16 columns a step: four steps in each 64-column tile
+            const uint64_t dq = hb_umma_desc_k128(hb_smem_u32(sQ + b * OPND + (kk >> 2) * TILE)) + 2 * (kk & 3);
+            const uint64_t dk = hb_umma_desc_k128(hb_smem_u32(sK + stage * OPND + (kk >> 2) * TILE)) + 2 * (kk & 3);
+            hb_umma_bf16(tmem + c * 128, dq, dk, idesc, kk != 0);
+          }
+          hb_umma_commit(&bar->s_full[c]);
+          n[c]++;
+          if (!w.wide || c == 1) {
+            hb_umma_commit(&bar->k_free[stage]);
+            if (++stage == NK) { stage = 0; use++; }
+          }
+          if (u == units - 1 || (w.wide && u == units - 2)) hb_umma_commit(&bar->q_free[b]);
+        }
+        if (!w.wide) qb ^= 1;
+      }
+    }
+  } else {  // ---------------- tensor cores: O += P V
+    if (hb_elect()) {
+      constexpr uint32_t idesc = hb_umma_idesc_bf16(ST_ROWS, D) | (1u << 16);      // B is MN-major
+      uint32_t stage = 0, use = 0, n[2] = {0, 0};
+      bool ok = true;
+      Work ahead = work_of(items, it0, it1, RT);
+      for (int it = it0; it < it1 && ok; it++) {
+        const Work w = ahead;
+        ahead = work_of(items, it + 1, it1, RT);
+        const int units = w.units();
+        for (int u = 0; u < units && ok; u++) {
+          const uint32_t c = u & 1;
+          ok = hb_mbar_wait(&bar->v_full[stage], use & 1, abort_flag) && hb_mbar_wait(&bar->p_full[c], n[c] & 1, abort_flag);
+          if (!ok) break;
+          hb_tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < ST_KEYS / 16; kk++)          // 16 keys: eight columns of P, 16 rows of V
+            umma_ts(tmem + 256 + c * 128, tmem + c * 128 + 8 * kk, desc_mn128(hb_smem_u32(sV + stage * OPND + kk * 16 * 128), TILE), idesc, u > 1 || kk != 0);
+          hb_umma_commit(&bar->pv_done[c]);
+          n[c]++;
+          if (!w.wide || c == 1) {
+            hb_umma_commit(&bar->v_free[stage]);
+            if (++stage == NV) { stage = 0; use++; }
+          }
+        }
+      }
+    }
+  }
+  } else {  // ---------------- softmax: warpgroup c is chain c, a thread a query row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int c = warp >> 2, w4 = warp & 3, r = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(w4 * 32) << 16, tmem_s = tmem + c * 128 + lanes, tmem_o = tmem + 256 + c * 128 + lanes;
+    uint32_t n = 0, vt0 = 0;       // the chain's units, and the V tiles of the items before
+    bool ok = true;                // every wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide
+    auto wait = [&](uint64_t* b, uint32_t parity) { ok = __all_sync(0xffffffffu, hb_mbar_wait(b, parity, abort_flag)); return ok; };
+    const uint64_t scale2 = pack2(scale_log2, scale_log2);
+    Work ahead = work_of(items, it0, it1, RT);
+    for (int it = it0; it < it1 && ok; it++) {
+      const Work w = ahead;
+      ahead = work_of(items, it + 1, it1, RT);
+      const int first = w.wide ? c * RT : 0, rows = min(RT, w.e.tokens - first) * G;           // the chain's rows
+      const bool idle = w4 * 32 >= rows;
+      const int last_key = min(w.e.hi - 1, w.e.pos == SP_NO_MASK ? SP_NO_MASK : w.e.pos + first + r / G);
+      const int sure = w.e.pos == SP_NO_MASK ? w.e.hi : min(w.e.hi, w.e.pos + first + 1);      // the keys below are seen by all rows
+      float m_run = -INFINITY, l_run = 0.f;
+      int units = 0;
+      for (int i = w.wide ? 0 : c; i < w.tiles; i += w.wide ? 1 : 2, units++, n++) {
+        const int k_base = (w.kt0 + i) * ST_KEYS;
+        if (!wait(&bar->s_full[c], n & 1)) break;
+        hb_tc_fence_after();
+        if (!idle) {
+          uint32_t sr[128];
+#pragma unroll
+          for (int q = 0; q < 128; q += 32) ld32(tmem_s + q, sr + q);
+          hb_tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 128; q += 32) ld32_fence(sr + q);
+          if (k_base < w.e.lo || k_base + ST_KEYS > sure) {
+            const int lo_j = w.e.lo - k_base, hi_j = last_key - k_base;
+#pragma unroll
+            for (int j = 0; j < 128; j++)
+              if (j < lo_j || j > hi_j) sr[j] = __float_as_uint(-INFINITY);
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], __uint_as_float(sr[j])), __uint_as_float(sr[j + 1]));
+          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+          const bool grow = m_tile > m_run + ST_SLACK;   // also the first tile with a visible key: m_run is -inf
+          float corr = 1.f;
+          if (grow) {
+            corr = hb_exp2(m_run - m_tile);              // 0 while nothing has been summed
+            m_run = m_tile;
+          }
+          const float sub = m_run == -INFINITY ? 0.f : m_run;
+          const uint64_t sub2 = pack2(-sub, -sub);
+          uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+          for (int j = 0; j < 128; j += 4) {             // masked scores are -inf: 2^-inf = 0
+            float p0, p1, p2, p3;
+            unpack2(fma2(pack2(__uint_as_float(sr[j]), __uint_as_float(sr[j + 1])), scale2, sub2), p0, p1);
+            unpack2(fma2(pack2(__uint_as_float(sr[j + 2]), __uint_as_float(sr[j + 3])), scale2, sub2), p2, p3);
+            p0 = hb_exp2(p0); p1 = hb_exp2(p1); p2 = hb_exp2(p2); p3 = hb_exp2(p3);
+            sum2[0] = add2(sum2[0], pack2(p0, p1));
+            sum2[1] = add2(sum2[1], pack2(p2, p3));
+            // P is rounded to bfloat16, the operand's type; the sum is of the unrounded numbers
+            sr[j >> 1] = hb_pack_bf16(p0, p1);
+            sr[(j >> 1) + 1] = hb_pack_bf16(p2, p3);
+          }
+          st32(tmem_s, sr);
+          st32(tmem_s + 32, sr + 32);
+          float s0, s1, s2, s3;
+          unpack2(sum2[0], s0, s1);
+          unpack2(sum2[1], s2, s3);
+          l_run = l_run * corr + ((s0 + s1) + (s2 + s3));
+          if (units > 0 && __any_sync(0xffffffffu, grow)) {   // the rows of O so far: the product before was done when these scores were begun
+#pragma unroll
+            for (int q = 0; q < D / 32; q++) {
+              uint32_t o[32];
+              ld32(tmem_o + q * 32, o);
+              hb_tmem_ld_wait();
+              ld32_fence(o);
+#pragma unroll
+              for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr);
+              st32(tmem_o + q * 32, o);
+            }
+          }
+          hb_tmem_st_wait();
+        }
+        if (k_base < w.e.lo || k_base + ST_KEYS > w.e.hi) {      // thread r clears row r of V where the item does not reach
+          const uint32_t vt = vt0 + i, stage = vt % NV;
+          if (!wait(&bar->v_full[stage], (vt / NV) & 1)) break;
+          if (k_base + r < w.e.lo || k_base + r >= w.e.hi) {
+            const uint32_t dst = hb_smem_u32(sV + stage * OPND) + r * 128;
+#pragma unroll
+            for (int hf = 0; hf < NH; hf++)
+#pragma unroll
+              for (int q = 0; q < 8; q++)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * TILE + q * 16), "r"(0) : "memory");
+          }
+          hb_fence_proxy_async();
+        }
+        hb_tc_fence_before();
+        __syncwarp();
+        if (lane == 0) hb_mbar_arrive(&bar->p_full[c]);
+      }
+      vt0 += w.tiles;
+      if (!ok) break;
+      // ---- the item's end: the rows' parts
+      const size_t part = (size_t)w.e.part + (c == 0 ? 0 : w.wide ? RT * G : rows);
+      if (units > 0) {
+        if (!wait(&bar->pv_done[c], (n - 1) & 1)) break;
+        hb_tc_fence_after();
+      }
+      if (r < rows) part_ml[part + r] = make_float2(m_run, l_run);
+      if (units > 0 && !idle) {
+        float* dst = part_o + (part + r) * D;
+#pragma unroll
+        for (int q = 0; q < D / 32; q++) {
+          uint32_t o[32];
+          ld32(tmem_o + q * 32, o);
+          hb_tmem_ld_wait();
+          ld32_fence(o);
+          if (r < rows) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4) *(uint4*)(dst + q * 32 + d) = make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          }
+        }
+        hb_tc_fence_before();
+      }
+    }
+  }
+
+  hb_tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicExch(status, 1);
+    __nanosleep(100000);
+  }
+  if (warp == 10) {
+    __syncwarp();
+    hb_tmem_dealloc(tmem, 512);
+  }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeFn)p;
+  }
+  return fn;
+}
+// A bfloat16 map with the 128-byte swizzle; strides in bytes of dimension 1 (and 2).
+int make_map(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  EncodeFn fn = encode_fn();
+  if (!fn) HB_FAIL("cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) HB_FAIL("hb_shared_items_tc: cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return 0;
+}
+
+}  // namespace
+
+// Whether the kernel takes these sizes (whatever they are, rows of q and pages have to lie on 16 bytes).
+HB_EXPORT int hb_shared_items_tc_supported(int Hq, int Hkv, int D, int page_size) {
+  return Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= ST_ROWS && (D == 64 || D == 128) && page_size >= 8 && page_size <= ST_KEYS &&
+         (page_size & (page_size - 1)) == 0;
+}
+
+// As hb_shared_items, for a plan whose items have up to 2 * (128 / G) tokens, of which those of up to 128 / G leave two parts; `status` is set to 1 if
+// a bounded wait ran out.
+HB_EXPORT int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan,
+                                 int ctas, int T, float* part_o, void* part_ml, int Hq, int Hkv, int D, int page_size, float scale, int* status,
+                                 cudaStream_t s) {
+  if (!hb_shared_items_tc_supported(Hq, Hkv, D, page_size))
+    HB_FAIL("hb_shared_items_tc: %d/%d heads of %d with pages of %d are not supported", Hq, Hkv, D, page_size);
+  if (ctas <= 0 || T <= 0) return 0;
+  if (!status) HB_FAIL("hb_shared_items_tc: no status word");
+  if ((((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15) || (ldq * 2) % 16 || ldq < (long)Hq * D)
+    HB_FAIL("hb_shared_items_tc: rows of q and pages have to lie on 16 bytes");
+  const long rows = num_pages * Hkv * page_size;
+  if (rows > 0x7fffffff) HB_FAIL("hb_shared_items_tc: %ld pages are beyond the maps' limit", num_pages);
+  const int G = Hq / Hkv;
+  CUtensorMap mq, mk, mv;
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)T}, strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)ldq * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(ST_ROWS / G)};
+    if (make_map(&mq, q, 3, dims, strides, box)) return -1;
+  }
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)D * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)page_size};
+    if (make_map(&mk, kc, 2, dims, strides, box) || make_map(&mv, vc, 2, dims, strides, box)) return -1;
+  }
+  cudaError_t e = cudaSuccess;
+#define ST_LAUNCH(DD)                                                                                                               \
+  do {                                                                                                                             \
+    static bool configured = false;                                                                                                \
+    if (!configured) {                                                                                                             \
+      e = cudaFuncSetAttribute(shared_items_tc_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, st_smem<DD>());             \
+      if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));                                               \
+      configured = true;                                                                                                           \
+    }                                                                                                                              \
+    e = hb_launch(shared_items_tc_kernel<DD>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, plan, part_o,          \
+                  (float2*)part_ml, Hkv, G, page_size, scale * 1.4426950408889634f, status);                                        \
+  } while (0)
+  if (D == 64) ST_LAUNCH(64);
+  else ST_LAUNCH(128);
+#undef ST_LAUNCH
+  if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));
+  HB_CHECK_LAUNCH("hb_shared_items_tc");
+  return 0;
+}

@@ -18,7 +18,9 @@ from . import library, ops
 _p, _i, _l, _f = C.c_void_p, C.c_int, C.c_long, C.c_float
 ops._SIGS["drafts"] = {
     "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i],
-    "hb_shared_items": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _i, _p, _p, _i, _i, _i, _i, _f, _i, _p],
+    "hb_shared_items": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _i, _i, _p, _p, _i, _i, _i, _i, _f, _i, _p],
+    "hb_shared_items_tc": [_p, _l, _p, _p, _l, _p, _i, _p, _i, _i, _p, _p, _i, _i, _i, _i, _f, _p, _p],
+    "hb_shared_items_tc_supported": [_i, _i, _i, _i],
     "hb_shared_join": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _p, _p, _p, _i, _i, _i, _i, _f, _i, _p],
     "hb_verify_drafts": [_p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _l, _p, _i, _l, _l, _p, _p, _p, _p, _p],
 }
@@ -68,8 +70,15 @@ class SharedPlan:
         self.device = torch.device(device)
         self.n_requests = len(q_lens)
         group = n_heads // n_kv_heads
-        tile, narrow, key_tile, ctas, item_cost, part_cost = max(1, 64 // group), 0, 64, 2 * _sms(self.device), 1.0, head_dim * 2e-6
+        # on the tensor cores: one CTA an SM, items of two chains of up to 128 rows each
+        self.tensor_cores = (dtype == torch.bfloat16 and ops.fast_kernels_on()
+                             and bool(ops._fn("drafts", "hb_shared_items_tc_supported")(n_heads, n_kv_heads, head_dim, page_size)))
+        if self.tensor_cores:
+            tile, narrow, key_tile, ctas, item_cost, part_cost = 2 * (128 // group), 128 // group, 128, _sms(self.device), 1.5, head_dim * 2e-6
+        else:
+            tile, narrow, key_tile, ctas, item_cost, part_cost = max(1, 64 // group), 0, 64, 2 * _sms(self.device), 1.0, head_dim * 2e-6
         numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, tile, narrow, key_tile, ctas, item_cost, part_cost)
+        self.narrow = narrow
         self.rows, self.parts = int(numbers[_TOKENS]), int(numbers[_PARTS])
         self.ctas, self.max_rows = int(numbers[_CTAS]), int(numbers[_MAX_ROWS])
         self.most_keys = max((int(c) + int(n) for c, n in zip(ctx_lens, q_lens) if n), default=0)
@@ -114,10 +123,14 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     part_o = None if ws is None else ws.data_ptr()
     part_ml = None if ws is None else part_o + 4 * (plan.parts * D + (-plan.parts * D) % 4)
     size = q.element_size()
-    vec = int(D % 4 == 0 and (q.stride(0) * size) % 16 == 0 and not any(x.data_ptr() % 16 for x in (q, k_cache, v_cache, out)))
-    if plan.ctas:
+    aligned = (q.stride(0) * size) % 16 == 0 and not any(x.data_ptr() % 16 for x in (q, k_cache, v_cache, out))
+    vec = int(aligned and D % 4 == 0)
+    if plan.ctas and plan.tensor_cores and aligned:
+        ops._call("drafts", "hb_shared_items_tc", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_table.data_ptr(),
+                  bts, plan.numbers.data_ptr(), plan.ctas, T, part_o, part_ml, Hq, Hkv, D, ps, scale, ops.fast._status_ptr(), st)
+    elif plan.ctas:
         ops._call("drafts", "hb_shared_items", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), dt, block_table.data_ptr(), bts,
-                  plan.numbers.data_ptr(), plan.ctas, plan.max_rows, part_o, part_ml, Hq, Hkv, D, ps, scale, vec, st)
+                  plan.numbers.data_ptr(), plan.ctas, plan.max_rows, plan.narrow, part_o, part_ml, Hq, Hkv, D, ps, scale, vec, st)
     ops._call("drafts", "hb_shared_join", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), dt, block_table.data_ptr(), bts,
               plan.numbers.data_ptr(), T, part_o, part_ml, out.data_ptr(), Hq, Hkv, D, ps, scale, vec, st)
     return out

@@ -33,7 +33,7 @@ LIBRARIES: Dict[str, List[str]] = {
     "mixers": ["mixers_entry.cu", "delta_rule.cu", "attention_window.cu", "attention_window_flash.cu"],
     "seqmix": ["seqmix_entry.cu", "attention_masked.cu", "attention_masked_flash.cu", "attention_masked_heads.cu", "latent.cu", "gla.cu"],
     "hybrid": ["hybrid_entry.cu", "hyper_streams.cu", "ssd.cu", "moe.cu", "selective_scan.cu"],
-    "drafts": ["drafts_entry.cu", "shared_plan.cu", "attention_shared.cu", "verify_drafts.cu"],
+    "drafts": ["drafts_entry.cu", "shared_plan.cu", "attention_shared.cu", "attention_shared_tc.cu", "verify_drafts.cu"],
     "memory": ["memory_entry.cu", "matrix_state.cu", "depth_average.cu"],
     "fast": ["fast_entry.cu", "gemm_tc.cu", "gemm_stream.cu", "gemm_stream_consumers.cu", "gemm_rows.cu", "gemm_split.cu", "attention_fast.cu", "attention_prefill.cu", "attention_prefill_tc.cu", "attention_diff_tc.cu", "wait_selftest.cu"],
 }
