@@ -314,55 +314,50 @@ int launch_items(const void* q, long ldq, const void* kc, const void* vc, const 
   return 0;
 }
 
-int check_sizes(const char* who, int Hq, int Hkv, int D, int page_size) {
-  if (Hkv < 1 || Hq < Hkv || Hq % Hkv) HB_FAIL("%s: %d heads are not a multiple of %d kv heads", who, Hq, Hkv);
-  if (D < 1 || D > 256) HB_FAIL("%s: heads of %d (1 to 256 are supported)", who, D);
-  if (page_size < 1) HB_FAIL("%s: pages of %d", who, page_size);
-  return 0;
-}
-
 }  // namespace
 
-// q [T, ldq] (heads of D side by side), caches [page, Hkv, page_size, D], bt [R, bt_stride], plan on the device (see shared_plan.cu) and its
-// n_ctas, max_rows and narrow_tokens; part_o [parts][D], part_ml [parts] (16-byte aligned). vec: all rows start on 16 bytes.
-HB_EXPORT int hb_shared_items(const void* q, long ldq, const void* kc, const void* vc, int dt, const int* bt, int bt_stride, const int* plan, int ctas,
-                              int max_rows, int narrow, float* part_o, void* part_ml, int Hq, int Hkv, int D, int page_size, float scale, int vec,
-                              cudaStream_t s) {
-  if (check_sizes("hb_shared_items", Hq, Hkv, D, page_size)) return -1;
-  if (ctas <= 0 || max_rows <= 0) return 0;
-  const float sl2 = scale * 1.4426950408889634f;
-  int r = -1;
-#define SI_LAUNCH(RM, NC) \
-  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, plan, ctas, max_rows, narrow, part_o, (float2*)part_ml, Hq, Hkv, D, page_size, sl2, vec, s)
-  HB_DISPATCH_1(dt, "hb_shared_items", {
-    if (max_rows <= 16) {
-      if (D <= 64) SI_LAUNCH(1, 1); else if (D <= 128) SI_LAUNCH(1, 2); else SI_LAUNCH(1, 4);
-    } else {
-      if (D <= 64) SI_LAUNCH(4, 1); else if (D <= 128) SI_LAUNCH(4, 2); else SI_LAUNCH(4, 4);
-    }
-  });
-#undef SI_LAUNCH
-  if (r) return r;
-  HB_CHECK_LAUNCH("hb_shared_items");
-  return 0;
-}
+// What a call has of its plan, in host memory: the numbers that the launches want.
+struct SharedLaunch { int T, ctas, max_rows, narrow, parts, tensor_cores, dt, Hq, Hkv, D, page_size; };
 
-// out [T, Hq, D] from the parts and the keys of the step's own rows. T as in the plan.
-HB_EXPORT int hb_shared_join(const void* q, long ldq, const void* kc, const void* vc, int dt, const int* bt, int bt_stride, const int* plan, int T,
-                             const float* part_o, const void* part_ml, void* out, int Hq, int Hkv, int D, int page_size, float scale, int vec,
-                             cudaStream_t s) {
-  if (check_sizes("hb_shared_join", Hq, Hkv, D, page_size)) return -1;
+// q [T, ldq] (heads of D side by side), caches [num_pages, Hkv, page_size, D], bt [R, bt_stride], plan on the device (see shared_plan.cu) and `h` of it;
+// workspace parts * (D + 2) + 4 floats, 16-byte aligned; out [T, Hq, D]. aligned: rows of q, pages and out start on 16 bytes. `status` is set to 1 if
+// a bounded wait ran out.
+HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan,
+                                  const SharedLaunch* h, float* workspace, void* out, float scale, int aligned, int* status, cudaStream_t s) {
+  const int Hq = h->Hq, Hkv = h->Hkv, D = h->D, ps = h->page_size, T = h->T;
+  if (Hkv < 1 || Hq < Hkv || Hq % Hkv) HB_FAIL("hb_attention_shared: %d heads are not a multiple of %d kv heads", Hq, Hkv);
+  if (D < 1 || D > 256 || ps < 1) HB_FAIL("hb_attention_shared: heads of %d (1 to 256 are supported), pages of %d", D, ps);
   if (T <= 0) return 0;
   const long warps = (long)T * Hq;
-  if (warps > (1l << 30)) HB_FAIL("hb_shared_join: %d rows of %d heads are beyond the grid limit", T, Hq);
+  if (warps > (1l << 30)) HB_FAIL("hb_attention_shared: %d rows of %d heads are beyond the grid limit", T, Hq);
+  if (h->parts > 0 && (!workspace || ((uintptr_t)workspace & 15))) HB_FAIL("hb_attention_shared: the workspace must be 16-byte aligned");
+  float* part_o = workspace;
+  float2* part_ml = (float2*)(workspace + ((long)h->parts * D + 3) / 4 * 4);
+  const int vec = aligned && D % 4 == 0;
   const float sl2 = scale * 1.4426950408889634f;
+  if (h->ctas > 0 && h->tensor_cores && aligned) {
+    if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, plan, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
+  } else if (h->ctas > 0) {
+    int r = -1;
+#define SI_LAUNCH(RM, NC) \
+  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, plan, h->ctas, h->max_rows, h->narrow, part_o, part_ml, Hq, Hkv, D, ps, sl2, vec, s)
+    HB_DISPATCH_1(h->dt, "hb_attention_shared", {
+      if (h->max_rows <= 16) {
+        if (D <= 64) SI_LAUNCH(1, 1); else if (D <= 128) SI_LAUNCH(1, 2); else SI_LAUNCH(1, 4);
+      } else {
+        if (D <= 64) SI_LAUNCH(4, 1); else if (D <= 128) SI_LAUNCH(4, 2); else SI_LAUNCH(4, 4);
+      }
+    });
+#undef SI_LAUNCH
+    if (r) return r;
+  }
   cudaError_t e = cudaSuccess;
 #define SJ_LAUNCH(E)                                                                                                                     \
   e = hb_launch(shared_join_kernel<TA, E>, dim3((unsigned)((warps + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq,   \
-                (const TA*)kc, (const TA*)vc, bt, bt_stride, plan, part_o, (const float2*)part_ml, (TA*)out, Hq, Hkv, D, page_size, sl2, vec)
-  HB_DISPATCH_1(dt, "hb_shared_join", { if (D <= 64) SJ_LAUNCH(2); else if (D <= 128) SJ_LAUNCH(4); else SJ_LAUNCH(8); });
+                (const TA*)kc, (const TA*)vc, bt, bt_stride, plan, part_o, part_ml, (TA*)out, Hq, Hkv, D, ps, sl2, vec)
+  HB_DISPATCH_1(h->dt, "hb_attention_shared", { if (D <= 64) SJ_LAUNCH(2); else if (D <= 128) SJ_LAUNCH(4); else SJ_LAUNCH(8); });
 #undef SJ_LAUNCH
-  if (e != cudaSuccess) HB_FAIL("hb_shared_join: %s", cudaGetErrorString(e));
-  HB_CHECK_LAUNCH("hb_shared_join");
+  if (e != cudaSuccess) HB_FAIL("hb_attention_shared: %s", cudaGetErrorString(e));
+  HB_CHECK_LAUNCH("hb_attention_shared");
   return 0;
 }

@@ -441,11 +441,8 @@ HB_EXPORT int hb_shared_items_tc_supported(int Hq, int Hkv, int D, int page_size
          (page_size & (page_size - 1)) == 0;
 }
 
-// As hb_shared_items, for a plan whose items have up to 2 * (128 / G) tokens, of which those of up to 128 / G leave two parts; `status` is set to 1 if
-// a bounded wait ran out.
-HB_EXPORT int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan,
-                                 int ctas, int T, float* part_o, void* part_ml, int Hq, int Hkv, int D, int page_size, float scale, int* status,
-                                 cudaStream_t s) {
+int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan, int ctas,
+                       int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s) {
   if (!hb_shared_items_tc_supported(Hq, Hkv, D, page_size))
     HB_FAIL("hb_shared_items_tc: %d/%d heads of %d with pages of %d are not supported", Hq, Hkv, D, page_size);
   if (ctas <= 0 || T <= 0) return 0;
@@ -476,7 +473,7 @@ HB_EXPORT int hb_shared_items_tc(const void* q, long ldq, const void* kc, const 
       configured = true;                                                                                                           \
     }                                                                                                                              \
     e = hb_launch(shared_items_tc_kernel<DD>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, plan, part_o,          \
-                  (float2*)part_ml, Hkv, G, page_size, scale * 1.4426950408889634f, status);                                        \
+                  part_ml, Hkv, G, page_size, scale_log2, status);                                        \
   } while (0)
   if (D == 64) ST_LAUNCH(64);
   else ST_LAUNCH(128);

@@ -1,5 +1,6 @@
 // What the planner of the shared-prefix attention hands to its kernels (shared_plan.cu, attention_shared*.cu).
 #pragma once
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 // Keys [lo, hi) of one kv head against `tokens` consecutive rows of q with all heads of the group: read through block table row
@@ -19,3 +20,8 @@ constexpr int SP_NO_MASK = 1 << 30;
 // A request of up to this many rows in the step has its rows' own keys (they are causal among themselves) added by the joining kernel; the
 // items then have no mask, and what stands behind a row, whatever it is, is never multiplied by a probability of 0.
 constexpr int SP_FRESH = 16;
+
+// The items on the tensor cores (attention_shared_tc.cu): bfloat16, for a plan whose items have up to 2 * (128 / G) tokens, of which those of up to
+// 128 / G leave two parts. scale_log2: the scale times log2(e).
+int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan, int ctas,
+                       int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s);

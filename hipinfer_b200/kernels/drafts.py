@@ -7,6 +7,7 @@ logits and leaves the choice to the caller."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -18,11 +19,10 @@ from . import library, ops
 _p, _i, _l, _f = C.c_void_p, C.c_int, C.c_long, C.c_float
 ops._SIGS["drafts"] = {
     "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i],
-    "hb_shared_items": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _i, _i, _p, _p, _i, _i, _i, _i, _f, _i, _p],
-    "hb_shared_items_tc": [_p, _l, _p, _p, _l, _p, _i, _p, _i, _i, _p, _p, _i, _i, _i, _i, _f, _p, _p],
+    "hb_attention_shared": [_p, _l, _p, _p, _l, _p, _i, _p, _p, _p, _p, _f, _i, _p, _p],
     "hb_shared_items_tc_supported": [_i, _i, _i, _i],
-    "hb_shared_join": [_p, _l, _p, _p, _i, _p, _i, _p, _i, _p, _p, _p, _i, _i, _i, _i, _f, _i, _p],
     "hb_verify_drafts": [_p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _l, _p, _i, _l, _l, _p, _p, _p, _p, _p],
+    "hb_verify_drafts_workspace": [_i, _i, _i, _i],
 }
 MAX_DRAFTS = 63
 
@@ -78,10 +78,15 @@ class SharedPlan:
         else:
             tile, narrow, key_tile, ctas, item_cost, part_cost = max(1, 64 // group), 0, 64, 2 * _sms(self.device), 1.0, head_dim * 2e-6
         numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, tile, narrow, key_tile, ctas, item_cost, part_cost)
-        self.narrow = narrow
         self.rows, self.parts = int(numbers[_TOKENS]), int(numbers[_PARTS])
         self.ctas, self.max_rows = int(numbers[_CTAS]), int(numbers[_MAX_ROWS])
         self.most_keys = max((int(c) + int(n) for c, n in zip(ctx_lens, q_lens) if n), default=0)
+        self.q_shape, self.page_shape = (self.rows, n_heads * head_dim), (n_kv_heads, page_size, head_dim)
+        self.size, self.default_scale = 2 if dtype == torch.bfloat16 else 4, 1.0 / math.sqrt(head_dim)
+        self.workspace = self.parts * (head_dim + 2) + 4           # floats
+        self._launch = np.array([self.rows, self.ctas, self.max_rows, narrow, self.parts, self.tensor_cores, ops._DT[dtype], n_heads, n_kv_heads,
+                                 head_dim, page_size], dtype=np.int32)      # SharedLaunch of csrc/attention_shared.cu
+        self.launch = self._launch.ctypes.data
         host = torch.from_numpy(numbers)
         if self.device.type == "cuda":
             host = host.pin_memory()
@@ -98,47 +103,36 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of the plan's rows over their requests' pages. q [T, Hq D] (rows may be part of wider ones); caches [page, Hkv, page_size, D]
     of the same type; block_table int32 [R, pages]; out [T, Hq D]; scale 1 / sqrt(D) by default. Scores, softmax and sums are 32-bit; the
     keys' cut, and with it a result's last bits, is a matter of the plan."""
-    ops._need_cuda(q, k_cache, v_cache, block_table, out)
-    Hq, Hkv, D, ps, T = plan.n_heads, plan.n_kv_heads, plan.head_dim, plan.page_size, plan.rows
-    if q.dim() != 2 or q.shape != (T, Hq * D) or q.stride(1) != 1 or q.dtype != plan.dtype:
-        raise ops.KernelError(f"attention_shared: q {tuple(q.shape)} {q.dtype}, strides {q.stride()}; the plan has {T} rows of {Hq} heads of {D}, {plan.dtype}")
+    if not (q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and block_table.is_cuda):
+        ops._need_cuda(q, k_cache, v_cache, block_table)
+    width, dtype, T = plan.n_heads * plan.head_dim, plan.dtype, plan.rows
+    if q.dim() != 2 or q.shape != plan.q_shape or q.dtype != dtype or q.stride(1) != 1:
+        raise ops.KernelError(f"attention_shared: q {tuple(q.shape)} {q.dtype}, strides {q.stride()}; the plan has {T} rows of {plan.n_heads} heads of "
+                              f"{plan.head_dim}, {dtype}")
+    pages = k_cache.shape[0]
     for name, x in (("keys", k_cache), ("values", v_cache)):
-        if x.dim() != 4 or x.shape[1:] != (Hkv, ps, D) or not x.is_contiguous() or x.dtype != plan.dtype:
-            raise ops.KernelError(f"attention_shared: {name} {tuple(x.shape)} {x.dtype} are no pages of {Hkv} heads x {ps} tokens x {D}, {plan.dtype}")
-    if k_cache.shape[0] != v_cache.shape[0]:
-        raise ops.KernelError(f"attention_shared: {k_cache.shape[0]} pages of keys, {v_cache.shape[0]} of values")
+        if x.shape != (pages, *plan.page_shape) or x.dtype != dtype or not x.is_contiguous():
+            raise ops.KernelError(f"attention_shared: {name} {tuple(x.shape)} {x.dtype}, {pages} pages of {plan.n_kv_heads} heads x {plan.page_size} tokens x "
+                                  f"{plan.head_dim}, {dtype}, are expected")
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1 or block_table.shape[0] != plan.n_requests \
-            or block_table.shape[1] * ps < plan.most_keys:
+            or block_table.shape[1] * plan.page_size < plan.most_keys:
         raise ops.KernelError(f"attention_shared: block table {tuple(block_table.shape)} {block_table.dtype}; the plan has {plan.n_requests} requests of up "
-                              f"to {plan.most_keys} tokens in pages of {ps}")
+                              f"to {plan.most_keys} tokens in pages of {plan.page_size}")
     if out is None:
-        out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device)
-    elif out.shape != (T, Hq * D) or out.dtype != q.dtype or not out.is_contiguous():
+        out = q.new_empty(T, width)
+    elif out.shape != plan.q_shape or out.dtype != dtype or not out.is_contiguous() or not out.is_cuda:
+        ops._need_cuda(out)
         raise ops.KernelError(f"attention_shared: out {tuple(out.shape)} {out.dtype}, strides {out.stride()}")
     if not T:
         return out
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    dt, st, bts = ops._DT[q.dtype], library.current_stream(), block_table.stride(0)
-    ws = torch.empty(plan.parts * (D + 2) + 4, dtype=torch.float32, device=q.device) if plan.parts else None
-    part_o = None if ws is None else ws.data_ptr()
-    part_ml = None if ws is None else part_o + 4 * (plan.parts * D + (-plan.parts * D) % 4)
-    size = q.element_size()
-    aligned = (q.stride(0) * size) % 16 == 0 and not any(x.data_ptr() % 16 for x in (q, k_cache, v_cache, out))
-    vec = int(aligned and D % 4 == 0)
-    if plan.ctas and plan.tensor_cores and aligned:
-        ops._call("drafts", "hb_shared_items_tc", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_table.data_ptr(),
-                  bts, plan.numbers.data_ptr(), plan.ctas, T, part_o, part_ml, Hq, Hkv, D, ps, scale, ops.fast._status_ptr(), st)
-    elif plan.ctas:
-        ops._call("drafts", "hb_shared_items", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), dt, block_table.data_ptr(), bts,
-                  plan.numbers.data_ptr(), plan.ctas, plan.max_rows, plan.narrow, part_o, part_ml, Hq, Hkv, D, ps, scale, vec, st)
-    ops._call("drafts", "hb_shared_join", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), dt, block_table.data_ptr(), bts,
-              plan.numbers.data_ptr(), T, part_o, part_ml, out.data_ptr(), Hq, Hkv, D, ps, scale, vec, st)
+    ws = torch.empty(plan.workspace, dtype=torch.float32, device=q.device) if plan.parts else None
+    qp, kp, vp, op, ld = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), q.stride(0)
+    aligned = int((ld * plan.size) % 16 == 0 and (qp | kp | vp | op) % 16 == 0)
+    library.launches[0] += plan.ctas > 0
+    ops._call("drafts", "hb_attention_shared", qp, ld, kp, vp, pages, block_table.data_ptr(), block_table.stride(0), plan.numbers.data_ptr(), plan.launch,
+              None if ws is None else ws.data_ptr(), op, plan.default_scale if scale is None else scale, aligned, ops.fast._status_ptr(),
+              library.current_stream())
     return out
-
-
-def _vector(x, dtype, n, what):
-    if x.dtype != dtype or x.numel() != n or not x.is_contiguous():
-        raise ops.KernelError(f"verify_drafts: {what} {tuple(x.shape)} {x.dtype}, {n} of {dtype} side by side are expected")
 
 
 def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Tensor, drafts: torch.Tensor, temperature: torch.Tensor,
@@ -146,7 +140,7 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
     """Accepts or refuses drafted tokens so that what is produced is distributed as if the target alone had drawn it.
 
     Request r has n_drafts[r] drafts in row r of `drafts` (int32 [R, K]) and n_drafts[r] + 1 rows of logits ([T, V], float32 or bfloat16) from row
-    start[r] on; p_i is the softmax of the i-th over `temperature[r]` (float32 [R]; 0: greedy, a point mass on the lowest index of the largest
+    start[r] on; p_i is the softmax of the i-th over `temperature[r]` (float32 [R]; 0 or less: greedy, a point mass on the lowest index of the largest
     logit, which is also what a row without a finite largest logit is; NaN counts as above all). Draft i is accepted iff all before it are and
     uniform[r, i] * q_i(draft) < p_i(draft), with q_i = draft_probs[r, i] ([R, K, V], float32 or bfloat16), or 1 where no distributions are given (drafts
     that were looked up). The token behind the accepted ones is the arg max of w / noise[r] (float32 [R, V], exponential variates; ties: the lowest
@@ -156,36 +150,50 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
     log p_i of each, at temperature 1 for a greedy request, 0 for a row without a finite largest logit and behind the last). A request whose
     rows lie outside the logits gets no token."""
     ops._need_cuda(logits, start, n_drafts, drafts, temperature, uniform, noise, draft_probs)
-    ops._rows_contiguous(logits, "verify_drafts logits")
-    if drafts.dim() != 2 or drafts.dtype != torch.int32 or not drafts.is_contiguous():
-        raise ops.KernelError(f"verify_drafts: drafts {tuple(drafts.shape)} {drafts.dtype}, strides {drafts.stride()}; int32 [R, K] is expected")
+    if logits.dim() != 2 or drafts.dim() != 2:
+        raise ops.KernelError(f"verify_drafts: logits {tuple(logits.shape)} and drafts {tuple(drafts.shape)}, [T, V] and [R, K] are expected")
     (T, V), (R, K) = logits.shape, drafts.shape
+    if logits.stride(1) != 1 and V > 1:
+        raise ops.KernelError(f"verify_drafts: logits with strides {logits.stride()}, rows side by side are expected")
     if K > MAX_DRAFTS:
         raise ops.KernelError(f"verify_drafts: {K} drafts a request, at most {MAX_DRAFTS}")
+    _vector(drafts, torch.int32, R * K, "drafts")
     _vector(start, torch.int32, R, "start")
     _vector(n_drafts, torch.int32, R, "n_drafts")
     _vector(temperature, torch.float32, R, "temperature")
     _vector(uniform, torch.float32, R * K, "uniform")
     if noise.shape != (R, V) or noise.dtype != torch.float32 or (V > 1 and noise.stride(1) != 1):
         raise ops.KernelError(f"verify_drafts: noise {tuple(noise.shape)} {noise.dtype}, strides {noise.stride()}; float32 [{R}, {V}] is expected")
-    if draft_probs is not None and (draft_probs.shape != (R, K, V) or draft_probs.dtype not in ops._DT or (V > 1 and draft_probs.stride(2) != 1)):
-        raise ops.KernelError(f"verify_drafts: draft_probs {tuple(draft_probs.shape)} {draft_probs.dtype}, strides {draft_probs.stride()}; [{R}, {K}, {V}] is "
-                              f"expected")
+    probs = (None, 0, 0, 0)
+    if draft_probs is not None:
+        if draft_probs.shape != (R, K, V) or draft_probs.dtype not in ops._DT or (V > 1 and draft_probs.stride(2) != 1):
+            raise ops.KernelError(f"verify_drafts: draft_probs {tuple(draft_probs.shape)} {draft_probs.dtype}, strides {draft_probs.stride()}; [{R}, {K}, {V}] "
+                                  f"is expected")
+        if K:
+            probs = (draft_probs.data_ptr(), ops._DT[draft_probs.dtype], draft_probs.stride(0), draft_probs.stride(1))
     dt = ops._dt(logits)
-    numbers = torch.empty(R * (K + 2), dtype=torch.int32, device=logits.device)
-    tokens, counts = numbers[:R * (K + 1)].view(R, K + 1), numbers[R * (K + 1):]
-    logprobs = torch.empty(R, K + 1, dtype=torch.float32, device=logits.device)
+    tokens, counts, logprobs = drafts.new_empty((R, K + 1)), n_drafts.new_empty((R,)), uniform.new_empty((R, K + 1))
     if not R:
         return tokens, counts, logprobs
     if not V:
         raise ops.KernelError("verify_drafts: empty vocabulary")
-    lib = library.load("drafts")
-    lib.hb_verify_drafts_workspace.restype = C.c_long
-    ws = torch.empty(lib.hb_verify_drafts_workspace(R, K, V, dt), dtype=torch.uint8, device=logits.device)
-    probs = draft_probs if K else None
+    ws = noise.new_empty((_workspace(R, K, V, dt),))
     library.launches[0] += 1
     ops._call("drafts", "hb_verify_drafts", logits.data_ptr(), dt, logits.stride(0), T, V, start.data_ptr(), n_drafts.data_ptr(), drafts.data_ptr(), R, K,
-              temperature.data_ptr(), uniform.data_ptr(), noise.data_ptr(), noise.stride(0), ops._ptr(probs), 0 if probs is None else ops._dt(probs),
-              0 if probs is None else probs.stride(0), 0 if probs is None else probs.stride(1), ws.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
+              temperature.data_ptr(), uniform.data_ptr(), noise.data_ptr(), noise.stride(0), *probs, ws.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
               logprobs.data_ptr(), library.current_stream())
     return tokens, counts, logprobs
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(R: int, K: int, V: int, dt: int) -> int:
+    """Floats that the two kernels of a verification of this size meet in."""
+    n = ops._fn("drafts", "hb_verify_drafts_workspace")(R, K, V, dt)
+    if n < 0:
+        raise ops.KernelError(f"verify_drafts: {R} requests of {K} drafts, a vocabulary of {V}: too many")
+    return n
+
+
+def _vector(x, dtype, n, what):
+    if x.dtype is not dtype or x.numel() != n or not x.is_contiguous():
+        raise ops.KernelError(f"verify_drafts: {what} {tuple(x.shape)} {x.dtype}, strides {x.stride()}; {n} of {dtype} side by side are expected")

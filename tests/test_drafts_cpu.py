@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from hipinfer_b200.kernels import drafts, library, ops
+from hipinfer_b200.kernels import drafts, fast, library, ops
 
 pytestmark = pytest.mark.skipif(not (os.path.isfile("/usr/local/cuda/bin/nvcc") or os.environ.get("HIPINFER_B200_NVCC")), reason="no nvcc")
 NO_MASK, FRESH = 1 << 30, 16
@@ -140,6 +140,7 @@ def launches(monkeypatch):
     monkeypatch.setattr(ops, "_call", lambda lib, name, *a: calls.append(name))
     monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)
     monkeypatch.setattr(library, "current_stream", lambda: 0)
+    monkeypatch.setattr(fast, "_status_ptr", lambda: 0)
     return calls
 
 
@@ -151,7 +152,7 @@ def attend(plan_kw={}, **kw):
 
 
 def test_attention_shared_takes_what_it_is_made_for(launches):
-    assert attend().shape == (3, 256) and launches == ["hb_shared_items", "hb_shared_join"]
+    assert attend().shape == (3, 256) and launches == ["hb_attention_shared"]
     assert attend(q=torch.zeros(3, 300)[:, :256]).is_contiguous()
 
 
