@@ -36,7 +36,8 @@ template <int RM, int NC> constexpr int items_smem() {
 // A thread has RM rows (ty RM ..) by four keys (tx, tx + 16, ..) of the scores, and RM rows by 4 NC columns of the output.
 template <typename T, int RM, int NC>
 __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
-                                                                  const int* plan, int narrow, float* part_o, float2* part_ml, int Hq, int Hkv,
+                                                                  const SharedItem* items, const int* ctas, int narrow, float* part_o,
+                                                                  float2* part_ml, int Hq, int Hkv,
                                                                   int D, int page_size, float scale_log2, int vec) {
   constexpr int R = 16 * RM, DP = 64 * NC, LD = DP + 4, LP = SI_KEYS + 4;
   extern __shared__ __align__(16) float sh[];
@@ -44,8 +45,6 @@ __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, lo
   hb_pdl_wait();
   hb_pdl_launch();
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = Hq / Hkv;
-  const SharedItem* items = (const SharedItem*)(plan + plan[SP_OFF_ITEMS]);
-  const int* ctas = plan + plan[SP_OFF_CTAS];
   for (int it = ctas[blockIdx.x]; it < ctas[blockIdx.x + 1]; it++) {
     const SharedItem e = items[it];
     const int rows = e.tokens * G;
@@ -199,15 +198,15 @@ constexpr int SJ_WARPS = 4;
 // A warp per row of q and head; a lane has E columns.
 template <typename T, int E>
 __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
-                                                                    const int* plan, const float* part_o, const float2* part_ml, T* out, int Hq,
+                                                                    const SharedToken* tokens, int T_rows, const float* part_o, const float2* part_ml, T* out, int Hq,
                                                                     int Hkv, int D, int page_size, float scale_log2, int vec) {
   hb_pdl_wait();
   hb_pdl_launch();
   const int lane = threadIdx.x & 31, c = lane * E, G = Hq / Hkv;
-  const int u = blockIdx.x * SJ_WARPS + (threadIdx.x >> 5), T_rows = plan[SP_TOKENS];
+  const int u = blockIdx.x * SJ_WARPS + (threadIdx.x >> 5);
   if (u >= T_rows * Hq) return;
   const int t = u / Hq, head = u % Hq, h = head / G, g = head % G;
-  const SharedToken e = ((const SharedToken*)(plan + plan[SP_OFF_TOKENS]))[t];
+  const SharedToken e = tokens[t];
   float m = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; i++) acc[i] = 0.f;
@@ -297,8 +296,8 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
 }
 
 template <typename T, int RM, int NC>
-int launch_items(const void* q, long ldq, const void* kc, const void* vc, const int* bt, int bt_stride, const int* plan, int ctas, int max_rows,
-                 int narrow, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
+int launch_items(const void* q, long ldq, const void* kc, const void* vc, const int* bt, int bt_stride, const SharedItem* items, const int* cta_items,
+                 int ctas, int max_rows, int narrow, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
   constexpr int smem = items_smem<RM, NC>();
   auto kern = shared_items_kernel<T, RM, NC>;
   static bool configured = false;
@@ -309,7 +308,7 @@ int launch_items(const void* q, long ldq, const void* kc, const void* vc, const 
   }
   const int blocks = (max_rows + 16 * RM - 1) / (16 * RM);
   const cudaError_t e = hb_launch(kern, dim3(ctas, blocks < 65535 ? blocks : 65535), SI_THREADS, smem, s, (const T*)q, ldq, (const T*)kc, (const T*)vc, bt,
-                                  bt_stride, plan, narrow, part_o, part_ml, Hq, Hkv, D, page_size, scale_log2, vec);
+                                  bt_stride, items, cta_items, narrow, part_o, part_ml, Hq, Hkv, D, page_size, scale_log2, vec);
   if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
   return 0;
 }
@@ -317,7 +316,7 @@ int launch_items(const void* q, long ldq, const void* kc, const void* vc, const 
 }  // namespace
 
 // What a call has of its plan, in host memory: the numbers that the launches want.
-struct SharedLaunch { int T, ctas, max_rows, narrow, parts, tensor_cores, dt, Hq, Hkv, D, page_size; };
+struct SharedLaunch { int T, ctas, max_rows, narrow, parts, tensor_cores, dt, Hq, Hkv, D, page_size, off_items, off_ctas, off_tokens; };
 
 // q [T, ldq] (heads of D side by side), caches [num_pages, Hkv, page_size, D], bt [R, bt_stride], plan on the device (see shared_plan.cu) and `h` of it;
 // workspace parts * (D + 2) + 4 floats, 16-byte aligned; out [T, Hq, D]. aligned: rows of q, pages and out start on 16 bytes. `status` is set to 1 if
@@ -333,14 +332,17 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   if (h->parts > 0 && (!workspace || ((uintptr_t)workspace & 15))) HB_FAIL("hb_attention_shared: the workspace must be 16-byte aligned");
   float* part_o = workspace;
   float2* part_ml = (float2*)(workspace + ((long)h->parts * D + 3) / 4 * 4);
+  const SharedItem* items = (const SharedItem*)(plan + h->off_items);
+  const int* cta_items = plan + h->off_ctas;
+  const SharedToken* tokens = (const SharedToken*)(plan + h->off_tokens);
   const int vec = aligned && D % 4 == 0;
   const float sl2 = scale * 1.4426950408889634f;
   if (h->ctas > 0 && h->tensor_cores && aligned) {
-    if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, plan, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
+    if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, items, cta_items, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
   } else if (h->ctas > 0) {
     int r = -1;
 #define SI_LAUNCH(RM, NC) \
-  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, plan, h->ctas, h->max_rows, h->narrow, part_o, part_ml, Hq, Hkv, D, ps, sl2, vec, s)
+  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, items, cta_items, h->ctas, h->max_rows, h->narrow, part_o, part_ml, Hq, Hkv, D, ps, sl2, vec, s)
     HB_DISPATCH_1(h->dt, "hb_attention_shared", {
       if (h->max_rows <= 16) {
         if (D <= 64) SI_LAUNCH(1, 1); else if (D <= 128) SI_LAUNCH(1, 2); else SI_LAUNCH(1, 4);
@@ -354,7 +356,7 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   cudaError_t e = cudaSuccess;
 #define SJ_LAUNCH(E)                                                                                                                     \
   e = hb_launch(shared_join_kernel<TA, E>, dim3((unsigned)((warps + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq,   \
-                (const TA*)kc, (const TA*)vc, bt, bt_stride, plan, part_o, part_ml, (TA*)out, Hq, Hkv, D, ps, sl2, vec)
+                (const TA*)kc, (const TA*)vc, bt, bt_stride, tokens, T, part_o, part_ml, (TA*)out, Hq, Hkv, D, ps, sl2, vec)
   HB_DISPATCH_1(h->dt, "hb_attention_shared", { if (D <= 64) SJ_LAUNCH(2); else if (D <= 128) SJ_LAUNCH(4); else SJ_LAUNCH(8); });
 #undef SJ_LAUNCH
   if (e != cudaSuccess) HB_FAIL("hb_attention_shared: %s", cudaGetErrorString(e));

@@ -1,19 +1,20 @@
 // The items of the shared-prefix attention (shared_plan.cu, attention_shared.cu) on the 5th-generation tensor cores: bfloat16, heads of 64 or 128.
 //
 // Persistent CTAs, one an SM, walk the items that the plan gives them. An item is up to 2 x 128 query rows (consecutive tokens times the heads
-// of a kv head) against a range of keys, in tiles of 128 absolute positions. Two CHAINS, a softmax warpgroup, a score tile, an accumulator
-// and running maxima and sums each, work in turn: where an item has more rows than 128 a chain has half of them and every key tile, and
-// a tile of K and V that was loaded once serves both; where it has fewer, both chains have the same rows and take the key tiles in turn, and
-// leave a part of the result each. Either way the exponentials of one chain run beside the products of the other.
-//   softmax warps   a thread owns a query row: reads its row of S from tensor memory, masks it where the tile reaches over the item's
-//                   range or the row's position, exponentiates in 32 bits, and writes P as bfloat16 over S in tensor memory, from where the second
-//                   product reads it as its A operand (shared memory then feeds K and V alone);
-//   K and V loaders TMA, a page and 64 columns a box, a lane holds a page's number; Q comes with K, one box of (64 columns, heads, tokens);
-//   two MMA warps   S = Q K^T of the next units, and O += P V of those whose P is written.
-// A score tile and its P are the same tensor memory: the next scores wait until the product behind them is done, so when they arrive the
-// accumulator is complete and may be rescaled (only when a row's maximum grew by more than 2^8: any reference value gives the same quotient).
+// of a kv head) against a range of keys, in tiles of 128 absolute positions. Two CHAINS, a softmax warpgroup, an MMA warp, score tiles, an
+// accumulator and running maxima and sums each, work beside each other in STEPS of 128 rows by 64 keys: where an item has more rows than 128 a
+// chain has half of them and takes a tile in two steps, and the tile of K and V that was loaded once serves both; where it has fewer, both
+// chains have the same rows, each a half of every tile's keys, and each leaves a part of the result.
+//   softmax warps   a thread owns a query row: reads a step's scores from tensor memory, masks them where the tile reaches over the item's range or the
+//                   row's position, exponentiates in 32 bits, and writes P as bfloat16 over the scores, from where the second product reads
+//                   it as its A operand (shared memory then feeds Q, K and V alone);
+//   an MMA warp a chain   O += P V of a step as soon as its P is written, and right behind it S = Q K^T of the step after the next into the
+//                   same tensor memory (the tensor core works in the order of issue), which is done while the softmax warps are at the next step;
+//   K and V loaders TMA, a page and 64 columns a box, a lane holds a page's number; Q comes with K, one box of (64 columns, heads, tokens).
+// The accumulator is rescaled only when a row's maximum grew by more than 2^8 (any reference value gives the same quotient).
 // V rows outside of the item's range, which may hold anything, are set to zero in shared memory by the softmax threads that mask them: P
-// is 0 there, and 0 times an infinity is no 0. Every wait is bounded.
+// is 0 there, and 0 times an infinity is no 0. Every wait is bounded; both chains wait for and release every tile and every Q, so that a
+// barrier is never more than a phase ahead of one that waits for it.
 #include "shared_plan.h"
 #include "tc_common.cuh"
 
@@ -25,13 +26,14 @@ constexpr float ST_SLACK = 8.f;
 template <int D> struct StSizes {
   static constexpr int TILE = 128 * 64 * 2;                 // [128][64] bfloat16; an operand of D columns is D / 64 of them
   static constexpr int OPND = D / 64 * TILE;
-  static constexpr int NK = D == 128 ? 2 : 5, NV = D == 128 ? 3 : 6;
+  static constexpr int NK = D == 128 ? 2 : 4, NV = D == 128 ? 3 : 8;
 };
 template <int D> struct StBars {
   uint64_t q_full[2], q_free[2], k_full[StSizes<D>::NK], k_free[StSizes<D>::NK], v_full[StSizes<D>::NV], v_free[StSizes<D>::NV];
-  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];      // [chain][step & 1]
   uint32_t tmem_slot;
   int abort_flag;
+  alignas(16) SharedItem kept[64];
 };
 template <int D> constexpr int st_smem() { return (2 + StSizes<D>::NK + StSizes<D>::NV) * StSizes<D>::OPND + (int)sizeof(StBars<D>); }
 static_assert(st_smem<128>() <= 227 * 1024 && st_smem<64>() <= 227 * 1024, "shared memory of a block");
@@ -83,28 +85,53 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uin
       : "memory");
 }
 
+// Whether a phase is over, without waiting; and a wait, of which only the first look stands in line (a loop at every place it is used made the
+// kernel 60 KB of code, and every role's instructions came late).
+__device__ __forceinline__ bool is_over(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(hb_smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, volatile int* abort) { return hb_mbar_wait(bar, parity, abort); }
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return hb_mbar_try_wait(bar, parity) || wait_longer(bar, parity, abort);
+}
+
+// The CTA's items: the first ST_KEPT of them are in shared memory.
+constexpr int ST_KEPT = 64;
+struct Items {
+  const SharedItem *kept, *all;
+  int n, tokens_a_chain;
+};
 struct Work {      // an item as the roles go through it
   SharedItem e;
   int kt0, tiles;  // its key tiles
-  bool wide;       // a chain has half of the rows (else half of the tiles)
-  __device__ __forceinline__ int units() const { return wide ? 2 * tiles : tiles; }
+  bool wide;       // a chain has half of the rows (else half of a tile's keys)
 };
-__device__ __forceinline__ Work work_of(const SharedItem* items, int it, int last, int tokens_a_chain) {
+__device__ __forceinline__ Work work_of(const Items& items, int it) {
   Work w;
-  const int4* src = (const int4*)(items + (it < last ? it : last - 1));
+  const int4* src = (const int4*)(it < ST_KEPT ? items.kept + it : items.all + it);
   *(int4*)&w.e = src[0];
   *((int4*)&w.e + 1) = src[1];
   w.kt0 = w.e.lo / ST_KEYS;
   w.tiles = (w.e.hi - 1) / ST_KEYS - w.kt0 + 1;
-  w.wide = w.e.tokens > tokens_a_chain;
+  w.wide = w.e.tokens > items.tokens_a_chain;
   return w;
 }
 
 template <int D>
 __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const int* bt, int bt_stride,
-                                                                        const int* plan, float* part_o, float2* part_ml, int Hkv, int G, int page_size,
-                                                                        float scale_log2, int* status) {
+                                                                        const SharedItem* plan_items, const int* ctas, float* part_o, float2* part_ml,
+                                                                        int Hkv, int G, int page_size, float scale_log2, int* status) {
   using S = StSizes<D>;
   constexpr int NH = D / 64, TILE = S::TILE, OPND = S::OPND, NK = S::NK, NV = S::NV;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -119,12 +146,13 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
     return;
   }
   if (threadIdx.x == 0) {
+    // (what is loaded has to be let go by both chains)
     for (int b = 0; b < 2; b++) {
-      hb_mbar_init(&bar->q_full[b], 1); hb_mbar_init(&bar->q_free[b], 1);
-      hb_mbar_init(&bar->s_full[b], 1); hb_mbar_init(&bar->p_full[b], 4); hb_mbar_init(&bar->pv_done[b], 1);
+      hb_mbar_init(&bar->q_full[b], 1); hb_mbar_init(&bar->q_free[b], 2);
+      for (int h = 0; h < 2; h++) { hb_mbar_init(&bar->s_full[b][h], 1); hb_mbar_init(&bar->p_full[b][h], 4); hb_mbar_init(&bar->pv_done[b][h], 1); }
     }
-    for (int b = 0; b < NK; b++) { hb_mbar_init(&bar->k_full[b], 1); hb_mbar_init(&bar->k_free[b], 1); }
-    for (int b = 0; b < NV; b++) { hb_mbar_init(&bar->v_full[b], 1); hb_mbar_init(&bar->v_free[b], 1); }
+    for (int b = 0; b < NK; b++) { hb_mbar_init(&bar->k_full[b], 1); hb_mbar_init(&bar->k_free[b], 2); }
+    for (int b = 0; b < NV; b++) { hb_mbar_init(&bar->v_full[b], 1); hb_mbar_init(&bar->v_free[b], 2); }
     bar->abort_flag = 0;
     hb_fence_barrier_init();
   }
@@ -133,22 +161,20 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
     hb_tmem_alloc(&bar->tmem_slot, 512);
     hb_tmem_relinquish();
   }
+  // (the plan and the block tables are copied before the step's first kernel begins: they may be read ahead of the wait)
+  const int it0 = ctas[blockIdx.x], RT = ST_ROWS / G;
+  Items items = {bar->kept, plan_items + it0, ctas[blockIdx.x + 1] - it0, RT};
+  for (int i = threadIdx.x; i < 2 * min(items.n, ST_KEPT); i += ST_THREADS) ((int4*)bar->kept)[i] = ((const int4*)items.all)[i];
   hb_tc_fence_before();
   __syncthreads();
   hb_tc_fence_after();
   const uint32_t tmem = bar->tmem_slot;   // S and P of chain c at c * 128, its O at 256 + c * 128
   hb_pdl_wait();
   hb_pdl_launch();
-  const SharedItem* items = (const SharedItem*)(plan + plan[SP_OFF_ITEMS]);
-  const int* ctas = plan + plan[SP_OFF_CTAS];
-  const int it0 = ctas[blockIdx.x], it1 = ctas[blockIdx.x + 1], RT = ST_ROWS / G;
 
-  // Units (a chain's work on a key tile) are numbered through all items, chain = unit & 1; wide: units 2 i and 2 i + 1 are tile i, else unit i is.
-  // The next item begins with chain 0 again, so a chain counts its own units.
-  // Q buffers: a wide item has both, a narrow one the one that the item before did not have.
-  // Registers: 3 x 128 threads were launched with 168; a softmax thread holds a row of scores and takes 208, the other warps keep 88 (2 x 208 + 88 = 3 x 168).
+  // Key tiles are numbered through all items of the CTA, a chain's steps too. Q buffers: a wide item has both, a narrow one the one that the narrow item
+  // before did not have.
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < 10) {  // ---------------- TMA
     const bool is_k = warp == 8;
     const CUtensorMap* map = is_k ? &map_k : &map_v;
@@ -156,19 +182,22 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
     uint8_t* ring = is_k ? sK : sV;
     const uint32_t stages = is_k ? NK : NV;
     const int places = ST_KEYS / page_size;
-    uint32_t stage = 0, use = 0, q_use[2] = {0, 0}, qb = 0;
+    uint32_t stage = 0, parity = 1, q_parity = 3, qb = 0;
     bool ok = true;
-    Work ahead = work_of(items, it0, it1, RT);
-    for (int it = it0; it < it1 && ok; it++) {
-      const Work w = ahead;
-      ahead = work_of(items, it + 1, it1, RT);
-      const int* table = bt + (size_t)w.e.table * bt_stride;
-      if (is_k) {
-        for (int c = 0; c < (w.wide ? 2 : 1) && ok; c++) {
+    auto wait = [&](uint64_t* b, uint32_t p) { return ok = __all_sync(0xffffffffu, wait_for(b, p, abort_flag)); };
+    // the page of this lane's place in tile t, asked for a tile ahead
+    auto page = [&](const Work& w, int t) {
+      const int pg = (w.kt0 + t) * places + lane;
+      return lane < places && pg * page_size < w.e.hi && (pg + 1) * page_size > w.e.lo ? bt[(size_t)w.e.table * bt_stride + pg] : -1;
+    };
+    Work w = work_of(items, 0);
+    int ahead = page(w, 0);
+    for (int it = 0, t = 0; it < items.n && ok;) {
+      if (is_k && t == 0) {
+        for (int c = 0; c < (w.wide ? 2 : 1); c++) {
           const uint32_t b = w.wide ? (uint32_t)c : qb;
-          ok = __all_sync(0xffffffffu, hb_mbar_wait(&bar->q_free[b], (q_use[b] & 1) ^ 1, abort_flag));
-          if (!ok) break;
-          q_use[b]++;
+          if (!wait(&bar->q_free[b], q_parity >> b & 1)) break;
+          q_parity ^= 1u << b;
           if (hb_elect()) {
             hb_mbar_expect_tx(&bar->q_full[b], (uint32_t)(RT * G * D * 2));
 #pragma unroll
@@ -177,211 +206,222 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
           }
           __syncwarp();
         }
-        if (!w.wide) qb ^= 1;
-      }
-      auto page = [&](int t) {
-        const int pg = (w.kt0 + t) * places + lane;
-        return lane < places && pg * page_size < w.e.hi && (pg + 1) * page_size > w.e.lo ? table[pg] : -1;
-      };
-      int next = page(0);
-      for (int t = 0; t < w.tiles && ok; t++) {
-        const uint32_t boxes = __ballot_sync(0xffffffffu, next >= 0);
-        const int row = (next * Hkv + w.e.head) * page_size;
-        next = t + 1 < w.tiles ? page(t + 1) : -1;
-        ok = __all_sync(0xffffffffu, hb_mbar_wait(&free[stage], (use & 1) ^ 1, abort_flag));
         if (!ok) break;
-        if (hb_elect()) hb_mbar_expect_tx(&full[stage], (uint32_t)__popc(boxes) * page_size * D * 2);
-        __syncwarp();
-        for (int p = 0; p < places; p += 4) {       // four boxes an election
-          int from[4];
-#pragma unroll
-          for (int j = 0; j < 4; j++) from[j] = __shfl_sync(0xffffffffu, row, (p + j) & 31);
-          if (hb_elect()) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              if (p + j < places && (boxes >> (p + j) & 1)) {
-                uint8_t* dst = ring + stage * OPND + (p + j) * page_size * 128;            // rows of 128 bytes in each 64-column tile
-#pragma unroll
-                for (int hf = 0; hf < NH; hf++) hb_tma_load_2d(dst + hf * TILE, map, &full[stage], hf * 64, from[j]);
-              }
-          }
-          __syncwarp();
-        }
-        if (++stage == stages) { stage = 0; use++; }
-      }
-    }
-  } else if (warp == 10) {  // ---------------- tensor cores: S = Q K^T
-    if (hb_elect()) {
-      constexpr uint32_t idesc = hb_umma_idesc_bf16(ST_ROWS, ST_KEYS);
-      uint32_t stage = 0, use = 0, q_use[2] = {0, 0}, qb = 0, n[2] = {0, 0};
-      bool ok = true;
-      Work ahead = work_of(items, it0, it1, RT);
-      for (int it = it0; it < it1 && ok; it++) {
-        const Work w = ahead;
-        ahead = work_of(items, it + 1, it1, RT);
-        const int units = w.units();
-        for (int u = 0; u < units && ok; u++) {
-          const uint32_t c = u & 1, b = w.wide ? c : qb;
-          if (u == 0 || (w.wide && u == 1)) {
-            ok = hb_mbar_wait(&bar->q_full[b], q_use[b] & 1, abort_flag);
-            q_use[b]++;
-          }
-          // the product behind the chain's unit before has read its P
-          ok = ok && hb_mbar_wait(&bar->k_full[stage], use & 1, abort_flag) && (n[c] == 0 || hb_mbar_wait(&bar->pv_done[c], (n[c] - 1) & 1, abort_flag));
-          if (!ok) break;
-          hb_tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < D / 16; kk++) {   // 16 columns a step: four steps in each 64-column tile
-            const uint64_t dq = hb_umma_desc_k128(hb_smem_u32(sQ + b * OPND + (kk >> 2) * TILE)) + 2 * (kk & 3);
-            const uint64_t dk = hb_umma_desc_k128(hb_smem_u32(sK + stage * OPND + (kk >> 2) * TILE)) + 2 * (kk & 3);
-            hb_umma_bf16(tmem + c * 128, dq, dk, idesc, kk != 0);
-          }
-          hb_umma_commit(&bar->s_full[c]);
-          n[c]++;
-          if (!w.wide || c == 1) {
-            hb_umma_commit(&bar->k_free[stage]);
-            if (++stage == NK) { stage = 0; use++; }
-          }
-          if (u == units - 1 || (w.wide && u == units - 2)) hb_umma_commit(&bar->q_free[b]);
-        }
         if (!w.wide) qb ^= 1;
       }
-    }
-  } else {  // ---------------- tensor cores: O += P V
-    if (hb_elect()) {
-      constexpr uint32_t idesc = hb_umma_idesc_bf16(ST_ROWS, D) | (1u << 16);      // B is MN-major
-      uint32_t stage = 0, use = 0, n[2] = {0, 0};
-      bool ok = true;
-      Work ahead = work_of(items, it0, it1, RT);
-      for (int it = it0; it < it1 && ok; it++) {
-        const Work w = ahead;
-        ahead = work_of(items, it + 1, it1, RT);
-        const int units = w.units();
-        for (int u = 0; u < units && ok; u++) {
-          const uint32_t c = u & 1;
-          ok = hb_mbar_wait(&bar->v_full[stage], use & 1, abort_flag) && hb_mbar_wait(&bar->p_full[c], n[c] & 1, abort_flag);
-          if (!ok) break;
-          hb_tc_fence_after();
+      const uint32_t boxes = __ballot_sync(0xffffffffu, ahead >= 0);
+      const int row = (ahead * Hkv + w.e.head) * page_size;
+      if (++t == w.tiles) {
+        t = 0;
+        if (++it < items.n) w = work_of(items, it);
+      }
+      if (it < items.n) ahead = page(w, t);
+      if (!wait(&free[stage], parity)) break;
+      if (hb_elect()) hb_mbar_expect_tx(&full[stage], (uint32_t)__popc(boxes) * page_size * D * 2);
+      __syncwarp();
+      for (int p = 0; p < places; p += 4) {       // four boxes an election
+        int from[4];
 #pragma unroll
-          for (int kk = 0; kk < ST_KEYS / 16; kk++)          // 16 keys: eight columns of P, 16 rows of V
-            umma_ts(tmem + 256 + c * 128, tmem + c * 128 + 8 * kk, desc_mn128(hb_smem_u32(sV + stage * OPND + kk * 16 * 128), TILE), idesc, u > 1 || kk != 0);
-          hb_umma_commit(&bar->pv_done[c]);
-          n[c]++;
-          if (!w.wide || c == 1) {
-            hb_umma_commit(&bar->v_free[stage]);
-            if (++stage == NV) { stage = 0; use++; }
+        for (int j = 0; j < 4; j++) from[j] = __shfl_sync(0xffffffffu, row, (p + j) & 31);
+        if (hb_elect()) {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (p + j < places && (boxes >> (p + j) & 1)) {
+              uint8_t* dst = ring + stage * OPND + (p + j) * page_size * 128;            // rows of 128 bytes in each 64-column tile
+#pragma unroll
+              for (int hf = 0; hf < NH; hf++) hb_tma_load_2d(dst + hf * TILE, map, &full[stage], hf * 64, from[j]);
+            }
+        }
+        __syncwarp();
+      }
+      if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
+  } else {  // ---------------- tensor cores: warp 10 + c issues the products of chain c
+    if (hb_elect()) {
+      const uint32_t c = warp - 10, tmem_s = tmem + c * 128, tmem_o = tmem + 256 + c * 128;
+      constexpr uint32_t idesc_s = hb_umma_idesc_bf16(ST_ROWS, 64), idesc_o = hb_umma_idesc_bf16(ST_ROWS, D) | (1u << 16);      // (V is MN-major)
+      const uint64_t q_desc = hb_umma_desc_k128(hb_smem_u32(sQ)), k_desc = hb_umma_desc_k128(hb_smem_u32(sK)), v_desc = desc_mn128(hb_smem_u32(sV), TILE);
+      // Where the scores are, and where the products: an item's tiles and kind, the tile in it and its half, the tile's stage and the parity of
+      // the stage's use.
+      struct At {
+        int it, tile, tiles;
+        uint32_t wide, half, stage, parity;
+      };
+      auto item = [&](At& a) {
+        const Work w = work_of(items, a.it);
+        a.tile = 0;
+        a.tiles = w.tiles;
+        a.wide = w.wide;
+        a.half = w.wide ? 0 : c;
+      };
+      auto next = [&](At& a, uint32_t stages) {
+        if (a.wide && a.half == 0) {
+          a.half = 1;
+          return;
+        }
+        if (++a.stage == stages) { a.stage = 0; a.parity ^= 1; }
+        a.half = a.wide ? 0 : c;
+        if (++a.tile == a.tiles && ++a.it < items.n) item(a);
+      };
+      At s = {0, 0, 0, 0, 0, 0, 0}, o;
+      item(s);
+      o = s;
+      uint32_t q_parity = 0, qb = 0;               // of the two Q buffers as bits; the narrow items' buffer
+      uint32_t ms = 0, mo = 0, polls = 0;          // steps whose scores, and whose products, were issued: at most two of the former ahead
+      while (o.it < items.n) {
+        polls++;
+        const bool first = !s.wide || s.half == 0;           // the step is its tile's first of this chain
+        const uint32_t b = s.wide ? c : qb;
+        if (s.it < items.n && ms < mo + 2 &&
+            (!first || (is_over(&bar->k_full[s.stage], s.parity) &&
+                        (s.tile > 0 || (is_over(&bar->q_full[b], q_parity >> b & 1) && (!s.wide || is_over(&bar->q_full[b ^ 1], q_parity >> (b ^ 1) & 1))))))) {
+          if (s.tile == 0 && first) q_parity ^= s.wide ? 3u : 1u << b;
+          hb_tc_fence_after();
+          const uint64_t dq = q_desc + b * (OPND >> 4), dk = k_desc + s.stage * (OPND >> 4) + s.half * (64 * 128 >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk++)     // 16 columns a step: four steps in each 64-column tile
+            hb_umma_bf16(tmem_s + (ms & 1) * 64, dq + (kk >> 2) * (TILE >> 4) + 2 * (kk & 3), dk + (kk >> 2) * (TILE >> 4) + 2 * (kk & 3), idesc_s, kk != 0);
+          hb_umma_commit(&bar->s_full[c][ms & 1]);
+          if (!s.wide || s.half) {
+            hb_umma_commit(&bar->k_free[s.stage]);
+            if (s.tile == s.tiles - 1) {
+              hb_umma_commit(&bar->q_free[b]);
+              if (s.wide) hb_umma_commit(&bar->q_free[b ^ 1]);
+              else qb ^= 1;
+            }
           }
+          next(s, NK);
+          ms++;
+          polls = 0;
+        }
+        if (mo < ms && is_over(&bar->p_full[c][mo & 1], mo >> 1 & 1) && is_over(&bar->v_full[o.stage], o.parity)) {
+          hb_tc_fence_after();
+          const uint32_t fresh = o.tile == 0 && (!o.wide || o.half == 0);           // the accumulator's first step
+          const uint64_t dv = v_desc + o.stage * (OPND >> 4) + o.half * (64 * 128 >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)          // 16 keys: eight columns of P, 16 rows of V
+            umma_ts(tmem_o, tmem_s + (mo & 1) * 64 + 8 * kk, dv + kk * (16 * 128 >> 4), idesc_o, kk != 0 || !fresh);
+          hb_umma_commit(&bar->pv_done[c][mo & 1]);
+          if (!o.wide || o.half) hb_umma_commit(&bar->v_free[o.stage]);
+          next(o, NV);
+          mo++;
+          polls = 0;
+        }
+        if ((polls & 63) == 63 && *abort_flag) break;
+        if (polls > 16 * HB_WAIT_LIMIT) {          // (these looks do not suspend)
+          *abort_flag = 1;
+          break;
         }
       }
     }
   }
   } else {  // ---------------- softmax: warpgroup c is chain c, a thread a query row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int c = warp >> 2, w4 = warp & 3, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(w4 * 32) << 16, tmem_s = tmem + c * 128 + lanes, tmem_o = tmem + 256 + c * 128 + lanes;
-    uint32_t n = 0, vt0 = 0;       // the chain's units, and the V tiles of the items before
+    uint32_t m = 0, v_stage = 0, v_parity = 0;       // steps; where V is
     bool ok = true;                // every wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide
-    auto wait = [&](uint64_t* b, uint32_t parity) { ok = __all_sync(0xffffffffu, hb_mbar_wait(b, parity, abort_flag)); return ok; };
+    auto wait = [&](uint64_t* b, uint32_t parity) { return ok = __all_sync(0xffffffffu, wait_for(b, parity, abort_flag)); };
     const uint64_t scale2 = pack2(scale_log2, scale_log2);
-    Work ahead = work_of(items, it0, it1, RT);
-    for (int it = it0; it < it1 && ok; it++) {
-      const Work w = ahead;
-      ahead = work_of(items, it + 1, it1, RT);
+    const int token = r / G;       // the row's, counted from the chain's first
+    for (int it = 0; it < items.n && ok; it++) {
+      const Work w = work_of(items, it);
       const int first = w.wide ? c * RT : 0, rows = min(RT, w.e.tokens - first) * G;           // the chain's rows
       const bool idle = w4 * 32 >= rows;
-      const int last_key = min(w.e.hi - 1, w.e.pos == SP_NO_MASK ? SP_NO_MASK : w.e.pos + first + r / G);
+      const int last_key = min(w.e.hi - 1, w.e.pos == SP_NO_MASK ? SP_NO_MASK : w.e.pos + first + token);
       const int sure = w.e.pos == SP_NO_MASK ? w.e.hi : min(w.e.hi, w.e.pos + first + 1);      // the keys below are seen by all rows
       float m_run = -INFINITY, l_run = 0.f;
-      int units = 0;
-      for (int i = w.wide ? 0 : c; i < w.tiles; i += w.wide ? 1 : 2, units++, n++) {
-        const int k_base = (w.kt0 + i) * ST_KEYS;
-        if (!wait(&bar->s_full[c], n & 1)) break;
-        hb_tc_fence_after();
-        if (!idle) {
-          uint32_t sr[128];
+      const uint32_t m0 = m;
+      for (int i = 0; i < w.tiles && ok; i++) {
+        const int tile = (w.kt0 + i) * ST_KEYS;
+        for (int h = w.wide ? 0 : c; h < (w.wide ? 2 : c + 1); h++, m++) {
+          const int k_base = tile + 64 * h;
+          const uint32_t sp = tmem_s + (m & 1) * 64;           // S and P of the step
+          if (!wait(&bar->s_full[c][m & 1], m >> 1 & 1)) break;
+          hb_tc_fence_after();
+          const bool cut = k_base < w.e.lo || k_base + 64 > w.e.hi;
+          if (cut) {      // the rows of V, of the step's keys, where the item does not reach: a thread has half of one
+            const int row = 64 * h + (r >> 1);
+            if (!wait(&bar->v_full[v_stage], v_parity)) break;
+            if (tile + row < w.e.lo || tile + row >= w.e.hi) {
+              const uint32_t dst = hb_smem_u32(sV + v_stage * OPND) + row * 128 + (r & 1) * (D == 128 ? TILE : 64);
 #pragma unroll
-          for (int q = 0; q < 128; q += 32) ld32(tmem_s + q, sr + q);
-          hb_tmem_ld_wait();
-#pragma unroll
-          for (int q = 0; q < 128; q += 32) ld32_fence(sr + q);
-          if (k_base < w.e.lo || k_base + ST_KEYS > sure) {
-            const int lo_j = w.e.lo - k_base, hi_j = last_key - k_base;
-#pragma unroll
-            for (int j = 0; j < 128; j++)
-              if (j < lo_j || j > hi_j) sr[j] = __float_as_uint(-INFINITY);
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], __uint_as_float(sr[j])), __uint_as_float(sr[j + 1]));
-          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
-          const bool grow = m_tile > m_run + ST_SLACK;   // also the first tile with a visible key: m_run is -inf
-          float corr = 1.f;
-          if (grow) {
-            corr = hb_exp2(m_run - m_tile);              // 0 while nothing has been summed
-            m_run = m_tile;
-          }
-          const float sub = m_run == -INFINITY ? 0.f : m_run;
-          const uint64_t sub2 = pack2(-sub, -sub);
-          uint64_t sum2[2] = {0ull, 0ull};
-#pragma unroll
-          for (int j = 0; j < 128; j += 4) {             // masked scores are -inf: 2^-inf = 0
-            float p0, p1, p2, p3;
-            unpack2(fma2(pack2(__uint_as_float(sr[j]), __uint_as_float(sr[j + 1])), scale2, sub2), p0, p1);
-            unpack2(fma2(pack2(__uint_as_float(sr[j + 2]), __uint_as_float(sr[j + 3])), scale2, sub2), p2, p3);
-            p0 = hb_exp2(p0); p1 = hb_exp2(p1); p2 = hb_exp2(p2); p3 = hb_exp2(p3);
-            sum2[0] = add2(sum2[0], pack2(p0, p1));
-            sum2[1] = add2(sum2[1], pack2(p2, p3));
-            // P is rounded to bfloat16, the operand's type; the sum is of the unrounded numbers
-            sr[j >> 1] = hb_pack_bf16(p0, p1);
-            sr[(j >> 1) + 1] = hb_pack_bf16(p2, p3);
-          }
-          st32(tmem_s, sr);
-          st32(tmem_s + 32, sr + 32);
-          float s0, s1, s2, s3;
-          unpack2(sum2[0], s0, s1);
-          unpack2(sum2[1], s2, s3);
-          l_run = l_run * corr + ((s0 + s1) + (s2 + s3));
-          if (units > 0 && __any_sync(0xffffffffu, grow)) {   // the rows of O so far: the product before was done when these scores were begun
-#pragma unroll
-            for (int q = 0; q < D / 32; q++) {
-              uint32_t o[32];
-              ld32(tmem_o + q * 32, o);
-              hb_tmem_ld_wait();
-              ld32_fence(o);
-#pragma unroll
-              for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr);
-              st32(tmem_o + q * 32, o);
+              for (int q = 0; q < D / 16; q++)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + q * 16), "r"(0) : "memory");
             }
+            hb_fence_proxy_async();
           }
-          hb_tmem_st_wait();
-        }
-        if (k_base < w.e.lo || k_base + ST_KEYS > w.e.hi) {      // thread r clears row r of V where the item does not reach
-          const uint32_t vt = vt0 + i, stage = vt % NV;
-          if (!wait(&bar->v_full[stage], (vt / NV) & 1)) break;
-          if (k_base + r < w.e.lo || k_base + r >= w.e.hi) {
-            const uint32_t dst = hb_smem_u32(sV + stage * OPND) + r * 128;
+          if (!idle) {
+            uint32_t x[64];
 #pragma unroll
-            for (int hf = 0; hf < NH; hf++)
+            for (int q = 0; q < 64; q += 32) ld32(sp + q, x + q);
+            hb_tmem_ld_wait();
 #pragma unroll
-              for (int q = 0; q < 8; q++)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * TILE + q * 16), "r"(0) : "memory");
+            for (int q = 0; q < 64; q += 32) ld32_fence(x + q);
+            if (cut || k_base + 64 > sure) {
+              const int lo_j = w.e.lo - k_base, hi_j = last_key - k_base;
+#pragma unroll
+              for (int j = 0; j < 64; j++)
+                if (j < lo_j || j > hi_j) x[j] = __float_as_uint(-INFINITY);
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
+            const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+            const bool grow = m_step > m_run + ST_SLACK;   // also the first step with a visible key: m_run is -inf
+            if (__any_sync(0xffffffffu, grow)) {
+              const float m_new = grow ? m_step : m_run, corr = grow ? hb_exp2(m_run - m_new) : 1.f;      // 0 while nothing has been summed
+              m_run = m_new;
+              l_run *= corr;
+              if (m > m0) {       // the rows of O so far
+                if (!wait(&bar->pv_done[c][(m - 1) & 1], (m - 1) >> 1 & 1)) break;
+                hb_tc_fence_after();
+#pragma unroll
+                for (int q = 0; q < D / 32; q++) {
+                  uint32_t o[32];
+                  ld32(tmem_o + q * 32, o);
+                  hb_tmem_ld_wait();
+                  ld32_fence(o);
+#pragma unroll
+                  for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr);
+                  st32(tmem_o + q * 32, o);
+                }
+              }
+            }
+            const float sub = m_run == -INFINITY ? 0.f : m_run;
+            const uint64_t sub2 = pack2(-sub, -sub);
+            uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {              // masked scores are -inf: 2^-inf = 0
+              float p0, p1, p2, p3;
+              unpack2(fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, sub2), p0, p1);
+              unpack2(fma2(pack2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), scale2, sub2), p2, p3);
+              p0 = hb_exp2(p0); p1 = hb_exp2(p1); p2 = hb_exp2(p2); p3 = hb_exp2(p3);
+              sum2[0] = add2(sum2[0], pack2(p0, p1));
+              sum2[1] = add2(sum2[1], pack2(p2, p3));
+              // P is rounded to bfloat16, the operand's type; the sum is of the unrounded numbers
+              x[j >> 1] = hb_pack_bf16(p0, p1);
+              x[(j >> 1) + 1] = hb_pack_bf16(p2, p3);
+            }
+            st32(sp, x);
+            hb_tmem_st_wait();
+            float s0, s1, s2, s3;
+            unpack2(sum2[0], s0, s1);
+            unpack2(sum2[1], s2, s3);
+            l_run += (s0 + s1) + (s2 + s3);
           }
-          hb_fence_proxy_async();
+          hb_tc_fence_before();
+          __syncwarp();
+          if (lane == 0) hb_mbar_arrive(&bar->p_full[c][m & 1]);
         }
-        hb_tc_fence_before();
-        __syncwarp();
-        if (lane == 0) hb_mbar_arrive(&bar->p_full[c]);
+        if (++v_stage == NV) { v_stage = 0; v_parity ^= 1; }
       }
-      vt0 += w.tiles;
       if (!ok) break;
       // ---- the item's end: the rows' parts
-      const size_t part = (size_t)w.e.part + (c == 0 ? 0 : w.wide ? RT * G : rows);
-      if (units > 0) {
-        if (!wait(&bar->pv_done[c], (n - 1) & 1)) break;
-        hb_tc_fence_after();
-      }
+      const size_t part = (size_t)w.e.part + (w.wide ? c * RT * G : c * rows);
+      if (!wait(&bar->pv_done[c][(m - 1) & 1], (m - 1) >> 1 & 1)) break;
+      hb_tc_fence_after();
       if (r < rows) part_ml[part + r] = make_float2(m_run, l_run);
-      if (units > 0 && !idle) {
+      if (!idle) {
         float* dst = part_o + (part + r) * D;
 #pragma unroll
         for (int q = 0; q < D / 32; q++) {
@@ -441,8 +481,8 @@ HB_EXPORT int hb_shared_items_tc_supported(int Hq, int Hkv, int D, int page_size
          (page_size & (page_size - 1)) == 0;
 }
 
-int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan, int ctas,
-                       int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s) {
+int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const SharedItem* items,
+                       const int* cta_items, int ctas, int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s) {
   if (!hb_shared_items_tc_supported(Hq, Hkv, D, page_size))
     HB_FAIL("hb_shared_items_tc: %d/%d heads of %d with pages of %d are not supported", Hq, Hkv, D, page_size);
   if (ctas <= 0 || T <= 0) return 0;
@@ -472,8 +512,8 @@ int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, 
       if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));                                               \
       configured = true;                                                                                                           \
     }                                                                                                                              \
-    e = hb_launch(shared_items_tc_kernel<DD>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, plan, part_o,          \
-                  part_ml, Hkv, G, page_size, scale_log2, status);                                        \
+    e = hb_launch(shared_items_tc_kernel<DD>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, items, cta_items,      \
+                  part_o, part_ml, Hkv, G, page_size, scale_log2, status);                                        \
   } while (0)
   if (D == 64) ST_LAUNCH(64);
   else ST_LAUNCH(128);

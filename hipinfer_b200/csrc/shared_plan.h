@@ -23,5 +23,5 @@ constexpr int SP_FRESH = 16;
 
 // The items on the tensor cores (attention_shared_tc.cu): bfloat16, for a plan whose items have up to 2 * (128 / G) tokens, of which those of up to
 // 128 / G leave two parts. scale_log2: the scale times log2(e).
-int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* plan, int ctas,
-                       int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s);
+int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const SharedItem* items,
+                       const int* cta_items, int ctas, int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s);
