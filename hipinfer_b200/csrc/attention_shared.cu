@@ -7,7 +7,7 @@
 // shared_items_kernel leaves (m, l) and o of every item's rows in the workspace; any head size up to 256, page size and group, both element
 // types: 16 or 64 rows a block by 64 keys a tile, products on the FMA pipe, everything widened to 32 bits in shared memory. bfloat16 heads of
 // 64 and 128 go to the tensor cores instead (attention_shared_tc.cu).
-// shared_join_kernel, a warp per row and head, adds the keys of the step's own rows (a row sees those up to itself, so that the items need no mask) and
+// shared_join_kernel, one or four warps per row and head, adds the keys of the step's own rows (a row sees those up to itself, so that the items need no mask) and
 // joins the parts in a fixed order: the same plan and inputs give the same bits.
 #include "common.cuh"
 #include "shared_plan.h"
@@ -193,26 +193,29 @@ template <int E, typename T> __device__ __forceinline__ void load_elements(const
   }
 }
 
-constexpr int SJ_WARPS = 4;
+constexpr int SJ_WARPS = 4, SJ_AHEAD = 8;
 
-// A warp per row of q and head; a lane has E columns.
-template <typename T, int E>
+// W warps per row of q and head (a block has SJ_WARPS); a lane has E columns. The parts go to the warps in turn, the keys of the step's own rows to
+// the last warp; W > 1: the warps' results meet in shared memory, in their order.
+template <typename T, int E, int W>
 __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
-                                                                    const SharedToken* tokens, int T_rows, const float* part_o, const float2* part_ml, T* out, int Hq,
-                                                                    int Hkv, int D, int page_size, float scale_log2, int vec) {
-  hb_pdl_wait();
-  hb_pdl_launch();
-  const int lane = threadIdx.x & 31, c = lane * E, G = Hq / Hkv;
-  const int u = blockIdx.x * SJ_WARPS + (threadIdx.x >> 5);
-  if (u >= T_rows * Hq) return;
-  const int t = u / Hq, head = u % Hq, h = head / G, g = head % G;
-  const SharedToken e = tokens[t];
+                                                                    const SharedToken* tokens, int T_rows, const float* part_o, const float2* part_ml, T* out,
+                                                                    int Hq, int Hkv, int D, int page_size, float scale_log2, int vec) {
+  __shared__ float2 sh_ml[SJ_WARPS];
+  __shared__ float sh_acc[W > 1 ? SJ_WARPS : 1][W > 1 ? 32 * E : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % W, c = lane * E, G = Hq / Hkv;
+  const int u = blockIdx.x * (SJ_WARPS / W) + warp / W;
+  const bool some = u < T_rows * Hq;
+  const int t = some ? u / Hq : 0, head = some ? u % Hq : 0, h = head / G, g = head % G;
+  const SharedToken e = tokens[t];                   // (of the plan, as the block table: in place before the step's first kernel)
   float m = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; i++) acc[i] = 0.f;
+  hb_pdl_wait();
+  hb_pdl_launch();
 
   // the keys of the step's own rows
-  if (e.fresh > 0) {
+  if (some && mine == W - 1 && e.fresh > 0) {
     float x[E];
     load_elements<E>(q + (size_t)t * ldq + (size_t)head * D, c, D, vec, x);
     for (int j0 = 0; j0 < e.fresh; j0 += 4) {
@@ -249,12 +252,12 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
     }
   }
 
-  // the parts, 32 at a time: a lane holds one's maximum and sum
-  const int n = e.pre_n + e.own_n;
+  // this warp's parts, 32 at a time: a lane holds one's maximum and sum
+  const int all = some ? e.pre_n + e.own_n : 0, n = (all - mine + W - 1) / W;
   for (int k0 = 0; k0 < n; k0 += 32) {
-    const int k = k0 + lane;
+    const int k = (k0 + lane) * W + mine;
     const int row = k < e.pre_n ? e.pre_base + (h * e.pre_n + k) * e.pre_rows + g : e.own_base + (h * e.own_n + k - e.pre_n) * e.own_rows + g;
-    const float2 ml = k < n ? part_ml[row] : make_float2(-INFINITY, 0.f);
+    const float2 ml = k < all ? part_ml[row] : make_float2(-INFINITY, 0.f);
     const float mx = hb_warp_max(fmaxf(ml.x, m)), sub = mx == -INFINITY ? 0.f : mx, corr = exp2_of(m - sub);
     // a part without a visible key has sum 0 and no output; one whose sum is NaN makes the row NaN
     const float w = ml.y == 0.f ? 0.f : ml.y != ml.y ? ml.y : exp2_of(ml.x - sub);
@@ -263,23 +266,44 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
 #pragma unroll
     for (int i = 0; i < E; i++) acc[i] *= corr;
     const int in = min(32, n - k0);
-    for (int j0 = 0; j0 < in; j0 += 4) {
-      float o[4][E], wj[4];
+    for (int j0 = 0; j0 < in; j0 += SJ_AHEAD) {
+      float o[SJ_AHEAD][E], wj[SJ_AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < SJ_AHEAD; j++) {
         const int from = __shfl_sync(0xffffffffu, row, min(j0 + j, in - 1));
         wj[j] = __shfl_sync(0xffffffffu, w, min(j0 + j, in - 1));
         if (j0 + j >= in) wj[j] = 0.f;
         if (wj[j] != 0.f) load_elements<E>(part_o + (size_t)from * D, c, D, vec, o[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < SJ_AHEAD; j++)
         if (wj[j] != 0.f) {
 #pragma unroll
           for (int i = 0; i < E; i++) acc[i] = fmaf(wj[j], o[j][i], acc[i]);
         }
     }
   }
+  if (W > 1) {
+    if (lane == 0) sh_ml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int i = 0; i < E; i++) sh_acc[warp][c + i] = acc[i];
+    __syncthreads();
+    if (mine != 0) return;
+    for (int k = warp; k < warp + W; k++) m = fmaxf(m, sh_ml[k].x);
+    const float sub = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; i++) acc[i] = 0.f;
+    for (int k = warp; k < warp + W; k++) {
+      const float2 ml = sh_ml[k];
+      if (ml.y == 0.f) continue;
+      const float w = ml.y != ml.y ? ml.y : exp2_of(ml.x - sub);
+      l = fmaf(w, ml.y, l);
+#pragma unroll
+      for (int i = 0; i < E; i++) acc[i] = fmaf(w, sh_acc[k][c + i], acc[i]);
+    }
+  }
+  if (!some) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;       // a row that sees nothing is 0
   T* dst = out + ((size_t)t * Hq + head) * D;
 #pragma unroll
@@ -354,11 +378,19 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
     if (r) return r;
   }
   cudaError_t e = cudaSuccess;
-#define SJ_LAUNCH(E)                                                                                                                     \
-  e = hb_launch(shared_join_kernel<TA, E>, dim3((unsigned)((warps + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq,   \
+  // few rows of many parts: four warps share one's (8 rows x 32 heads of 34 parts 13 -> 8 us; 2,048 rows of 8 parts 5 us slower, beyond one round)
+  const int W = warps > 1024 || h->parts < 6 * warps ? 1 : 4;
+#define SJ_LAUNCH(E, W)                                                                                                                          \
+  e = hb_launch(shared_join_kernel<TA, E, W>, dim3((unsigned)((warps * W + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq,      \
                 (const TA*)kc, (const TA*)vc, bt, bt_stride, tokens, T, part_o, part_ml, (TA*)out, Hq, Hkv, D, ps, sl2, vec)
-  HB_DISPATCH_1(h->dt, "hb_attention_shared", { if (D <= 64) SJ_LAUNCH(2); else if (D <= 128) SJ_LAUNCH(4); else SJ_LAUNCH(8); });
+#define SJ_LAUNCH_W(E)               \
+  do {                               \
+    if (W == 1) SJ_LAUNCH(E, 1);     \
+    else SJ_LAUNCH(E, 4);            \
+  } while (0)
+  HB_DISPATCH_1(h->dt, "hb_attention_shared", { if (D <= 64) SJ_LAUNCH_W(2); else if (D <= 128) SJ_LAUNCH_W(4); else SJ_LAUNCH_W(8); });
 #undef SJ_LAUNCH
+#undef SJ_LAUNCH_W
   if (e != cudaSuccess) HB_FAIL("hb_attention_shared: %s", cudaGetErrorString(e));
   HB_CHECK_LAUNCH("hb_attention_shared");
   return 0;

@@ -3,14 +3,13 @@
 // A group's shared range and a request's own range are SEGMENTS: some rows against a range of keys. A segment's keys are cut into equal
 // chunks, an item is (chunk, kv head, up to tile_tokens rows), and each CTA gets a list of items: the shared items in the order of their keys,
 // so that the CTAs at work at one time read the same tiles (once from memory, then from L2), each to the CTA with the least work so
-// far, then the requests' own, longest first. The number of keys in a chunk is the one among a few multiples of an even share whose longest CTA, and whose
-// partial results, cost least.
+// far, then the requests' own, longest first. A chunk is the one among a few fractions of an even share of the work whose longest CTA, and whose partial
+// results, cost least.
 #include "common.cuh"
 #include "shared_plan.h"
 
 #include <algorithm>
 #include <exception>
-#include <queue>
 #include <utility>
 #include <vector>
 
@@ -28,47 +27,72 @@ struct Cut {
 
 struct Planner {
   int Hkv, G, key_tile, n_ctas, narrow_tokens;
-  double item_cost, part_cost;
+  double item_cost, wide_cost, part_cost;
+  static constexpr double row_cost = 0.02;               // of a part of the row that has most of them (they are joined one after another)
   std::vector<Segment> segs;
   std::vector<std::vector<std::pair<int, int>>> lists;   // a CTA's (segment, head * chunks + chunk)
 
-  int parts_of(const Segment& s, int chunks) const { return chunks * (s.tokens <= narrow_tokens ? 2 : 1); }
-  // Cuts the segments into chunks of at most `len` tiles and gives the items to the CTAs.
-  Cut cut(int len, bool keep) {
+  bool narrow(const Segment& s) const { return s.tokens <= narrow_tokens; }
+  double tile_cost(const Segment& s) const { return narrow(s) ? 1.0 : wide_cost; }
+  // What chunks of about `cost` come to: the longest CTA, if the shared items fill rounds of all CTAs and the requests' own ones what is left of the
+  // last of them, and the partial results.
+  Cut cut(double cost) {
     Cut c;
-    typedef std::pair<double, int> Load;
-    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> q;
-    for (int i = 0; i < n_ctas; i++) q.push(Load(0.0, i));
-    if (keep) lists.assign(n_ctas, {});
-    double longest = 0;
-    auto give = [&](int s, int item, double cost) {
-      Load l = q.top();
-      q.pop();
-      l.first += cost;
-      longest = std::max(longest, l.first);
-      if (keep) lists[l.second].push_back({s, item});
-      q.push(l);
+    double sum[2] = {0, 0}, most[2] = {0, 0};
+    long items[2] = {0, 0};
+    int parts[2] = {0, 0};
+    for (Segment& s : segs) {
+      const int len = std::max(1, (int)(cost / tile_cost(s) + 0.999));
+      s.chunks = (s.tiles + len - 1) / len;
+      s.parts = s.chunks * (narrow(s) ? 2 : 1);
+      s.base = (int)std::min<long>(c.parts, 0x7fffffff);
+      c.parts += (long)Hkv * s.parts * s.tokens * G;
+      const int k = s.shared ? 0 : 1;
+      const double all = item_cost * s.chunks + tile_cost(s) * s.tiles;
+      sum[k] += Hkv * all;
+      most[k] = std::max(most[k], all / s.chunks);
+      items[k] += (long)Hkv * s.chunks;
+      parts[k] = std::max(parts[k], s.parts);
+    }
+    auto rounds = [&](int k) { return items[k] ? (items[k] + n_ctas - 1) / n_ctas * (sum[k] / items[k]) : 0.0; };
+    const double even = (sum[0] + sum[1]) / n_ctas;
+    double longest = std::max(even, rounds(0));
+    if (!items[0]) longest = std::max(even, rounds(1));
+    if (items[1] && even >= rounds(0)) longest = std::max(longest, even + most[1] / 2);
+    c.cost = std::max(longest, std::max(most[0], most[1])) + part_cost * c.parts + row_cost * (parts[0] + parts[1]);
+    return c;
+  }
+  // Gives the items to the CTAs.
+  void deal() {
+    // the CTAs as a heap, the one with the least work (of these the lowest) on top
+    std::vector<std::pair<float, int>> load(n_ctas);
+    for (int i = 0; i < n_ctas; i++) load[i] = {0.f, i};
+    lists.assign(n_ctas, {});
+    auto give = [&](int s, int item) {
+      std::pair<float, int> l = load[0];
+      l.first += (float)(item_cost + tile_cost(segs[s]) * segs[s].tiles / segs[s].chunks);
+      lists[l.second].push_back({s, item});
+      int at = 0;
+      for (int child; (child = 2 * at + 1) < n_ctas; at = child) {
+        if (child + 1 < n_ctas && load[child + 1] < load[child]) child++;
+        if (!(load[child] < l)) break;
+        load[at] = load[child];
+      }
+      load[at] = l;
     };
     std::vector<int> own, shared;
     int most = 0;
     for (size_t i = 0; i < segs.size(); i++) {
-      Segment& s = segs[i];
-      s.chunks = (s.tiles + len - 1) / len;
-      s.parts = parts_of(s, s.chunks);
-      s.base = (int)std::min<long>(c.parts, 0x7fffffff);
-      c.parts += (long)Hkv * s.parts * s.tokens * G;
-      (s.shared ? shared : own).push_back((int)i);
-      if (s.shared) most = std::max(most, s.chunks);
+      (segs[i].shared ? shared : own).push_back((int)i);
+      if (segs[i].shared) most = std::max(most, segs[i].chunks);
     }
     for (int k = 0; k < most; k++)
       for (int h = 0; h < Hkv; h++)
         for (int i : shared)
-          if (k < segs[i].chunks) give(i, h * segs[i].chunks + k, item_cost + double(segs[i].tiles) / segs[i].chunks);
+          if (k < segs[i].chunks) give(i, h * segs[i].chunks + k);
     std::stable_sort(own.begin(), own.end(), [&](int a, int b) { return (long)segs[a].tiles * segs[b].chunks > (long)segs[b].tiles * segs[a].chunks; });
     for (int i : own)
-      for (int u = 0; u < Hkv * segs[i].chunks; u++) give(i, u, item_cost + double(segs[i].tiles) / segs[i].chunks);
-    c.cost = longest + part_cost * c.parts;
-    return c;
+      for (int u = 0; u < Hkv * segs[i].chunks; u++) give(i, u);
   }
 };
 
@@ -77,9 +101,10 @@ struct Planner {
 // q_len, ctx_len [R]; groups [n_groups][3]: first request, requests, shared tokens. out: SP_HEADER ints, then items, each CTA's first item (one more
 // for the end), tokens; returns the ints that were written, or, where `cap` is too small, minus the number that is needed; 0 with a message in
 // hb_last_error for lengths that make no plan. tile_tokens: rows of q in an item; narrow_tokens: items of at most so many rows leave two
-// parts (their key tiles go to two chains in turn), 0: none do.
+// parts (two chains share their keys), 0: none do. Costs are in key tiles of a narrow item: an item's beginning and end, a tile of another item, a part row.
 HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const int* groups, int n_groups, int Hq, int Hkv, int tile_tokens,
-                             int narrow_tokens, int key_tile, int n_ctas, float item_cost, float part_cost, int* out, int cap) {
+                             int narrow_tokens, int key_tile, int n_ctas, float item_cost, float wide_cost, float part_cost, int* out,
+                             int cap) {
   try {
     if (R < 0 || n_groups < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv || tile_tokens < 1 || key_tile < 1 || n_ctas < 1) {
       hb_set_error("hb_shared_plan: bad sizes (%d requests, %d groups, %d/%d heads, %d rows an item)", R, n_groups, Hq, Hkv, tile_tokens);
@@ -125,6 +150,7 @@ HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const 
     p.n_ctas = n_ctas;
     p.narrow_tokens = narrow_tokens;
     p.item_cost = item_cost;
+    p.wide_cost = wide_cost;
     p.part_cost = part_cost;
     const int T = start[R];
     std::vector<SharedToken> tokens(T);
@@ -169,27 +195,24 @@ HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const 
         t.fresh = fresh ? i + 1 : 0;
       }
     }
-    long tiles = 0, longest = 1;
-    for (const Segment& s : p.segs) {
-      tiles += (long)s.tiles * Hkv;
-      longest = std::max<long>(longest, s.tiles);
-    }
-    const double share = std::max(1.0, double(tiles) / n_ctas);
-    int best = 1;
-    double cost = -1;
-    for (double f : {1.0, 1.1, 1.25, 2.0, 0.75, 0.5, 0.4, 0.34, 0.25, 4.0}) {
-      const int len = (int)std::max(1.0, std::min(double(longest), share * f + 0.999));
-      const Cut c = p.cut(len, false);
+    double all = 0;
+    for (const Segment& s : p.segs) all += (p.item_cost + p.tile_cost(s) * s.tiles) * Hkv;
+    const double share = std::max(1.0, all / n_ctas);
+    double best = 1, cost = -1;
+    for (double f = 2.0; f > 0.1; f *= 0.93) {
+      const double chunk = std::max(1.0, share * f - p.item_cost);
+      const Cut c = p.cut(chunk);
       if (c.parts < 0x7fffffff && (cost < 0 || c.cost < cost)) {
         cost = c.cost;
-        best = len;
+        best = chunk;
       }
     }
     if (cost < 0) {
       hb_set_error("hb_shared_plan: the partial results of %d rows are too many", T);
       return 0;
     }
-    const Cut c = p.cut(best, true);
+    const Cut c = p.cut(best);
+    p.deal();
     std::vector<SharedItem> items;
     std::vector<int> ctas;
     int max_rows = 0;

@@ -18,7 +18,7 @@ from . import library, ops
 
 _p, _i, _l, _f = C.c_void_p, C.c_int, C.c_long, C.c_float
 ops._SIGS["drafts"] = {
-    "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i],
+    "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _f, _p, _i],
     "hb_attention_shared": [_p, _l, _p, _p, _l, _p, _i, _p, _p, _p, _p, _f, _i, _p, _p],
     "hb_shared_items_tc_supported": [_i, _i, _i, _i],
     "hb_verify_drafts": [_p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _l, _p, _i, _l, _l, _p, _p, _p, _p, _p],
@@ -32,7 +32,7 @@ _HEADER = 16
 
 
 def plan_numbers(q_lens, ctx_lens, groups, n_heads: int, n_kv_heads: int, tile_tokens: int, narrow_tokens: int, key_tile: int, n_ctas: int,
-                 item_cost: float, part_cost: float) -> np.ndarray:
+                 item_cost: float, wide_cost: float, part_cost: float) -> np.ndarray:
     """The plan as int32 numbers (csrc/shared_plan.cu, which runs on the host); raises KernelError for lengths that make none."""
     q, c = (np.ascontiguousarray(x, dtype=np.int32) for x in (q_lens, ctx_lens))
     g = np.ascontiguousarray(groups, dtype=np.int32).reshape(-1, 3)
@@ -43,7 +43,7 @@ def plan_numbers(q_lens, ctx_lens, groups, n_heads: int, n_kv_heads: int, tile_t
     while True:
         out = np.empty(cap, dtype=np.int32)
         n = fn(q.ctypes.data, c.ctypes.data, len(q), g.ctypes.data, len(g), n_heads, n_kv_heads, tile_tokens, narrow_tokens, key_tile, n_ctas,
-               item_cost, part_cost, out.ctypes.data, cap)
+               item_cost, wide_cost, part_cost, out.ctypes.data, cap)
         if n > 0:
             return out[:n]
         if n == 0:
@@ -73,18 +73,19 @@ class SharedPlan:
         # on the tensor cores: one CTA an SM, items of two chains of up to 128 rows each
         self.tensor_cores = (dtype == torch.bfloat16 and ops.fast_kernels_on()
                              and bool(ops._fn("drafts", "hb_shared_items_tc_supported")(n_heads, n_kv_heads, head_dim, page_size)))
+        # (costs in key tiles of an item of few rows, as measured: 1.3 us; see csrc/shared_plan.cu)
         if self.tensor_cores:
-            tile, narrow, key_tile, ctas, item_cost, part_cost = 2 * (128 // group), 128 // group, 128, _sms(self.device), 1.5, head_dim * 2e-6
+            cut, costs = (2 * (128 // group), 128 // group, 128, _sms(self.device)), (0.9, 1.7, head_dim * 1e-6)
         else:
-            tile, narrow, key_tile, ctas, item_cost, part_cost = max(1, 64 // group), 0, 64, 2 * _sms(self.device), 1.0, head_dim * 2e-6
-        numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, tile, narrow, key_tile, ctas, item_cost, part_cost)
+            cut, costs = (max(1, 64 // group), 0, 64, 2 * _sms(self.device)), (1.0, 1.0, head_dim * 1e-6)
+        numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, *cut, *costs)
         self.rows, self.parts = int(numbers[_TOKENS]), int(numbers[_PARTS])
         self.ctas, self.max_rows = int(numbers[_CTAS]), int(numbers[_MAX_ROWS])
         self.most_keys = max((int(c) + int(n) for c, n in zip(ctx_lens, q_lens) if n), default=0)
         self.q_shape, self.page_shape = (self.rows, n_heads * head_dim), (n_kv_heads, page_size, head_dim)
         self.size, self.default_scale = 2 if dtype == torch.bfloat16 else 4, 1.0 / math.sqrt(head_dim)
         self.workspace = self.parts * (head_dim + 2) + 4           # floats
-        self._launch = np.array([self.rows, self.ctas, self.max_rows, narrow, self.parts, self.tensor_cores, ops._DT[dtype], n_heads, n_kv_heads,
+        self._launch = np.array([self.rows, self.ctas, self.max_rows, cut[1], self.parts, self.tensor_cores, ops._DT[dtype], n_heads, n_kv_heads,
                                  head_dim, page_size, numbers[_OFF_ITEMS], numbers[_OFF_CTAS], numbers[_OFF_TOKENS]], dtype=np.int32)      # SharedLaunch of csrc/attention_shared.cu
         self.launch = self._launch.ctypes.data
         host = torch.from_numpy(numbers)

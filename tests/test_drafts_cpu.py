@@ -12,8 +12,8 @@ pytestmark = pytest.mark.skipif(not (os.path.isfile("/usr/local/cuda/bin/nvcc") 
 NO_MASK, FRESH = 1 << 30, 16
 
 
-def plan(q, c, groups, Hq=8, Hkv=2, tile=16, narrow=0, key_tile=64, ctas=10, item_cost=1.0, part_cost=1e-4):
-    return drafts.plan_numbers(q, c, groups, Hq, Hkv, tile, narrow, key_tile, ctas, item_cost, part_cost)
+def plan(q, c, groups, Hq=8, Hkv=2, tile=16, narrow=0, key_tile=64, ctas=10, item_cost=1.0, wide_cost=1.5, part_cost=1e-4):
+    return drafts.plan_numbers(q, c, groups, Hq, Hkv, tile, narrow, key_tile, ctas, item_cost, wide_cost, part_cost)
 
 
 def seen_keys(n, Hkv, G, narrow=0, key_tile=64):
@@ -25,15 +25,14 @@ def seen_keys(n, Hkv, G, narrow=0, key_tile=64):
     owner = {}
     for table, token, count, pos, lo, hi, head, part in items.tolist():
         assert lo < hi and count > 0
-        chains = 2 if count <= narrow else 1
+        chains = 2 if count <= narrow else 1         # (two share a tile's keys)
         for ch in range(chains):
             for i in range(count):
                 for g in range(G):
                     p = part + (ch * count + i) * G + g
                     assert p not in owner and 0 <= p < n[drafts._PARTS]
                     keys = [k for k in range(lo, hi) if k <= pos + i]
-                    if chains == 2:      # its key tiles in turn
-                        keys = [k for k in keys if (k // key_tile - lo // key_tile) % 2 == ch]
+                    keys = [k for k in keys if k % key_tile // (key_tile // chains) == ch]
                     owner[p] = (token + i, head, g, table, keys)
     assert len(owner) == n[drafts._PARTS]
     out = []
