@@ -12,6 +12,8 @@
 #include "common.cuh"
 #include "shared_plan.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int SI_KEYS = 64, SI_THREADS = 256;
@@ -29,142 +31,231 @@ template <typename T> __device__ __forceinline__ float4 row4(const T* row, int c
   return v;
 }
 
-template <int RM, int NC> constexpr int items_smem() {
-  return (16 * RM * (64 * NC + 4) + 2 * SI_KEYS * (64 * NC + 4) + 16 * RM * (SI_KEYS + 4)) * 4;
+// Two numbers at a time: the FMA pipe takes as long, the issue slots are half of them.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool some) {      // zeros where there is nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(some ? 16 : 0) : "memory");
 }
 
-// A thread has RM rows (ty RM ..) by four keys (tx, tx + 16, ..) of the scores, and RM rows by 4 NC columns of the output.
+template <int NC> struct ItemsShared {
+  static constexpr int LD = 64 * NC + 4, LP = SI_KEYS + 4, TILE = SI_KEYS * LD, STAGES = NC <= 2 ? 2 : 1;
+  static constexpr int BYTES = (64 * LD + 2 * STAGES * TILE + 64 * LP) * 4 + 2 * SI_KEYS * 8;
+};
+
+// A block of up to 16 RM rows of an item. A thread has RM rows (ty RM ..) by four keys (tx, tx + 16, ..) of the scores, and RM rows by 4 NC columns of
+// the output. Tiles of K and V come by asynchronous copies a tile ahead, where rows start on 16 bytes, are 32-bit and two tiles fit (heads of up to
+// 128); else through registers.
 template <typename T, int RM, int NC>
+__device__ __forceinline__ void item_rows(const SharedItem& e, int r0, float* sh, const T* q, long ldq, const T* kc, const T* vc, const int* bt,
+                                          int bt_stride, int narrow, float* part_o, float2* part_ml, int G, int Hkv, int D, int page_size,
+                                          float scale_log2, int vec) {
+  using S = ItemsShared<NC>;
+  constexpr int R = 16 * RM, DP = 64 * NC, LD = S::LD, LP = S::LP;
+  constexpr bool CAN = S::STAGES == 2 && sizeof(T) == 4;
+  float *sQ = sh, *sKV = sQ + 64 * LD, *sP = sKV + 2 * S::STAGES * S::TILE;     // stage s: K at 2 s, V at 2 s + 1
+  long* sRow = (long*)(sP + 64 * LP);                                           // [stage][key]: where the key's row is, -1: nowhere
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, rows = e.tokens * G;
+  const bool copies = CAN && vec;
+  auto find = [&](int k0, int s) {                    // rows of the keys from k0 on
+    if (threadIdx.x < SI_KEYS) {
+      const int p = k0 + (int)threadIdx.x;
+      sRow[s * SI_KEYS + threadIdx.x] =
+          p < e.hi ? (((long)bt[(size_t)e.table * bt_stride + p / page_size] * Hkv + e.head) * page_size + p % page_size) * D : -1;
+    }
+  };
+  auto bring = [&](int s) {                           // their keys and values into stage s
+    float *sK = sKV + 2 * s * S::TILE, *sV = sK + S::TILE;
+    for (int i = threadIdx.x; i < SI_KEYS * (DP / 4); i += SI_THREADS) {
+      const int j = i / (DP / 4), c = 4 * (i % (DP / 4));
+      const long row = sRow[s * SI_KEYS + j];
+      if (copies) {
+        const bool some = row >= 0 && c < D;
+        copy16(sK + j * LD + c, kc + (some ? row + c : 0), some);
+        copy16(sV + j * LD + c, vc + (some ? row + c : 0), some);
+      } else {
+        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+        if (row >= 0) {
+          k = row4(kc + row, c, D, vec);
+          v = row4(vc + row, c, D, vec);
+        }
+        *(float4*)(sK + j * LD + c) = k;
+        *(float4*)(sV + j * LD + c) = v;
+      }
+    }
+    if (CAN) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+        __syncthreads();
+        find(e.lo, 0);
+        for (int i = threadIdx.x; i < R * (DP / 4); i += SI_THREADS) {
+          const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r0 + r < rows) v = row4(q + (size_t)(e.token + (r0 + r) / G) * ldq + (size_t)(e.head * G + (r0 + r) % G) * D, c, D, vec);
+          *(float4*)(sQ + r * LD + c) = v;
+        }
+        __syncthreads();
+        if (copies) bring(0);
+        float m[RM], l[RM];
+        uint64_t acc[RM][2 * NC];
+        int last[RM];                                     // the last key that the row sees
+  #pragma unroll
+        for (int i = 0; i < RM; i++) {
+          m[i] = -INFINITY;
+          l[i] = 0.f;
+          last[i] = e.pos == SP_NO_MASK ? SP_NO_MASK : e.pos + (r0 + ty * RM + i) / G;
+  #pragma unroll
+          for (int c = 0; c < 2 * NC; c++) acc[i][c] = 0ull;
+        }
+        int stage = 0;
+        for (int k0 = e.lo; k0 < e.hi; k0 += SI_KEYS) {
+          if (copies) {
+            if (k0 + SI_KEYS < e.hi) find(k0 + SI_KEYS, stage ^ 1);
+            __syncthreads();                              // (the other stage has been read, too)
+            if (k0 + SI_KEYS < e.hi) {
+              bring(stage ^ 1);
+              asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+              asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+          } else {
+            if (k0 > e.lo) {
+              __syncthreads();
+              find(k0, 0);
+              __syncthreads();
+            }
+            bring(0);
+          }
+          __syncthreads();
+          const float *sK = sKV + 2 * stage * S::TILE, *sV = sK + S::TILE;
+          if (copies) stage ^= 1;
+          uint64_t s2[RM][4];
+  #pragma unroll
+          for (int i = 0; i < RM; i++)
+  #pragma unroll
+            for (int j = 0; j < 4; j++) s2[i][j] = 0ull;
+  #pragma unroll 4
+          for (int c = 0; c < DP; c += 4) {
+            ulonglong2 a[RM], b[4];
+  #pragma unroll
+            for (int i = 0; i < RM; i++) a[i] = *(const ulonglong2*)(sQ + (ty * RM + i) * LD + c);
+  #pragma unroll
+            for (int j = 0; j < 4; j++) b[j] = *(const ulonglong2*)(sK + (tx + 16 * j) * LD + c);
+  #pragma unroll
+            for (int i = 0; i < RM; i++)
+  #pragma unroll
+              for (int j = 0; j < 4; j++) s2[i][j] = fma2(a[i].x, b[j].x, fma2(a[i].y, b[j].y, s2[i][j]));
+          }
+          float corr[RM];
+  #pragma unroll
+          for (int i = 0; i < RM; i++) {
+            float s[4], mx = -INFINITY;
+  #pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int p = k0 + tx + 16 * j;
+              const float2 y = both(s2[i][j]);
+              s[j] = p < e.hi && p <= last[i] ? (y.x + y.y) * scale_log2 : -INFINITY;
+              mx = fmaxf(mx, s[j]);
+            }
+  #pragma unroll
+            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float mn = fmaxf(m[i], mx), sub = mn == -INFINITY ? 0.f : mn;
+            corr[i] = exp2_of(m[i] - sub);
+            m[i] = mn;
+            float sum = 0.f;
+  #pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float p = exp2_of(s[j] - sub);
+              sum += p;
+              sP[(ty * RM + i) * LP + tx + 16 * j] = p;
+            }
+  #pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[i] = l[i] * corr[i] + sum;
+          }
+          __syncwarp();               // the 16 lanes that share a row of P are of one warp
+  #pragma unroll
+          for (int i = 0; i < RM; i++) {
+            const uint64_t w = pair(corr[i], corr[i]);
+  #pragma unroll
+            for (int c = 0; c < 2 * NC; c++) acc[i][c] = fma2(acc[i][c], w, 0ull);
+          }
+          // a value behind a row is not multiplied by 0 (it may be an infinity or NaN), where rows do not see all keys
+          auto products = [&](auto careful) {
+  #pragma unroll 2
+            for (int j = 0; j < SI_KEYS; j += 4) {
+              float pr[RM][4];
+  #pragma unroll
+              for (int i = 0; i < RM; i++) *(float4*)pr[i] = *(const float4*)(sP + (ty * RM + i) * LP + j);
+  #pragma unroll
+              for (int jj = 0; jj < 4; jj++)
+  #pragma unroll
+                for (int n = 0; n < NC; n++) {
+                  const ulonglong2 v = *(const ulonglong2*)(sV + (j + jj) * LD + 64 * n + 4 * tx);
+  #pragma unroll
+                  for (int i = 0; i < RM; i++) {
+                    const uint64_t p = pair(pr[i][jj], pr[i][jj]);
+                    if (!decltype(careful)::value || pr[i][jj] != 0.f) {
+                      acc[i][2 * n] = fma2(p, v.x, acc[i][2 * n]);
+                      acc[i][2 * n + 1] = fma2(p, v.y, acc[i][2 * n + 1]);
+                    }
+                  }
+                }
+            }
+          };
+          if (e.pos == SP_NO_MASK) products(std::false_type());
+          else products(std::true_type());
+        }
+  #pragma unroll
+        for (int i = 0; i < RM; i++) {
+          const int r = r0 + ty * RM + i;
+          if (r >= rows) continue;
+          const size_t row = (size_t)e.part + r;
+          if (tx == 0) {
+            part_ml[row] = make_float2(m[i], l[i]);
+            // a plan that was made for the tensor cores has a second part here (rows of q that TMA cannot address)
+            if (e.tokens <= narrow) part_ml[row + rows] = make_float2(-INFINITY, 0.f);
+          }
+  #pragma unroll
+          for (int n = 0; n < NC; n++) {
+            const float2 y[2] = {both(acc[i][2 * n]), both(acc[i][2 * n + 1])};
+            const float o[4] = {y[0].x, y[0].y, y[1].x, y[1].y};
+  #pragma unroll
+            for (int c = 0; c < 4; c++)
+              if (64 * n + 4 * tx + c < D) part_o[row * D + 64 * n + 4 * tx + c] = o[c];
+          }
+        }
+}
+
+// Items of up to 16 rows, and the last rows of others, take a row a thread (LSU-bound: a key's loads serve 16 rows), the rest four.
+template <typename T, int NC>
 __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
                                                                   const SharedItem* items, const int* ctas, int narrow, float* part_o,
-                                                                  float2* part_ml, int Hq, int Hkv,
-                                                                  int D, int page_size, float scale_log2, int vec) {
-  constexpr int R = 16 * RM, DP = 64 * NC, LD = DP + 4, LP = SI_KEYS + 4;
+                                                                  float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec) {
   extern __shared__ __align__(16) float sh[];
-  float *sQ = sh, *sK = sQ + R * LD, *sV = sK + SI_KEYS * LD, *sP = sV + SI_KEYS * LD;
+  const int G = Hq / Hkv, it0 = ctas[blockIdx.x], it1 = ctas[blockIdx.x + 1];
   hb_pdl_wait();
   hb_pdl_launch();
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, G = Hq / Hkv;
-  for (int it = ctas[blockIdx.x]; it < ctas[blockIdx.x + 1]; it++) {
+  for (int it = it0; it < it1; it++) {
     const SharedItem e = items[it];
     const int rows = e.tokens * G;
-    for (int r0 = blockIdx.y * R; r0 < rows; r0 += gridDim.y * R) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < R * (DP / 4); i += SI_THREADS) {
-        const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r0 + r < rows) v = row4(q + (size_t)(e.token + (r0 + r) / G) * ldq + (size_t)(e.head * G + (r0 + r) % G) * D, c, D, vec);
-        *(float4*)(sQ + r * LD + c) = v;
-      }
-      float m[RM], l[RM], acc[RM][4 * NC];
-      int last[RM];                                     // the last key that the row sees
-#pragma unroll
-      for (int i = 0; i < RM; i++) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
-        last[i] = e.pos == SP_NO_MASK ? SP_NO_MASK : e.pos + (r0 + ty * RM + i) / G;
-#pragma unroll
-        for (int c = 0; c < 4 * NC; c++) acc[i][c] = 0.f;
-      }
-      for (int k0 = e.lo; k0 < e.hi; k0 += SI_KEYS) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < SI_KEYS * (DP / 4); i += SI_THREADS) {
-          const int j = i / (DP / 4), c = 4 * (i % (DP / 4)), p = k0 + j;
-          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-          if (p < e.hi) {
-            const size_t row = ((size_t)bt[(size_t)e.table * bt_stride + p / page_size] * Hkv + e.head) * page_size + p % page_size;
-            k = row4(kc + row * D, c, D, vec);
-            v = row4(vc + row * D, c, D, vec);
-          }
-          *(float4*)(sK + j * LD + c) = k;
-          *(float4*)(sV + j * LD + c) = v;
-        }
-        __syncthreads();
-        float s[RM][4] = {};
-#pragma unroll 4
-        for (int c = 0; c < DP; c += 4) {
-          float4 a[RM], b[4];
-#pragma unroll
-          for (int i = 0; i < RM; i++) a[i] = *(const float4*)(sQ + (ty * RM + i) * LD + c);
-#pragma unroll
-          for (int j = 0; j < 4; j++) b[j] = *(const float4*)(sK + (tx + 16 * j) * LD + c);
-#pragma unroll
-          for (int i = 0; i < RM; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
-        }
-        float corr[RM];
-#pragma unroll
-        for (int i = 0; i < RM; i++) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const int p = k0 + tx + 16 * j;
-            s[i][j] = p < e.hi && p <= last[i] ? s[i][j] * scale_log2 : -INFINITY;
-            mx = fmaxf(mx, s[i][j]);
-          }
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float mn = fmaxf(m[i], mx), sub = mn == -INFINITY ? 0.f : mn;
-          corr[i] = exp2_of(m[i] - sub);
-          m[i] = mn;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float p = exp2_of(s[i][j] - sub);
-            sum += p;
-            sP[(ty * RM + i) * LP + tx + 16 * j] = p;
-          }
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          l[i] = l[i] * corr[i] + sum;
-        }
-        __syncwarp();               // the 16 lanes that share a row of P are of one warp
-#pragma unroll
-        for (int i = 0; i < RM; i++)
-#pragma unroll
-          for (int c = 0; c < 4 * NC; c++) acc[i][c] *= corr[i];
-#pragma unroll 4
-        for (int j = 0; j < SI_KEYS; j += 4) {
-          float pr[RM][4];
-#pragma unroll
-          for (int i = 0; i < RM; i++) *(float4*)pr[i] = *(const float4*)(sP + (ty * RM + i) * LP + j);
-#pragma unroll
-          for (int jj = 0; jj < 4; jj++)
-#pragma unroll
-            for (int n = 0; n < NC; n++) {
-              const float4 v = *(const float4*)(sV + (j + jj) * LD + 64 * n + 4 * tx);
-#pragma unroll
-              for (int i = 0; i < RM; i++) {
-                // a value behind the row is not multiplied by 0: it may be an infinity or NaN
-                const float p = pr[i][jj];
-                if (p != 0.f) {
-                  acc[i][4 * n] = fmaf(p, v.x, acc[i][4 * n]);
-                  acc[i][4 * n + 1] = fmaf(p, v.y, acc[i][4 * n + 1]);
-                  acc[i][4 * n + 2] = fmaf(p, v.z, acc[i][4 * n + 2]);
-                  acc[i][4 * n + 3] = fmaf(p, v.w, acc[i][4 * n + 3]);
-                }
-              }
-            }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < RM; i++) {
-        const int r = r0 + ty * RM + i;
-        if (r >= rows) continue;
-        const size_t row = (size_t)e.part + r;
-        if (tx == 0) {
-          part_ml[row] = make_float2(m[i], l[i]);
-          // a plan that was made for the tensor cores has a second part here (rows of q that TMA cannot address)
-          if (e.tokens <= narrow) part_ml[row + rows] = make_float2(-INFINITY, 0.f);
-        }
-#pragma unroll
-        for (int n = 0; n < NC; n++)
-#pragma unroll
-          for (int c = 0; c < 4; c++)
-            if (64 * n + 4 * tx + c < D) part_o[row * D + 64 * n + 4 * tx + c] = acc[i][4 * n + c];
-      }
+    for (int r0 = blockIdx.y * 64; r0 < rows; r0 += gridDim.y * 64) {
+      if (rows - r0 <= 16)
+        item_rows<T, 1, NC>(e, r0, sh, q, ldq, kc, vc, bt, bt_stride, narrow, part_o, part_ml, G, Hkv, D, page_size, scale_log2, vec);
+      else
+        item_rows<T, 4, NC>(e, r0, sh, q, ldq, kc, vc, bt, bt_stride, narrow, part_o, part_ml, G, Hkv, D, page_size, scale_log2, vec);
     }
   }
 }
@@ -319,18 +410,18 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
   }
 }
 
-template <typename T, int RM, int NC>
+template <typename T, int NC>
 int launch_items(const void* q, long ldq, const void* kc, const void* vc, const int* bt, int bt_stride, const SharedItem* items, const int* cta_items,
                  int ctas, int max_rows, int narrow, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
-  constexpr int smem = items_smem<RM, NC>();
-  auto kern = shared_items_kernel<T, RM, NC>;
+  constexpr int smem = ItemsShared<NC>::BYTES;
+  auto kern = shared_items_kernel<T, NC>;
   static bool configured = false;
   if (!configured) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
     configured = true;
   }
-  const int blocks = (max_rows + 16 * RM - 1) / (16 * RM);
+  const int blocks = (max_rows + 63) / 64;
   const cudaError_t e = hb_launch(kern, dim3(ctas, blocks < 65535 ? blocks : 65535), SI_THREADS, smem, s, (const T*)q, ldq, (const T*)kc, (const T*)vc, bt,
                                   bt_stride, items, cta_items, narrow, part_o, part_ml, Hq, Hkv, D, page_size, scale_log2, vec);
   if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
@@ -365,15 +456,9 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
     if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, items, cta_items, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
   } else if (h->ctas > 0) {
     int r = -1;
-#define SI_LAUNCH(RM, NC) \
-  r = launch_items<TA, RM, NC>(q, ldq, kc, vc, bt, bt_stride, items, cta_items, h->ctas, h->max_rows, h->narrow, part_o, part_ml, Hq, Hkv, D, ps, sl2, vec, s)
-    HB_DISPATCH_1(h->dt, "hb_attention_shared", {
-      if (h->max_rows <= 16) {
-        if (D <= 64) SI_LAUNCH(1, 1); else if (D <= 128) SI_LAUNCH(1, 2); else SI_LAUNCH(1, 4);
-      } else {
-        if (D <= 64) SI_LAUNCH(4, 1); else if (D <= 128) SI_LAUNCH(4, 2); else SI_LAUNCH(4, 4);
-      }
-    });
+#define SI_LAUNCH(NC) \
+  r = launch_items<TA, NC>(q, ldq, kc, vc, bt, bt_stride, items, cta_items, h->ctas, h->max_rows, h->narrow, part_o, part_ml, Hq, Hkv, D, ps, sl2, vec, s)
+    HB_DISPATCH_1(h->dt, "hb_attention_shared", { if (D <= 64) SI_LAUNCH(1); else if (D <= 128) SI_LAUNCH(2); else SI_LAUNCH(4); });
 #undef SI_LAUNCH
     if (r) return r;
   }

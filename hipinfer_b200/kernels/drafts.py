@@ -77,7 +77,8 @@ class SharedPlan:
         if self.tensor_cores:
             cut, costs = (2 * (128 // group), 128 // group, 128, _sms(self.device)), (0.9, 1.7, head_dim * 1e-6)
         else:
-            cut, costs = (max(1, 64 // group), 0, 64, 2 * _sms(self.device)), (1.0, 1.0, head_dim * 1e-6)
+            cut = (max(1, 64 // group), 0, 64, (2 if head_dim <= 64 else 1) * _sms(self.device))         # (as many as are resident)
+            costs = (1.0, 1.0, head_dim * 1e-6)
         numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, *cut, *costs)
         self.rows, self.parts = int(numbers[_TOKENS]), int(numbers[_PARTS])
         self.ctas, self.max_rows = int(numbers[_CTAS]), int(numbers[_MAX_ROWS])
