@@ -14,6 +14,10 @@ logical page (position // page_size); a released entry reads -1. All pages retur
 pool when the request ends. A freed page is handed out again, lowest id first, so that which
 page a request gets is reproducible.
 
+A request may be FORKED: the new one names the whole pages that its parent has filled, and each page counts who holds it;
+it is free again when the last of them lets go. A page held twice is never written: both requests go on in pages of their
+own. A request may also be TRUNCATED, when drafted tokens that it was run with are refused.
+
 Beside the pages there are STATE SLOTS: one integer per live request, handed out at admission
 and returned at the end, which indexes tensors of fixed per-request state (a recurrent or
 convolution state of another mixer, a sampler's counters). This architecture's attention
@@ -98,13 +102,13 @@ class CacheGroupSpec:
 
 
 class PagePool:
-    """Page ids 0..n-1 of one group; lowest free id first; every id is either free or held once."""
+    """Page ids 0..n-1 of one group; lowest free id first; every id is either free or held, as often as requests share it."""
 
     def __init__(self, num_pages: int):
         self.num_pages = int(num_pages)
         self._free = list(range(self.num_pages))
         heapq.heapify(self._free)
-        self._held = [False] * self.num_pages
+        self._held = [0] * self.num_pages
 
     @property
     def free_count(self) -> int:
@@ -114,14 +118,25 @@ class PagePool:
         if not self._free:
             raise OutOfPages("page pool is empty")
         p = heapq.heappop(self._free)
-        self._held[p] = True
+        self._held[p] = 1
         return p
+
+    def share(self, page: int) -> int:
+        """One more request holds the page."""
+        if not (0 <= page < self.num_pages) or not self._held[page]:
+            raise CacheError(f"page {page} is shared but not held")
+        self._held[page] += 1
+        return page
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
 
     def release(self, page: int) -> None:
         if not (0 <= page < self.num_pages) or not self._held[page]:
             raise CacheError(f"page {page} is released but not held")
-        self._held[page] = False
-        heapq.heappush(self._free, page)
+        self._held[page] -= 1
+        if not self._held[page]:
+            heapq.heappush(self._free, page)
 
     def held(self) -> List[int]:
         return [p for p, h in enumerate(self._held) if h]
@@ -198,7 +213,7 @@ class CacheManager:
             raise CacheError(f"request {request_id!r} is not live") from None
 
     def free_request(self, request_id) -> None:
-        """Give back every page and the state slot of a request that has ended."""
+        """Give back every page (a shared one stays with who else holds it) and the state slot of a request that has ended."""
         rc = self.get(request_id)
         for g, table in enumerate(rc.tables):
             for p in table:
@@ -206,6 +221,54 @@ class CacheManager:
                     self.pools[g].release(p)
         self.slots.release(rc.state_slot)
         del self.requests[request_id]
+
+    def fork(self, request_id, new_id) -> RequestCache:
+        """A new request that holds the whole pages of `request_id`: its length is theirs, and the tokens behind them, if it
+        shall have them too, are run again. State slots are not copied: a request whose model keeps per-request state has
+        nothing to be forked from. Raises CacheError where the retention rule has given back pages that a query behind the
+        whole pages reads (at a page's end it never has)."""
+        rc = self.get(request_id)
+        whole = rc.length // self.page_size
+        if not self._kept(rc, whole * self.page_size):
+            raise CacheError(f"request {request_id!r} cannot be forked at {whole * self.page_size} of its {rc.length} tokens: pages "
+                             f"that would be read are gone")
+        new = self.add_request(new_id)
+        new.length = whole * self.page_size
+        for g, table in enumerate(rc.tables):
+            new.tables[g] = [self.pools[g].share(p) if p >= 0 else -1 for p in table[:whole]]
+        return new
+
+    def truncate(self, request_id, length: int) -> int:
+        """The request's tokens from position `length` on are taken back; pages behind it are released. Returns how many.
+        Raises CacheError (nothing changed) for a length above the request's, for one inside a page that another request
+        holds too (the next token would be written there), and where the retention rule has given back pages that a query
+        at `length` reads again."""
+        rc = self.get(request_id)
+        if not 0 <= length <= rc.length:
+            raise CacheError(f"request {request_id!r} holds {rc.length} tokens and cannot be cut to {length}")
+        keep = -(-length // self.page_size)
+        for g, table in enumerate(rc.tables):
+            if length % self.page_size and table[keep - 1] >= 0 and self.pools[g].holders(table[keep - 1]) > 1:
+                raise CacheError(f"request {request_id!r} cannot be cut to {length} tokens: page {table[keep - 1]} is shared")
+        if not self._kept(rc, length):
+            raise CacheError(f"request {request_id!r} cannot be cut to {length} tokens: pages that it would read are gone")
+        released = 0
+        for g, table in enumerate(rc.tables):
+            for p in table[keep:]:
+                if p >= 0:
+                    self.pools[g].release(p)
+                    released += 1
+            del table[keep:]
+        rc.length = length
+        return released
+
+    def _kept(self, rc: RequestCache, length: int) -> bool:
+        """Are all pages there that a query at position `length` and later ones read?"""
+        for spec, table in zip(self.groups, rc.tables):
+            dead = [(-(-lo // self.page_size), hi // self.page_size) for lo, hi in RETENTION[spec.kind](spec, length)]
+            if any(table[lp] < 0 and not any(lo <= lp < hi for lo, hi in dead) for lp in range(-(-length // self.page_size))):
+                return False
+        return True
 
     # ---------------------------------------------------------------- pages
     def pages_needed(self, request_id, n_tokens: int) -> List[int]:
@@ -274,16 +337,16 @@ class CacheManager:
         return [p.free_count for p in self.pools]
 
     def check(self) -> None:
-        """Every page is free or held by exactly one request; every slot likewise. For tests."""
+        """Every page is free or held by as many requests as it counts; every slot is free or held by one. For tests."""
         for g, pool in enumerate(self.pools):
-            owned: Dict[int, object] = {}
+            owned: Dict[int, list] = {}
             for rid, rc in self.requests.items():
                 for p in rc.tables[g]:
-                    if p < 0:
-                        continue
-                    if p in owned:
-                        raise CacheError(f"group {g}: page {p} is held by {owned[p]!r} and {rid!r}")
-                    owned[p] = rid
+                    if p >= 0:
+                        owned.setdefault(p, []).append(rid)
+            for p, rids in owned.items():
+                if len(rids) != pool.holders(p) or len(set(rids)) != len(rids):
+                    raise CacheError(f"group {g}: page {p} is held by {rids!r} and counts {pool.holders(p)}")
             held = set(pool.held())
             if held != set(owned):
                 raise CacheError(f"group {g}: pool holds {sorted(held)}, requests hold {sorted(owned)}")

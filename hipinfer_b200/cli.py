@@ -4,6 +4,7 @@ are kept, with --model for a folder of config.json and model.safetensors.
 
     python -m hipinfer_b200 generate --model DIR --tokens 1 2 3 --new 8 [--mode bf16|fp32]
                                      [--temperature T --seed S] [--max-batch --max-seq --max-prefill]
+                                     [--samples N --drafts K]
     python -m hipinfer_b200 random-model --config config.json --out DIR --seed 0 [--std 0.02] [--dtype bfloat16]
     python -m hipinfer_b200 replay --model DIR --dtype bfloat16 --out DIR --max-tokens N   (steps on stdin)
     python -m hipinfer_b200 bench [bench.py's options]        (the measurement program beside the package)
@@ -25,6 +26,8 @@ def main(argv=None) -> int:
     g.add_argument("--mode", "--dtype", dest="mode", default="bf16", choices=["bf16", "fp32", "bfloat16", "float32"])
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--seed", type=int, default=0)
+    g.add_argument("--samples", type=int, default=0, help="continuations of the one prompt, which share its cache")
+    g.add_argument("--drafts", type=int, default=0, help="with --samples: tokens a step looks up in a sample's text and verifies")
     g.add_argument("--max-batch", type=int, default=8)
     g.add_argument("--max-seq", type=int, default=2048)
     g.add_argument("--max-prefill", type=int, default=1024)
@@ -64,7 +67,11 @@ def main(argv=None) -> int:
         eng = Engine(a.model, max_batch=a.max_batch, max_seq=a.max_seq, max_prefill=a.max_prefill, dtype=a.mode)
         print({k: getattr(eng, k) for k in ("vocab", "hidden", "inter", "layers", "heads", "kv_heads", "head_dim",
                                             "max_pos", "tied")})
-        print(eng.generate(a.tokens, a.new, temperature=a.temperature, seed=a.seed))
+        if a.samples or a.drafts:
+            for tokens in eng.sample_many(a.tokens, max(1, a.samples), a.new, temperature=a.temperature, seed=a.seed, n_draft=a.drafts):
+                print(tokens)
+        else:
+            print(eng.generate(a.tokens, a.new, temperature=a.temperature, seed=a.seed))
         eng.close()
         return 0
     if a.cmd == "random-model":

@@ -9,7 +9,7 @@ max_pos, tied, weight_bytes, kv_bytes_per_token`), the slot calls `prefill(slot,
 `prefill_logits`, `decode(B, steps)`, `history(slot, start, n)`, `logits(B)`, and `ValueError`
 for bad arguments (scripts/hipinfer.py:386-390). What is new beside them: `dtype`
 ("bfloat16" or "float32"), temperature sampling, requests through the scheduler
-(`add_request`, `step`, `run`), random weights, and `runner` for the step function itself.
+(`add_request`, `step`, `run`), many samples of one prompt (`sample_many`), random weights, and `runner` for the step function itself.
 
 `max_batch` is the most requests live at a time, `max_seq` the longest sequence, `max_prefill`
 the token budget of a step (the reference's prefill chunk, src/api.cu:1788).
@@ -224,6 +224,18 @@ class Engine:
         res = self.run()
         outs = [res[i] for i in ids]
         return outs if many else outs[0]
+
+    def sample_many(self, prompt: Sequence[int], n: int, n_new: int, temperature: float = 0.0, seed: int = 0, n_draft: int = 0,
+                    stop_token_ids: Sequence[int] = (), ignore_eos: bool = True, logprobs: bool = False):
+        """n continuations of one prompt, each of n_new tokens or up to a stop token. The prompt is run and kept once; with n_draft
+        a step runs up to that many tokens more per sample, looked up in its own text, and keeps those that the model would have
+        drawn. Returns the n lists of tokens; with `logprobs` also the n lists of their logarithms of probability (at temperature
+        1 for greedy samples). Temperature draws come from a generator seeded with `seed`, one after the other: they repeat for
+        equal arguments, and are other draws than generate()'s."""
+        from .samples import sample_many
+
+        call = sample_many(self, prompt, n, n_new, temperature, seed, n_draft, stop_token_ids, ignore_eos)
+        return (call.outputs, call.logprobs) if logprobs else call.outputs
 
     # ---------------------------------------------------------------- the reference's slot calls
     def _slot_ok(self, slot):

@@ -50,6 +50,7 @@ class StepBatch:
     max_q_len: int = 0
     extra: dict = field(default_factory=dict)  # what a kernel dispatcher derived for this batch (cached per step)
     short_list: Optional[torch.Tensor] = None  # int32: rows of requests with fewer than SHORT_ROWS rows, in a step with longer ones
+    shared: Sequence[list] = ()   # per cache group: (first request, requests, tokens) that hold the same pages (shared_prefixes)
     dump: Optional[dict] = None   # debug: planes of the step are recorded here, keyed (order index, name) (parts/planes.py)
     dump_step: int = -1           # the order index the decoder is at
 
@@ -64,6 +65,25 @@ class StepBatch:
                 rows = torch.from_numpy(_rows_of(short, self.h_q_start, self.h_q_len)).to(self.tokens.device)
             self.extra[key] = rows, max((self.h_ctx_len[r] + self.h_q_len[r] - 1 for r in short), default=0)
         return self.extra[key]
+
+
+def shared_prefixes(tables: Sequence[np.ndarray], ctx_lens: Sequence[int], page_size: int) -> list:
+    """(first request, requests, tokens) of neighbours whose block tables begin with the same pages, in whole pages that all of
+    them have filled. A neighbour joins the run before it if more keys are then read once for all than without it."""
+    out, first, pages = [], 0, 0
+    for r in range(1, len(tables) + 1):
+        common = 0
+        if r < len(tables) and len(tables[r]) and len(tables[first]) and tables[r][0] == tables[first][0] >= 0:
+            n = min(len(tables[r]), len(tables[first]), min(ctx_lens[first], ctx_lens[r]) // page_size)
+            differ = np.flatnonzero((tables[r][:n] != tables[first][:n]) | (tables[r][:n] < 0))
+            common = min(int(differ[0]) if len(differ) else n, pages if r - first > 1 else n)
+        if common * (r - first) > pages * (r - first - 1):
+            pages = common
+            continue
+        if r - first > 1:
+            out.append((first, r - first, pages * page_size))
+        first, pages = r, 0
+    return out
 
 
 SHORT_ROWS = 16     # portions of fewer rows are computed row by row (kernels/fast.py: FLASH_MIN_ROWS)

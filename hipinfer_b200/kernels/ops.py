@@ -808,6 +808,12 @@ def linear_deferred(a: torch.Tensor, w: Weight, out: torch.Tensor, accumulate: b
 
 def attention(q, k_cache, v_cache, batch, group: int, out, n_heads, n_kv_heads, head_dim, page_size, window, scale):
     """Attention of the step's rows over their requests' pages of cache group `group`."""
+    if window <= 0 and getattr(batch, "shared", ()) and batch.shared[group] and head_dim <= 256:
+        key = ("shared", group, n_heads, n_kv_heads, head_dim)       # requests that hold the same pages: one plan for the step's layers
+        if key not in batch.extra:
+            batch.extra[key] = SharedPlan(batch.h_q_len, batch.h_ctx_len, batch.shared[group], n_heads, n_kv_heads, head_dim, page_size,
+                                          q.dtype, q.device)
+        return attention_shared(q, k_cache, v_cache, batch.block_tables[group], batch.extra[key], out=out, scale=scale)
     if fast.attention(q, k_cache, v_cache, batch, group, out, n_heads, n_kv_heads, head_dim, page_size, window, scale):
         return out
     return attention_rows(q, k_cache, v_cache, batch.block_tables[group], batch.row_request, batch.positions, out,
@@ -1744,4 +1750,4 @@ def output_norm(x: torch.Tensor, y, weight: torch.Tensor, bias: Optional[torch.T
 
 
 # Attention over shared prefixes and the verification of drafted tokens (kernels/drafts.py)
-from .drafts import SharedPlan, attention_shared, verify_drafts  # noqa: E402,F401
+from .drafts import MAX_DRAFTS, SharedPlan, attention_shared, verify_drafts  # noqa: E402,F401
