@@ -260,71 +260,85 @@ __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, lo
   }
 }
 
-// E elements of a row of D from column c on as floats.
-template <int E, typename T> __device__ __forceinline__ void load_elements(const T* row, int c, int D, bool vec, float* x) {
-  if constexpr (E >= 4) {
+// E elements of a row of D from column c on as floats; FULL: a row is 32 E elements and starts on 16 bytes.
+template <int E, bool FULL, typename T> __device__ __forceinline__ void load_elements(const T* row, int c, int D, float* x) {
+  if constexpr (!FULL) {
+#pragma unroll
+    for (int i = 0; i < E; i++) x[i] = c + i < D ? hb_to_float(row[c + i]) : 0.f;
+  } else if constexpr (E >= 4) {
 #pragma unroll
     for (int i = 0; i < E; i += 4) {
-      const float4 v = row4(row, c + i, D, vec);
+      const float4 v = hb_load4(row + c + i);
       x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
     }
   } else {
-    if (vec && c + 2 <= D) {
-      if constexpr (sizeof(T) == 4) {
-        const float2 v = *(const float2*)(row + c);
-        x[0] = v.x; x[1] = v.y;
-      } else {
-        const float2 v = __bfloat1622float2(*(const __nv_bfloat162*)(row + c));
-        x[0] = v.x; x[1] = v.y;
-      }
-    } else {
-      x[0] = c < D ? hb_to_float(row[c]) : 0.f;
-      x[1] = c + 1 < D ? hb_to_float(row[c + 1]) : 0.f;
-    }
+    float2 v;
+    if constexpr (sizeof(T) == 4) v = *(const float2*)(row + c);
+    else v = __bfloat1622float2(*(const __nv_bfloat162*)(row + c));
+    x[0] = v.x; x[1] = v.y;
   }
 }
 
-constexpr int SJ_WARPS = 4, SJ_AHEAD = 8;
+constexpr int SJ_WARPS = 4;
+
+// Four sums over the warp at a time, all of them in every lane: a lane that halves what it sums also halves the shuffles.
+__device__ __forceinline__ void warp_sums(float* s, int lane) {
+  const bool hi = lane & 16, odd = lane & 8;
+  const float a0 = (hi ? s[2] : s[0]) + __shfl_xor_sync(0xffffffffu, hi ? s[0] : s[2], 16);
+  const float a1 = (hi ? s[3] : s[1]) + __shfl_xor_sync(0xffffffffu, hi ? s[1] : s[3], 16);
+  float c = (odd ? a1 : a0) + __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+#pragma unroll
+  for (int j = 0; j < 4; j++) s[j] = __shfl_sync(0xffffffffu, c, 8 * j);
+}
 
 // W warps per row of q and head (a block has SJ_WARPS); a lane has E columns. The parts go to the warps in turn, the keys of the step's own rows to
-// the last warp; W > 1: the warps' results meet in shared memory, in their order.
-template <typename T, int E, int W>
-__global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
-                                                                    const SharedToken* tokens, int T_rows, const float* part_o, const float2* part_ml, T* out,
-                                                                    int Hq, int Hkv, int D, int page_size, float scale_log2, int vec) {
+// the last warp; W > 1: the warps' results meet in shared memory, in their order. Latency is what it takes, a few loads that wait for one another:
+// the pages of all own keys are looked up at once, a lane a key, and parts are asked for before their weights are known. The own keys come ahead
+// of the wait for the items' kernel (behind_items: that one starts this one behind its own wait, when all they need is in place).
+template <typename T, int E, int W, bool FULL>
+__global__ void __launch_bounds__(SJ_WARPS * 32, E <= 4 ? 8 : 4) shared_join_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
+                                                                    const SharedToken* tokens, const float* part_o, const float2* part_ml, T* out, int Hq,
+                                                                    int Hkv, int G, int D, int page_size, float scale_log2, int behind_items) {
   __shared__ float2 sh_ml[SJ_WARPS];
   __shared__ float sh_acc[W > 1 ? SJ_WARPS : 1][W > 1 ? 32 * E : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % W, c = lane * E, G = Hq / Hkv;
-  const int u = blockIdx.x * (SJ_WARPS / W) + warp / W;
-  const bool some = u < T_rows * Hq;
-  const int t = some ? u / Hq : 0, head = some ? u % Hq : 0, h = head / G, g = head % G;
-  const SharedToken e = tokens[t];                   // (of the plan, as the block table: in place before the step's first kernel)
+  constexpr int AHEAD = W == 1 ? 4 : 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % W, c = lane * E;
+  const int t = blockIdx.x, head = blockIdx.y * (SJ_WARPS / W) + warp / W, h = head / G, g = head - h * G;
+  const bool some = head < Hq;
+  const SharedToken e = tokens[t];                   // (of the plan: in place before the step's first kernel)
   float m = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; i++) acc[i] = 0.f;
-  hb_pdl_wait();
-  hb_pdl_launch();
+  if (!behind_items) hb_pdl_wait();
 
   // the keys of the step's own rows
   if (some && mine == W - 1 && e.fresh > 0) {
+    static_assert(SP_FRESH <= 32, "a lane a key");
     float x[E];
-    load_elements<E>(q + (size_t)t * ldq + (size_t)head * D, c, D, vec, x);
+    load_elements<E, FULL>(q + (size_t)t * ldq + (size_t)head * D, c, D, x);
+    const int p = e.first + min(lane, e.fresh - 1);
+    const int page = p / page_size;
+    const long at = (((long)bt[(size_t)e.table * bt_stride + page] * Hkv + h) * page_size + (p - page * page_size)) * D;
     for (int j0 = 0; j0 < e.fresh; j0 += 4) {
-      float k[4][E], v[4][E];
+      float k[4][E], v[4][E], s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int p = e.first + min(j0 + j, e.fresh - 1);
-        const size_t row = ((size_t)bt[(size_t)e.table * bt_stride + p / page_size] * Hkv + h) * page_size + p % page_size;
-        load_elements<E>(kc + row * D, c, D, vec, k[j]);
-        load_elements<E>(vc + row * D, c, D, vec, v[j]);
+      for (int j = 0; j < 4; j++) {              // (the last key again behind it, without a branch)
+        const long row = __shfl_sync(0xffffffffu, at, j0 + j);
+        load_elements<E, FULL>(kc + row, c, D, k[j]);
+        load_elements<E, FULL>(vc + row, c, D, v[j]);
       }
-      float s[4], mx = m;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < E; i++) s[j] = fmaf(x[i], k[j][i], s[j]);
+      if (j0 + 1 < e.fresh) warp_sums(s, lane);
+      else s[0] = hb_warp_sum(s[0]);
+      float mx = m;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        float a = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; i++) a = fmaf(x[i], k[j][i], a);
-        s[j] = j0 + j < e.fresh ? hb_warp_sum(a) * scale_log2 : -INFINITY;
+        s[j] = j0 + j < e.fresh ? s[j] * scale_log2 : -INFINITY;
         mx = fmaxf(mx, s[j]);
       }
       const float sub = mx == -INFINITY ? 0.f : mx, corr = exp2_of(m - sub);
@@ -342,13 +356,23 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
         }
     }
   }
+  if (behind_items) hb_pdl_wait();
+  hb_pdl_launch();
 
   // this warp's parts, 32 at a time: a lane holds one's maximum and sum
   const int all = some ? e.pre_n + e.own_n : 0, n = (all - mine + W - 1) / W;
+  const int pre0 = e.pre_base + h * e.pre_n * e.pre_rows + g, own0 = e.own_base + (h * e.own_n - e.pre_n) * e.own_rows + g;
+  auto row_of = [&](int k) { return k < e.pre_n ? pre0 + k * e.pre_rows : own0 + k * e.own_rows; };
   for (int k0 = 0; k0 < n; k0 += 32) {
-    const int k = (k0 + lane) * W + mine;
-    const int row = k < e.pre_n ? e.pre_base + (h * e.pre_n + k) * e.pre_rows + g : e.own_base + (h * e.own_n + k - e.pre_n) * e.own_rows + g;
-    const float2 ml = k < all ? part_ml[row] : make_float2(-INFINITY, 0.f);
+    const int k = (k0 + lane) * W + mine, in = min(32, n - k0);
+    const float2 ml = k < all ? part_ml[row_of(k)] : make_float2(-INFINITY, 0.f);
+    float o[AHEAD][E];
+    auto ask = [&](int j0) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; j++)
+        load_elements<E, FULL>(part_o + (size_t)row_of((k0 + min(j0 + j, in - 1)) * W + mine) * D, c, D, o[j]);
+    };
+    ask(0);
     const float mx = hb_warp_max(fmaxf(ml.x, m)), sub = mx == -INFINITY ? 0.f : mx, corr = exp2_of(m - sub);
     // a part without a visible key has sum 0 and no output; one whose sum is NaN makes the row NaN
     const float w = ml.y == 0.f ? 0.f : ml.y != ml.y ? ml.y : exp2_of(ml.x - sub);
@@ -356,22 +380,16 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
     l = l * corr + hb_warp_sum(w == 0.f ? 0.f : w * ml.y);
 #pragma unroll
     for (int i = 0; i < E; i++) acc[i] *= corr;
-    const int in = min(32, n - k0);
-    for (int j0 = 0; j0 < in; j0 += SJ_AHEAD) {
-      float o[SJ_AHEAD][E], wj[SJ_AHEAD];
+    for (int j0 = 0; j0 < in; j0 += AHEAD) {
+      if (j0) ask(j0);
 #pragma unroll
-      for (int j = 0; j < SJ_AHEAD; j++) {
-        const int from = __shfl_sync(0xffffffffu, row, min(j0 + j, in - 1));
-        wj[j] = __shfl_sync(0xffffffffu, w, min(j0 + j, in - 1));
-        if (j0 + j >= in) wj[j] = 0.f;
-        if (wj[j] != 0.f) load_elements<E>(part_o + (size_t)from * D, c, D, vec, o[j]);
-      }
+      for (int j = 0; j < AHEAD; j++) {
+        const float wj = __shfl_sync(0xffffffffu, w, j0 + j);       // (0 behind the last part)
+        if (wj != 0.f) {
 #pragma unroll
-      for (int j = 0; j < SJ_AHEAD; j++)
-        if (wj[j] != 0.f) {
-#pragma unroll
-          for (int i = 0; i < E; i++) acc[i] = fmaf(wj[j], o[j][i], acc[i]);
+          for (int i = 0; i < E; i++) acc[i] = fmaf(wj, o[j][i], acc[i]);
         }
+      }
     }
   }
   if (W > 1) {
@@ -399,10 +417,9 @@ __global__ void __launch_bounds__(SJ_WARPS * 32) shared_join_kernel(const T* q, 
   T* dst = out + ((size_t)t * Hq + head) * D;
 #pragma unroll
   for (int i = 0; i < E; i++) acc[i] *= inv;
-  if (vec && E >= 4) {
+  if constexpr (FULL && E >= 4) {
 #pragma unroll
-    for (int i = 0; i < E; i += 4)
-      if (c + i < D) hb_store4(dst + c + i, make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]));
+    for (int i = 0; i < E; i += 4) hb_store4(dst + c + i, make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]));
   } else {
 #pragma unroll
     for (int i = 0; i < E; i++)
@@ -443,7 +460,7 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   if (D < 1 || D > 256 || ps < 1) HB_FAIL("hb_attention_shared: heads of %d (1 to 256 are supported), pages of %d", D, ps);
   if (T <= 0) return 0;
   const long warps = (long)T * Hq;
-  if (warps > (1l << 30)) HB_FAIL("hb_attention_shared: %d rows of %d heads are beyond the grid limit", T, Hq);
+  if (warps > (1l << 30) || Hq > 65535) HB_FAIL("hb_attention_shared: %d rows of %d heads are beyond the grid limit", T, Hq);
   if (h->parts > 0 && (!workspace || ((uintptr_t)workspace & 15))) HB_FAIL("hb_attention_shared: the workspace must be 16-byte aligned");
   float* part_o = workspace;
   float2* part_ml = (float2*)(workspace + ((long)h->parts * D + 3) / 4 * 4);
@@ -465,13 +482,14 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   cudaError_t e = cudaSuccess;
   // few rows of many parts: four warps share one's (8 rows x 32 heads of 34 parts 13 -> 8 us; 2,048 rows of 8 parts 5 us slower, beyond one round)
   const int W = warps > 1024 || h->parts < 6 * warps ? 1 : 4;
-#define SJ_LAUNCH(E, W)                                                                                                                          \
-  e = hb_launch(shared_join_kernel<TA, E, W>, dim3((unsigned)((warps * W + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq,      \
-                (const TA*)kc, (const TA*)vc, bt, bt_stride, tokens, T, part_o, part_ml, (TA*)out, Hq, Hkv, D, ps, sl2, vec)
-#define SJ_LAUNCH_W(E)               \
-  do {                               \
-    if (W == 1) SJ_LAUNCH(E, 1);     \
-    else SJ_LAUNCH(E, 4);            \
+#define SJ_LAUNCH(E, W, FULL)                                                                                                                    \
+  e = hb_launch(shared_join_kernel<TA, E, W, FULL>, dim3((unsigned)T, (unsigned)((Hq * W + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq, \
+                (const TA*)kc, (const TA*)vc, bt, bt_stride, tokens, part_o, part_ml, (TA*)out, Hq, Hkv, Hq / Hkv, D, ps, sl2, (int)(h->ctas > 0))
+#define SJ_LAUNCH_W(E)                                       \
+  do {                                                       \
+    if (!(aligned && D == 32 * E)) SJ_LAUNCH(E, 1, false);   \
+    else if (W == 1) SJ_LAUNCH(E, 1, true);                  \
+    else SJ_LAUNCH(E, 4, true);                              \
   } while (0)
   HB_DISPATCH_1(h->dt, "hb_attention_shared", { if (D <= 64) SJ_LAUNCH_W(2); else if (D <= 128) SJ_LAUNCH_W(4); else SJ_LAUNCH_W(8); });
 #undef SJ_LAUNCH

@@ -105,36 +105,50 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of the plan's rows over their requests' pages. q [T, Hq D] (rows may be part of wider ones); caches [page, Hkv, page_size, D]
     of the same type; block_table int32 [R, pages]; out [T, Hq D]; scale 1 / sqrt(D) by default. Scores, softmax and sums are 32-bit; the
     keys' cut, and with it a result's last bits, is a matter of the plan."""
+    width, dtype, T, pages = plan.n_heads * plan.head_dim, plan.dtype, plan.rows, k_cache.shape
     if not (q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and block_table.is_cuda):
         ops._need_cuda(q, k_cache, v_cache, block_table)
-    width, dtype, T = plan.n_heads * plan.head_dim, plan.dtype, plan.rows
-    if q.dim() != 2 or q.shape != plan.q_shape or q.dtype != dtype or q.stride(1) != 1:
+    if q.shape != plan.q_shape or q.dtype is not dtype or q.stride(1) != 1:
         raise ops.KernelError(f"attention_shared: q {tuple(q.shape)} {q.dtype}, strides {q.stride()}; the plan has {T} rows of {plan.n_heads} heads of "
                               f"{plan.head_dim}, {dtype}")
-    pages = k_cache.shape[0]
-    for name, x in (("keys", k_cache), ("values", v_cache)):
-        if x.shape != (pages, *plan.page_shape) or x.dtype != dtype or not x.is_contiguous():
-            raise ops.KernelError(f"attention_shared: {name} {tuple(x.shape)} {x.dtype}, {pages} pages of {plan.n_kv_heads} heads x {plan.page_size} tokens x "
-                                  f"{plan.head_dim}, {dtype}, are expected")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1 or block_table.shape[0] != plan.n_requests \
+    if not (pages == v_cache.shape and pages[1:] == plan.page_shape and k_cache.dtype is dtype and v_cache.dtype is dtype and k_cache.is_contiguous()
+            and v_cache.is_contiguous()):
+        raise ops.KernelError(f"attention_shared: keys {tuple(pages)} {k_cache.dtype}, values {tuple(v_cache.shape)} {v_cache.dtype}; {pages[0]} pages of "
+                              f"{plan.n_kv_heads} heads x {plan.page_size} tokens x {plan.head_dim}, {dtype}, are expected")
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.stride(1) != 1 or block_table.shape[0] != plan.n_requests \
             or block_table.shape[1] * plan.page_size < plan.most_keys:
         raise ops.KernelError(f"attention_shared: block table {tuple(block_table.shape)} {block_table.dtype}; the plan has {plan.n_requests} requests of up "
                               f"to {plan.most_keys} tokens in pages of {plan.page_size}")
     if out is None:
-        out = q.new_empty(T, width)
-    elif out.shape != plan.q_shape or out.dtype != dtype or not out.is_contiguous() or not out.is_cuda:
+        out = torch.empty(T, width, dtype=dtype, device=q.device)
+    elif out.shape != plan.q_shape or out.dtype is not dtype or not out.is_contiguous() or not out.is_cuda:
         ops._need_cuda(out)
         raise ops.KernelError(f"attention_shared: out {tuple(out.shape)} {out.dtype}, strides {out.stride()}")
     if not T:
         return out
-    ws = torch.empty(plan.workspace, dtype=torch.float32, device=q.device) if plan.parts else None
+    stream = library.current_stream()
+    ws = _scratch(plan.workspace, q.device, stream) if plan.parts else None
     qp, kp, vp, op, ld = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), q.stride(0)
     aligned = int((ld * plan.size) % 16 == 0 and (qp | kp | vp | op) % 16 == 0)
     library.launches[0] += plan.ctas > 0
-    ops._call("drafts", "hb_attention_shared", qp, ld, kp, vp, pages, block_table.data_ptr(), block_table.stride(0), plan.numbers.data_ptr(), plan.launch,
-              None if ws is None else ws.data_ptr(), op, plan.default_scale if scale is None else scale, aligned, ops.fast._status_ptr(),
-              library.current_stream())
+    ops._call("drafts", "hb_attention_shared", qp, ld, kp, vp, pages[0], block_table.data_ptr(), block_table.stride(0), plan.numbers.data_ptr(), plan.launch,
+              None if ws is None else ws.data_ptr(), op, plan.default_scale if scale is None else scale, aligned, ops.fast._status_ptr(), stream)
     return out
+
+
+_scratches = {}
+SCRATCH_KEPT = 1 << 22        # floats; a call that wants more takes longer than an allocation by far
+
+
+def _scratch(n: int, device, stream: int) -> torch.Tensor:
+    """At least n floats in which a call's kernels meet. Calls on one stream follow one another, so that they share what is kept for it (an
+    allocation is 1.7 us of a call's 15); a captured graph has its own, since it may be replayed beside them."""
+    if n > SCRATCH_KEPT or device.type != "cuda" or torch.cuda.is_current_stream_capturing():
+        return torch.empty(n, dtype=torch.float32, device=device)
+    ws = _scratches.get((device, stream))
+    if ws is None or ws.numel() < n:
+        ws = _scratches[device, stream] = torch.empty(min(SCRATCH_KEPT, 2 * n), dtype=torch.float32, device=device)
+    return ws
 
 
 def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Tensor, drafts: torch.Tensor, temperature: torch.Tensor,
@@ -151,7 +165,8 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
     Returns (tokens int32 [R, K + 1]: accepted drafts, the token behind them, -1; counts int32 [R]: how many tokens; logprobs float32 [R, K + 1]:
     log p_i of each, at temperature 1 for a greedy request, 0 for a row without a finite largest logit and behind the last). A request whose
     rows lie outside the logits gets no token."""
-    ops._need_cuda(logits, start, n_drafts, drafts, temperature, uniform, noise, draft_probs)
+    if not (logits.is_cuda and start.is_cuda and n_drafts.is_cuda and drafts.is_cuda and temperature.is_cuda and uniform.is_cuda and noise.is_cuda):
+        ops._need_cuda(logits, start, n_drafts, drafts, temperature, uniform, noise)
     if logits.dim() != 2 or drafts.dim() != 2:
         raise ops.KernelError(f"verify_drafts: logits {tuple(logits.shape)} and drafts {tuple(drafts.shape)}, [T, V] and [R, K] are expected")
     (T, V), (R, K) = logits.shape, drafts.shape
@@ -168,22 +183,26 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
         raise ops.KernelError(f"verify_drafts: noise {tuple(noise.shape)} {noise.dtype}, strides {noise.stride()}; float32 [{R}, {V}] is expected")
     probs = (None, 0, 0, 0)
     if draft_probs is not None:
+        ops._need_cuda(draft_probs)
         if draft_probs.shape != (R, K, V) or draft_probs.dtype not in ops._DT or (V > 1 and draft_probs.stride(2) != 1):
             raise ops.KernelError(f"verify_drafts: draft_probs {tuple(draft_probs.shape)} {draft_probs.dtype}, strides {draft_probs.stride()}; [{R}, {K}, {V}] "
                                   f"is expected")
         if K:
             probs = (draft_probs.data_ptr(), ops._DT[draft_probs.dtype], draft_probs.stride(0), draft_probs.stride(1))
     dt = ops._dt(logits)
-    tokens, counts, logprobs = drafts.new_empty((R, K + 1)), n_drafts.new_empty((R,)), uniform.new_empty((R, K + 1))
+    device = logits.device
+    tokens, counts = torch.empty(R, K + 1, dtype=torch.int32, device=device), torch.empty(R, dtype=torch.int32, device=device)
+    logprobs = torch.empty(R, K + 1, dtype=torch.float32, device=device)
     if not R:
         return tokens, counts, logprobs
     if not V:
         raise ops.KernelError("verify_drafts: empty vocabulary")
-    ws = noise.new_empty((_workspace(R, K, V, dt),))
+    stream = library.current_stream()
+    ws = _scratch(_workspace(R, K, V, dt), device, stream)
     library.launches[0] += 1
     ops._call("drafts", "hb_verify_drafts", logits.data_ptr(), dt, logits.stride(0), T, V, start.data_ptr(), n_drafts.data_ptr(), drafts.data_ptr(), R, K,
               temperature.data_ptr(), uniform.data_ptr(), noise.data_ptr(), noise.stride(0), *probs, ws.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
-              logprobs.data_ptr(), library.current_stream())
+              logprobs.data_ptr(), stream)
     return tokens, counts, logprobs
 
 
