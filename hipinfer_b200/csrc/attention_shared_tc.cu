@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int ST_ROWS = 128, ST_KEYS = 128, ST_THREADS = 384;
+constexpr int ST_ROWS = 128, ST_KEYS = 128, ST_THREADS = 384, ST_KEPT = 64;
 constexpr float ST_SLACK = 8.f;
 
 template <int D> struct StSizes {
@@ -33,7 +33,7 @@ template <int D> struct StBars {
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];      // [chain][step & 1]
   uint32_t tmem_slot;
   int abort_flag;
-  alignas(16) SharedItem kept[64];
+  alignas(16) SharedItem kept[ST_KEPT];
 };
 template <int D> constexpr int st_smem() { return (2 + StSizes<D>::NK + StSizes<D>::NV) * StSizes<D>::OPND + (int)sizeof(StBars<D>); }
 static_assert(st_smem<128>() <= 227 * 1024 && st_smem<64>() <= 227 * 1024, "shared memory of a block");
@@ -61,6 +61,11 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void ld32_fence(uint32_t* r) { asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory"); }
 __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+// 16 lanes by 64 columns: of each eight columns a thread has two neighbours (2 (lane % 4)) of rows lane / 4 and lane / 4 + 8.
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(taddr));
 }
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
   uint64_t r;
@@ -124,16 +129,41 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatil
   return hb_mbar_try_wait(bar, parity) || wait_longer(bar, parity, abort);
 }
 
+// A warp's rows of O from tensor memory to `dst`, the first n of 32. A store of a thread's own row would touch 32 lines of 128 bytes (256 rows of
+// 128 took 9,500 cycles): here four threads have 64 bytes of a row, neighbours having swapped two columns of eight for two of the next eight.
+template <int D> __device__ __noinline__ void store_rows(uint32_t tmem_o, float* dst, int n) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, odd = lane & 1;
+  dst += r * D + 8 * odd + 4 * (lane >> 1 & 1);
+  for (int half = 0; half < 2 && 16 * half < n; half++) {
+#pragma unroll 1
+    for (int q = 0; q < D / 64; q++) {
+      uint32_t o[32];
+      ld16(tmem_o + ((uint32_t)(16 * half) << 16) + q * 64, o);
+      hb_tmem_ld_wait();
+      ld32_fence(o);
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)          // two eights of columns
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {       // the thread's two rows
+          const uint32_t x0 = __shfl_xor_sync(0xffffffffu, odd ? o[i + k] : o[i + 4 + k], 1);
+          const uint32_t x1 = __shfl_xor_sync(0xffffffffu, odd ? o[i + k + 1] : o[i + 5 + k], 1);
+          const uint4 v = odd ? make_uint4(x0, x1, o[i + 4 + k], o[i + 5 + k]) : make_uint4(o[i + k], o[i + k + 1], x0, x1);
+          if (r + 16 * half + 4 * k < n) *(uint4*)(dst + (16 * half + 4 * k) * D + q * 64 + 2 * i) = v;
+        }
+    }
+  }
+}
+
 // The CTA's items: the first ST_KEPT of them are in shared memory.
-constexpr int ST_KEPT = 64;
 struct Items {
   const SharedItem *kept, *all;
-  int n, tokens_a_chain;
+  int n, tokens_a_chain, tokens_low;
 };
 struct Work {      // an item as the roles go through it
   SharedItem e;
   int kt0, tiles;  // its key tiles
   bool wide;       // a chain has half of the rows (else half of a tile's keys)
+  bool low;        // at most 64 rows: chain 1 has them in its rows 64 .., so that the two chains' warps are not of the same schedulers
 };
 __device__ __forceinline__ Work work_of(const Items& items, int it) {
   Work w;
@@ -143,6 +173,7 @@ __device__ __forceinline__ Work work_of(const Items& items, int it) {
   w.kt0 = w.e.lo / ST_KEYS;
   w.tiles = (w.e.hi - 1) / ST_KEYS - w.kt0 + 1;
   w.wide = w.e.tokens > items.tokens_a_chain;
+  w.low = w.e.tokens <= items.tokens_low;
   return w;
 }
 
@@ -154,7 +185,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
   using S = StSizes<D>;
   constexpr int NH = D / 64, TILE = S::TILE, OPND = S::OPND, NK = S::NK, NV = S::NV;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t *sQ = smem, *sK = sQ + 2 * OPND, *sV = sK + NK * OPND;
+  uint8_t *sK = smem, *sQ = sK + NK * OPND, *sV = sQ + 2 * OPND;      // (chain 1 of a low item reads 64 rows from below Q: K, whatever is there)
   StBars<D>* bar = (StBars<D>*)(sV + NV * OPND);
   volatile int* abort_flag = &bar->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -180,9 +211,9 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
     hb_tmem_alloc(&bar->tmem_slot, 512);
     hb_tmem_relinquish();
   }
-  // (the plan and the block tables are copied before the step's first kernel begins: they may be read ahead of the wait)
+  // (the plan is copied before the step's first kernel begins: it may be read ahead of the wait; block tables are read behind it)
   const int it0 = ctas[blockIdx.x], RT = ST_ROWS / G;
-  Items items = {bar->kept, plan_items + it0, ctas[blockIdx.x + 1] - it0, RT};
+  Items items = {bar->kept, plan_items + it0, ctas[blockIdx.x + 1] - it0, RT, 64 / G};
   for (int i = threadIdx.x; i < 2 * min(items.n, ST_KEPT); i += ST_THREADS) ((int4*)bar->kept)[i] = ((const int4*)items.all)[i];
   hb_tc_fence_before();
   __syncthreads();
@@ -264,7 +295,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
       // the stage's use.
       struct At {
         int it, tile, tiles;
-        uint32_t wide, half, stage, parity;
+        uint32_t wide, half, stage, parity, below;
       };
       auto item = [&](At& a) {
         const Work w = work_of(items, a.it);
@@ -272,6 +303,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
         a.tiles = w.tiles;
         a.wide = w.wide;
         a.half = w.wide ? 0 : c;
+        a.below = w.low && c ? 64 * 128 >> 4 : 0;
       };
       auto next = [&](At& a, uint32_t stages) {
         if (a.wide && a.half == 0) {
@@ -282,7 +314,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
         a.half = a.wide ? 0 : c;
         if (++a.tile == a.tiles && ++a.it < items.n) item(a);
       };
-      At s = {0, 0, 0, 0, 0, 0, 0}, o;
+      At s = {0, 0, 0, 0, 0, 0, 0, 0}, o;
       item(s);
       o = s;
       uint32_t q_parity = 0, qb = 0;               // of the two Q buffers as bits; the narrow items' buffer
@@ -296,7 +328,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
                         (s.tile > 0 || (is_over(&bar->q_full[b], q_parity >> b & 1) && (!s.wide || is_over(&bar->q_full[b ^ 1], q_parity >> (b ^ 1) & 1))))))) {
           if (s.tile == 0 && first) q_parity ^= s.wide ? 3u : 1u << b;
           hb_tc_fence_after();
-          const uint64_t dq = q_desc + b * (OPND >> 4), dk = k_desc + s.stage * (OPND >> 4) + s.half * (64 * 128 >> 4);
+          const uint64_t dq = q_desc + b * (OPND >> 4) - s.below, dk = k_desc + s.stage * (OPND >> 4) + s.half * (64 * 128 >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk++)     // 16 columns a step: four steps in each 64-column tile
             hb_umma_bf16(tmem_s + (ms & 1) * 64, dq + (kk >> 2) * (TILE >> 4) + 2 * (kk & 3), dk + (kk >> 2) * (TILE >> 4) + 2 * (kk & 3), idesc_s, kk != 0);
@@ -335,18 +367,18 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
     }
   }
   } else {  // ---------------- softmax: warpgroup c is chain c, a thread a query row
-    const int c = warp >> 2, w4 = warp & 3, r = threadIdx.x & 127;
+    const int c = warp >> 2, w4 = warp & 3;
     const uint32_t lanes = (uint32_t)(w4 * 32) << 16, tmem_s = tmem + c * 128 + lanes, tmem_o = tmem + 256 + c * 128 + lanes;
     uint32_t m = 0, v_stage = 0, v_parity = 0;       // steps; where V is
     bool ok = true;                // every wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide
     auto wait = [&](uint64_t* b, uint32_t parity) { return ok = __all_sync(0xffffffffu, wait_for(b, parity, abort_flag)); };
     const uint64_t scale2 = pack2(scale_log2, scale_log2);
-    const int token = r / G;       // the row's, counted from the chain's first
     for (int it = 0; it < items.n && ok; it++) {
       const Work w = work_of(items, it);
       const int first = w.wide ? c * RT : 0, rows = min(RT, w.e.tokens - first) * G;           // the chain's rows
-      const bool idle = w4 * 32 >= rows;
-      const int last_key = min(w.e.hi - 1, w.e.pos == SP_NO_MASK ? SP_NO_MASK : w.e.pos + first + token);
+      const int below = w.low && c ? 64 : 0, r = (int)(threadIdx.x & 127) - below;      // the thread's row of the chain's
+      const bool idle = w4 * 32 < below || w4 * 32 - below >= rows;
+      const int last_key = min(w.e.hi - 1, w.e.pos == SP_NO_MASK ? SP_NO_MASK : w.e.pos + first + r / G);
       const int sure = w.e.pos == SP_NO_MASK ? w.e.hi : min(w.e.hi, w.e.pos + first + 1);      // the keys below are seen by all rows
       float m_run = -INFINITY, l_run = 0.f;
       const uint32_t m0 = m;
@@ -359,10 +391,10 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
           hb_tc_fence_after();
           const bool cut = k_base < w.e.lo || k_base + 64 > w.e.hi;
           if (cut) {      // the rows of V, of the step's keys, where the item does not reach: a thread has half of one
-            const int row = 64 * h + (r >> 1);
+            const int row = 64 * h + ((threadIdx.x & 127) >> 1);
             if (!wait(&bar->v_full[v_stage], v_parity)) break;
             if (tile + row < w.e.lo || tile + row >= w.e.hi) {
-              const uint32_t dst = hb_smem_u32(sV + v_stage * OPND) + row * 128 + (r & 1) * (D == 128 ? TILE : 64);
+              const uint32_t dst = hb_smem_u32(sV + v_stage * OPND) + row * 128 + (threadIdx.x & 1) * (D == 128 ? TILE : 64);
 #pragma unroll
               for (int q = 0; q < D / 16; q++)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + q * 16), "r"(0) : "memory");
@@ -446,20 +478,9 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
       const size_t part = (size_t)w.e.part + (w.wide ? c * RT * G : c * rows);
       if (!wait(&bar->pv_done[c][(m - 1) & 1], (m - 1) >> 1 & 1)) break;
       hb_tc_fence_after();
-      if (r < rows) part_ml[part + r] = make_float2(m_run, l_run);
+      if (r >= 0 && r < rows) part_ml[part + r] = make_float2(m_run, l_run);
       if (!idle) {
-        float* dst = part_o + (part + r) * D;
-#pragma unroll
-        for (int q = 0; q < D / 32; q++) {
-          uint32_t o[32];
-          ld32(tmem_o + q * 32, o);
-          hb_tmem_ld_wait();
-          ld32_fence(o);
-          if (r < rows) {
-#pragma unroll
-            for (int d = 0; d < 32; d += 4) *(uint4*)(dst + q * 32 + d) = make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-          }
-        }
+        store_rows<D>(tmem_o, part_o + (part + w4 * 32 - below) * D, rows - (w4 * 32 - below));
         hb_tc_fence_before();
       }
     }
