@@ -154,6 +154,20 @@ template <int D> __device__ __noinline__ void store_rows(uint32_t tmem_o, float*
   }
 }
 
+// This thread's row of O times `by`.
+template <int D> __device__ __noinline__ void scale_rows(uint32_t tmem_o, float by) {
+#pragma unroll 1
+  for (int q = 0; q < D / 32; q++) {
+    uint32_t o[32];
+    ld32(tmem_o + q * 32, o);
+    hb_tmem_ld_wait();
+    ld32_fence(o);
+#pragma unroll
+    for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * by);
+    st32(tmem_o + q * 32, o);
+  }
+}
+
 // The CTA's items: the first ST_KEPT of them are in shared memory.
 struct Items {
   const SharedItem *kept, *all;
@@ -426,16 +440,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
               if (m > m0) {       // the rows of O so far
                 if (!wait(&bar->pv_done[c][(m - 1) & 1], (m - 1) >> 1 & 1)) break;
                 hb_tc_fence_after();
-#pragma unroll
-                for (int q = 0; q < D / 32; q++) {
-                  uint32_t o[32];
-                  ld32(tmem_o + q * 32, o);
-                  hb_tmem_ld_wait();
-                  ld32_fence(o);
-#pragma unroll
-                  for (int d = 0; d < 32; d++) o[d] = __float_as_uint(__uint_as_float(o[d]) * corr);
-                  st32(tmem_o + q * 32, o);
-                }
+                scale_rows<D>(tmem_o, corr);
               }
             }
             const float sub = m_run == -INFINITY ? 0.f : m_run;
