@@ -102,8 +102,8 @@ __device__ __forceinline__ RowPart warp_join(u64 key, float sum, float c) {
   return r;
 }
 
-// A row is some elements up to its first 16-byte boundary (a row of an odd vocabulary starts anywhere), whole vectors, of which a slice has up to
-// U * VD_THREADS, and some elements more.
+// A row is some elements up to its first 16-byte boundary (a row of an odd vocabulary starts anywhere), whole vectors, of which a slice has
+// U * VD_THREADS (the last one what is left), and some elements more.
 template <typename T, int U>
 __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const T* logits, long ld, int T_rows, int V, const int* start, const int* n_drafts, int K,
                                                                  const float* temperature, RowPart* parts, int slices) {
@@ -116,9 +116,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const T* logits
   const int row = start[r] + i;
   if (i > clamped(n_drafts[r], K) || row < 0 || row >= T_rows) return;
   const T* x = logits + (size_t)row * ld;
-  // `head` elements, n whole vectors, and the rest; of the vectors this thread has lo, lo + VD_THREADS, .. below hi
-  const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), n = (V - head) / N, share = (n + slices - 1) / slices;
-  const int lo = s * share + (int)threadIdx.x, hi = min(n, (s + 1) * share);
+  // `head` elements, n whole vectors, and the rest; of the vectors this thread has U at most: lo, lo + VD_THREADS, .. below hi
+  const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), n = (V - head) / N;
+  const int lo = s * U * VD_THREADS + (int)threadIdx.x, hi = n;
   const uint4* vec = (const uint4*)(x + head) + lo;
   uint4 raw[U];
 #pragma unroll
@@ -268,14 +268,16 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
       const int skip = attempt < 2 && taken < n && !probs ? s.d - begin : VD_NONE;      // (places from `begin` on)
       auto walk = [&](auto flag, auto unroll) {
         constexpr bool WITH_Q = decltype(flag)::value;
-        constexpr int U = decltype(unroll)::value;
+        constexpr int U = decltype(unroll)::value, STEP = U * VP_THREADS;
         const T* xp = x + begin;
         const Q* qp = q + begin;
-        for (int k = threadIdx.x; k < end - begin; k += U * VP_THREADS) {
+        const int all = end - begin;
+        auto chunk = [&](int k, auto whole) {           // U candidates a thread, all of them there or not
+          constexpr bool WHOLE = decltype(whole)::value;
           float xs[U], qs[U];
 #pragma unroll
           for (int u = 0; u < U; u++) {
-            const bool in = k < end - begin - u * VP_THREADS;
+            const bool in = WHOLE || k < all - u * VP_THREADS;
             xs[u] = -INFINITY;
             qs[u] = 0.f;
             if (in) xs[u] = hb_to_float(xp[k + u * VP_THREADS]);
@@ -293,11 +295,16 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
               at = k + u * VP_THREADS;
             }
           }
-          if (U > 1)
+        };
+        int k = threadIdx.x, from = 0;
+        for (; U > 1 && from + STEP <= all; from += STEP, k += STEP) {
+          chunk(k, std::true_type());
+          const bool more = from + 2 * STEP <= all;
 #pragma unroll
-            for (int u = 0; u < U; u++)
-              if (k < end - begin - (u + U) * VP_THREADS) es[u] = e[begin + k + (u + U) * VP_THREADS];
+          for (int u = 0; u < U; u++)
+            if (more || k < all - STEP - u * VP_THREADS) es[u] = e[begin + k + STEP + u * VP_THREADS];
         }
+        for (; k < all; k += STEP) chunk(k, std::false_type());
       };
       if (attempt == 0 && dist) walk(std::true_type(), std::integral_constant<int, VP_U>());
       else if (attempt == 0) walk(std::false_type(), std::integral_constant<int, VP_U>());
@@ -335,13 +342,14 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
   if (lane == 0) counts[r] = any ? taken + 1 : 0;
 }
 
-// The cut: U vectors a thread (four where that leaves blocks for all SMs; few rows are cut finer), and CTAs a request for the last token, up to 16 of
+// The cut: U vectors a thread (32 elements where that leaves blocks for all SMs, 64 of bfloat16 would take
+// the registers of half of the warps; few rows are cut finer), and CTAs a request for the last token, up to 16 of
 // at least 1,024 candidates.
 struct Cut { int u, slices, ranks; };
 Cut cut(int V, int dt, int R, int K) {
   const int n = V / (dt == HB_BF16 ? 8 : 4);
   Cut c;
-  for (c.u = 4; c.u > 1; c.u >>= 1)
+  for (c.u = dt == HB_BF16 ? 4 : 8; c.u > 1; c.u >>= 1)
     if ((long)R * (K + 1) * (n / (c.u * VD_THREADS)) >= 4 * 148) break;
   c.slices = n / (c.u * VD_THREADS) + 1;
   c.ranks = 1;
@@ -389,7 +397,7 @@ HB_EXPORT int hb_verify_drafts(const void* logits, int dt, long ld, int T_rows, 
   cudaError_t e = cudaSuccess;
 #define VD_LAUNCH_ROWS(U) e = hb_launch(verify_rows_kernel<TA, U>, dim3(k.slices, K + 1, R), VD_THREADS, 0, s, (const TA*)logits, ld, T_rows, V, start, \
                                         n_drafts, K, temperature, parts, k.slices)
-  HB_DISPATCH_1(dt, "hb_verify_drafts", { if (k.u == 4) VD_LAUNCH_ROWS(4); else if (k.u == 2) VD_LAUNCH_ROWS(2); else VD_LAUNCH_ROWS(1); });
+  HB_DISPATCH_1(dt, "hb_verify_drafts", { if (k.u == 8 && sizeof(TA) == 4) VD_LAUNCH_ROWS(sizeof(TA) == 4 ? 8 : 4); else if (k.u == 4) VD_LAUNCH_ROWS(4); else if (k.u == 2) VD_LAUNCH_ROWS(2); else VD_LAUNCH_ROWS(1); });
 #undef VD_LAUNCH_ROWS
   if (e != cudaSuccess) HB_FAIL("hb_verify_drafts: %s", cudaGetErrorString(e));
   HB_DISPATCH_2(dt, probs ? probs_dt : HB_F32, "hb_verify_drafts",
