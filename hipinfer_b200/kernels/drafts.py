@@ -94,6 +94,11 @@ class SharedPlan:
             host = host.pin_memory()
         self.numbers = host.to(self.device, non_blocking=True)
         self._host = host                     # until the copy is over
+        # as the binding reads it (Plan in csrc/drafts_binding.cpp)
+        self._native = np.array([self.rows, n_heads * head_dim, n_kv_heads, page_size, head_dim, ops._DT[dtype], self.n_requests, self.most_keys,
+                                 self.workspace if self.parts else 0, self.ctas, self.numbers.data_ptr(), self.launch, 0], dtype=np.int64)
+        self._native[12:].view(np.float64)[0] = self.default_scale
+        self.native = self._native.ctypes.data
 
 
 def _sms(device) -> int:
@@ -105,6 +110,12 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of the plan's rows over their requests' pages. q [T, Hq D] (rows may be part of wider ones); caches [page, Hkv, page_size, D]
     of the same type; block_table int32 [R, pages]; out [T, Hq D]; scale 1 / sqrt(D) by default. Scores, softmax and sums are 32-bit; the
     keys' cut, and with it a result's last bits, is a matter of the plan."""
+    if q.is_cuda:
+        bound = _binding() if _bound is None else _bound
+        if bound:
+            result = bound.attend(q, k_cache, v_cache, block_table, plan.native, out, scale, ops.fast._status_ptr())
+            if result is not None:
+                return _done(result, 1 + (plan.ctas > 0))
     width, dtype, T, pages = plan.n_heads * plan.head_dim, plan.dtype, plan.rows, k_cache.shape
     if not (q.is_cuda and k_cache.is_cuda and v_cache.is_cuda and block_table.is_cuda):
         ops._need_cuda(q, k_cache, v_cache, block_table)
@@ -126,29 +137,36 @@ def attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ops.KernelError(f"attention_shared: out {tuple(out.shape)} {out.dtype}, strides {out.stride()}")
     if not T:
         return out
-    stream = library.current_stream()
-    ws = _scratch(plan.workspace, q.device, stream) if plan.parts else None
+    ws = torch.empty(plan.workspace, dtype=torch.float32, device=q.device) if plan.parts else None
     qp, kp, vp, op, ld = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), q.stride(0)
     aligned = int((ld * plan.size) % 16 == 0 and (qp | kp | vp | op) % 16 == 0)
     library.launches[0] += plan.ctas > 0
     ops._call("drafts", "hb_attention_shared", qp, ld, kp, vp, pages[0], block_table.data_ptr(), block_table.stride(0), plan.numbers.data_ptr(), plan.launch,
-              None if ws is None else ws.data_ptr(), op, plan.default_scale if scale is None else scale, aligned, ops.fast._status_ptr(), stream)
+              None if ws is None else ws.data_ptr(), op, plan.default_scale if scale is None else scale, aligned, ops.fast._status_ptr(),
+              library.current_stream())
     return out
 
 
-_scratches = {}
-SCRATCH_KEPT = 1 << 22        # floats; a call that wants more takes longer than an allocation by far
+_bound = None
 
 
-def _scratch(n: int, device, stream: int) -> torch.Tensor:
-    """At least n floats in which a call's kernels meet. Calls on one stream follow one another, so that they share what is kept for it (an
-    allocation is 1.7 us of a call's 15); a captured graph has its own, since it may be replayed beside them."""
-    if n > SCRATCH_KEPT or device.type != "cuda" or torch.cuda.is_current_stream_capturing():
-        return torch.empty(n, dtype=torch.float32, device=device)
-    ws = _scratches.get((device, stream))
-    if ws is None or ws.numel() < n:
-        ws = _scratches[device, stream] = torch.empty(min(SCRATCH_KEPT, 2 * n), dtype=torch.float32, device=device)
-    return ws
+def _binding():
+    """The binding (csrc/drafts_binding.cpp), at the addresses of the library's calls; False where it cannot be had."""
+    global _bound
+    lib, module = library.load("drafts"), library.load_binding("drafts")
+    if module is not None:
+        module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value
+                      for name in ("hb_attention_shared", "hb_verify_drafts", "hb_verify_drafts_workspace")))
+    _bound = module or False
+    return _bound
+
+
+def _done(result, launches: int):
+    """What a call through the binding gave."""
+    if result.__class__ is int:
+        raise ops.KernelError(library.load("drafts").hb_last_error().decode())
+    library.launches[0] += launches
+    return result
 
 
 def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Tensor, drafts: torch.Tensor, temperature: torch.Tensor,
@@ -165,8 +183,13 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
     Returns (tokens int32 [R, K + 1]: accepted drafts, the token behind them, -1; counts int32 [R]: how many tokens; logprobs float32 [R, K + 1]:
     log p_i of each, at temperature 1 for a greedy request, 0 for a row without a finite largest logit and behind the last). A request whose
     rows lie outside the logits gets no token."""
-    if not (logits.is_cuda and start.is_cuda and n_drafts.is_cuda and drafts.is_cuda and temperature.is_cuda and uniform.is_cuda and noise.is_cuda):
-        ops._need_cuda(logits, start, n_drafts, drafts, temperature, uniform, noise)
+    if logits.is_cuda:
+        bound = _binding() if _bound is None else _bound
+        if bound:
+            result = bound.verify(logits, start, n_drafts, drafts, temperature, uniform, noise, draft_probs)
+            if result is not None:
+                return _done(result, 2)
+    ops._need_cuda(logits, start, n_drafts, drafts, temperature, uniform, noise, draft_probs)
     if logits.dim() != 2 or drafts.dim() != 2:
         raise ops.KernelError(f"verify_drafts: logits {tuple(logits.shape)} and drafts {tuple(drafts.shape)}, [T, V] and [R, K] are expected")
     (T, V), (R, K) = logits.shape, drafts.shape
@@ -183,7 +206,6 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
         raise ops.KernelError(f"verify_drafts: noise {tuple(noise.shape)} {noise.dtype}, strides {noise.stride()}; float32 [{R}, {V}] is expected")
     probs = (None, 0, 0, 0)
     if draft_probs is not None:
-        ops._need_cuda(draft_probs)
         if draft_probs.shape != (R, K, V) or draft_probs.dtype not in ops._DT or (V > 1 and draft_probs.stride(2) != 1):
             raise ops.KernelError(f"verify_drafts: draft_probs {tuple(draft_probs.shape)} {draft_probs.dtype}, strides {draft_probs.stride()}; [{R}, {K}, {V}] "
                                   f"is expected")
@@ -197,12 +219,11 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
         return tokens, counts, logprobs
     if not V:
         raise ops.KernelError("verify_drafts: empty vocabulary")
-    stream = library.current_stream()
-    ws = _scratch(_workspace(R, K, V, dt), device, stream)
+    ws = torch.empty(_workspace(R, K, V, dt), dtype=torch.float32, device=device)
     library.launches[0] += 1
     ops._call("drafts", "hb_verify_drafts", logits.data_ptr(), dt, logits.stride(0), T, V, start.data_ptr(), n_drafts.data_ptr(), drafts.data_ptr(), R, K,
               temperature.data_ptr(), uniform.data_ptr(), noise.data_ptr(), noise.stride(0), *probs, ws.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
-              logprobs.data_ptr(), stream)
+              logprobs.data_ptr(), library.current_stream())
     return tokens, counts, logprobs
 
 

@@ -7,6 +7,10 @@ file beside the .so holds their hash); what is compiled is only what was asked f
 files live in `hipinfer_b200/_lib/`; when that folder cannot be written they go to a
 per-user folder under the system's temporary directory. While nvcc runs, a line is printed
 now and then. There is no fallback: without the library every operation raises.
+
+A BINDING is a Python module of C++ that calls such a library for operations whose host time matters (no interpreter between
+the checks, the allocations and the launches). It is built with the host compiler against torch's headers; where they or the
+compiler are missing, that is said once and the operation goes through ctypes as the others do.
 """
 from __future__ import annotations
 
@@ -38,6 +42,10 @@ LIBRARIES: Dict[str, List[str]] = {
     "fast": ["fast_entry.cu", "gemm_tc.cu", "gemm_stream.cu", "gemm_stream_consumers.cu", "gemm_rows.cu", "gemm_split.cu", "attention_fast.cu", "attention_prefill.cu", "attention_prefill_tc.cu", "attention_diff_tc.cu", "wait_selftest.cu"],
 }
 HEADERS = ["common.cuh", "tc_common.cuh", "gemm_stream_static.h", "shared_plan.h"]
+
+
+# binding name -> its source; the module is called hipinfer_b200_<name>_binding
+BINDINGS: Dict[str, str] = {"drafts": "drafts_binding.cpp"}
 
 
 class KernelLibraryError(RuntimeError):
@@ -168,7 +176,61 @@ def load(name: str) -> ctypes.CDLL:
 
 
 def build_all(verbose: bool = True) -> List[str]:
-    return [build(n, verbose) for n in LIBRARIES]
+    return [build(n, verbose) for n in LIBRARIES] + [build_binding(n, verbose) for n in BINDINGS]
+
+
+def build_binding(name: str, verbose: bool = True) -> str:
+    """Path of the up-to-date binding `name`, compiling it if need be."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    source = os.path.join(CSRC, BINDINGS[name])
+    libs = cpp_extension.library_paths()
+    python = sysconfig.get_paths()["include"]
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    with open(source, "rb") as f:
+        stamp = hashlib.sha256(" ".join(flags + [torch.__version__, sys.version, python] + libs).encode() + f.read()).hexdigest()
+    so = _find_fresh(f"{name}_binding", stamp)
+    if so:
+        return so
+    compiler = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not compiler:
+        raise KernelLibraryError("no host C++ compiler was found (PATH, $CXX)")
+    out_dir = _writable_dir()
+    so = os.path.join(out_dir, f"libhipinfer_b200_{name}_binding.so")
+    tmp = os.path.join(out_dir, f".libhipinfer_b200_{name}_binding.{os.getpid()}.so")
+    includes = cpp_extension.include_paths() + [python, os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")]
+    cmd = ([compiler] + flags + [x for d in includes for x in ("-isystem", d)] + ["-o", tmp, source] + [f"-L{d}" for d in libs]
+           + [f"-Wl,-rpath,{d}" for d in libs] + ["-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
+    t0 = time.time()
+    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if proc.returncode != 0:
+        raise KernelLibraryError(f"the host compiler failed for binding '{name}':\n{' '.join(cmd)}\n{proc.stdout[-4000:]}")
+    os.replace(tmp, so)
+    with open(os.path.join(out_dir, f"libhipinfer_b200_{name}_binding.stamp"), "w") as f:
+        f.write(stamp)
+    if verbose:
+        _say(f"compiled binding '{name}' in {time.time() - t0:.0f} s -> {so}")
+    return so
+
+
+def load_binding(name: str):
+    """The module of binding `name` (built first if stale), or None where it cannot be had."""
+    import importlib.machinery
+    import importlib.util
+
+    with _lock:
+        try:
+            module = f"hipinfer_b200_{name}_binding"
+            loader = importlib.machinery.ExtensionFileLoader(module, build_binding(name))
+            found = importlib.util.module_from_spec(importlib.util.spec_from_loader(module, loader))
+            loader.exec_module(found)
+            return found
+        except (KernelLibraryError, ImportError, OSError) as e:
+            _say(f"binding '{name}' is not there, its operations go through ctypes: {e}")
+            return None
 
 
 _raw_stream = None
