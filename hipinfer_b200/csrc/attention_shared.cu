@@ -5,10 +5,10 @@
 //   ranges are joined as o = sum_A 2^(m_A - m) o_A / sum_A 2^(m_A - m) l_A, m = max m_A.
 //
 // shared_items_kernel leaves (m, l) and o of every item's rows in the workspace; any head size up to 256, page size and group, both element
-// types: 16 or 64 rows a block by 64 keys a tile, products on the FMA pipe, everything widened to 32 bits in shared memory. bfloat16 heads of
-// 64 and 128 go to the tensor cores instead (attention_shared_tc.cu).
-// shared_join_kernel, one or four warps per row and head, adds the keys of the step's own rows (a row sees those up to itself, so that the items need no mask) and
-// joins the parts in a fixed order: the same plan and inputs give the same bits.
+// types: 64 rows by 64 keys a tile in shared memory, or up to 16 rows without one; products on the FMA pipe, all numbers widened to 32 bits.
+// bfloat16 heads of 64 and 128 go to the tensor cores instead (attention_shared_tc.cu).
+// shared_join_kernel, one or four warps per row and head, adds the keys of the step's own rows (a row sees those up to itself, so that the
+// items need no mask) and joins the parts in a fixed order: the same plan and inputs give the same bits.
 #include "common.cuh"
 #include "shared_plan.h"
 
@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int SI_KEYS = 64, SI_THREADS = 256;
+constexpr int SI_KEYS = 64, SI_THREADS = 256, SI_FEW = 16;      // (rows: also in kernels/drafts.py)
 
 __device__ __forceinline__ float exp2_of(float x) { return exp2f(x); }
 
@@ -56,15 +56,14 @@ template <int NC> struct ItemsShared {
   static constexpr int BYTES = (64 * LD + 2 * STAGES * TILE + 64 * LP) * 4 + 2 * SI_KEYS * 8;
 };
 
-// A block of up to 16 RM rows of an item. A thread has RM rows (ty RM ..) by four keys (tx, tx + 16, ..) of the scores, and RM rows by 4 NC columns of
-// the output. Tiles of K and V come by asynchronous copies a tile ahead, where rows start on 16 bytes, are 32-bit and two tiles fit (heads of up to
+// 64 rows of an item. A thread has four rows (4 ty ..) by four keys (tx, tx + 16, ..) of the scores, and four rows by 4 NC columns of the output. Tiles of K and V come by asynchronous copies a tile ahead, where rows start on 16 bytes, are 32-bit and two tiles fit (heads of up to
 // 128); else through registers.
-template <typename T, int RM, int NC>
+template <typename T, int NC>
 __device__ __forceinline__ void item_rows(const SharedItem& e, int r0, float* sh, const T* q, long ldq, const T* kc, const T* vc, const int* bt,
                                           int bt_stride, int narrow, float* part_o, float2* part_ml, int G, int Hkv, int D, int page_size,
                                           float scale_log2, int vec) {
   using S = ItemsShared<NC>;
-  constexpr int R = 16 * RM, DP = 64 * NC, LD = S::LD, LP = S::LP;
+  constexpr int RM = 4, R = 16 * RM, DP = 64 * NC, LD = S::LD, LP = S::LP;
   constexpr bool CAN = S::STAGES == 2 && sizeof(T) == 4;
   float *sQ = sh, *sKV = sQ + 64 * LD, *sP = sKV + 2 * S::STAGES * S::TILE;     // stage s: K at 2 s, V at 2 s + 1
   long* sRow = (long*)(sP + 64 * LP);                                           // [stage][key]: where the key's row is, -1: nowhere
@@ -98,150 +97,318 @@ __device__ __forceinline__ void item_rows(const SharedItem& e, int r0, float* sh
     }
     if (CAN) asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  __syncthreads();
+  find(e.lo, 0);
+  for (int i = threadIdx.x; i < R * (DP / 4); i += SI_THREADS) {
+    const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r0 + r < rows) v = row4(q + (size_t)(e.token + (r0 + r) / G) * ldq + (size_t)(e.head * G + (r0 + r) % G) * D, c, D, vec);
+    *(float4*)(sQ + r * LD + c) = v;
+  }
+  __syncthreads();
+  if (copies) bring(0);
+  float m[RM], l[RM];
+  uint64_t acc[RM][2 * NC];
+  int last[RM];                                     // the last key that the row sees
+#pragma unroll
+  for (int i = 0; i < RM; i++) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    last[i] = e.pos == SP_NO_MASK ? SP_NO_MASK : e.pos + (r0 + ty * RM + i) / G;
+#pragma unroll
+    for (int c = 0; c < 2 * NC; c++) acc[i][c] = 0ull;
+  }
+  int stage = 0;
+  for (int k0 = e.lo; k0 < e.hi; k0 += SI_KEYS) {
+    if (copies) {
+      if (k0 + SI_KEYS < e.hi) find(k0 + SI_KEYS, stage ^ 1);
+      __syncthreads();                              // (the other stage has been read, too)
+      if (k0 + SI_KEYS < e.hi) {
+        bring(stage ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
+    } else {
+      if (k0 > e.lo) {
         __syncthreads();
-        find(e.lo, 0);
-        for (int i = threadIdx.x; i < R * (DP / 4); i += SI_THREADS) {
-          const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (r0 + r < rows) v = row4(q + (size_t)(e.token + (r0 + r) / G) * ldq + (size_t)(e.head * G + (r0 + r) % G) * D, c, D, vec);
-          *(float4*)(sQ + r * LD + c) = v;
-        }
+        find(k0, 0);
         __syncthreads();
-        if (copies) bring(0);
-        float m[RM], l[RM];
-        uint64_t acc[RM][2 * NC];
-        int last[RM];                                     // the last key that the row sees
-  #pragma unroll
-        for (int i = 0; i < RM; i++) {
-          m[i] = -INFINITY;
-          l[i] = 0.f;
-          last[i] = e.pos == SP_NO_MASK ? SP_NO_MASK : e.pos + (r0 + ty * RM + i) / G;
-  #pragma unroll
-          for (int c = 0; c < 2 * NC; c++) acc[i][c] = 0ull;
-        }
-        int stage = 0;
-        for (int k0 = e.lo; k0 < e.hi; k0 += SI_KEYS) {
-          if (copies) {
-            if (k0 + SI_KEYS < e.hi) find(k0 + SI_KEYS, stage ^ 1);
-            __syncthreads();                              // (the other stage has been read, too)
-            if (k0 + SI_KEYS < e.hi) {
-              bring(stage ^ 1);
-              asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-              asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
-          } else {
-            if (k0 > e.lo) {
-              __syncthreads();
-              find(k0, 0);
-              __syncthreads();
-            }
-            bring(0);
-          }
-          __syncthreads();
-          const float *sK = sKV + 2 * stage * S::TILE, *sV = sK + S::TILE;
-          if (copies) stage ^= 1;
-          uint64_t s2[RM][4];
-  #pragma unroll
-          for (int i = 0; i < RM; i++)
-  #pragma unroll
-            for (int j = 0; j < 4; j++) s2[i][j] = 0ull;
-  #pragma unroll 4
-          for (int c = 0; c < DP; c += 4) {
-            ulonglong2 a[RM], b[4];
-  #pragma unroll
-            for (int i = 0; i < RM; i++) a[i] = *(const ulonglong2*)(sQ + (ty * RM + i) * LD + c);
-  #pragma unroll
-            for (int j = 0; j < 4; j++) b[j] = *(const ulonglong2*)(sK + (tx + 16 * j) * LD + c);
-  #pragma unroll
-            for (int i = 0; i < RM; i++)
-  #pragma unroll
-              for (int j = 0; j < 4; j++) s2[i][j] = fma2(a[i].x, b[j].x, fma2(a[i].y, b[j].y, s2[i][j]));
-          }
-          float corr[RM];
-  #pragma unroll
-          for (int i = 0; i < RM; i++) {
-            float s[4], mx = -INFINITY;
-  #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const int p = k0 + tx + 16 * j;
-              const float2 y = both(s2[i][j]);
-              s[j] = p < e.hi && p <= last[i] ? (y.x + y.y) * scale_log2 : -INFINITY;
-              mx = fmaxf(mx, s[j]);
-            }
-  #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float mn = fmaxf(m[i], mx), sub = mn == -INFINITY ? 0.f : mn;
-            corr[i] = exp2_of(m[i] - sub);
-            m[i] = mn;
-            float sum = 0.f;
-  #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float p = exp2_of(s[j] - sub);
-              sum += p;
-              sP[(ty * RM + i) * LP + tx + 16 * j] = p;
-            }
-  #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l[i] = l[i] * corr[i] + sum;
-          }
-          __syncwarp();               // the 16 lanes that share a row of P are of one warp
-  #pragma unroll
-          for (int i = 0; i < RM; i++) {
-            const uint64_t w = pair(corr[i], corr[i]);
-  #pragma unroll
-            for (int c = 0; c < 2 * NC; c++) acc[i][c] = fma2(acc[i][c], w, 0ull);
-          }
-          // a value behind a row is not multiplied by 0 (it may be an infinity or NaN), where rows do not see all keys
-          auto products = [&](auto careful) {
-  #pragma unroll 2
-            for (int j = 0; j < SI_KEYS; j += 4) {
-              float pr[RM][4];
-  #pragma unroll
-              for (int i = 0; i < RM; i++) *(float4*)pr[i] = *(const float4*)(sP + (ty * RM + i) * LP + j);
-  #pragma unroll
-              for (int jj = 0; jj < 4; jj++)
-  #pragma unroll
-                for (int n = 0; n < NC; n++) {
-                  const ulonglong2 v = *(const ulonglong2*)(sV + (j + jj) * LD + 64 * n + 4 * tx);
-  #pragma unroll
-                  for (int i = 0; i < RM; i++) {
-                    const uint64_t p = pair(pr[i][jj], pr[i][jj]);
-                    if (!decltype(careful)::value || pr[i][jj] != 0.f) {
-                      acc[i][2 * n] = fma2(p, v.x, acc[i][2 * n]);
-                      acc[i][2 * n + 1] = fma2(p, v.y, acc[i][2 * n + 1]);
-                    }
-                  }
-                }
-            }
-          };
-          if (e.pos == SP_NO_MASK) products(std::false_type());
-          else products(std::true_type());
-        }
-  #pragma unroll
-        for (int i = 0; i < RM; i++) {
-          const int r = r0 + ty * RM + i;
-          if (r >= rows) continue;
-          const size_t row = (size_t)e.part + r;
-          if (tx == 0) {
-            part_ml[row] = make_float2(m[i], l[i]);
-            // a plan that was made for the tensor cores has a second part here (rows of q that TMA cannot address)
-            if (e.tokens <= narrow) part_ml[row + rows] = make_float2(-INFINITY, 0.f);
-          }
-  #pragma unroll
+      }
+      bring(0);
+    }
+    __syncthreads();
+    const float *sK = sKV + 2 * stage * S::TILE, *sV = sK + S::TILE;
+    if (copies) stage ^= 1;
+    uint64_t s2[RM][4];
+#pragma unroll
+    for (int i = 0; i < RM; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) s2[i][j] = 0ull;
+#pragma unroll 4
+    for (int c = 0; c < DP; c += 4) {
+      ulonglong2 a[RM], b[4];
+#pragma unroll
+      for (int i = 0; i < RM; i++) a[i] = *(const ulonglong2*)(sQ + (ty * RM + i) * LD + c);
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j] = *(const ulonglong2*)(sK + (tx + 16 * j) * LD + c);
+#pragma unroll
+      for (int i = 0; i < RM; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s2[i][j] = fma2(a[i].x, b[j].x, fma2(a[i].y, b[j].y, s2[i][j]));
+    }
+    float corr[RM];
+#pragma unroll
+    for (int i = 0; i < RM; i++) {
+      float s[4], mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int p = k0 + tx + 16 * j;
+        const float2 y = both(s2[i][j]);
+        s[j] = p < e.hi && p <= last[i] ? (y.x + y.y) * scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[j]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(m[i], mx), sub = mn == -INFINITY ? 0.f : mn;
+      corr[i] = exp2_of(m[i] - sub);
+      m[i] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float p = exp2_of(s[j] - sub);
+        sum += p;
+        sP[(ty * RM + i) * LP + tx + 16 * j] = p;
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l[i] = l[i] * corr[i] + sum;
+    }
+    __syncwarp();               // the 16 lanes that share a row of P are of one warp
+#pragma unroll
+    for (int i = 0; i < RM; i++) {
+      const uint64_t w = pair(corr[i], corr[i]);
+#pragma unroll
+      for (int c = 0; c < 2 * NC; c++) acc[i][c] = fma2(acc[i][c], w, 0ull);
+    }
+    // a value behind a row is not multiplied by 0 (it may be an infinity or NaN), where rows do not see all keys
+    auto products = [&](auto careful) {
+#pragma unroll 2
+      for (int j = 0; j < SI_KEYS; j += 4) {
+        float pr[RM][4];
+#pragma unroll
+        for (int i = 0; i < RM; i++) *(float4*)pr[i] = *(const float4*)(sP + (ty * RM + i) * LP + j);
+#pragma unroll
+        for (int jj = 0; jj < 4; jj++)
+#pragma unroll
           for (int n = 0; n < NC; n++) {
-            const float2 y[2] = {both(acc[i][2 * n]), both(acc[i][2 * n + 1])};
-            const float o[4] = {y[0].x, y[0].y, y[1].x, y[1].y};
-  #pragma unroll
-            for (int c = 0; c < 4; c++)
-              if (64 * n + 4 * tx + c < D) part_o[row * D + 64 * n + 4 * tx + c] = o[c];
+            const ulonglong2 v = *(const ulonglong2*)(sV + (j + jj) * LD + 64 * n + 4 * tx);
+#pragma unroll
+            for (int i = 0; i < RM; i++) {
+              const uint64_t p = pair(pr[i][jj], pr[i][jj]);
+              if (!decltype(careful)::value || pr[i][jj] != 0.f) {
+                acc[i][2 * n] = fma2(p, v.x, acc[i][2 * n]);
+                acc[i][2 * n + 1] = fma2(p, v.y, acc[i][2 * n + 1]);
+              }
+            }
           }
-        }
+      }
+    };
+    if (e.pos == SP_NO_MASK) products(std::false_type());
+    else products(std::true_type());
+  }
+#pragma unroll
+  for (int i = 0; i < RM; i++) {
+    const int r = r0 + ty * RM + i;
+    if (r >= rows) continue;
+    const size_t row = (size_t)e.part + r;
+    if (tx == 0) {
+      part_ml[row] = make_float2(m[i], l[i]);
+      // a plan that was made for the tensor cores has a second part here (rows of q that TMA cannot address)
+      if (e.tokens <= narrow) part_ml[row + rows] = make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+      const float2 y[2] = {both(acc[i][2 * n]), both(acc[i][2 * n + 1])};
+      const float o[4] = {y[0].x, y[0].y, y[1].x, y[1].y};
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        if (64 * n + 4 * tx + c < D) part_o[row * D + 64 * n + 4 * tx + c] = o[c];
+    }
+  }
 }
 
-// Items of up to 16 rows, and the last rows of others, take a row a thread (LSU-bound: a key's loads serve 16 rows), the rest four.
+// Few rows of an item, RR at a time, without shared tiles: a lane has E columns of all RR rows of q and of O in registers, LPK lanes are a key, and
+// a warp goes through eight keys at a time (four a half-warp; four a warp for heads above 64) on its own, the warps in turn. The sums over a key's
+// lanes come by exchanging halves, so that every lane ends with whole scores of one row, and P goes round through 32 numbers of shared memory.
+// The warps' results meet at the end. A tile through shared memory has one load of 16 bytes for four products where it serves few rows: 32 requests
+// of one row behind 2,048 tokens of their own, 32 heads over 8 of 64 in 32 bits, 185 us through tiles, 66 so (4.1 TB/s); heads of 128 343 and 189.
+// Up to 16 rows go this way (24, with the rest of a long prefix's rows, made 25 us 36).
+template <int NC> struct FewRows {
+  // (four rows leave two blocks an SM; more columns a lane have one in any case)
+  static constexpr int RR = NC == 1 ? 4 : 8, LPK = NC == 1 ? 16 : 32, E = 64 * NC / LPK, HALVES = 32 / LPK, KEYS = 4 * HALVES;
+  // what a warp has of the shared memory: m, l and O of its rows at the end; P before it
+  static constexpr int FLOATS = RR * 2 + RR * 64 * NC;
+};
 template <typename T, int NC>
-__global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
+__device__ __forceinline__ void item_few_rows(const SharedItem& e, int r0, float* sh, const T* q, long ldq, const T* kc, const T* vc, const int* bt,
+                                              int bt_stride, int narrow, float* part_o, float2* part_ml, int G, int Hkv, int D, int page_size,
+                                              float scale_log2, int vec) {
+  using F = FewRows<NC>;
+  constexpr int RR = F::RR, LPK = F::LPK, E = F::E, E2 = E / 2, KEYS = F::KEYS, DP = 64 * NC, WARPS = SI_THREADS / 32;
+  constexpr int PER = RR * 4 / LPK;                    // scores a lane ends with: of row `mine`, keys key0 ..
+  static_assert(PER == 1 || PER == 2, "a lane's scores are of one row");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPK, half = lane / LPK, c = sub * E, rows = e.tokens * G;
+  const int mine = sub * PER / 4, key0 = sub * PER % 4;
+  float* own = sh + warp * F::FLOATS;
+  __syncthreads();                                     // (the shared memory's last readers)
+  auto load = [&](const T* row, uint64_t* x) {         // this lane's columns
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const float4 v = row4(row, c + i, D, vec);
+      x[i / 2] = pair(v.x, v.y);
+      x[i / 2 + 1] = pair(v.z, v.w);
+    }
+  };
+  uint64_t x[RR][E2], acc[RR][E2];
+#pragma unroll
+  for (int r = 0; r < RR; r++) {
+    const int row = min(r0 + r, rows - 1);             // (the last row again behind it)
+    load(q + (size_t)(e.token + row / G) * ldq + (size_t)(e.head * G + row % G) * D, x[r]);
+#pragma unroll
+    for (int i = 0; i < E2; i++) acc[r][i] = 0ull;
+  }
+  const int last = e.pos == SP_NO_MASK ? e.hi - 1 : min(e.hi - 1, e.pos + min(r0 + mine, rows - 1) / G);      // the last key that row `mine` sees
+  float m = -INFINITY, l = 0.f;                        // of row `mine`; l of this lane's keys
+  auto walk = [&](auto careful) {
+    for (int k0 = e.lo + warp * KEYS; k0 < e.hi; k0 += WARPS * 32) {
+      const int p = min(k0 + (lane / KEYS) * WARPS * KEYS + lane % KEYS, e.hi - 1), page = p / page_size;      // of this warp's keys of the next 256
+      const long at = (((long)bt[(size_t)e.table * bt_stride + page] * Hkv + e.head) * page_size + (p - page * page_size)) * D;
+      for (int j0 = 0, first = k0 + 4 * half; j0 < 32 && first - 4 * half < e.hi; j0 += KEYS, first += WARPS * KEYS) {      // (the last key again behind it)
+        uint64_t k[4][E2], v[4][E2];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const long row = __shfl_sync(0xffffffffu, at, j0 + 4 * half + u);
+          load(kc + row, k[u]);
+          load(vc + row, v[u]);
+        }
+        float s[RR * 4];
+#pragma unroll
+        for (int r = 0; r < RR; r++)
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            uint64_t a = 0ull;
+#pragma unroll
+            for (int i = 0; i < E2; i++) a = fma2(x[r][i], k[u][i], a);
+            const float2 y = both(a);
+            s[4 * r + u] = y.x + y.y;
+          }
+        // sums over a key's lanes: who has the upper half of the lanes keeps the upper half of the sums
+#pragma unroll
+        for (int o = LPK / 2, n = RR * 2; o > 0; o >>= 1, n >>= 1) {
+          const bool up = sub & o;
+          if (n > 0) {
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+              const float keep = up ? s[n + i] : s[i], give = up ? s[i] : s[n + i];
+              s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+          } else {
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          s[i] = first + key0 + i <= last ? s[i] * scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[i]);
+        }
+#pragma unroll
+        for (int o = 4 / PER / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (F::HALVES == 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        if (__any_sync(0xffffffffu, mx > m)) {
+          const float mn = fmaxf(m, mx), corr = m == mn ? 1.f : exp2_of(m - mn);
+          m = mn;
+          l *= corr;
+#pragma unroll
+          for (int r = 0; r < RR; r++) {
+            const float f = __shfl_sync(0xffffffffu, corr, r * 4 / PER);
+#pragma unroll
+            for (int i = 0; i < E2; i++) acc[r][i] = fma2(acc[r][i], pair(f, f), 0ull);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        __syncwarp();                                  // P's last readers
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          s[i] = exp2_of(s[i] - ref);
+          l += s[i];
+          own[half * RR * 4 + sub * PER + i] = s[i];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+          const float4 w = *(const float4*)(own + half * RR * 4 + 4 * r);
+          const float ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            // a value behind a row is not multiplied by 0 (it may be an infinity or NaN), where rows do not see all keys
+            if (!decltype(careful)::value || ws[u] != 0.f) {
+#pragma unroll
+              for (int i = 0; i < E2; i++) acc[r][i] = fma2(pair(ws[u], ws[u]), v[u][i], acc[r][i]);
+            }
+        }
+      }
+    }
+  };
+  if (e.pos == SP_NO_MASK) walk(std::false_type());
+  else walk(std::true_type());
+  // this warp's rows into its part of the shared memory
+#pragma unroll
+  for (int o = 4 / PER / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (F::HALVES == 2) l += __shfl_xor_sync(0xffffffffu, l, 16);
+  __syncwarp();
+  if (half == 0 && key0 == 0) {
+    own[mine] = m;
+    own[RR + mine] = l;
+  }
+#pragma unroll
+  for (int r = 0; r < RR; r++)
+#pragma unroll
+    for (int i = 0; i < E2; i++) {
+      float2 y = both(acc[r][i]);
+      if (F::HALVES == 2) {
+        y.x += __shfl_xor_sync(0xffffffffu, y.x, 16);
+        y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
+      }
+      if (half == 0) *(float2*)(own + 2 * RR + r * DP + c + 2 * i) = y;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < RR * DP; i += SI_THREADS) {
+    const int r = i / DP, col = i % DP;
+    if (r0 + r >= rows) break;
+    float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) top = fmaxf(top, sh[w * F::FLOATS + r]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float f = exp2_of(sh[w * F::FLOATS + r] - ref);              // 0 for a warp without keys
+      sum = fmaf(f, sh[w * F::FLOATS + RR + r], sum);
+      o = fmaf(f, sh[w * F::FLOATS + 2 * RR + i], o);
+    }
+    const size_t part = (size_t)e.part + r0 + r;
+    if (col == 0) {
+      part_ml[part] = make_float2(top, sum);
+      if (e.tokens <= narrow) part_ml[part + rows] = make_float2(-INFINITY, 0.f);        // (as below)
+    }
+    if (col < D) part_o[part * D + col] = o;
+  }
+}
+
+// An item's rows, 64 at a time, or where they are few, four or eight.
+template <typename T, int NC>
+__global__ void __launch_bounds__(SI_THREADS, NC == 1 ? 2 : 1) shared_items_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
                                                                   const SharedItem* items, const int* ctas, int narrow, float* part_o,
                                                                   float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec) {
   extern __shared__ __align__(16) float sh[];
@@ -252,10 +419,11 @@ __global__ void __launch_bounds__(SI_THREADS) shared_items_kernel(const T* q, lo
     const SharedItem e = items[it];
     const int rows = e.tokens * G;
     for (int r0 = blockIdx.y * 64; r0 < rows; r0 += gridDim.y * 64) {
-      if (rows - r0 <= 16)
-        item_rows<T, 1, NC>(e, r0, sh, q, ldq, kc, vc, bt, bt_stride, narrow, part_o, part_ml, G, Hkv, D, page_size, scale_log2, vec);
+      if (rows - r0 <= SI_FEW)
+        for (int r = r0; r < rows; r += FewRows<NC>::RR)
+          item_few_rows<T, NC>(e, r, sh, q, ldq, kc, vc, bt, bt_stride, narrow, part_o, part_ml, G, Hkv, D, page_size, scale_log2, vec);
       else
-        item_rows<T, 4, NC>(e, r0, sh, q, ldq, kc, vc, bt, bt_stride, narrow, part_o, part_ml, G, Hkv, D, page_size, scale_log2, vec);
+        item_rows<T, NC>(e, r0, sh, q, ldq, kc, vc, bt, bt_stride, narrow, part_o, part_ml, G, Hkv, D, page_size, scale_log2, vec);
     }
   }
 }

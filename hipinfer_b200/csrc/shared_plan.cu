@@ -26,14 +26,14 @@ struct Cut {
 };
 
 struct Planner {
-  int Hkv, G, key_tile, n_ctas, narrow_tokens;
-  double item_cost, wide_cost, part_cost;
+  int Hkv, G, key_tile, n_ctas, narrow_tokens, few_tokens;
+  double item_cost, wide_cost, few_cost, part_cost;
   static constexpr double row_cost = 0.02;               // of a part of the row that has most of them (they are joined one after another)
   std::vector<Segment> segs;
   std::vector<std::vector<std::pair<int, int>>> lists;   // a CTA's (segment, head * chunks + chunk)
 
   bool narrow(const Segment& s) const { return s.tokens <= narrow_tokens; }
-  double tile_cost(const Segment& s) const { return narrow(s) ? 1.0 : wide_cost; }
+  double tile_cost(const Segment& s) const { return s.tokens <= few_tokens ? few_cost : narrow(s) ? 1.0 : wide_cost; }
   // What chunks of about `cost` come to: the longest CTA, if the shared items fill rounds of all CTAs and the requests' own ones what is left of the
   // last of them, and the partial results.
   Cut cut(double cost) {
@@ -101,10 +101,11 @@ struct Planner {
 // q_len, ctx_len [R]; groups [n_groups][3]: first request, requests, shared tokens. out: SP_HEADER ints, then items, each CTA's first item (one more
 // for the end), tokens; returns the ints that were written, or, where `cap` is too small, minus the number that is needed; 0 with a message in
 // hb_last_error for lengths that make no plan. tile_tokens: rows of q in an item; narrow_tokens: items of at most so many rows leave two
-// parts (two chains share their keys), 0: none do. Costs are in key tiles of a narrow item: an item's beginning and end, a tile of another item, a part row.
+// parts (two chains share their keys), 0: none do. Costs are in key tiles of a narrow item: an item's beginning and end, a tile of another
+// item, a part row; a tile of an item of up to few_tokens rows (0: as another).
 HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const int* groups, int n_groups, int Hq, int Hkv, int tile_tokens,
-                             int narrow_tokens, int key_tile, int n_ctas, float item_cost, float wide_cost, float part_cost, int* out,
-                             int cap) {
+                             int narrow_tokens, int key_tile, int n_ctas, float item_cost, float wide_cost, float part_cost, int few_tokens, float few_cost,
+                             int* out, int cap) {
   try {
     if (R < 0 || n_groups < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv || tile_tokens < 1 || key_tile < 1 || n_ctas < 1) {
       hb_set_error("hb_shared_plan: bad sizes (%d requests, %d groups, %d/%d heads, %d rows an item)", R, n_groups, Hq, Hkv, tile_tokens);
@@ -152,6 +153,8 @@ HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const 
     p.item_cost = item_cost;
     p.wide_cost = wide_cost;
     p.part_cost = part_cost;
+    p.few_tokens = few_tokens;
+    p.few_cost = few_cost;
     const int T = start[R];
     std::vector<SharedToken> tokens(T);
     std::vector<int> pre_seg(T, -1), own_seg(T, -1), pre_row(T, 0), own_row(T, 0);

@@ -18,7 +18,7 @@ from . import library, ops
 
 _p, _i, _l, _f = C.c_void_p, C.c_int, C.c_long, C.c_float
 ops._SIGS["drafts"] = {
-    "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _f, _p, _i],
+    "hb_shared_plan": [_p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _f, _i, _f, _p, _i],
     "hb_attention_shared": [_p, _l, _p, _p, _l, _p, _i, _p, _p, _p, _p, _f, _i, _p, _p],
     "hb_shared_items_tc_supported": [_i, _i, _i, _i],
     "hb_verify_drafts": [_p, _i, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _l, _p, _i, _l, _l, _p, _p, _p, _p, _p],
@@ -32,7 +32,7 @@ _HEADER = 16
 
 
 def plan_numbers(q_lens, ctx_lens, groups, n_heads: int, n_kv_heads: int, tile_tokens: int, narrow_tokens: int, key_tile: int, n_ctas: int,
-                 item_cost: float, wide_cost: float, part_cost: float) -> np.ndarray:
+                 item_cost: float, wide_cost: float, part_cost: float, few_tokens: int = 0, few_cost: float = 1.0) -> np.ndarray:
     """The plan as int32 numbers (csrc/shared_plan.cu, which runs on the host); raises KernelError for lengths that make none."""
     q, c = (np.ascontiguousarray(x, dtype=np.int32) for x in (q_lens, ctx_lens))
     g = np.ascontiguousarray(groups, dtype=np.int32).reshape(-1, 3)
@@ -43,7 +43,7 @@ def plan_numbers(q_lens, ctx_lens, groups, n_heads: int, n_kv_heads: int, tile_t
     while True:
         out = np.empty(cap, dtype=np.int32)
         n = fn(q.ctypes.data, c.ctypes.data, len(q), g.ctypes.data, len(g), n_heads, n_kv_heads, tile_tokens, narrow_tokens, key_tile, n_ctas,
-               item_cost, wide_cost, part_cost, out.ctypes.data, cap)
+               item_cost, wide_cost, part_cost, few_tokens, few_cost, out.ctypes.data, cap)
         if n > 0:
             return out[:n]
         if n == 0:
@@ -78,7 +78,7 @@ class SharedPlan:
             cut, costs = (2 * (128 // group), 128 // group, 128, _sms(self.device)), (1.6, 1.8, head_dim * 1e-6)
         else:
             cut = (max(1, 64 // group), 0, 64, (2 if head_dim <= 64 else 1) * _sms(self.device))         # (as many as are resident)
-            costs = (1.0, 1.0, head_dim * 1e-6)
+            costs = (0.6, 1.0, head_dim * 1e-6, 16 // group, 0.4)      # (in tiles of 64 rows; up to 16 rows go another way)
         numbers = plan_numbers(q_lens, ctx_lens, groups, n_heads, n_kv_heads, *cut, *costs)
         self.rows, self.parts = int(numbers[_TOKENS]), int(numbers[_PARTS])
         self.ctas, self.max_rows = int(numbers[_CTAS]), int(numbers[_MAX_ROWS])
