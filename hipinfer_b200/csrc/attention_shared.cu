@@ -56,7 +56,7 @@ template <int NC> struct ItemsShared {
   static constexpr int BYTES = (64 * LD + 2 * STAGES * TILE + 64 * LP) * 4 + 2 * SI_KEYS * 8;
 };
 
-// 64 rows of an item. A thread has four rows (4 ty ..) by four keys (tx, tx + 16, ..) of the scores, and four rows by 4 NC columns of the output. Tiles of K and V come by asynchronous copies a tile ahead, where rows start on 16 bytes, are 32-bit and two tiles fit (heads of up to
+// 64 rows of an item, FMA-bound: 192 rows of 32 heads over 8 of 64 behind 8,192 tokens 369 us, 35 TFLOP/s of 72. A thread has four rows (4 ty ..) by four keys (tx, tx + 16, ..) of the scores, and four rows by 4 NC columns of the output. Tiles of K and V come by asynchronous copies a tile ahead, where rows start on 16 bytes, are 32-bit and two tiles fit (heads of up to
 // 128); else through registers.
 template <typename T, int NC>
 __device__ __forceinline__ void item_rows(const SharedItem& e, int r0, float* sh, const T* q, long ldq, const T* kc, const T* vc, const int* bt,
@@ -464,7 +464,8 @@ __device__ __forceinline__ void warp_sums(float* s, int lane) {
 // W warps per row of q and head (a block has SJ_WARPS); a lane has E columns. The parts go to the warps in turn, the keys of the step's own rows to
 // the last warp; W > 1: the warps' results meet in shared memory, in their order. Latency is what it takes, a few loads that wait for one another:
 // the pages of all own keys are looked up at once, a lane a key, and parts are asked for before their weights are known. The own keys come ahead
-// of the wait for the items' kernel (behind_items: that one starts this one behind its own wait, when all they need is in place).
+// of the wait for the items' kernel (behind_items: that one starts this one behind its own wait, when all they need is in place). 384 rows of 32
+// heads with four parts each take 15 us, 8 rows 2.
 template <typename T, int E, int W, bool FULL>
 __global__ void __launch_bounds__(SJ_WARPS * 32, E <= 4 ? 8 : 4) shared_join_kernel(const T* q, long ldq, const T* kc, const T* vc, const int* bt, int bt_stride,
                                                                     const SharedToken* tokens, const float* part_o, const float2* part_ml, T* out, int Hq,
@@ -648,7 +649,8 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
     if (r) return r;
   }
   cudaError_t e = cudaSuccess;
-  // few rows of many parts: four warps share one's (8 rows x 32 heads of 34 parts 13 -> 8 us; 2,048 rows of 8 parts 5 us slower, beyond one round)
+  // few rows of many parts: four warps share one's (8 rows of 32 heads behind 24,560 tokens 26.7 -> 23.8 us a call; 190 rows of 24 heads with 5 parts
+  // 34.8 -> 44: more blocks than a round)
   const int W = warps > 1024 || h->parts < 6 * warps ? 1 : 4;
 #define SJ_LAUNCH(E, W, FULL)                                                                                                                    \
   e = hb_launch(shared_join_kernel<TA, E, W, FULL>, dim3((unsigned)T, (unsigned)((Hq * W + SJ_WARPS - 1) / SJ_WARPS)), SJ_WARPS * 32, 0, s, (const TA*)q, ldq, \

@@ -13,8 +13,15 @@
 //   K and V loaders TMA, a page and 64 columns a box, a lane holds a page's number; Q comes with K, one box of (64 columns, heads, tokens).
 // The accumulator is rescaled only when a row's maximum grew by more than a power of 2 (any reference value gives the same quotient).
 // V rows outside of the item's range, which may hold anything, are set to zero in shared memory by the softmax threads that mask them: P
-// is 0 there, and 0 times an infinity is no 0. Every wait is bounded; both chains wait for and release every tile and every Q, so that a
-// barrier is never more than a phase ahead of one that waits for it.
+// is 0 there, and 0 times an infinity is no 0. (Keys inside of the range that a row of the item does not see, as only portions of more than
+// SP_FRESH rows have them, do meet a P of 0: a value there that is not finite makes the rows before it NaN.) Every wait is bounded; both chains wait
+// for and release every tile and every Q, so that a barrier is never more than a phase ahead of one that waits for it.
+//
+// What bounds it: with many rows the softmax (a step is 64 exponentials of 128 rows for two products of 128 x 64 x D; two warps share a scheduler):
+// 384 rows of 32 heads over 8 of 128 behind 24,560 shared tokens take 143 us, 1,082 TFLOP/s. With few rows the memory: 32 requests of one row
+// behind 8,192 tokens of their own 170 us, 6.3 TB/s. In short calls latency: an item's first tile and its end, 2 us each. A chain takes
+// 64 keys a step so that its scores fit into registers beside the running numbers; two chains an SM, since one alone leaves the tensor core idle during
+// its softmax and four, with the registers for half of the keys each, were slower.
 #include "shared_plan.h"
 #include "tc_common.cuh"
 
@@ -450,7 +457,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
               float p0, p1, p2, p3;
               const uint64_t t0 = fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, sub2);
               const uint64_t t1 = fma2(pack2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), scale2, sub2);
-              if (j % 12 == 0) {       // 6 of 16 groups: the special-function unit has 8 cycles for each of the others (none 170 us, these 160, half of them 179)
+              if (j % 12 == 0) {       // 6 of 16 groups: the special-function unit has 8 cycles for each of the others (none 150 us, these 143, half of them 148: 384 rows behind 24,560 tokens)
                 exp2_poly(t0, p0, p1);
                 exp2_poly(t1, p2, p3);
               } else {

@@ -1,6 +1,7 @@
 """Operators of a step that samples many continuations behind shared pages, with drafted tokens: attention over a paged cache in which
 groups of requests share a long prefix (computed once for all of a group's rows), and the verification of drafted tokens against the
-target's logits. Reached as `ops.SharedPlan`, `ops.attention_shared` and `ops.verify_drafts` (csrc/shared_plan.cu, attention_shared.cu, verify_drafts.cu).
+target's logits. Reached as `ops.SharedPlan`, `ops.attention_shared` and `ops.verify_drafts` (csrc/shared_plan.cu, attention_shared.cu, attention_shared_tc.cu,
+verify_drafts.cu; drafts_binding.cpp makes the calls whose arguments are as they should be).
 
 The reference has neither: its batch slots hold a copy of the prompt each (src/api.cu:1409-1411), and its `verify_step` (2029-2060) returns
 logits and leaves the choice to the caller."""
@@ -58,7 +59,8 @@ class SharedPlan:
     q_lens[r] rows of request r (its rows are consecutive, requests one after the other) stand at positions ctx_lens[r], ...; a row sees the
     keys up to its own. groups: (first request, requests, shared tokens): the block tables of these requests name the same pages for the
     positions below `shared tokens` (which need not be a multiple of the page size). Requests of no group, and groups of which fewer than two
-    bring rows, attend on their own."""
+    bring rows, attend on their own. The plan's numbers are copied to the device on the current stream, and a call's kernels read them: on
+    another stream it is used, and let go, only when that one has waited for this and the other way round, as with any tensor."""
 
     def __init__(self, q_lens: Sequence[int], ctx_lens: Sequence[int], groups: Sequence[Tuple[int, int, int]], n_heads: int, n_kv_heads: int,
                  head_dim: int, page_size: int, dtype: torch.dtype, device="cuda:0"):
