@@ -358,7 +358,7 @@ Cut cut(int V, int dt, int R, int K) {
     if ((long)R * (K + 1) * (n / (c.u * VD_THREADS)) >= 4 * 148) break;
   c.slices = n / (c.u * VD_THREADS) + 1;
   c.ranks = 1;
-  while (c.ranks < VP_MAX_RANKS && (long)R * c.ranks < 4 * 148 && V > c.ranks * 1024) c.ranks *= 2;
+  while (c.ranks < VP_MAX_RANKS && (long)R * c.ranks * 2 <= 4 * 148 && V > c.ranks * 1024) c.ranks *= 2;
   return c;
 }
 
