@@ -7,7 +7,7 @@
 // with e_v ~ Exp(1) given: the smallest of exponential variables of rates w_v is v with probability w_v / sum w.
 //
 // Bytes bound it: every logit once, one row of q and the noise a request. 24 requests of up to five drafts over 128,256 entries, 32-bit, take 17.5 us
-// (3.7 TB/s), 96 of up to seven over 50,021 in bfloat16 31 (2.4: half of the blocks are drafts that are not there, and an exponential, a
+// (3.7 TB/s), 96 of up to seven over 50,021 in bfloat16 28 (2.6: half of the blocks are drafts that are not there, and an exponential, a
 // conversion and two sums for two bytes keep the issue slots half full). One request of three takes 6: two kernels and what they wait for.
 //
 // Two kernels. verify_rows_kernel reads every logit once: a block has a slice of a row in registers and leaves its maximum and sum of
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
 
 // The cut: U vectors a thread (32 elements where that leaves blocks for all SMs, 64 of bfloat16 would take
 // the registers of half of the warps; few rows are cut finer), and CTAs a request for the last token, up to 16 of
-// at least 1,024 candidates.
+// at least 1,024 candidates, as many as one round of the SMs has (two rounds: 96 requests 31 us instead of 28).
 struct Cut { int u, slices, ranks; };
 Cut cut(int V, int dt, int R, int K) {
   const int n = V / (dt == HB_BF16 ? 8 : 4);
