@@ -627,6 +627,7 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   const int Hq = h->Hq, Hkv = h->Hkv, D = h->D, ps = h->page_size, T = h->T;
   if (Hkv < 1 || Hq < Hkv || Hq % Hkv) HB_FAIL("hb_attention_shared: %d heads are not a multiple of %d kv heads", Hq, Hkv);
   if (D < 1 || D > 256 || ps < 1) HB_FAIL("hb_attention_shared: heads of %d (1 to 256 are supported), pages of %d", D, ps);
+  if (!(scale >= 0.f && scale < INFINITY)) HB_FAIL("hb_attention_shared: a scale of %g", scale);
   if (T <= 0) return 0;
   const long warps = (long)T * Hq;
   if (warps > (1l << 30) || Hq > 65535) HB_FAIL("hb_attention_shared: %d rows of %d heads are beyond the grid limit", T, Hq);
@@ -637,7 +638,7 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   const int* cta_items = plan + h->off_ctas;
   const SharedToken* tokens = (const SharedToken*)(plan + h->off_tokens);
   const int vec = aligned && D % 4 == 0;
-  const float sl2 = scale * 1.4426950408889634f;
+  const float sl2 = fmaxf(scale * 1.4426950408889634f, 1.17549435e-38f);      // (masked scores are -inf ahead of it: 0 would make them NaN)
   if (h->ctas > 0 && h->tensor_cores && aligned) {
     if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, items, cta_items, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
   } else if (h->ctas > 0) {

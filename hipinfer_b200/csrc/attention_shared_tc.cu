@@ -89,13 +89,19 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The largest of three numbers, NaN if there is one.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // 2^t of two numbers, t <= 8, on the FMA pipe: t = n + f with n its nearest integer, 2^f for |f| <= 1/2 as a polynomial of degree 4 that is 1 at 0
-// (fitted to the least relative error, 2.9e-6), n added to the exponent. Below -127, -inf too, it is 0; NaN does not stay finite through P.
+// (fitted to the least relative error, 2.9e-6), n added to the exponent. Below -127, -inf too, it is 0; of NaN it is any number.
 __device__ __forceinline__ void exp2_poly(uint64_t t2, float& p0, float& p1) {
   float t0, t1;
   unpack2(t2, t0, t1);
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t0));       // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t1));
+  t0 = fmaxf(t0, -127.f);
+  t1 = fmaxf(t1, -127.f);
   const uint64_t t = pack2(t0, t1), magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f);
   const uint64_t y = add2(t, magic), n = add2(y, minus), f = fma2(n, pack2(-1.f, -1.f), t);
   uint64_t p = fma2(f, pack2(0.009582818485796452f, 0.009582818485796452f), pack2(0.05590637028217316f, 0.05590637028217316f));
@@ -436,8 +442,9 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
-            const float m_step = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+            for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = max_nan(mx[(j >> 1) & 3], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+            const float m_step = max_nan(max_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale_log2;
+            if (!(m_step < INFINITY)) l_run = __uint_as_float(0x7fc00000u);      // a score that is NaN or infinite: so is the row
             const bool grow = m_step > m_run + slack;   // also the first step with a visible key: m_run is -inf
             if (__any_sync(0xffffffffu, grow)) {
               const float m_new = grow ? m_step : m_run, corr = grow ? hb_exp2(m_run - m_new) : 1.f;      // 0 while nothing has been summed

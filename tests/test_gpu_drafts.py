@@ -413,3 +413,63 @@ def test_verification_again_on_another_stream_and_captured():
     graph.replay()
     graph.replay()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q,c,groups", [([1, 2], [200, 210], [(0, 2, 192)]), ([20, 40], [200, 210], [(0, 2, 192)])], ids=["few rows", "many rows"])
+def test_a_score_that_is_not_finite_makes_its_rows_nan(q, c, groups, dtype):
+    """At every place of a tile's steps, in the prefix, a request's own keys and the step's: NaN and +inf scores are NaN rows, -inf ones weigh nothing."""
+    Hq, Hkv, D, ps = 8, 2, 64, 16
+    x, k, v, table, scale = case(q, c, groups, Hq, Hkv, D, ps, dtype, poison=False)
+    plan = ops.SharedPlan(q, c, groups, Hq, Hkv, D, ps, dtype, DEV)
+    first = torch.tensor([[i] for n in q for i in range(n)], device=DEV)
+    held = torch.tensor([[c[r]] for r, n in enumerate(q) for _ in range(n)], device=DEV)
+    own = torch.tensor([[r == 1] for r, n in enumerate(q) for _ in range(n)], device=DEV)
+    sign = x.view(-1, Hq, D)[:, :, 0]
+    for pos in list(range(64, 192, 3)) + list(range(128, 192)) + [192, 200, 209, 210]:
+        r = 1 if pos >= 192 else 0            # (the prefix is read through the first request's table)
+        sees = (held + first >= pos) & (own if r == 1 else torch.ones_like(own))
+        for bad in (math.nan, math.inf):
+            k2 = k.clone()
+            k2[int(table[r, pos // ps]), :, pos % ps, 0] = bad
+            got = ops.attention_shared(x, k2, v, table, plan).view(-1, Hq, D)
+            hit = sees & (torch.ones_like(sign, dtype=torch.bool) if math.isnan(bad) else sign > 0)
+            assert got[hit].isnan().all() and torch.isfinite(got[~hit]).all(), (pos, bad)
+    ops.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scales(dtype):
+    """A scale of 0 is the mean of the values; one that is negative or no number is refused."""
+    x, k, v, table, _ = case([1, 3], [130, 140], [(0, 2, 128)], 4, 2, 64, 16, dtype)
+    plan = ops.SharedPlan([1, 3], [130, 140], [(0, 2, 128)], 4, 2, 64, 16, dtype, DEV)
+    out, mag, most, keys = oracle(x, k, v, table, [1, 3], [130, 140], [(0, 2, 128)], 4, 2, 64, 16, 0.0)
+    got = ops.attention_shared(x, k, v, table, plan, scale=0.0)
+    assert ((got.double() - out).abs() <= bound(dtype, out, mag, most, keys, 64)).all()
+    for bad in (-0.1, math.nan, math.inf):
+        with pytest.raises(ops.KernelError, match="scale"):
+            ops.attention_shared(x, k, v, table, plan, scale=bad)
+
+
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (BF16, 64), (BF16, 80)])
+def test_a_cache_of_more_than_32_bits_of_elements(dtype, D):
+    """Pages at the far end of a cache of more than 2^31 elements give the bits that the same pages give in a small one."""
+    q, c, groups, Hkv, ps = [2, 1, 18], [150, 171, 133], [(0, 2, 128)], 2, 16
+    x, k, v, table, scale = case(q, c, groups, 4, Hkv, D, ps, dtype, poison=False)
+    plan = ops.SharedPlan(q, c, groups, 4, Hkv, D, ps, dtype, DEV)
+    want = ops.attention_shared(x, k, v, table, plan)
+    pages = k.shape[0]
+    total = 2 ** 31 // (Hkv * ps * D) + 2 * pages
+    if torch.cuda.mem_get_info()[0] < 3 * total * Hkv * ps * D * x.element_size():
+        pytest.skip("not enough free memory")
+    far = []
+    for small in (k, v):
+        big = torch.empty(total, Hkv, ps, D, dtype=dtype, device=DEV)
+        big[total - pages:] = small
+        far.append(big)
+    assert far[0].numel() > 2 ** 31
+    got = ops.attention_shared(x, *far, torch.where(table < 0, table, table + (total - pages)), plan)
+    assert torch.equal(got, want)
+    ops.check_device_status()
+    del far, big
+    torch.cuda.empty_cache()
