@@ -40,7 +40,7 @@ def plan_numbers(q_lens, ctx_lens, groups, n_heads: int, n_kv_heads: int, tile_t
     if q.ndim != 1 or q.shape != c.shape:
         raise ops.KernelError(f"a plan needs one number of rows and one length a request, got {q.shape} and {c.shape}")
     fn = ops._fn("drafts", "hb_shared_plan")
-    cap = 4096 + 16 * int(q.clip(0).sum())
+    cap = 32768 + 16 * int(q.clip(0).sum())
     while True:
         out = np.empty(cap, dtype=np.int32)
         n = fn(q.ctypes.data, c.ctypes.data, len(q), g.ctypes.data, len(g), n_heads, n_kv_heads, tile_tokens, narrow_tokens, key_tile, n_ctas,
