@@ -97,6 +97,11 @@ __device__ __forceinline__ void cluster_sync() {       // (the barrier's instruc
   __syncwarp();
   hb_cluster_sync();
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 // The lanes' parts as one.
 __device__ __forceinline__ RowPart warp_join(u64 key, float sum, float c) {
   RowPart r;
@@ -195,6 +200,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
   struct Row { float m, s; int at, ok, d; float logp; };
   __shared__ Row rows[VD_MAX_DRAFTS + 1];
   __shared__ u64 warp_key[VP_WARPS], rank_key[VP_MAX_RANKS];
+  cluster_arrive();                                   // this CTA runs: the others may write to it
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t ranks;
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
@@ -253,6 +259,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
     }
   }
   __syncthreads();
+  cluster_wait();                                     // and they run
   int taken = 0;
   while (taken < n && rows[taken].ok) taken++;
   const Row s = any ? rows[taken] : Row{INFINITY, 1.f, -1, 0, -1, 0.f};
