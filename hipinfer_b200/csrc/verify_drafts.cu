@@ -55,9 +55,9 @@ __device__ __forceinline__ float2 both(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {   // two fmaf, each rounded by itself
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -88,10 +88,13 @@ __device__ __forceinline__ float unordered(uint32_t k) {
   return k == 0xffffffffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// A slice's largest logit (with its lowest index, where the request is greedy or the number not finite), and the sum of 2^(x c - ref) with
-// ref = m c rounded (any reference gives the same quotients, so its rounding does not show).
+// A slice's largest logit (with its lowest index, where the request is greedy or the number not finite), and the sum of 2^((x - m) c), c = log2(e) / t.
+// The subtraction comes before the factor: at the largest logit the exponent is 0 at any temperature, where x c minus a rounded m c is
+// off by 2^-24 |m c| (above 126 from m / t of 1.5e9 on: sums of 0 and infinity).
 struct RowPart { u64 key; float sum; int pad; };
-__device__ __forceinline__ float reference(float m, float c) { return m == -INFINITY ? 0.f : m * c; }
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+// (c is finite and not 0, so that neither 0 c nor -inf c is NaN)
+__device__ __forceinline__ float factor(float t) { return fminf(fmaxf(VD_LOG2E / (t > 0.f ? t : 1.f), 1.17549435e-38f), 3.40282347e38f); }
 __device__ __forceinline__ int clamped(int n, int K) { return n < 0 ? 0 : n > K ? K : n; }
 __device__ __forceinline__ void cluster_sync() {       // (the barrier's instructions want whole warps)
   __syncwarp();
@@ -107,7 +110,7 @@ __device__ __forceinline__ RowPart warp_join(u64 key, float sum, float c) {
   RowPart r;
   r.key = warp_larger(key);
   const float m = unordered((uint32_t)(key >> 32)), top = unordered((uint32_t)(r.key >> 32));
-  r.sum = hb_warp_sum(key == 0 || sum == 0.f ? 0.f : sum * hb_exp2(reference(m, c) - reference(top, c)));
+  r.sum = hb_warp_sum(key == 0 || sum == 0.f ? 0.f : sum * hb_exp2((m - base_of(top)) * c));
   r.pad = 0;
   return r;
 }
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const T* logits
   const float ex = edge >= 0 ? hb_to_float(x[edge]) : -INFINITY;
   const float t = temperature[r];
   const bool greedy = !(t > 0.f);
-  const float c = VD_LOG2E / (greedy ? 1.f : t);
+  const float c = factor(t);
   float mx[U], m = ex;
 #pragma unroll
   for (int u = 0; u < U; u++) {
@@ -149,18 +152,18 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const T* logits
     m = fmaxf(m, mx[u]);
   }
   m = warp_max(m);
-  const float ref = reference(m, c);
-  const uint64_t c2 = pair(__float_as_uint(c), __float_as_uint(c)), ref2 = pair(__float_as_uint(-ref), __float_as_uint(-ref));
+  const float base = base_of(m);
+  const uint64_t c2 = pair(__float_as_uint(c), __float_as_uint(c)), minus2 = pair(__float_as_uint(-base), __float_as_uint(-base));
   uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
     for (int j = 0; j < N / 2; j++) {
-      const float2 y = both(fma2(pair_of(T(), raw[u], j), c2, ref2));
+      const float2 y = both(mul2(add2(pair_of(T(), raw[u], j), minus2), c2));
       sums[j & 1] = add2(sums[j & 1], pair(__float_as_uint(hb_exp2(y.x)), __float_as_uint(hb_exp2(y.y))));
     }
   const float2 ab = both(add2(sums[0], sums[1]));
-  const float sum = hb_warp_sum(ab.x + ab.y + hb_exp2(fmaf(ex, c, -ref)));
+  const float sum = hb_warp_sum(ab.x + ab.y + hb_exp2((ex - base) * c));
   const bool odd = !(fabsf(m) < INFINITY) || sum != sum;           // (NaN hides from the maximum and shows in the sum)
   uint32_t value = ordered(m);
   int at = VD_NONE;
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
   const bool any = row0 >= 0 && n >= 0;                               // rows outside of the logits: no token
   const float t = temperature[r];
   const bool greedy = !(t > 0.f);
-  const float c = VD_LOG2E / (greedy ? 1.f : t);
+  const float c = factor(t);
   const float* e = noise + (size_t)r * noise_ld;
   const int share = (V >> shift) + 1, begin = min(V, rank * share), end = min(V, begin + share);
   // what a draft is decided by: lane j of warp w has row w + VP_WARPS j
@@ -245,16 +248,16 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
       all = warp_join(p.key, p.sum, c);
     }
     if (lane == i / VP_WARPS) {
-      const float m = unordered((uint32_t)(all.key >> 32)), ref = reference(m, c);
+      const float m = unordered((uint32_t)(all.key >> 32)), y = (xd - base_of(m)) * c;
       const bool finite = fabsf(m) < INFINITY;
       Row w;
       w.m = finite ? m : INFINITY;
       w.s = finite ? all.sum : 1.f;
       w.at = index_of(all.key);
       w.d = d;
-      const float p = d < 0 || d >= V ? 0.f : greedy || !finite ? (d == w.at ? 1.f : 0.f) : hb_exp2(fmaf(xd, c, -ref)) / all.sum;
+      const float p = d < 0 || d >= V ? 0.f : greedy || !finite ? (d == w.at ? 1.f : 0.f) : hb_exp2(y) / all.sum;
       w.ok = ud * qd < p;
-      w.logp = finite ? fmaf(xd, c, -ref) * VD_LN2 - logf(all.sum) : 0.f;
+      w.logp = finite ? y * VD_LN2 - logf(all.sum) : 0.f;
       rows[i] = w;
     }
   }
@@ -264,7 +267,6 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
   while (taken < n && rows[taken].ok) taken++;
   const Row s = any ? rows[taken] : Row{INFINITY, 1.f, -1, 0, -1, 0.f};
   const bool point = greedy || !(s.m < INFINITY);
-  const float ref = reference(s.m, c);
   const T* x = logits + (size_t)(row0 + taken) * ld;
   int final = s.at;
   if (!point) {
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
           }
 #pragma unroll
           for (int u = 0; u < U; u++) {
-            float w = hb_exp2(fmaf(xs[u], c, -ref));                  // (the sum matters beside q alone)
+            float w = hb_exp2((xs[u] - s.m) * c);                  // (the sum matters beside q alone)
             if (WITH_Q) w = fmaf(w, inv, -qs[u]);
             float score = w * reciprocal(es[u]);                      // infinite without noise
             if (U == 1) score = w > 0.f ? fmaxf(score, 0.f) : -1.f;   // (attempts after the first; NaN counts as 0)
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
       lp = rows[i].logp;
     } else if (any && i == taken) {
       token = final;
-      if (s.m < INFINITY) lp = fmaf(hb_to_float(x[final]), c, -ref) * VD_LN2 - logf(s.s);
+      if (s.m < INFINITY) lp = (hb_to_float(x[final]) - s.m) * c * VD_LN2 - logf(s.s);
     }
     tokens[(size_t)r * (K + 1) + i] = token;
     logprobs[(size_t)r * (K + 1) + i] = lp;
