@@ -158,7 +158,7 @@ def sample_many(engine, prompt, n, n_new, temperature, seed, n_draft, stop_token
     runner, prompt = engine.runner, [int(t) for t in prompt]
     if not prompt or any(not 0 <= t < engine.vocab for t in prompt):
         raise ValueError(f"sample_many needs a prompt of tokens below {engine.vocab}")
-    if n < 1 or n_new < 1 or temperature < 0:
+    if n < 1 or n_new < 1 or not temperature >= 0:      # (a NaN too)
         raise ValueError(f"sample_many: {n} samples of {n_new} tokens at temperature {temperature}")
     if not 0 <= n_draft <= ops.MAX_DRAFTS:
         raise ValueError(f"sample_many: {n_draft} drafts a step, 0 to {ops.MAX_DRAFTS} are possible")
