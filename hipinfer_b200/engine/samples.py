@@ -101,13 +101,39 @@ class Sampling:
                     self.runner.fork(self.rids[0], rid)
         return logits
 
+    def _behind(self, i) -> int:
+        """Tokens of sample i that are still to be run: its newest, and in a fork's first step the prompt's last, partial page."""
+        return len(self.texts[i].tokens) - self.runner.length(self.rids[i])
+
     def _step(self, live) -> None:
+        """The live samples' newest tokens with drafts behind them, in one step where there are no more samples than a step may have rows."""
+        if sum(map(self._behind, live)) > self.max_prefill:
+            self._catch_up(live)
+        for at in range(0, len(live), self.max_prefill):
+            self._step_of(live[at:at + self.max_prefill])
+
+    def _catch_up(self, live) -> None:
+        """All but their newest tokens, which do not fit into one step beside each other."""
+        entries, room = [], self.max_prefill
+        for i in live:
+            at, rows = self.runner.length(self.rids[i]), self.texts[i].tokens[:-1]
+            while at < len(rows):
+                part = rows[at:at + room]
+                entries.append(StepEntry(self.rids[i], part, []))
+                at, room = at + len(part), room - len(part)
+                if not room:
+                    self.runner.step(entries)
+                    entries, room = [], self.max_prefill
+        if entries:
+            self.runner.step(entries)
+
+    def _step_of(self, live) -> None:
+        most = min(self.n_draft, (self.max_prefill - sum(map(self._behind, live))) // len(live))      # (the rest of the step's rows)
         entries, starts, drafts, row = [], [], [], 0
         for i in live:
             text = self.texts[i]
-            d = text.propose(min(self.n_draft, self.n_new - len(self.outputs[i]) - 1))
-            held = self.runner.length(self.rids[i])          # a fork's first step also runs the prompt's last, partial page
-            rows = text.tokens[held:] + d
+            d = text.propose(min(most, self.n_new - len(self.outputs[i]) - 1))
+            rows = text.tokens[-self._behind(i):] + d
             entries.append(StepEntry(self.rids[i], rows, range(len(rows) - 1 - len(d), len(rows))))
             starts.append(row)
             drafts.append(d)
