@@ -50,7 +50,8 @@ class StepBatch:
     max_q_len: int = 0
     extra: dict = field(default_factory=dict)  # what a kernel dispatcher derived for this batch (cached per step)
     short_list: Optional[torch.Tensor] = None  # int32: rows of requests with fewer than SHORT_ROWS rows, in a step with longer ones
-    shared: Sequence[list] = ()   # per cache group: (first request, requests, tokens) that hold the same pages (shared_prefixes)
+    shared: Sequence[list] = ()   # per cache group: (first request, requests, tokens) that hold the same pages (shared_prefixes), for
+                                  # groups with layers of Mixer.reads_shared_pages
     dump: Optional[dict] = None   # debug: planes of the step are recorded here, keyed (order index, name) (parts/planes.py)
     dump_step: int = -1           # the order index the decoder is at
 

@@ -178,11 +178,12 @@ class ModelRunner:
         return logits
 
     def _shared_prefixes(self, tables, ctx_lens):
-        """Per cache group that keeps everything, the neighbours in this step that hold the same pages (of forked requests)."""
+        """Per cache group that keeps everything and whose layers make use of it, the neighbours in this step that hold the same pages
+        (of forked requests)."""
         if not self._forked:
             return ()
-        return [shared_prefixes([t[g] for t in tables], ctx_lens, self.page_size) if spec.kind == "full" else []
-                for g, spec in enumerate(self.cache.groups)]
+        return [shared_prefixes([t[g] for t in tables], ctx_lens, self.page_size) if spec.kind == "full" and self.model.shared_layers[g]
+                else [] for g, spec in enumerate(self.cache.groups)]
 
     # A decode-only step of forked requests may be replayed from its graph, every request reading all its pages, or run eagerly with
     # attention over the shared pages (whose plan changes every step). Reading is 6 TB/s; launching a layer eagerly takes the host
@@ -191,8 +192,9 @@ class ModelRunner:
     SHARED_STEP_BYTES = 0.7e9
 
     def _saved_bytes(self, shared) -> float:
-        """Bytes of the cache that a step reads once instead of once a request."""
-        per_token = [spec.elements_per_token() * torch.empty((), dtype=self.dtype).element_size() for spec in self.cache.groups]
+        """Bytes of the cache that the step's layers read once instead of once a request."""
+        per_token = [spec.elements_per_token() // spec.n_layers * n * self.dtype.itemsize
+                     for spec, n in zip(self.cache.groups, self.model.shared_layers)]
         return sum((n - 1) * tokens * b for runs, b in zip(shared, per_token) for _, n, tokens in runs)
 
     def _table_rows(self, rc):

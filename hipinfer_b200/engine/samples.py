@@ -1,5 +1,6 @@
 """Many continuations of one prompt. The prompt is run once; every sample is a fork of it that holds the prompt's pages, so that a step
-reads their keys and values once for all samples (ops.attention_shared). A sample brings its newest token and, after it, tokens drafted by
+reads their keys and values once for all samples (ops.attention_shared) where a layer's attention does that
+(Mixer.reads_shared_pages: attention without a window; others share the memory alone). A sample brings its newest token and, after it, tokens drafted by
 looking up what followed the same tokens earlier in its own text; the step's logits accept or refuse them (ops.verify_drafts), and the
 cache gives back what was refused. What is drawn is distributed as if each token had been drawn alone.
 

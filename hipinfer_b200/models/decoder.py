@@ -89,6 +89,9 @@ class DecoderModel:
             counts[g] += 1
         self.cache_groups = [CacheGroupSpec(f"{k[0]}{k[1] or ''}-h{k[2]}-d{k[3]}" + "".join(f"-{p[0]}" for p in k[4]),
                                             k[0], n, k[2], k[3], k[1], k[4], k[5]) for k, n in zip(keys, counts)]
+        # per group: layers of the order whose attention reads pages that requests share once for all of them
+        self.shared_layers = [sum(plan is not None and plan.group == g and getattr(self.layers[st.layer].mixer, "reads_shared_pages", False)
+                                  for plan, st in zip(self.cache_plan, self.spec.order)) for g in range(len(keys))]
 
     # ---------------------------------------------------------------- weights
     def param_specs(self):

@@ -34,6 +34,7 @@ class AttentionMixer(Mixer):
         if self.n_heads % self.n_kv_heads:
             raise ValueError(f"attention: {self.n_heads} heads are not a multiple of {self.n_kv_heads} kv heads")
         self.window = int(p.get("window") or 0)
+        self.reads_shared_pages = not self.window and self.head_dim <= 256      # (ops.attention)
         self.scale = float(p.get("scale") or 1.0 / math.sqrt(self.head_dim))
         self.names = {k: prefix + p.get(k + "_name", f"self_attn.{k}_proj.weight") for k in ("q", "k", "v", "o")}
         self.position = build_part("position", p["position"], ctx, prefix)

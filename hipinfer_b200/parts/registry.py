@@ -85,6 +85,9 @@ class Part:
 
 
 class Mixer(Part):
+    # Its attention reads the pages that neighbours in a step hold together once for all of them (StepBatch.shared).
+    reads_shared_pages = False
+
     def cache_need(self) -> Optional[CacheNeed]:
         return None
 
