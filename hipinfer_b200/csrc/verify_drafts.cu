@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(VP_THREADS, 4) verify_pick_kernel(const T* log
   const int rank = (int)hb_cluster_ctarank(), shift = __ffs(ranks) - 1, r = blockIdx.x >> shift;      // (a power of two)
   // The rows' kernel lets this one start behind its own wait: everything but its parts is in place.
   const int row0 = start[r], n = min(clamped(n_drafts[r], K), T_rows - 1 - row0);
-  const bool any = row0 >= 0 && n >= 0;                               // rows outside of the logits: no token
+  const bool any = row0 >= 0 && n >= 0;                               // the first row outside of the logits: no token (the last ones: fewer drafts)
   const float t = temperature[r];
   const bool greedy = !(t > 0.f);
   const float c = factor(t);

@@ -184,7 +184,8 @@ def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Ten
 
     Returns (tokens int32 [R, K + 1]: accepted drafts, the token behind them, -1; counts int32 [R]: how many tokens; logprobs float32 [R, K + 1]:
     log p_i of each, at temperature 1 for a greedy request, 0 for a row without a finite largest logit and behind the last). A request whose
-    rows lie outside the logits gets no token."""
+    first row lies outside the logits gets no token; where only its last ones do, the drafts that have no row behind them are not looked
+    at, and the last row that is there is the one behind all drafts."""
     if logits.is_cuda:
         bound = _binding() if _bound is None else _bound
         if bound:
