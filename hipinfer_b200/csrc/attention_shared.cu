@@ -639,7 +639,9 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   const SharedToken* tokens = (const SharedToken*)(plan + h->off_tokens);
   const int vec = aligned && D % 4 == 0;
   const float sl2 = fmaxf(scale * 1.4426950408889634f, 1.17549435e-38f);      // (masked scores are -inf ahead of it: 0 would make them NaN)
-  if (h->ctas > 0 && h->tensor_cores && aligned) {
+  if (T == 1) ldq = (long)Hq * D;                        // (one row has no stride)
+  // rows of q that lie over each other (one row for all, say) have no copies by boxes: they go the way of those off 16 bytes
+  if (h->ctas > 0 && h->tensor_cores && aligned && ldq >= (long)Hq * D) {
     if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, items, cta_items, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
   } else if (h->ctas > 0) {
     int r = -1;
