@@ -601,11 +601,13 @@ int launch_items(const void* q, long ldq, const void* kc, const void* vc, const 
                  int ctas, int max_rows, int narrow, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int vec, cudaStream_t s) {
   constexpr int smem = ItemsShared<NC>::BYTES;
   auto kern = shared_items_kernel<T, NC>;
-  static bool configured = false;
-  if (!configured) {
+  static bool configured[64] = {};      // the attribute belongs to a device: set once on each
+  int dev = -1;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) HB_FAIL("hb_shared_items: %s", cudaGetErrorString(e));
-    configured = true;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int blocks = (max_rows + 63) / 64;
   const cudaError_t e = hb_launch(kern, dim3(ctas, blocks < 65535 ? blocks : 65535), SI_THREADS, smem, s, (const T*)q, ldq, (const T*)kc, (const T*)vc, bt,

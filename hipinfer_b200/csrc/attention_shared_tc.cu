@@ -573,16 +573,18 @@ int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, 
   // new one waits for the product before: 64 users 33 us at 8, 39 at 2. Calls of fewer than 256 rows times heads take as long with either.
   const float slack = (long)T * Hq < 256 ? 1.f : 8.f;
   cudaError_t e = cudaSuccess;
+  int dev = -1;
+  cudaGetDevice(&dev);
 #define ST_LAUNCH(DD)                                                                                                               \
-  do {                                                                                                                             \
-    static bool configured = false;                                                                                                \
-    if (!configured) {                                                                                                             \
+  do {                                                                                                                              \
+    static bool configured[64] = {}; /* the attribute belongs to a device: set once on each */                                      \
+    if (dev < 0 || dev >= 64 || !configured[dev]) {                                                                                 \
       e = cudaFuncSetAttribute(shared_items_tc_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, st_smem<DD>());             \
       if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));                                               \
-      configured = true;                                                                                                           \
-    }                                                                                                                              \
+      if (dev >= 0 && dev < 64) configured[dev] = true;                                                                             \
+    }                                                                                                                               \
     e = hb_launch(shared_items_tc_kernel<DD>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, items, cta_items,      \
-                  part_o, part_ml, Hkv, G, page_size, scale_log2, slack, status);                                        \
+                  part_o, part_ml, Hkv, G, page_size, scale_log2, slack, status);                                                 \
   } while (0)
   if (D == 64) ST_LAUNCH(64);
   else ST_LAUNCH(128);

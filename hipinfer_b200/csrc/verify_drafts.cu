@@ -376,11 +376,13 @@ cudaError_t launch_pick(const Cut& k, const void* logits, long ld, int T_rows, i
                         const float* temperature, const float* uniform, const float* noise, long noise_ld, const void* probs, long probs_r,
                         long probs_i, const RowPart* parts, int* tokens, int* counts, float* logprobs, cudaStream_t s) {
   auto kern = verify_pick_kernel<T, Q>;
-  static bool configured = false;
-  if (!configured) {
+  static bool configured[64] = {};      // the attribute belongs to a device: set once on each
+  int dev = -1;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    configured = true;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   return hb_launch_cluster(kern, dim3((unsigned)R * k.ranks), VP_THREADS, 0, s, dim3(k.ranks, 1, 1), (const T*)logits, ld, T_rows, V, start, n_drafts, drafts, K,
                            temperature, uniform, noise, noise_ld, (const Q*)probs, probs_r, probs_i, parts, k.slices, tokens, counts, logprobs);
