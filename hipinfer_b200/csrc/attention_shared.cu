@@ -619,7 +619,7 @@ int launch_items(const void* q, long ldq, const void* kc, const void* vc, const 
 }  // namespace
 
 // What a call has of its plan, in host memory: the numbers that the launches want.
-struct SharedLaunch { int T, ctas, max_rows, narrow, parts, tensor_cores, dt, Hq, Hkv, D, page_size, off_items, off_ctas, off_tokens; };
+struct SharedLaunch { int T, ctas, max_rows, narrow, parts, tensor_cores, dt, Hq, Hkv, D, page_size, off_items, off_ctas, off_tokens, masked; };
 
 // q [T, ldq] (heads of D side by side), caches [num_pages, Hkv, page_size, D], bt [R, bt_stride], plan on the device (see shared_plan.cu) and `h` of it;
 // workspace parts * (D + 2) + 4 floats, 16-byte aligned; out [T, Hq, D]. aligned: rows of q, pages and out start on 16 bytes. `status` is set to 1 if
@@ -644,7 +644,7 @@ HB_EXPORT int hb_attention_shared(const void* q, long ldq, const void* kc, const
   if (T == 1) ldq = (long)Hq * D;                        // (one row has no stride)
   // rows of q that lie over each other (one row for all, say) have no copies by boxes: they go the way of those off 16 bytes
   if (h->ctas > 0 && h->tensor_cores && aligned && ldq >= (long)Hq * D) {
-    if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, items, cta_items, h->ctas, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
+    if (hb_shared_items_tc(q, ldq, kc, vc, num_pages, bt, bt_stride, items, cta_items, h->ctas, h->masked, T, part_o, part_ml, Hq, Hkv, D, ps, sl2, status, s)) return -1;
   } else if (h->ctas > 0) {
     int r = -1;
 #define SI_LAUNCH(NC) \

@@ -13,9 +13,11 @@
 //   K and V loaders TMA, a page and 64 columns a box, a lane holds a page's number; Q comes with K, one box of (64 columns, heads, tokens).
 // The accumulator is rescaled only when a row's maximum grew by more than a power of 2 (any reference value gives the same quotient).
 // V rows outside of the item's range, which may hold anything, are set to zero in shared memory by the softmax threads that mask them: P
-// is 0 there, and 0 times an infinity is no 0. (Keys inside of the range that a row of the item does not see, as only portions of more than
-// SP_FRESH rows have them, do meet a P of 0: a value there that is not finite makes the rows before it NaN.) Every wait is bounded; both chains wait
-// for and release every tile and every Q, so that a barrier is never more than a phase ahead of one that waits for it.
+// is 0 there, and 0 times an infinity is no 0. For the same reason, where a step has keys that some rows of the item do not see (portions of more
+// than SP_FRESH rows), values that are not finite are looked for, set to zero, and make the rows that do see them NaN (scan_values).
+// That is an instance of the kernel by itself: a portion of 4,096 rows of 32 heads of 128 takes 210 us, 194 without, and the registers cost
+// steps without such keys 2 to 5 %. Every wait is bounded; both chains wait for and release every tile and every Q, so that a barrier is never
+// more than a phase ahead of one that waits for it.
 //
 // What bounds it: with many rows the softmax (a step is 64 exponentials of 128 rows for two products of 128 x 64 x D; two warps share a scheduler):
 // 384 rows of 32 heads over 8 of 128 behind 24,560 shared tokens take 143 us, 1,082 TFLOP/s. With few rows the memory: 32 requests of one row
@@ -37,6 +39,8 @@ template <int D> struct StSizes {
 template <int D> struct StBars {
   uint64_t q_full[2], q_free[2], k_full[StSizes<D>::NK], k_free[StSizes<D>::NK], v_full[StSizes<D>::NV], v_free[StSizes<D>::NV];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];      // [chain][step & 1]
+  uint64_t scanned[2];                                     // a chain's warps have all looked through a step's values
+  alignas(8) uint32_t bad[StSizes<D>::NV][4];              // a tile's values that are not finite, a bit a row
   uint32_t tmem_slot;
   int abort_flag;
   alignas(16) SharedItem kept[ST_KEPT];
@@ -180,6 +184,38 @@ template <int D> __device__ __noinline__ void scale_rows(uint32_t tmem_o, float 
   }
 }
 
+// The values of a step that not all rows of the item see, keys [lo, hi) of its 64: those that are not finite are set to zero. Two threads have a row
+// of V; what they find they mark in `bad` first, so that the other chain, which goes through the same tile of a wide item, knows of rows
+// that this one has emptied. 1: there is one among the keys up to `last`, which this thread's row sees; 2: a wait ran out.
+template <int D> __device__ __noinline__ int scan_values(uint8_t* rows, uint32_t* bad, uint64_t* bar, uint32_t parity, int lo, int hi, int last, volatile int* abort) {
+  const int row = (threadIdx.x & 127) >> 1;
+  const uint32_t mine = hb_smem_u32(rows) + row * 128 + (threadIdx.x & 1) * (D == 128 ? StSizes<D>::TILE : 64);
+  if (row >= lo && row < hi) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int q = 0; q < D / 16; q++) {
+      uint32_t x[4];
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(mine + q * 16) : "memory");
+#pragma unroll
+      for (int i = 0; i < 4; i++) found |= __vcmpeq2(x[i] & 0x7f807f80u, 0x7f807f80u);
+    }
+    if (found) {
+      atomicOr(bad + (row >> 5), 1u << (row & 31));
+      __threadfence_block();
+    }
+  }
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) hb_mbar_arrive(bar);
+  if (!__all_sync(0xffffffffu, wait_for(bar, parity, abort))) return 2;
+  const unsigned long long all = *(volatile unsigned long long*)bad;
+  if (!all) return 0;
+  if (all >> row & 1) {
+#pragma unroll
+    for (int q = 0; q < D / 16; q++) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(mine + q * 16), "r"(0) : "memory");
+  }
+  return last >= 0 && (all & (~0ull >> (63 - min(last, 63)))) != 0;
+}
+
 // The CTA's items: the first ST_KEPT of them are in shared memory.
 struct Items {
   const SharedItem *kept, *all;
@@ -203,7 +239,8 @@ __device__ __forceinline__ Work work_of(const Items& items, int it) {
   return w;
 }
 
-template <int D>
+// MASKED: there are items whose rows do not see all keys.
+template <int D, bool MASKED>
 __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const int* bt, int bt_stride,
                                                                         const SharedItem* plan_items, const int* ctas, float* part_o, float2* part_ml,
@@ -224,7 +261,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
   if (threadIdx.x == 0) {
     // (what is loaded has to be let go by both chains)
     for (int b = 0; b < 2; b++) {
-      hb_mbar_init(&bar->q_full[b], 1); hb_mbar_init(&bar->q_free[b], 2);
+      hb_mbar_init(&bar->q_full[b], 1); hb_mbar_init(&bar->q_free[b], 2); hb_mbar_init(&bar->scanned[b], 4);
       for (int h = 0; h < 2; h++) { hb_mbar_init(&bar->s_full[b][h], 1); hb_mbar_init(&bar->p_full[b][h], 4); hb_mbar_init(&bar->pv_done[b][h], 1); }
     }
     for (int b = 0; b < NK; b++) { hb_mbar_init(&bar->k_full[b], 1); hb_mbar_init(&bar->k_free[b], 2); }
@@ -293,6 +330,8 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
       }
       if (it < items.n) ahead = page(w, t);
       if (!wait(&free[stage], parity)) break;
+      if (MASKED && !is_k && lane < 4) bar->bad[stage][lane] = 0;
+      __syncwarp();
       if (hb_elect()) hb_mbar_expect_tx(&full[stage], (uint32_t)__popc(boxes) * page_size * D * 2);
       __syncwarp();
       for (int p = 0; p < places; p += 4) {       // four boxes an election
@@ -395,7 +434,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
   } else {  // ---------------- softmax: warpgroup c is chain c, a thread a query row
     const int c = warp >> 2, w4 = warp & 3;
     const uint32_t lanes = (uint32_t)(w4 * 32) << 16, tmem_s = tmem + c * 128 + lanes, tmem_o = tmem + 256 + c * 128 + lanes;
-    uint32_t m = 0, v_stage = 0, v_parity = 0;       // steps; where V is
+    uint32_t m = 0, scans = 0, v_stage = 0, v_parity = 0;       // steps, and those whose values were looked through; where V is
     bool ok = true;                // every wait's outcome is made uniform over the warp: the tensor-memory accesses below are warp-wide
     auto wait = [&](uint64_t* b, uint32_t parity) { return ok = __all_sync(0xffffffffu, wait_for(b, parity, abort_flag)); };
     const uint64_t scale2 = pack2(scale_log2, scale_log2);
@@ -404,8 +443,8 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
       const int first = w.wide ? c * RT : 0, rows = min(RT, w.e.tokens - first) * G;           // the chain's rows
       const int below = w.low && c ? 64 : 0, r = (int)(threadIdx.x & 127) - below;      // the thread's row of the chain's
       const bool idle = w4 * 32 < below || w4 * 32 - below >= rows;
-      const int last_key = min(w.e.hi - 1, w.e.pos == SP_NO_MASK ? SP_NO_MASK : w.e.pos + first + r / G);
-      const int sure = w.e.pos == SP_NO_MASK ? w.e.hi : min(w.e.hi, w.e.pos + first + 1);      // the keys below are seen by all rows
+      const int last_key = !MASKED || w.e.pos == SP_NO_MASK ? w.e.hi - 1 : min(w.e.hi - 1, w.e.pos + first + r / G);
+      const int sure = !MASKED || w.e.pos == SP_NO_MASK ? w.e.hi : min(w.e.hi, w.e.pos + first + 1);      // the keys below are seen by all rows
       float m_run = -INFINITY, l_run = 0.f;
       const uint32_t m0 = m;
       for (int i = 0; i < w.tiles && ok; i++) {
@@ -416,14 +455,22 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_items_tc_kernel(const __
           if (!wait(&bar->s_full[c][m & 1], m >> 1 & 1)) break;
           hb_tc_fence_after();
           const bool cut = k_base < w.e.lo || k_base + 64 > w.e.hi;
-          if (cut) {      // the rows of V, of the step's keys, where the item does not reach: a thread has half of one
-            const int row = 64 * h + ((threadIdx.x & 127) >> 1);
+          const bool open = MASKED && k_base + 64 > w.e.pos + 1;      // some row does not see all keys (the same steps for both chains of a wide item)
+          if (cut || open) {
             if (!wait(&bar->v_full[v_stage], v_parity)) break;
+            // the rows of V, of the step's keys, where the item does not reach: a thread has half of one
+            const int row = 64 * h + ((threadIdx.x & 127) >> 1);
             if (tile + row < w.e.lo || tile + row >= w.e.hi) {
               const uint32_t dst = hb_smem_u32(sV + v_stage * OPND) + row * 128 + (threadIdx.x & 1) * (D == 128 ? TILE : 64);
 #pragma unroll
               for (int q = 0; q < D / 16; q++)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + q * 16), "r"(0) : "memory");
+            }
+            if (open) {
+              const int found = scan_values<D>(sV + v_stage * OPND + 64 * h * 128, &bar->bad[v_stage][2 * h], &bar->scanned[c], scans++ & 1,
+                                               max(w.e.lo, w.e.pos + 1) - k_base, w.e.hi - k_base, last_key - k_base, abort_flag);
+              if (!(ok = found != 2)) break;
+              if (found == 1) l_run = __uint_as_float(0x7fc00000u);
             }
             hb_fence_proxy_async();
           }
@@ -547,7 +594,7 @@ HB_EXPORT int hb_shared_items_tc_supported(int Hq, int Hkv, int D, int page_size
 }
 
 int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const SharedItem* items,
-                       const int* cta_items, int ctas, int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s) {
+                       const int* cta_items, int ctas, int masked, int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s) {
   if (!hb_shared_items_tc_supported(Hq, Hkv, D, page_size))
     HB_FAIL("hb_shared_items_tc: %d/%d heads of %d with pages of %d are not supported", Hq, Hkv, D, page_size);
   if (ctas <= 0 || T <= 0) return 0;
@@ -575,19 +622,21 @@ int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, 
   cudaError_t e = cudaSuccess;
   int dev = -1;
   cudaGetDevice(&dev);
-#define ST_LAUNCH(DD)                                                                                                               \
-  do {                                                                                                                              \
-    static bool configured[64] = {}; /* the attribute belongs to a device: set once on each */                                      \
-    if (dev < 0 || dev >= 64 || !configured[dev]) {                                                                                 \
-      e = cudaFuncSetAttribute(shared_items_tc_kernel<DD>, cudaFuncAttributeMaxDynamicSharedMemorySize, st_smem<DD>());             \
-      if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));                                               \
-      if (dev >= 0 && dev < 64) configured[dev] = true;                                                                             \
-    }                                                                                                                               \
-    e = hb_launch(shared_items_tc_kernel<DD>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, items, cta_items,      \
-                  part_o, part_ml, Hkv, G, page_size, scale_log2, slack, status);                                                 \
+#define ST_LAUNCH(DD, M)                                                                                                                    \
+  do {                                                                                                                                      \
+    static bool configured[64] = {}; /* the attribute belongs to a device: set once on each */                                              \
+    if (dev < 0 || dev >= 64 || !configured[dev]) {                                                                                         \
+      e = cudaFuncSetAttribute(shared_items_tc_kernel<DD, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, st_smem<DD>());                  \
+      if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));                                                       \
+      if (dev >= 0 && dev < 64) configured[dev] = true;                                                                                     \
+    }                                                                                                                                       \
+    e = hb_launch(shared_items_tc_kernel<DD, M>, ctas, ST_THREADS, st_smem<DD>(), s, mq, mk, mv, bt, bt_stride, items, cta_items,           \
+                  part_o, part_ml, Hkv, G, page_size, scale_log2, slack, status);                                                           \
   } while (0)
-  if (D == 64) ST_LAUNCH(64);
-  else ST_LAUNCH(128);
+  if (D == 64 && masked) ST_LAUNCH(64, true);
+  else if (D == 64) ST_LAUNCH(64, false);
+  else if (masked) ST_LAUNCH(128, true);
+  else ST_LAUNCH(128, false);
 #undef ST_LAUNCH
   if (e != cudaSuccess) HB_FAIL("hb_shared_items_tc: %s", cudaGetErrorString(e));
   HB_CHECK_LAUNCH("hb_shared_items_tc");

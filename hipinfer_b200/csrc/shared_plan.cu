@@ -218,7 +218,7 @@ HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const 
     p.deal();
     std::vector<SharedItem> items;
     std::vector<int> ctas;
-    int max_rows = 0;
+    int max_rows = 0, masked = 0;
     for (auto& list : p.lists) {
       if (list.empty()) continue;
       ctas.push_back((int)items.size());
@@ -237,6 +237,7 @@ HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const 
         x.part = s.base + (h * s.parts + k * (s.parts / s.chunks)) * rows_of;
         items.push_back(x);
         max_rows = std::max(max_rows, rows_of);
+        masked |= s.pos != SP_NO_MASK;
       }
     }
     const int n_cta = (int)ctas.size();
@@ -273,6 +274,7 @@ HB_EXPORT int hb_shared_plan(const int* q_len, const int* ctx_len, int R, const 
     out[SP_OFF_CTAS] = (int)off_ctas;
     out[SP_OFF_TOKENS] = (int)off_tokens;
     out[SP_INTS] = (int)ints;
+    out[SP_MASKED] = masked;
     static_assert(sizeof(SharedItem) == 32 && sizeof(SharedToken) == 48, "as the offsets have it");
     std::copy(items.begin(), items.end(), (SharedItem*)(out + off_items));
     std::copy(ctas.begin(), ctas.end(), out + off_ctas);

@@ -15,13 +15,13 @@ struct SharedToken {
   int pre_base, pre_n, pre_rows, own_base, own_n, own_rows, table, first, fresh, pad[3];
 };
 constexpr int SP_HEADER = 16;
-enum { SP_ITEMS, SP_CTAS, SP_PARTS, SP_TOKENS, SP_MAX_ROWS, SP_OFF_ITEMS, SP_OFF_CTAS, SP_OFF_TOKENS, SP_INTS };
+enum { SP_ITEMS, SP_CTAS, SP_PARTS, SP_TOKENS, SP_MAX_ROWS, SP_OFF_ITEMS, SP_OFF_CTAS, SP_OFF_TOKENS, SP_INTS, SP_MASKED };
 constexpr int SP_NO_MASK = 1 << 30;
 // A request of up to this many rows in the step has its rows' own keys (they are causal among themselves) added by the joining kernel; the
 // items then have no mask, and what stands behind a row, whatever it is, is never multiplied by a probability of 0.
 constexpr int SP_FRESH = 16;
 
 // The items on the tensor cores (attention_shared_tc.cu): bfloat16, for a plan whose items have up to 2 * (128 / G) tokens, of which those of up to
-// 128 / G leave two parts. scale_log2: the scale times log2(e).
+// 128 / G leave two parts. masked: whether any of them has a `pos`. scale_log2: the scale times log2(e).
 int hb_shared_items_tc(const void* q, long ldq, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const SharedItem* items,
-                       const int* cta_items, int ctas, int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s);
+                       const int* cta_items, int ctas, int masked, int T, float* part_o, float2* part_ml, int Hq, int Hkv, int D, int page_size, float scale_log2, int* status, cudaStream_t s);

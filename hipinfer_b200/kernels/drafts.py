@@ -28,7 +28,7 @@ ops._SIGS["drafts"] = {
 MAX_DRAFTS = 63
 
 # the header of a plan (csrc/shared_plan.h)
-_ITEMS, _CTAS, _PARTS, _TOKENS, _MAX_ROWS, _OFF_ITEMS, _OFF_CTAS, _OFF_TOKENS, _INTS = range(9)
+_ITEMS, _CTAS, _PARTS, _TOKENS, _MAX_ROWS, _OFF_ITEMS, _OFF_CTAS, _OFF_TOKENS, _INTS, _MASKED = range(10)
 _HEADER = 16
 
 
@@ -89,7 +89,8 @@ class SharedPlan:
         self.size, self.default_scale = 2 if dtype == torch.bfloat16 else 4, 1.0 / math.sqrt(head_dim)
         self.workspace = self.parts * (head_dim + 2) + 4           # floats
         self._launch = np.array([self.rows, self.ctas, self.max_rows, cut[1], self.parts, self.tensor_cores, ops._DT[dtype], n_heads, n_kv_heads,
-                                 head_dim, page_size, numbers[_OFF_ITEMS], numbers[_OFF_CTAS], numbers[_OFF_TOKENS]], dtype=np.int32)      # SharedLaunch of csrc/attention_shared.cu
+                                 head_dim, page_size, numbers[_OFF_ITEMS], numbers[_OFF_CTAS], numbers[_OFF_TOKENS], numbers[_MASKED]],
+                                dtype=np.int32)      # SharedLaunch of csrc/attention_shared.cu
         self.launch = self._launch.ctypes.data
         host = torch.from_numpy(numbers)
         if self.device.type == "cuda":
