@@ -187,9 +187,10 @@ class ModelRunner:
 
     # A decode-only step of forked requests may be replayed from its graph, every request reading all its pages, or run eagerly with
     # attention over the shared pages (whose plan changes every step). Reading is 6 TB/s; launching a layer eagerly takes the host
-    # 60 us more. Measured on 16 layers of 32 heads over 8 of 64 in bfloat16, ms a step from the graph and shared: 32 requests behind
-    # 8,000 tokens (0.51 GB a layer saved) 3.07 and 3.47, 64 behind 8,000 (1.03 GB) 5.16 and 4.59, 64 behind 15,000 9.27 and 5.70.
-    SHARED_STEP_BYTES = 0.7e9
+    # 50 us more. Measured on 16 layers of 32 heads over 8 of 64 in bfloat16, ms a step from the graph and shared: 32 requests behind
+    # 2,000 tokens (0.13 GB a layer saved) 1.81 and 2.44, 32 behind 8,000 (0.51 GB) 2.42 and 2.47, 64 behind 4,000 (0.52 GB) 2.95 and 2.90,
+    # 128 behind 2,000 (0.52 GB) 4.09 and 3.71, 64 behind 8,000 (1.03 GB) 3.94 and 2.95, 64 behind 15,000 5.86 and 2.99.
+    SHARED_STEP_BYTES = 0.5e9
 
     def _saved_bytes(self, shared) -> float:
         """Bytes of the cache that the step's layers read once instead of once a request."""
