@@ -1,0 +1,33 @@
+// A paged cache in 8 bits: codes [page][kv head][page_size][D], int8 or e4m3, and one float32 scale for each block of 16 places of
+// a page and head, [page][kv head][ceil(page_size / 16)]; a place's numbers are code * scale. Keys and values have their own.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_fp8.h>
+
+enum { HB_I8 = 2, HB_E4M3 = 3 };                // codes of the code types, beside HB_F32 and HB_BF16
+constexpr int C8_BLOCK = 16;                    // places that share a scale
+constexpr float C8_LEAST = 1e-30f;              // below it a block's largest number counts as this: no scale is 0 or denormal
+
+__host__ __device__ constexpr int c8_blocks(int page_size) { return (page_size + C8_BLOCK - 1) / C8_BLOCK; }
+
+// A code type: its largest number, code to number, and number (already within +- the largest) to the nearest code, ties to the even one.
+struct C8Int8 {
+  static constexpr float MOST = 127.f;
+  static __device__ __forceinline__ float value(uint8_t c) { return (float)(int8_t)c; }
+  static __device__ __forceinline__ uint8_t code(float x) { return (uint8_t)(int8_t)__float2int_rn(x); }
+};
+struct C8E4m3 {
+  static constexpr float MOST = 448.f;
+  static __device__ __forceinline__ float value(uint8_t c) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+  }
+  static __device__ __forceinline__ uint8_t code(float x) { return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+};
+
+#define C8_DISPATCH(ct, NAME, ...)                                  \
+  do {                                                              \
+    if ((ct) == HB_I8) { using CT = C8Int8; __VA_ARGS__; }          \
+    else if ((ct) == HB_E4M3) { using CT = C8E4m3; __VA_ARGS__; }   \
+    else HB_FAIL("%s: unknown code type %d", NAME, (int)(ct));      \
+  } while (0)

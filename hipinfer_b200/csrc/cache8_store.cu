@@ -1,0 +1,193 @@
+// Storing rows into a cache in 8 bits, and reading pages of it back as numbers.
+#include "cache8.cuh"
+
+// Rows of K and V [T][Hkv * D] go to the places slot[t] = page * page_size + place, in any order; of several rows for one place the last
+// counts. A block (16 places of a page) is taken over by the first row of the call that goes to it: the CTAs of that row look through all
+// slots for the others (a block's places are consecutive slots), and each of their warps has one kv head of K or V: it takes the largest |x| of
+// the block's rows, a; the block's scale becomes max(a, 1e-30) / M where a row goes to its first place, else the larger of that and what
+// it was, and where it grew the block's codes are rounded once more, to r(code * (old / new)); then the rows' codes, r(x * (1 / scale)),
+// overwrite theirs. Numbers that are not finite have no part in a; infinities become the largest code, NaN 0. All arithmetic is 32-bit,
+// each operation rounded by itself (no contraction), so that a block's bits are a matter of its rows and what it held alone.
+constexpr int C8S_WARPS = 8, C8S_ROWS = 16;
+
+// E numbers side by side, as floats, and as codes to memory.
+template <int E> __device__ __forceinline__ void c8_load(const float* p, float* x) {
+  if constexpr (E == 4) *(float4*)x = *(const float4*)p;
+  else x[0] = *p;
+}
+template <int E> __device__ __forceinline__ void c8_load(const __nv_bfloat16* p, float* x) {
+  if constexpr (E == 8) {
+    const uint4 r = *(const uint4*)p;
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  } else {
+    x[0] = __bfloat162float(*p);
+  }
+}
+template <int E> __device__ __forceinline__ void c8_store(uint8_t* p, const uint8_t* c) {
+  if constexpr (E == 8) *(uint2*)p = *(const uint2*)c;
+  else if constexpr (E == 4) *(uint32_t*)p = *(const uint32_t*)c;
+  else *p = *c;
+}
+
+// E numbers are loaded at a time; ITEMS > 0: a lane's numbers of a block (16 rows of D are 32 lanes x ITEMS x E) stay in registers between
+// the maximum and the rounding; 0: any D, loaded twice.
+template <typename CT, typename T, int E, int ITEMS>
+__global__ void __launch_bounds__(32 * C8S_WARPS) cache8_store_kernel(const T* k, const T* v, long ld_k, long ld_v, const int* slot, int n_rows, int rows_cta,
+                                                                      int Hkv, int page_size, int D, long n_slots, uint8_t* kc, uint8_t* vc, float* ks,
+                                                                      float* vs) {
+  __shared__ int win[C8_BLOCK], earlier;
+  hb_pdl_launch();
+  hb_pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, pair = blockIdx.y * C8S_WARPS + (tid >> 5), h = pair >> 1;
+  const bool mine = h < Hkv, is_v = pair & 1;
+  const T* x = (is_v ? v : k) + (long)h * D;
+  const long ld = is_v ? ld_v : ld_k;
+  const int t0 = blockIdx.x * rows_cta;
+  for (int t = t0; t < min(t0 + rows_cta, n_rows); t++) {
+    const int s = slot[t];
+    if (s < 0 || s >= n_slots) continue;
+    const int page = s / page_size, first = s % page_size / C8_BLOCK * C8_BLOCK, places = min(C8_BLOCK, page_size - first);
+    const int lo = page * page_size + first;                     // the block's places are slots lo .. lo + places - 1
+    if (t > 0 && (unsigned)(slot[t - 1] - lo) < (unsigned)places) continue;
+    __syncthreads();
+    if (tid < C8_BLOCK) win[tid] = -1;
+    if (tid == C8_BLOCK) earlier = 0;
+    __syncthreads();
+    for (int i = tid; i < n_rows; i += 32 * C8S_WARPS) {
+      const unsigned place = (unsigned)(slot[i] - lo);
+      if (place < (unsigned)places) {
+        if (i < t) earlier = 1;
+        atomicMax(&win[place], i);
+      }
+    }
+    __syncthreads();
+    if (earlier) continue;                                       // (uniform; the next round's first barrier is behind every read)
+    if (!mine) continue;
+    uint8_t* at = (is_v ? vc : kc) + ((long)page * Hkv + h) * page_size * D + (long)first * D;
+    float* scale = (is_v ? vs : ks) + ((long)page * Hkv + h) * c8_blocks(page_size) + first / C8_BLOCK;
+    const bool fresh = win[0] >= 0;
+    const float old = fresh ? 0.f : *scale;
+    const int pieces = D / E, items = places * pieces;           // piece i: place i / pieces, numbers i % pieces * E ..
+    float kept[ITEMS ? ITEMS : 1][E], most = 0.f;
+    const auto largest = [&](const float* y) {
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (fabsf(y[e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(y[e]));
+    };
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int j = 0; j < ITEMS; j++) {
+        const int i = j * 32 + lane, row = win[i / pieces];
+        if (row >= 0) c8_load<E>(x + row * ld + i % pieces * E, kept[j]);
+        else
+#pragma unroll
+          for (int e = 0; e < E; e++) kept[j][e] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < ITEMS; j++) largest(kept[j]);
+    } else {
+      for (int i = lane; i < items; i += 32)
+        if (win[i / pieces] >= 0) {
+          c8_load<E>(x + win[i / pieces] * ld + i % pieces * E, kept[0]);
+          largest(kept[0]);
+        }
+    }
+    float now = __fdiv_rn(fmaxf(hb_warp_max(most), C8_LEAST), CT::MOST);
+    if (!fresh && now > old) {
+      const float f = __fdiv_rn(old, now);
+      for (int i = lane; i < items; i += 32)
+        if (win[i / pieces] < 0) {
+          uint8_t c[E];
+#pragma unroll
+          for (int e = 0; e < E; e++) c[e] = CT::code(__fmul_rn(CT::value(at[(long)i * E + e]), f));
+          c8_store<E>(at + (long)i * E, c);
+        }
+    } else if (!fresh) {
+      now = old;
+    }
+    if (lane == 0) *scale = now;
+    const float inv = __fdiv_rn(1.f, now);
+    const auto put = [&](int i, const float* y) {
+      __align__(8) uint8_t c[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float z = __fmul_rn(y[e], inv);
+        c[e] = CT::code(z != z ? 0.f : fminf(fmaxf(z, -CT::MOST), CT::MOST));
+      }
+      c8_store<E>(at + (long)i * E, c);
+    };
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int j = 0; j < ITEMS; j++)
+        if (win[(j * 32 + lane) / pieces] >= 0) put(j * 32 + lane, kept[j]);
+    } else {
+      for (int i = lane; i < items; i += 32)
+        if (win[i / pieces] >= 0) {
+          c8_load<E>(x + win[i / pieces] * ld + i % pieces * E, kept[0]);
+          put(i, kept[0]);
+        }
+    }
+  }
+}
+
+// ct: HB_I8 or HB_E4M3; dt: the rows' type. n_pages * page_size places; slots outside of them (negative ones among them) store nothing.
+HB_EXPORT int hb_cache8_store(const void* k, const void* v, long ld_k, long ld_v, int dt, const int* slot, int n_rows, int Hkv, int page_size,
+                              int D, long n_pages, int ct, void* kc, void* vc, float* ks, float* vs, cudaStream_t st) {
+  if (n_rows <= 0) return 0;
+  if (Hkv < 1 || Hkv > 65535 || page_size < 1 || D < 1 || n_pages * page_size > 0x7fffffffL)
+    HB_FAIL("hb_cache8_store: %d kv heads of %d, %ld pages of %d", Hkv, D, n_pages, page_size);
+  const size_t size = dt == HB_F32 ? 4 : 2;
+  // 16 bytes of a row at a time
+  const bool wide = (D == 64 || D == 128) && page_size % C8_BLOCK == 0 &&
+                    !(((uintptr_t)k | (uintptr_t)v | ld_k * size | ld_v * size | (uintptr_t)kc | (uintptr_t)vc) & 15);
+  // a row a CTA while those that have nothing to do are few, else as many as a block has places
+  const int rows_cta = n_rows <= 512 ? 1 : C8S_ROWS;
+  const dim3 grid((n_rows + rows_cta - 1) / rows_cta, (2 * Hkv + C8S_WARPS - 1) / C8S_WARPS);
+#define C8S_LAUNCH(E, ITEMS)                                                                                                                        \
+  hb_launch(cache8_store_kernel<CT, TA, E, ITEMS>, grid, dim3(32 * C8S_WARPS), 0, st, (const TA*)k, (const TA*)v, ld_k, ld_v, slot, n_rows, rows_cta, \
+            Hkv, page_size, D, n_pages * page_size, (uint8_t*)kc, (uint8_t*)vc, ks, vs)
+  C8_DISPATCH(ct, "hb_cache8_store", HB_DISPATCH_1(dt, "hb_cache8_store", {
+    constexpr int E = 16 / sizeof(TA);
+    if (wide && D == 64) C8S_LAUNCH(E, 64 / (2 * E));
+    else if (wide) C8S_LAUNCH(E, 128 / (2 * E));
+    else C8S_LAUNCH(1, 0);
+  }));
+#undef C8S_LAUNCH
+  HB_CHECK_LAUNCH("hb_cache8_store");
+  return 0;
+}
+
+// Page i of the output [n][Hkv][page_size][D] is page table[index[i]] of the cache (table[i] without an index); a number outside of the
+// cache's pages gives zeros.
+template <typename CT, typename T>
+__global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, const int* table,
+                                                            const int* index, long n_pages, int Hkv, int page_size, int D, T* k, T* v) {
+  hb_pdl_launch();
+  hb_pdl_wait();
+  const long i = blockIdx.x;
+  const bool is_v = blockIdx.y;
+  const uint8_t* codes = is_v ? vc : kc;
+  const float* scales = is_v ? vs : ks;
+  T* out = (is_v ? v : k) + i * Hkv * page_size * D;
+  const long page = table[index ? index[i] : i];
+  const bool there = page >= 0 && page < n_pages;
+  for (int j = threadIdx.x; j < Hkv * page_size * D; j += 256) {
+    const int h = j / (page_size * D), place = j / D % page_size;
+    out[j] = hb_from_float<T>(there ? CT::value(codes[page * Hkv * page_size * D + j]) *
+                                          scales[(page * Hkv + h) * c8_blocks(page_size) + place / C8_BLOCK] : 0.f);
+  }
+}
+
+HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, const float* vs, int ct, const int* table, const int* index, long n,
+                               long n_pages, int Hkv, int page_size, int D, void* k, void* v, int dt, cudaStream_t st) {
+  if (n <= 0) return 0;
+  if (n > 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || (long)Hkv * page_size * D > 0x7fffffffL - 256)
+    HB_FAIL("hb_cache8_expand: %ld pages of %d heads, %d places and %d", n, Hkv, page_size, D);
+  C8_DISPATCH(ct, "hb_cache8_expand", HB_DISPATCH_1(dt, "hb_cache8_expand",
+      hb_launch(cache8_expand_kernel<CT, TA>, dim3(n, 2), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n_pages,
+                Hkv, page_size, D, (TA*)k, (TA*)v)));
+  HB_CHECK_LAUNCH("hb_cache8_expand");
+  return 0;
+}

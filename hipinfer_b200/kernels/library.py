@@ -38,10 +38,12 @@ LIBRARIES: Dict[str, List[str]] = {
     "seqmix": ["seqmix_entry.cu", "attention_masked.cu", "attention_masked_flash.cu", "attention_masked_heads.cu", "latent.cu", "gla.cu"],
     "hybrid": ["hybrid_entry.cu", "hyper_streams.cu", "ssd.cu", "moe.cu", "selective_scan.cu"],
     "drafts": ["drafts_entry.cu", "shared_plan.cu", "attention_shared.cu", "attention_shared_tc.cu", "verify_drafts.cu"],
+    "cache8": ["cache8_entry.cu", "cache8_store.cu", "cache8_attention.cu", "copy_pages.cu"],
     "memory": ["memory_entry.cu", "matrix_state.cu", "depth_average.cu"],
     "fast": ["fast_entry.cu", "gemm_tc.cu", "gemm_stream.cu", "gemm_stream_consumers.cu", "gemm_rows.cu", "gemm_split.cu", "attention_fast.cu", "attention_prefill.cu", "attention_prefill_tc.cu", "attention_diff_tc.cu", "wait_selftest.cu"],
 }
 HEADERS = ["common.cuh", "tc_common.cuh", "gemm_stream_static.h", "shared_plan.h"]
+OWN_HEADERS: Dict[str, List[str]] = {"cache8": ["cache8.cuh"]}      # headers of one library alone
 
 
 # binding name -> its source; the module is called hipinfer_b200_<name>_binding
@@ -72,7 +74,7 @@ def _nvcc() -> str:
 def _stamp(name: str) -> str:
     h = hashlib.sha256()
     h.update(" ".join(NVCC_FLAGS).encode())
-    for rel in LIBRARIES[name] + HEADERS:
+    for rel in LIBRARIES[name] + HEADERS + OWN_HEADERS.get(name, []):
         p = os.path.join(CSRC, rel)
         if os.path.isfile(p):
             with open(p, "rb") as f:
