@@ -1,0 +1,483 @@
+// Attention over a paged cache in 8 bits on warp MMAs: heads of 64 or 128, pages of whole blocks. Single tokens and short portions, whose time
+// is the reading of the cache.
+//
+// A TILE is up to 8 NT (row, query head) pairs of one request and kv head; a cluster of C blocks has a tile, and their warps take its keys in units
+// of 16 places (a block of the cache: one scale for K, one for V), every (4 C)th unit a warp. A warp keeps its own softmax of the units it has
+// seen and the warps and blocks are joined at the end, through shared memory and through the cluster's: no workspace, one launch.
+//
+// Scores are S^T = K Q^T and results O^T = V^T P^T, so that the 16 rows of an MMA are keys (or dimensions) and its 8 columns the pairs: eight
+// query heads fill it, where Q as the rows would leave half of it empty. The order of the dimensions within a product is free, and so K's
+// operand is what a thread has loaded: 16 bytes of key g and of key g + 8, four codes a step. V's needs two keys' codes of one dimension side by side:
+// bytes of four 16-byte loads are interleaved. Nothing goes through shared memory but the query.
+//
+// Codes are integers (or e4m3 numbers) of at most 8 significant bits, exact in f16. The query of a pair is scaled by a power of two to below 2^10 and
+// split into f16 parts: one holds all of a bf16 query, two hold 22 bits of a 32-bit one. Weights are taken at 2^7 of a running bound of the scores that
+// is raised only when a score passes it by 8 (in base 2), so that they stay below 2^15 in f16 (two parts where the rows are 32-bit), and
+// raising it, which costs a pass over the accumulators, is rare. Scales, sums and accumulators are 32-bit: V's scale multiplies a unit's product on its way
+// into the accumulator, so blocks of very unlike scales lose nothing.
+#include "cache8.cuh"
+#include "tc_common.cuh"
+
+#include <cuda_fp16.h>
+
+constexpr int C8M_WARPS = 4, C8M_RANKS = 8;      // warps of a block; blocks of a cluster at most
+
+struct C8Attend {
+  const void* q;
+  long ld_q;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  long n_pages;
+  int Hkv, upp;                // kv heads, units of a page
+  const int* bt;
+  long ld_table;
+  int table_rows, table_width;
+  const int *row_req, *pos;    // row_req null: row t is request t's
+  const int4* tiles;           // (request, its first row, first pair, pairs of its rows); null: single rows, tiles_row tiles each
+  int first_tile, tiles_row, G, window;
+  float scale_log2;
+  void* out;
+  int q_aligned;
+};
+
+// D += A B, f16 operands; D = A B without an addend.
+__device__ __forceinline__ void c8_mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void c8_mma_zero(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t c8_transpose(uint32_t x) {      // an 8 x 8 of f16, two numbers a thread
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 c8_load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 c8_load8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+
+// Four codes (two pairs) as two f16x2. int8: with the sign bit turned a byte u is code + 128, and f16 0x6400 | u is 1024 + u, exactly.
+template <typename CT> __device__ __forceinline__ void c8_halves(uint32_t w, uint32_t& lo, uint32_t& hi);
+template <> __device__ __forceinline__ void c8_halves<C8Int8>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 off = __half2half2(__ushort_as_half(0x6480));      // 1152
+  const __half2 x = __hsub2(*(const __half2*)&a, off), y = __hsub2(*(const __half2*)&b, off);
+  lo = *(const uint32_t*)&x;
+  hi = *(const uint32_t*)&y;
+}
+template <> __device__ __forceinline__ void c8_halves<C8E4m3>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+
+// PARTS numbers of f16 whose sum is x, two x at a time.
+template <int PARTS> __device__ __forceinline__ void c8_split(float x, float y, uint32_t* part) {
+  __half2 h = __floats2half2_rn(x, y);
+  part[0] = *(const uint32_t*)&h;
+  if constexpr (PARTS == 2) {
+    const float2 f = __half22float2(h);
+    h = __floats2half2_rn(x - f.x, y - f.y);
+    part[1] = *(const uint32_t*)&h;
+  }
+}
+
+template <int D> struct C8Unit {                  // what a thread holds of a unit
+  uint4 k[2][D / 64];                             // 16 codes of keys g and g + 8, of every 64 dimensions: 16 tq ..
+  uint32_t v[4][D / 32];                          // codes of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: dimensions g D / 8 ..
+};
+template <int D> __device__ __forceinline__ void c8_fetch(C8Unit<D>& u, const uint8_t* kc, const uint8_t* vc, int at, int g, int tq) {
+  const uint8_t *k = kc + (size_t)at * (C8_BLOCK * D) + g * D + tq * 16, *v = vc + (size_t)at * (C8_BLOCK * D) + tq * 2 * D + g * (D / 8);
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < D / 64; j++) u.k[i][j] = c8_load16(k + i * 8 * D + j * 64);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint8_t* p = v + ((i >> 1) * 8 + (i & 1)) * D;
+    if constexpr (D == 128) {
+      const uint4 x = c8_load16(p);
+      u.v[i][0] = x.x; u.v[i][1] = x.y; u.v[i][2] = x.z; u.v[i][3] = x.w;
+    } else {
+      const uint2 x = c8_load8(p);
+      u.v[i][0] = x.x; u.v[i][1] = x.y;
+    }
+  }
+}
+
+template <typename CT, typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(const C8Attend a) {
+  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, STEPS = D / 16, PAIRS = 8 * NT, PITCH = D + 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint2* q_sh = (uint2*)smem;                                           // [part][nt][step][lane]
+  float* o_sh = (float*)smem;                                           // [warp][pair][PITCH], over the query when it is done with
+  __shared__ float m_sh[C8M_WARPS][PAIRS], l_sh[C8M_WARPS][PAIRS], m_cta[PAIRS], l_cta[PAIRS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3, h = blockIdx.y;
+  const int ranks = gridDim.x, rank = blockIdx.x;
+  hb_pdl_launch();
+  hb_pdl_wait();
+  int r, t0, pair0, pairs;
+  if (a.tiles) {
+    const int4 t = a.tiles[a.first_tile + blockIdx.z];
+    r = t.x, t0 = t.y, pair0 = t.z, pairs = t.w;
+  } else {
+    t0 = (a.first_tile + blockIdx.z) / a.tiles_row;
+    pair0 = (a.first_tile + blockIdx.z) % a.tiles_row * PAIRS, pairs = a.G;
+    r = a.row_req ? a.row_req[t0] : t0;
+  }
+  const int n = min(PAIRS, pairs - pair0);                              // pairs of this tile
+  const int row_first = t0 + pair0 / a.G, row_last = t0 + (pair0 + n - 1) / a.G;
+  // the keys that any of its rows sees, and those that all of them see (positions of a request's rows ascend)
+  const int p_lo = a.pos[row_first], p_hi = a.pos[row_last], window = a.window > 0 ? a.window : 0x7fffffff;
+  const int see_lo = max(0, p_lo < window ? 0 : p_lo - window + 1), all_lo = p_hi < window ? 0 : p_hi - window + 1;
+  const int u_lo = see_lo / C8_BLOCK;
+  const int u_hi = r >= 0 && r < a.table_rows ? (int)min((long)(p_hi < 0 ? -1 : p_hi / C8_BLOCK), (long)a.table_width * a.upp - 1) : -1;
+  const int* table = a.bt + r * a.ld_table;
+
+  // the query: pair g of a tile of 8, the dimensions of this thread's codes
+  float col[NT][2];                                                     // of columns 2 tq, 2 tq + 1: score = product * col * the unit's scale
+  int col_hi[NT][2];                                                    // their rows' positions
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const int pair = pair0 + nt * 8 + g;
+    float x[STEPS][4], most = 0.f;
+    if (nt * 8 + g < n) {
+      const T* q = (const T*)a.q + (t0 + pair / a.G) * a.ld_q + ((long)h * a.G + pair % a.G) * D;
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        const T* p = q + (s >> 2) * 64 + tq * 16 + (s & 3) * 4;
+        if (a.q_aligned) {
+          const float4 f = hb_load4(p);
+          x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[s][e] = hb_to_float(p[e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < STEPS; s++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[s][e] = 0.f;
+    }
+    bool odd = false;
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        most = fmaxf(most, fabsf(x[s][e]));
+        odd |= !(fabsf(x[s][e]) <= 3.402823466e38f);
+      }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    odd = __shfl_xor_sync(0xffffffffu, (int)odd, 1) | odd;
+    odd = __shfl_xor_sync(0xffffffffu, (int)odd, 2) | odd;
+    // 2^e <= most < 2^(e + 1); the query times 2^(9 - e). A query that is not finite: NaN, and so are its scores
+    const int e = max(-100, (int)(__float_as_uint(most) >> 23) - 127);
+    const float up = __uint_as_float((uint32_t)(9 - e + 127) << 23), down = odd ? NAN : a.scale_log2 * __uint_as_float((uint32_t)(e - 9 + 127) << 23);
+    if (warp == 0) {                                                    // (every warp knows `down`; one writes the query)
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        uint32_t lo[PARTS], hi[PARTS];
+        c8_split<PARTS>(odd ? 0.f : x[s][0] * up, odd ? 0.f : x[s][1] * up, lo);
+        c8_split<PARTS>(odd ? 0.f : x[s][2] * up, odd ? 0.f : x[s][3] * up, hi);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) q_sh[((p * NT + nt) * STEPS + s) * 32 + lane] = make_uint2(lo[p], hi[p]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      col[nt][c] = __shfl_sync(0xffffffffu, down, (2 * tq + c) * 4);
+      const int i = nt * 8 + 2 * tq + c;
+      col_hi[nt][c] = i < n ? a.pos[t0 + (pair0 + i) / a.G] : -1;
+    }
+  }
+  __syncthreads();
+
+  float o[STEPS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+  }
+
+  const auto compute = [&](C8Unit<D>& u, int key0, float k_scale, float v_scale) {
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+    for (int st = 0; st < STEPS; st++) {
+      const uint4 &x = u.k[0][st >> 2], &y = u.k[1][st >> 2];
+      const uint32_t wx = (st & 3) == 0 ? x.x : (st & 3) == 1 ? x.y : (st & 3) == 2 ? x.z : x.w;
+      const uint32_t wy = (st & 3) == 0 ? y.x : (st & 3) == 1 ? y.y : (st & 3) == 2 ? y.z : y.w;
+      uint32_t f[4];
+      c8_halves<CT>(wx, f[0], f[2]);
+      c8_halves<CT>(wy, f[1], f[3]);
+#pragma unroll
+      for (int p = 0; p < PARTS; p++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const uint2 b = q_sh[((p * NT + nt) * STEPS + st) * 32 + lane];
+          c8_mma(s[nt], f, b.x, b.y);
+        }
+    }
+    bool raise = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const float f0 = col[nt][0] * k_scale, f1 = col[nt][1] * k_scale;
+      s[nt][0] *= f0, s[nt][1] *= f1, s[nt][2] *= f0, s[nt][3] *= f1;
+    }
+    if (key0 < all_lo || key0 + C8_BLOCK - 1 > p_lo) {                  // not all of it is seen by all rows
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int key = key0 + g + (c >> 1) * 8, hi = col_hi[nt][c & 1];
+          if (key > hi || hi - key >= window) s[nt][c] = -INFINITY;
+        }
+      if constexpr (sizeof(CT) && CT::MOST == C8E4m3::MOST) {           // a place that nobody sees may hold a NaN
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int key = key0 + 2 * tq + (i >> 1) * 8 + (i & 1);
+          if (key < see_lo || key > p_hi)
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) u.v[i][j] = 0u;
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) raise |= s[nt][c] > m[nt][c & 1] + 8.f;
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          if (mx > m[nt][c] + 8.f) {
+            const float f = hb_exp2(m[nt][c] - mx);
+            m[nt][c] = mx;
+            l[nt][c] *= f;
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) o[i][nt][c] *= f, o[i][nt][c + 2] *= f;
+          }
+        }
+    }
+    uint32_t b[PARTS][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const float b0 = (m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 7.f, b1 = (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 7.f;
+      const float w0 = hb_exp2(s[nt][0] - b0), w1 = hb_exp2(s[nt][1] - b1), w2 = hb_exp2(s[nt][2] - b0), w3 = hb_exp2(s[nt][3] - b1);
+      l[nt][0] += w0 + w2;
+      l[nt][1] += w1 + w3;
+      uint32_t x[PARTS], y[PARTS];
+      c8_split<PARTS>(w0, w1, x);
+      c8_split<PARTS>(w2, w3, y);
+#pragma unroll
+      for (int p = 0; p < PARTS; p++) b[p][nt][0] = c8_transpose(x[p]), b[p][nt][1] = c8_transpose(y[p]);
+    }
+#pragma unroll
+    for (int j = 0; j < D / 32; j++) {
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const uint32_t sel = half ? 0x7362 : 0x5140;
+        const uint32_t x = __byte_perm(u.v[0][j], u.v[1][j], sel), y = __byte_perm(u.v[2][j], u.v[3][j], sel);
+        uint32_t f[4];
+        c8_halves<CT>(x, f[0], f[1]);
+        c8_halves<CT>(y, f[2], f[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float d[4];
+          c8_mma_zero(d, f, b[0][nt][0], b[0][nt][1]);
+          if constexpr (PARTS == 2) c8_mma(d, f, b[1][nt][0], b[1][nt][1]);
+#pragma unroll
+          for (int c = 0; c < 4; c++) o[2 * j + half][nt][c] = fmaf(v_scale, d[c], o[2 * j + half][nt][c]);
+        }
+      }
+    }
+  };
+
+  // this warp's units: u_lo + id, and every (ranks * WARPS)th from there; a lane looks up one of the next 32
+  const int id = rank * C8M_WARPS + warp, stride = ranks * C8M_WARPS;
+  for (int first = u_lo + id; first <= u_hi; first += 32 * stride) {
+    const int mine = first + lane * stride;
+    int at = -1;
+    float k_scale = 0.f, v_scale = 0.f;
+    if (mine <= u_hi) {
+      const int page = table[mine / a.upp];
+      if (page >= 0 && page < a.n_pages) {
+        at = (page * a.Hkv + h) * a.upp + mine % a.upp;
+        k_scale = a.ks[at];
+        v_scale = a.vs[at];
+      }
+    }
+    const int count = min(32, (u_hi - first) / stride + 1);
+    C8Unit<D> x, y;
+    int at_x = __shfl_sync(0xffffffffu, at, 0), at_y;
+    if (at_x >= 0) c8_fetch<D>(x, a.kc, a.vc, at_x, g, tq);
+    for (int i = 0; i < count; i += 2) {
+      at_y = i + 1 < count ? __shfl_sync(0xffffffffu, at, i + 1) : -1;
+      if (at_y >= 0) c8_fetch<D>(y, a.kc, a.vc, at_y, g, tq);
+      float fk = __shfl_sync(0xffffffffu, k_scale, i), fv = __shfl_sync(0xffffffffu, v_scale, i);
+      if (at_x >= 0) compute(x, (first + i * stride) * C8_BLOCK, fk, fv);
+      at_x = i + 2 < count ? __shfl_sync(0xffffffffu, at, i + 2) : -1;
+      if (at_x >= 0) c8_fetch<D>(x, a.kc, a.vc, at_x, g, tq);
+      fk = __shfl_sync(0xffffffffu, k_scale, (i + 1) & 31), fv = __shfl_sync(0xffffffffu, v_scale, (i + 1) & 31);
+      if (at_y >= 0) compute(y, (first + (i + 1) * stride) * C8_BLOCK, fk, fv);
+    }
+  }
+
+  // the warps' results, then the blocks'
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      float x = l[nt][c];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (g == 0) {
+        m_sh[warp][nt * 8 + 2 * tq + c] = m[nt][c];
+        l_sh[warp][nt * 8 + 2 * tq + c] = x;
+      }
+    }
+  __syncthreads();                                                      // (and the query is read no more)
+  // dimension d = g D / 8 + 2 i + e lies at 16 i + 8 e + g: the lanes of a store in different banks
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int i = 0; i < STEPS; i++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        o_sh[(warp * PAIRS + nt * 8 + 2 * tq + (c & 1)) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c];
+  __syncthreads();
+  for (int pair = tid; pair < PAIRS; pair += 32 * C8M_WARPS) {
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < C8M_WARPS; w++) mx = fmaxf(mx, m_sh[w][pair]);
+#pragma unroll
+    for (int w = 0; w < C8M_WARPS; w++) {
+      const float f = m_sh[w][pair] == mx && mx == -INFINITY ? 1.f : hb_exp2(m_sh[w][pair] - mx);
+      m_sh[w][pair] = f;                                                // from here on: what the warp's result is multiplied with
+      sum += l_sh[w][pair] * f;
+    }
+    m_cta[pair] = mx;
+    l_cta[pair] = sum;
+  }
+  __syncthreads();
+  const auto place = [](int d) { return d % (D / 8) / 2 * 16 + d % 2 * 8 + d / (D / 8); };
+  T* out = (T*)a.out;
+  const auto put = [&](int pair, int d, float x, float sum) {
+    const int i = pair0 + pair;
+    out[((long)(t0 + i / a.G) * a.Hkv * a.G + (long)h * a.G + i % a.G) * D + d] = hb_from_float<T>(sum == 0.f ? 0.f : x / sum);
+  };
+  for (int i = tid; i < n * D; i += 32 * C8M_WARPS) {
+    const int pair = i / D, d = i % D;
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < C8M_WARPS; w++) x = fmaf(o_sh[(w * PAIRS + pair) * PITCH + place(d)], m_sh[w][pair], x);
+    if (ranks == 1) put(pair, d, x, l_cta[pair]);
+    else o_sh[pair * PITCH + place(d)] = x;                             // (its warp 0's number was this thread's alone)
+  }
+  if (ranks == 1) return;
+  hb_cluster_sync();
+  const uint32_t o_at = hb_smem_u32(o_sh), m_at = hb_smem_u32(m_cta), l_at = hb_smem_u32(l_cta);
+  for (int i = rank * 32 * C8M_WARPS + tid; i < n * D; i += ranks * 32 * C8M_WARPS) {
+    const int pair = i / D, d = i % D;
+    float xs[C8M_RANKS], ms[C8M_RANKS], ls[C8M_RANKS], mx = -INFINITY, x = 0.f, sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < C8M_RANKS; c++)
+      if (c < ranks) {
+        const auto far = [&](uint32_t p) {
+          uint32_t q;
+          float f;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(q) : "r"(p), "r"(c));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(q) : "memory");
+          return f;
+        };
+        xs[c] = far(o_at + (pair * PITCH + place(d)) * 4), ms[c] = far(m_at + pair * 4), ls[c] = far(l_at + pair * 4);
+      }
+#pragma unroll
+    for (int c = 0; c < C8M_RANKS; c++)
+      if (c < ranks) mx = fmaxf(mx, ms[c]);
+#pragma unroll
+    for (int c = 0; c < C8M_RANKS; c++)
+      if (c < ranks) {
+        const float f = ms[c] == mx && mx == -INFINITY ? 1.f : hb_exp2(ms[c] - mx);
+        x = fmaf(xs[c], f, x);
+        sum = fmaf(ls[c], f, sum);
+      }
+    put(pair, d, x, sum);
+  }
+  hb_cluster_sync();                                                    // nobody leaves while its numbers are read
+}
+
+template <typename CT, typename T, int D, int NT>
+static cudaError_t launch(const C8Attend& a, int tiles, int ranks, cudaStream_t st) {
+  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+  constexpr int query = PARTS * NT * (D / 16) * 32 * 8, joined = C8M_WARPS * 8 * NT * (D + 4) * 4, smem = query > joined ? query : joined;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (smem > 40 * 1024 && (dev >= 64 || !configured[dev])) {
+    e = cudaFuncSetAttribute(cache8_attention_mma_kernel<CT, T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) configured[dev] = true;
+  }
+  C8Attend b = a;
+  for (int first = 0; first < tiles; first += 65535) {                  // (the grid's limit)
+    b.first_tile = first;
+    e = hb_launch_cluster(cache8_attention_mma_kernel<CT, T, D, NT>, dim3(ranks, a.Hkv, tiles - first < 65535 ? tiles - first : 65535),
+                          dim3(32 * C8M_WARPS), smem, st, dim3(ranks, 1, 1), b);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+HB_EXPORT int hb_cache8_attention_mma_supported(int Hkv, int page_size, int D, long n_pages) {
+  return Hkv >= 1 && Hkv <= 65535 && page_size >= C8_BLOCK && page_size % C8_BLOCK == 0 && (D == 64 || D == 128) &&
+         n_pages * Hkv * (page_size / C8_BLOCK) < (1L << 31);
+}
+
+// tiles: n_tiles int4 on the device (C8Attend), pairs in tiles of 8 nt; null: n_tiles rows of one token each, whose G heads are cut into tiles of 8 nt.
+// kc and vc are 16-byte aligned.
+HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const void* kc, const void* vc, const float* ks, const float* vs, int ct,
+                                      long n_pages, int Hkv, int page_size, int D, const int* bt, long ld_table, int table_rows, int table_width,
+                                      const int* row_req, const int* pos, const int* tiles, int n_tiles, int nt, int ranks, int G, int window,
+                                      float scale, void* out, cudaStream_t st) {
+  if (n_tiles <= 0) return 0;
+  if (!hb_cache8_attention_mma_supported(Hkv, page_size, D, n_pages) || G < 1 || ranks < 1 || ranks > C8M_RANKS || (((uintptr_t)kc | (uintptr_t)vc) & 15))
+    HB_FAIL("hb_cache8_attention_mma: %d kv heads of %d for %d heads each, pages of %d, %d ranks", Hkv, D, G, page_size, ranks);
+  const size_t size = dt == HB_F32 ? 4 : 2;
+  C8Attend a = {q, ld_q, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, n_pages, Hkv, page_size / C8_BLOCK, bt, ld_table, table_rows, table_width,
+                row_req, pos, (const int4*)tiles, 0, (G + 8 * nt - 1) / (8 * nt), G, window, scale * 1.4426950408889634f, out,
+                !(((uintptr_t)q | ld_q * size) & (4 * size - 1))};
+  const int count = tiles ? n_tiles : n_tiles * a.tiles_row;
+  cudaError_t e = cudaErrorInvalidValue;
+  C8_DISPATCH(ct, "hb_cache8_attention_mma", HB_DISPATCH_1(dt, "hb_cache8_attention_mma", {
+    if (D == 64) e = nt == 1 ? launch<CT, TA, 64, 1>(a, count, ranks, st) : nt == 2 ? launch<CT, TA, 64, 2>(a, count, ranks, st) : nt == 4 ? launch<CT, TA, 64, 4>(a, count, ranks, st) : e;
+    else e = nt == 1 ? launch<CT, TA, 128, 1>(a, count, ranks, st) : nt == 2 ? launch<CT, TA, 128, 2>(a, count, ranks, st) : nt == 4 ? launch<CT, TA, 128, 4>(a, count, ranks, st) : e;
+  }));
+  if (e != cudaSuccess) HB_FAIL("hb_cache8_attention_mma: %s", cudaGetErrorString(e));
+  HB_CHECK_LAUNCH("hb_cache8_attention_mma");
+  return 0;
+}

@@ -23,6 +23,8 @@ ops._SIGS["cache8"] = {
     "hb_cache8_store": [_p, _p, _l, _l, _i, _p, _i, _i, _i, _i, _l, _i, _p, _p, _p, _p, _p],
     "hb_cache8_expand": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _p, _p, _i, _p],
     "hb_cache8_attention_any": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _f, _p, _p],
+    "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p],
+    "hb_cache8_attention_mma_supported": [_i, _i, _i, _l],
     "hb_copy_pages": [_p, _i, _p, _p, _i, _p],
 }
 BLOCK8 = 16                                                        # places of a page that share a scale
@@ -165,11 +167,56 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
         return out
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     single = batch.max_q_len == 1 and T == batch.n_requests
+    if _on_tensor_cores(cache):
+        _attend_mma(q, dt, cache, batch, table, single, n_heads // cache.n_kv_heads, int(window), scale, out)
+        return out
     ops._call("cache8", "hb_cache8_attention_any", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
               cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
               None if single else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
               out.data_ptr(), ops._stream())
     return out
+
+
+def _on_tensor_cores(cache: Cache8) -> bool:
+    """Whether the kernel on warp MMAs takes the cache's sizes and place in memory (csrc/cache8_attention_mma.cu)."""
+    return (ops.fast_kernels_on() and (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0
+            and bool(ops._fn("cache8", "hb_cache8_attention_mma_supported")(cache.n_kv_heads, cache.page_size, cache.head_dim, cache.k.shape[0])))
+
+
+def _attend_mma(q, dt, cache: Cache8, batch, table, single: bool, G: int, window: int, scale: float, out) -> None:
+    pairs = G if single else batch.max_q_len * G
+    nt = 1 if pairs <= 8 else 2 if pairs <= 16 else 4
+    tiles = None if single else _tiles(batch, G, nt)
+    n_tiles = batch.n_rows if single else tiles.shape[0]
+    keys = min(batch.max_pos + 1, window + batch.max_q_len) if window else batch.max_pos + 1
+    ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
+              cache.n_kv_heads, cache.page_size, cache.head_dim, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
+              None, batch.positions.data_ptr(), ops._ptr(tiles), n_tiles, nt,
+              _ranks(n_tiles * (-(-G // (8 * nt)) if single else 1) * cache.n_kv_heads, keys), G, window, scale, out.data_ptr(), ops._stream())
+
+
+def _ranks(tiles: int, keys: int) -> int:
+    """Blocks that share a tile's keys."""
+    ranks = 1
+    while ranks < 8 and tiles * ranks < 4 * 148 and keys > 64 * ranks:
+        ranks *= 2
+    return ranks
+
+
+def _tiles(batch, G: int, nt: int) -> torch.Tensor:
+    """int32 [tiles, 4] on the device: (request, its first row, first (row, head) pair, pairs of its rows), pairs in tiles of 8 nt."""
+    key = ("cache8 tiles", G, nt)
+    if key not in batch.extra:
+        parts = []
+        for r, (start, n) in enumerate(zip(batch.h_q_start, batch.h_q_len)):
+            first = np.arange(0, n * G, 8 * nt, dtype=np.int32)
+            part = np.empty((len(first), 4), dtype=np.int32)
+            part[:, 0], part[:, 1], part[:, 2], part[:, 3] = r, start, first, n * G
+            parts.append(part)
+        host = torch.from_numpy(np.concatenate(parts))
+        host = host.pin_memory() if batch.tokens.is_cuda else host
+        batch.extra[key] = host.to(batch.tokens.device, non_blocking=True), host       # (the host's copy until the other is over)
+    return batch.extra[key][0]
 
 
 def copy_pages(planes: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
