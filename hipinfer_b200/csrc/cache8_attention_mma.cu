@@ -8,10 +8,17 @@
 // Scores are S^T = K Q^T and results O^T = V^T P^T, so that the 16 rows of an MMA are keys (or dimensions) and its 8 columns the pairs: eight
 // query heads fill it, where Q as the rows would leave half of it empty. The order of the dimensions within a product is free, and so K's
 // operand is what a thread has loaded: 16 bytes of key g and of key g + 8, four codes a step. V's needs two keys' codes of one dimension side by side:
-// bytes of four 16-byte loads are interleaved. Nothing goes through shared memory but the query.
+// bytes of four loads are interleaved.
+//
+// A warp's units come by cp.async through a ring of its own in shared memory, two or three units ahead, so that nothing waits for another warp and the
+// registers are left to the products: with the units ahead in registers (166 of them, 12 warps an SM) every second stall was for a result of the
+// warp's own, and 64 requests of 8,000 tokens (128) took 208 us. 16-byte pieces are exchanged within a unit so that the reads of a product's operand
+// touch every bank once.
 //
 // Codes are integers (or e4m3 numbers) of at most 8 significant bits, exact in f16. The query of a pair is scaled by a power of two to below 2^10 and
-// split into f16 parts: one holds all of a bf16 query, two hold 22 bits of a 32-bit one. Weights are taken at 2^7 of a running bound of the scores that
+// split into f16 parts: one holds all of a bf16 query, two hold 22 bits of a 32-bit one. A bf16 query meets int8 keys as they are: it is rounded to
+// 16 bits of its pair's largest number, two int8 parts (2^-16 of that number is less than what bf16 keeps of it), whose products with the codes are
+// exact in integers; the keys' conversion was a sixth of all instructions. Weights are taken at 2^7 of a running bound of the scores that
 // is raised only when a score passes it by 8 (in base 2), so that they stay below 2^15 in f16 (two parts where the rows are 32-bit), and
 // raising it, which costs a pass over the accumulators, is rare. Scales, sums and accumulators are 32-bit: V's scale multiplies a unit's product on its way
 // into the accumulator, so blocks of very unlike scales lose nothing.
@@ -19,6 +26,8 @@
 #include "tc_common.cuh"
 
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 constexpr int C8M_WARPS = 4, C8M_RANKS = 8;      // warps of a block; blocks of a cluster at most
 
@@ -58,17 +67,6 @@ __device__ __forceinline__ uint32_t c8_transpose(uint32_t x) {      // an 8 x 8 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 c8_load16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 c8_load8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
-}
-
 // Four codes (two pairs) as two f16x2. int8: with the sign bit turned a byte u is code + 128, and f16 0x6400 | u is 1024 + u, exactly.
 template <typename CT> __device__ __forceinline__ void c8_halves(uint32_t w, uint32_t& lo, uint32_t& hi);
 template <> __device__ __forceinline__ void c8_halves<C8Int8>(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -94,33 +92,60 @@ template <int PARTS> __device__ __forceinline__ void c8_split(float x, float y, 
   }
 }
 
-template <int D> struct C8Unit {                  // what a thread holds of a unit
-  uint4 k[2][D / 64];                             // 16 codes of keys g and g + 8, of every 64 dimensions: 16 tq ..
-  uint32_t v[4][D / 32];                          // codes of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: dimensions g D / 8 ..
-};
-template <int D> __device__ __forceinline__ void c8_fetch(C8Unit<D>& u, const uint8_t* kc, const uint8_t* vc, int at, int g, int tq) {
-  const uint8_t *k = kc + (size_t)at * (C8_BLOCK * D) + g * D + tq * 16, *v = vc + (size_t)at * (C8_BLOCK * D) + tq * 2 * D + g * (D / 8);
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) u.k[i][j] = c8_load16(k + i * 8 * D + j * 64);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint8_t* p = v + ((i >> 1) * 8 + (i & 1)) * D;
-    if constexpr (D == 128) {
-      const uint4 x = c8_load16(p);
-      u.v[i][0] = x.x; u.v[i][1] = x.y; u.v[i][2] = x.z; u.v[i][3] = x.w;
-    } else {
-      const uint2 x = c8_load8(p);
-      u.v[i][0] = x.x; u.v[i][1] = x.y;
-    }
-  }
+// Two int8 products of 32 dimensions.
+__device__ __forceinline__ void c8_imma(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A unit in shared memory: keys' codes [16][D], then values'. Piece c (16 bytes) of key row r lies at:
+template <int D> __device__ __forceinline__ uint32_t c8_at_k(int r, int c) {
+  return D == 128 ? r * 128 + ((c ^ ((r & 1) << 2)) << 4) : r * 64 + (c << 4);
+}
+template <int D> __device__ __forceinline__ uint32_t c8_at_v(int r, int c) {
+  if constexpr (D == 128) return r * 128 + ((c ^ (r & 6)) << 4);
+  const int p = (r >> 1) + (r & 1) * 8;                               // the rows that a product reads together stand side by side
+  return p * 64 + ((c ^ (p & 2)) << 4);
+}
+template <int D> __device__ __forceinline__ void c8_fetch(uint32_t stage, const uint8_t* kc, const uint8_t* vc, int at, int lane) {
+  const uint8_t *k = kc + (size_t)at * (C8_BLOCK * D), *v = vc + (size_t)at * (C8_BLOCK * D);
+#pragma unroll
+  for (int j = 0; j < D / 32; j++) {
+    const int i = j * 32 + lane, r = i / (D / 16), c = i % (D / 16);
+    hb_cp_async16(stage + c8_at_k<D>(r, c), k + i * 16);
+    hb_cp_async16(stage + C8_BLOCK * D + c8_at_v<D>(r, c), v + i * 16);
+  }
+}
+__device__ __forceinline__ uint4 c8_lds16(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 c8_lds8(uint32_t p) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
+  return v;
+}
+
+template <typename CT, typename T, int D, int NT> struct C8Sizes {
+  static constexpr bool Q_INT = sizeof(T) == 2 && CT::MOST == C8Int8::MOST;                       // the query in int8 parts
+  static constexpr int PARTS = sizeof(T) == 4 || Q_INT ? 2 : 1, W_PARTS = sizeof(T) == 4 ? 2 : 1;  // of the query, of the weights
+  static constexpr int STEPS = D / 16, Q_STEPS = Q_INT ? D / 32 : D / 16;
+  static constexpr int U = D == 128 ? 1 : 2, STAGES = 3;                                          // units of a stage (4 KB), stages of a ring
+  static constexpr bool Q_REGS = NT == 1 && (Q_INT || PARTS == 1);
+  static constexpr int QUERY = Q_REGS ? 0 : PARTS * NT * Q_STEPS * 32 * 8, UNIT = 2 * C8_BLOCK * D, RING = C8M_WARPS * STAGES * U * UNIT;
+  static constexpr int PITCH = D + 4, JOINED = C8M_WARPS * 8 * NT * PITCH * 4;
+  static constexpr int SMEM = QUERY + RING > JOINED ? QUERY + RING : JOINED;
+  static constexpr int BLOCKS = NT == 1 ? 4 : D == 64 ? (NT == 2 ? 4 : 3) : NT == 2 ? 3 : 2;      // an SM, by registers
+};
+
 template <typename CT, typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(const C8Attend a) {
-  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, STEPS = D / 16, PAIRS = 8 * NT, PITCH = D + 4;
-  extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS) cache8_attention_mma_kernel(const C8Attend a) {
+  using Z = C8Sizes<CT, T, D, NT>;
+  constexpr int PARTS = Z::PARTS, W_PARTS = Z::W_PARTS, STEPS = Z::STEPS, Q_STEPS = Z::Q_STEPS, PAIRS = 8 * NT, PITCH = Z::PITCH, STAGES = Z::STAGES, U = Z::U;
+  extern __shared__ __align__(128) uint8_t smem[];
   uint2* q_sh = (uint2*)smem;                                           // [part][nt][step][lane]
   float* o_sh = (float*)smem;                                           // [warp][pair][PITCH], over the query when it is done with
   __shared__ float m_sh[C8M_WARPS][PAIRS], l_sh[C8M_WARPS][PAIRS], m_cta[PAIRS], l_cta[PAIRS];
@@ -146,7 +171,40 @@ __global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(co
   const int u_hi = r >= 0 && r < a.table_rows ? (int)min((long)(p_hi < 0 ? -1 : p_hi / C8_BLOCK), (long)a.table_width * a.upp - 1) : -1;
   const int* table = a.bt + r * a.ld_table;
 
+  const uint32_t ring = hb_smem_u32(smem) + Z::QUERY + warp * STAGES * U * Z::UNIT;
+  // this warp's stages: U units each, the id-th and every (ranks * WARPS)th from there; a lane looks up one unit of 32, 32 units ahead
+  constexpr int BATCH = 32 / U;
+  const int id = rank * C8M_WARPS + warp, stride = ranks * C8M_WARPS, s_lo = u_lo / U, first = s_lo + id;
+  const int count = u_hi < first * U ? 0 : (u_hi / U - first) / stride + 1;
+  struct Units { int at; float k_scale, v_scale; };
+  const auto look = [&](int i) {                                        // stages i .. i + BATCH - 1
+    Units x = {-1, 0.f, 0.f};
+    const int unit = (first + (i + lane / U) * stride) * U + lane % U;
+    if (i + lane / U < count && unit >= u_lo && unit <= u_hi) {
+      const int page = table[unit / a.upp];
+      if (page >= 0 && page < a.n_pages) {
+        x.at = (page * a.Hkv + h) * a.upp + unit % a.upp;
+        x.k_scale = a.ks[x.at];
+        x.v_scale = a.vs[x.at];
+      }
+    }
+    return x;
+  };
+  Units now = look(0), next = {-1, 0.f, 0.f};
+  if (count > BATCH) next = look(BATCH);
+  const auto fetch = [&](int i, int base, int slot) {                   // stage i, of the BATCH from `base` on or the next
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int l = i % BATCH * U + u, x = __shfl_sync(0xffffffffu, now.at, l), y = __shfl_sync(0xffffffffu, next.at, l), at = i - base < BATCH ? x : y;
+      if (i < count && at >= 0) c8_fetch<D>(ring + (slot * U + u) * Z::UNIT, a.kc, a.vc, at, lane);
+    }
+    hb_cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; i++) fetch(i, 0, i);
+
   // the query: pair g of a tile of 8, the dimensions of this thread's codes
+  uint2 q_reg[Z::Q_REGS ? PARTS : 1][Z::Q_REGS ? Q_STEPS : 1];
   float col[NT][2];                                                     // of columns 2 tq, 2 tq + 1: score = product * col * the unit's scale
   int col_hi[NT][2];                                                    // their rows' positions
 #pragma unroll
@@ -184,17 +242,44 @@ __global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(co
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     odd = __shfl_xor_sync(0xffffffffu, (int)odd, 1) | odd;
     odd = __shfl_xor_sync(0xffffffffu, (int)odd, 2) | odd;
-    // 2^e <= most < 2^(e + 1); the query times 2^(9 - e). A query that is not finite: NaN, and so are its scores
-    const int e = max(-100, (int)(__float_as_uint(most) >> 23) - 127);
-    const float up = __uint_as_float((uint32_t)(9 - e + 127) << 23), down = odd ? NAN : a.scale_log2 * __uint_as_float((uint32_t)(e - 9 + 127) << 23);
-    if (warp == 0) {                                                    // (every warp knows `down`; one writes the query)
+    float up, down;
+    if constexpr (Z::Q_INT) {
+      most = fmaxf(most, 1e-33f);
+      up = odd ? 0.f : 32512.f / most, down = a.scale_log2 * (most / 32512.f);
+    } else {                                                            // 2^e <= most < 2^(e + 1); the query times 2^(9 - e)
+      const int e = max(-100, (int)(__float_as_uint(most) >> 23) - 127);
+      up = odd ? 0.f : __uint_as_float((uint32_t)(9 - e + 127) << 23), down = a.scale_log2 * __uint_as_float((uint32_t)(e - 9 + 127) << 23);
+    }
+    if (odd) down = NAN;                                                // a query that is not finite: its scores are NaN
+    const auto keep = [&](int part, int step, uint2 v) {
+      if constexpr (Z::Q_REGS) q_reg[part][step] = v;
+      else q_sh[((part * NT + nt) * Q_STEPS + step) * 32 + lane] = v;
+    };
+    if (Z::Q_REGS || warp == 0) {                                       // (every warp knows `down`; one writes the query)
+      if constexpr (Z::Q_INT) {
 #pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        uint32_t lo[PARTS], hi[PARTS];
-        c8_split<PARTS>(odd ? 0.f : x[s][0] * up, odd ? 0.f : x[s][1] * up, lo);
-        c8_split<PARTS>(odd ? 0.f : x[s][2] * up, odd ? 0.f : x[s][3] * up, hi);
+        for (int s = 0; s < Q_STEPS; s++) {
+          uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
 #pragma unroll
-        for (int p = 0; p < PARTS; p++) q_sh[((p * NT + nt) * STEPS + s) * 32 + lane] = make_uint2(lo[p], hi[p]);
+          for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int n16 = odd ? 0 : __float2int_rn(x[2 * s + w][e] * up), n8 = (n16 + 128) >> 8;
+              hi[w] |= (uint32_t)(n8 & 255) << (8 * e);
+              lo[w] |= (uint32_t)((n16 - n8 * 256) & 255) << (8 * e);
+            }
+          keep(0, s, make_uint2(hi[0], hi[1]));
+          keep(1, s, make_uint2(lo[0], lo[1]));
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q_STEPS; s++) {
+          uint32_t lo[PARTS], hi[PARTS];
+          c8_split<PARTS>(odd ? 0.f : x[s][0] * up, odd ? 0.f : x[s][1] * up, lo);
+          c8_split<PARTS>(odd ? 0.f : x[s][2] * up, odd ? 0.f : x[s][3] * up, hi);
+#pragma unroll
+          for (int p = 0; p < PARTS; p++) keep(p, s, make_uint2(lo[p], hi[p]));
+        }
       }
     }
 #pragma unroll
@@ -215,60 +300,97 @@ __global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(co
     for (int i = 0; i < STEPS; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
   }
 
-  const auto compute = [&](C8Unit<D>& u, int key0, float k_scale, float v_scale) {
-    float s[NT][4];
+  // the scores of a unit, in 32 bits
+  const auto products = [&](uint32_t stage, float k_scale, float (&s)[NT][4]) {
+    int si[2][NT][4];                                                   // two chains of products: of int8 parts, or of every second step
+    float sf[2][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-    for (int st = 0; st < STEPS; st++) {
-      const uint4 &x = u.k[0][st >> 2], &y = u.k[1][st >> 2];
-      const uint32_t wx = (st & 3) == 0 ? x.x : (st & 3) == 1 ? x.y : (st & 3) == 2 ? x.z : x.w;
-      const uint32_t wy = (st & 3) == 0 ? y.x : (st & 3) == 1 ? y.y : (st & 3) == 2 ? y.z : y.w;
-      uint32_t f[4];
-      c8_halves<CT>(wx, f[0], f[2]);
-      c8_halves<CT>(wy, f[1], f[3]);
-#pragma unroll
-      for (int p = 0; p < PARTS; p++)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          const uint2 b = q_sh[((p * NT + nt) * STEPS + st) * 32 + lane];
-          c8_mma(s[nt], f, b.x, b.y);
-        }
-    }
-    bool raise = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const float f0 = col[nt][0] * k_scale, f1 = col[nt][1] * k_scale;
-      s[nt][0] *= f0, s[nt][1] *= f1, s[nt][2] *= f0, s[nt][3] *= f1;
-    }
-    if (key0 < all_lo || key0 + C8_BLOCK - 1 > p_lo) {                  // not all of it is seen by all rows
+    for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const int key = key0 + g + (c >> 1) * 8, hi = col_hi[nt][c & 1];
-          if (key > hi || hi - key >= window) s[nt][c] = -INFINITY;
+        for (int c = 0; c < 4; c++) si[i][nt][c] = 0, sf[i][nt][c] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 64; j++) {
+      const uint4 x = c8_lds16(stage + c8_at_k<D>(g, j * 4 + tq)), y = c8_lds16(stage + c8_at_k<D>(g + 8, j * 4 + tq));
+      const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
+      const auto query = [&](int part, int nt, int step) {
+        if constexpr (Z::Q_REGS) return q_reg[part][step];
+        else return q_sh[((part * NT + nt) * Q_STEPS + step) * 32 + lane];
+      };
+      if constexpr (Z::Q_INT) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const uint32_t f[4] = {wx[2 * i], wy[2 * i], wx[2 * i + 1], wy[2 * i + 1]};
+#pragma unroll
+          for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              const uint2 b = query(p, nt, j * 2 + i);
+              c8_imma(si[p][nt], f, b.x, b.y);
+            }
         }
-      if constexpr (sizeof(CT) && CT::MOST == C8E4m3::MOST) {           // a place that nobody sees may hold a NaN
+      } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const int key = key0 + 2 * tq + (i >> 1) * 8 + (i & 1);
-          if (key < see_lo || key > p_hi)
+          uint32_t f[4];
+          c8_halves<CT>(wx[i], f[0], f[2]);
+          c8_halves<CT>(wy[i], f[1], f[3]);
 #pragma unroll
-            for (int j = 0; j < D / 32; j++) u.v[i][j] = 0u;
+          for (int p = 0; p < PARTS; p++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              const uint2 b = query(p, nt, j * 4 + i);
+              c8_mma(sf[i & 1][nt], f, b.x, b.y);
+            }
         }
       }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) raise |= s[nt][c] > m[nt][c & 1] + 8.f;
+      for (int c = 0; c < 4; c++)
+        s[nt][c] = (Z::Q_INT ? (float)(si[0][nt][c] * 256 + si[1][nt][c]) : sf[0][nt][c] + sf[1][nt][c]) * (col[nt][c & 1] * k_scale);
+  };
+  // U units side by side in shared memory, whose first place is key0; at < 0: one that is not there
+  const auto compute = [&](uint32_t stage, int key0, const int (&at)[U], const float (&k_scale)[U], const float (&v_scale)[U]) {
+    float s[U][NT][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (at[u] >= 0) {
+        products(stage + u * Z::UNIT, k_scale[u], s[u]);
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = -INFINITY;
+      }
+    }
+    const bool whole = key0 >= all_lo && key0 + U * C8_BLOCK - 1 <= p_lo;
+    if (!whole) {                                                       // not all of it is seen by all rows
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int key = key0 + u * C8_BLOCK + g + (c >> 1) * 8, hi = col_hi[nt][c & 1];
+            if (key > hi || hi - key >= window) s[u][nt][c] = -INFINITY;
+          }
+    }
+    bool raise = false;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) raise |= s[u][nt][c] > m[nt][c & 1] + 8.f;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+          float mx = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+          for (int u = 1; u < U; u++) mx = fmaxf(mx, fmaxf(s[u][nt][c], s[u][nt][c + 2]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -281,69 +403,89 @@ __global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(co
           }
         }
     }
-    uint32_t b[PARTS][NT][2];
+    uint32_t b[U][W_PARTS][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const float b0 = (m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 7.f, b1 = (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 7.f;
-      const float w0 = hb_exp2(s[nt][0] - b0), w1 = hb_exp2(s[nt][1] - b1), w2 = hb_exp2(s[nt][2] - b0), w3 = hb_exp2(s[nt][3] - b1);
-      l[nt][0] += w0 + w2;
-      l[nt][1] += w1 + w3;
-      uint32_t x[PARTS], y[PARTS];
-      c8_split<PARTS>(w0, w1, x);
-      c8_split<PARTS>(w2, w3, y);
 #pragma unroll
-      for (int p = 0; p < PARTS; p++) b[p][nt][0] = c8_transpose(x[p]), b[p][nt][1] = c8_transpose(y[p]);
+      for (int u = 0; u < U; u++) {
+        const float w0 = hb_exp2(s[u][nt][0] - b0), w1 = hb_exp2(s[u][nt][1] - b1), w2 = hb_exp2(s[u][nt][2] - b0), w3 = hb_exp2(s[u][nt][3] - b1);
+        l[nt][0] += w0 + w2;
+        l[nt][1] += w1 + w3;
+        uint32_t x[W_PARTS], y[W_PARTS];
+        c8_split<W_PARTS>(w0, w1, x);
+        c8_split<W_PARTS>(w2, w3, y);
+#pragma unroll
+        for (int p = 0; p < W_PARTS; p++) b[u][p][nt][0] = c8_transpose(x[p]), b[u][p][nt][1] = c8_transpose(y[p]);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < D / 32; j++) {
+    for (int u = 0; u < U; u++) {
+      if (at[u] < 0) continue;
+      uint32_t v[4][D / 32];                                            // codes of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: dimensions g D / 8 ..
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const uint32_t sel = half ? 0x7362 : 0x5140;
-        const uint32_t x = __byte_perm(u.v[0][j], u.v[1][j], sel), y = __byte_perm(u.v[2][j], u.v[3][j], sel);
-        uint32_t f[4];
-        c8_halves<CT>(x, f[0], f[1]);
-        c8_halves<CT>(y, f[2], f[3]);
+      for (int i = 0; i < 4; i++) {
+        const int r = 2 * tq + (i >> 1) * 8 + (i & 1);
+        const uint32_t from = stage + u * Z::UNIT + C8_BLOCK * D;
+        if constexpr (D == 128) {
+          const uint4 x = c8_lds16(from + c8_at_v<D>(r, g));
+          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+        } else {
+          const uint2 x = c8_lds8(from + c8_at_v<D>(r, g >> 1) + (g & 1) * 8);
+          v[i][0] = x.x, v[i][1] = x.y;
+        }
+        if constexpr (CT::MOST == C8E4m3::MOST) {                       // a place that nobody sees may hold a NaN
+          const int key = key0 + u * C8_BLOCK + r;
+          if (!whole && (key < see_lo || key > p_hi))
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          float d[4];
-          c8_mma_zero(d, f, b[0][nt][0], b[0][nt][1]);
-          if constexpr (PARTS == 2) c8_mma(d, f, b[1][nt][0], b[1][nt][1]);
+            for (int j = 0; j < D / 32; j++) v[i][j] = 0u;
+        }
+      }
 #pragma unroll
-          for (int c = 0; c < 4; c++) o[2 * j + half][nt][c] = fmaf(v_scale, d[c], o[2 * j + half][nt][c]);
+      for (int j = 0; j < D / 32; j++) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const uint32_t sel = half ? 0x7362 : 0x5140;
+          const uint32_t x = __byte_perm(v[0][j], v[1][j], sel), y = __byte_perm(v[2][j], v[3][j], sel);
+          uint32_t f[4];
+          c8_halves<CT>(x, f[0], f[1]);
+          c8_halves<CT>(y, f[2], f[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            float d[4];
+            c8_mma_zero(d, f, b[u][0][nt][0], b[u][0][nt][1]);
+            if constexpr (W_PARTS == 2) c8_mma(d, f, b[u][1][nt][0], b[u][1][nt][1]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[2 * j + half][nt][c] = fmaf(v_scale[u], d[c], o[2 * j + half][nt][c]);
+          }
         }
       }
     }
   };
 
-  // this warp's units: u_lo + id, and every (ranks * WARPS)th from there; a lane looks up one of the next 32
-  const int id = rank * C8M_WARPS + warp, stride = ranks * C8M_WARPS;
-  for (int first = u_lo + id; first <= u_hi; first += 32 * stride) {
-    const int mine = first + lane * stride;
-    int at = -1;
-    float k_scale = 0.f, v_scale = 0.f;
-    if (mine <= u_hi) {
-      const int page = table[mine / a.upp];
-      if (page >= 0 && page < a.n_pages) {
-        at = (page * a.Hkv + h) * a.upp + mine % a.upp;
-        k_scale = a.ks[at];
-        v_scale = a.vs[at];
-      }
+#pragma unroll 1
+  for (int i = 0, base = 0, slot = 0, ahead = STAGES - 1; i < count; i++) {      // (not unrolled: three times the code was 12 % slower)
+    if (i - base == BATCH) {
+      base = i;
+      now = next;
+      next = look(base + BATCH);
     }
-    const int count = min(32, (u_hi - first) / stride + 1);
-    C8Unit<D> x, y;
-    int at_x = __shfl_sync(0xffffffffu, at, 0), at_y;
-    if (at_x >= 0) c8_fetch<D>(x, a.kc, a.vc, at_x, g, tq);
-    for (int i = 0; i < count; i += 2) {
-      at_y = i + 1 < count ? __shfl_sync(0xffffffffu, at, i + 1) : -1;
-      if (at_y >= 0) c8_fetch<D>(y, a.kc, a.vc, at_y, g, tq);
-      float fk = __shfl_sync(0xffffffffu, k_scale, i), fv = __shfl_sync(0xffffffffu, v_scale, i);
-      if (at_x >= 0) compute(x, (first + i * stride) * C8_BLOCK, fk, fv);
-      at_x = i + 2 < count ? __shfl_sync(0xffffffffu, at, i + 2) : -1;
-      if (at_x >= 0) c8_fetch<D>(x, a.kc, a.vc, at_x, g, tq);
-      fk = __shfl_sync(0xffffffffu, k_scale, (i + 1) & 31), fv = __shfl_sync(0xffffffffu, v_scale, (i + 1) & 31);
-      if (at_y >= 0) compute(y, (first + (i + 1) * stride) * C8_BLOCK, fk, fv);
+    hb_cp_async_wait<STAGES - 2>();
+    __syncwarp();                                                       // the stage is there for all lanes, and all are done with the one before
+    fetch(i + STAGES - 1, base, ahead);
+    int at[U];
+    float fk[U], fv[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int l = i % BATCH * U + u;
+      at[u] = __shfl_sync(0xffffffffu, now.at, l);
+      fk[u] = __shfl_sync(0xffffffffu, now.k_scale, l), fv[u] = __shfl_sync(0xffffffffu, now.v_scale, l);
     }
+    compute(ring + slot * U * Z::UNIT, (first + i * stride) * U * C8_BLOCK, at, fk, fv);
+    ahead = slot;
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
   }
+  hb_cp_async_wait<0>();
 
   // the warps' results, then the blocks'
 #pragma unroll
@@ -432,8 +574,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS) cache8_attention_mma_kernel(co
 
 template <typename CT, typename T, int D, int NT>
 static cudaError_t launch(const C8Attend& a, int tiles, int ranks, cudaStream_t st) {
-  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
-  constexpr int query = PARTS * NT * (D / 16) * 32 * 8, joined = C8M_WARPS * 8 * NT * (D + 4) * 4, smem = query > joined ? query : joined;
+  constexpr int smem = C8Sizes<CT, T, D, NT>::SMEM;
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -474,8 +615,12 @@ HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const vo
   const int count = tiles ? n_tiles : n_tiles * a.tiles_row;
   cudaError_t e = cudaErrorInvalidValue;
   C8_DISPATCH(ct, "hb_cache8_attention_mma", HB_DISPATCH_1(dt, "hb_cache8_attention_mma", {
-    if (D == 64) e = nt == 1 ? launch<CT, TA, 64, 1>(a, count, ranks, st) : nt == 2 ? launch<CT, TA, 64, 2>(a, count, ranks, st) : nt == 4 ? launch<CT, TA, 64, 4>(a, count, ranks, st) : e;
-    else e = nt == 1 ? launch<CT, TA, 128, 1>(a, count, ranks, st) : nt == 2 ? launch<CT, TA, 128, 2>(a, count, ranks, st) : nt == 4 ? launch<CT, TA, 128, 4>(a, count, ranks, st) : e;
+    const auto go = [&](auto d) {
+      constexpr int N = decltype(d)::value;
+      return nt == 1 ? launch<CT, TA, N, 1>(a, count, ranks, st) : nt == 2 ? launch<CT, TA, N, 2>(a, count, ranks, st)
+           : nt == 3 ? launch<CT, TA, N, 3>(a, count, ranks, st) : nt == 4 ? launch<CT, TA, N, 4>(a, count, ranks, st) : cudaErrorInvalidValue;
+    };
+    e = D == 64 ? go(std::integral_constant<int, 64>()) : go(std::integral_constant<int, 128>());
   }));
   if (e != cudaSuccess) HB_FAIL("hb_cache8_attention_mma: %s", cudaGetErrorString(e));
   HB_CHECK_LAUNCH("hb_cache8_attention_mma");

@@ -160,34 +160,60 @@ HB_EXPORT int hb_cache8_store(const void* k, const void* v, long ld_k, long ld_v
 }
 
 // Page i of the output [n][Hkv][page_size][D] is page table[index[i]] of the cache (table[i] without an index); a number outside of the
-// cache's pages gives zeros.
-template <typename CT, typename T>
+// cache's pages gives zeros. E codes at a time: 8 of them are a load of 8 bytes and a store of 16 (bf16) or two, so that a warp's stores are
+// whole lines; a page of one plane is a block's.
+template <typename CT, typename T, int E>
 __global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, const int* table,
                                                             const int* index, long n_pages, int Hkv, int page_size, int D, T* k, T* v) {
   hb_pdl_launch();
   hb_pdl_wait();
   const long i = blockIdx.x;
   const bool is_v = blockIdx.y;
-  const uint8_t* codes = is_v ? vc : kc;
-  const float* scales = is_v ? vs : ks;
-  T* out = (is_v ? v : k) + i * Hkv * page_size * D;
+  const int pieces = Hkv * page_size * D / E, blocks = c8_blocks(page_size);
+  T* out = (is_v ? v : k) + i * pieces * E;
   const long page = table[index ? index[i] : i];
   const bool there = page >= 0 && page < n_pages;
-  for (int j = threadIdx.x; j < Hkv * page_size * D; j += 256) {
-    const int h = j / (page_size * D), place = j / D % page_size;
-    out[j] = hb_from_float<T>(there ? CT::value(codes[page * Hkv * page_size * D + j]) *
-                                          scales[(page * Hkv + h) * c8_blocks(page_size) + place / C8_BLOCK] : 0.f);
+  const uint8_t* codes = (is_v ? vc : kc) + (there ? page : 0) * pieces * E;
+  const float* scales = (is_v ? vs : ks) + (there ? page : 0) * Hkv * blocks;
+#pragma unroll 4
+  for (int j = threadIdx.x; j < pieces; j += 256) {
+    const int row = j / (D / E);                    // of the page's rows, head by head
+    const float f = there ? scales[row / page_size * blocks + row % page_size / C8_BLOCK] : 0.f;
+    if constexpr (E == 8) {
+      const uint2 w = there ? *(const uint2*)(codes + (long)j * E) : make_uint2(0u, 0u);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = CT::value((uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)))) * f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        if constexpr (sizeof(T) == 4) *(float4*)(out + (long)j * E + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+      }
+      if constexpr (sizeof(T) == 2) {
+        __nv_bfloat162 y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        *(uint4*)(out + (long)j * E) = *(const uint4*)y;
+      }
+    } else {
+      out[j] = hb_from_float<T>(there ? CT::value(codes[j]) * f : 0.f);
+    }
   }
 }
 
 HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, const float* vs, int ct, const int* table, const int* index, long n,
                                long n_pages, int Hkv, int page_size, int D, void* k, void* v, int dt, cudaStream_t st) {
   if (n <= 0) return 0;
-  if (n > 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || (long)Hkv * page_size * D > 0x7fffffffL - 256)
-    HB_FAIL("hb_cache8_expand: %ld pages of %d heads, %d places and %d", n, Hkv, page_size, D);
-  C8_DISPATCH(ct, "hb_cache8_expand", HB_DISPATCH_1(dt, "hb_cache8_expand",
-      hb_launch(cache8_expand_kernel<CT, TA>, dim3(n, 2), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n_pages,
-                Hkv, page_size, D, (TA*)k, (TA*)v)));
+  if (n > 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || (long)Hkv * page_size * D > 0x7fffffffL - 256 || n_pages < 1)
+    HB_FAIL("hb_cache8_expand: %ld of %ld pages of %d heads, %d places and %d", n, n_pages, Hkv, page_size, D);
+  const bool wide = D % 8 == 0 && !(((uintptr_t)kc | (uintptr_t)vc) & 7) && !(((uintptr_t)k | (uintptr_t)v) & 15);
+#define C8E_LAUNCH(E)                                                                                                                                   \
+  hb_launch(cache8_expand_kernel<CT, TA, E>, dim3(n, 2), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n_pages, Hkv, \
+            page_size, D, (TA*)k, (TA*)v)
+  C8_DISPATCH(ct, "hb_cache8_expand", HB_DISPATCH_1(dt, "hb_cache8_expand", {
+    if (wide) C8E_LAUNCH(8);
+    else C8E_LAUNCH(1);
+  }));
+#undef C8E_LAUNCH
   HB_CHECK_LAUNCH("hb_cache8_expand");
   return 0;
 }

@@ -1,7 +1,7 @@
 // Pages of a cache copied to other pages, in every layer and plane of a cache group at once.
 #include "common.cuh"
 
-constexpr int CP_PLANES = 8, CP_PAIRS = 240;      // a launch's arguments are at most 4 KB
+constexpr int CP_PLANES = 8, CP_PAIRS = 960, CP_THREADS = 256, CP_AHEAD = 4;      // a launch's arguments are at most 32 KB
 
 struct CopyPlane {
   char* base;              // [layer][page][bytes]
@@ -10,20 +10,33 @@ struct CopyPlane {
 };
 struct CopyArgs {          // by value: nothing of a call lives in memory that the next could change
   CopyPlane plane[CP_PLANES];
+  int n_planes;
   int src[CP_PAIRS], dst[CP_PAIRS];
 };
 
-// One block has a pair of pages in one layer of one plane.
+// One block has a pair of pages in one layer, in all planes. A thread asks for four of its vectors before it writes the first.
 template <typename V>
-__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+__global__ void __launch_bounds__(CP_THREADS) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
   hb_pdl_launch();
   hb_pdl_wait();
-  const CopyPlane& p = a.plane[blockIdx.z];
-  if ((int)blockIdx.y >= p.layers) return;
-  char* layer = p.base + blockIdx.y * p.layer_stride;
-  const V* from = (const V*)(layer + a.src[blockIdx.x] * p.page_stride);
-  V* to = (V*)(layer + a.dst[blockIdx.x] * p.page_stride);
-  for (long i = threadIdx.x; i < p.bytes / (long)sizeof(V); i += 256) to[i] = from[i];
+  const long src = a.src[blockIdx.x], dst = a.dst[blockIdx.x];
+  for (int i = 0; i < a.n_planes; i++) {
+    const CopyPlane& p = a.plane[i];
+    if ((int)blockIdx.y >= p.layers) continue;
+    char* layer = p.base + blockIdx.y * p.layer_stride;
+    const V* from = (const V*)(layer + src * p.page_stride);
+    V* to = (V*)(layer + dst * p.page_stride);
+    const long n = p.bytes / (long)sizeof(V);
+    for (long j = threadIdx.x; j < n; j += CP_AHEAD * CP_THREADS) {
+      V x[CP_AHEAD];
+#pragma unroll
+      for (int k = 0; k < CP_AHEAD; k++)
+        if (j + k * CP_THREADS < n) x[k] = from[j + k * CP_THREADS];
+#pragma unroll
+      for (int k = 0; k < CP_AHEAD; k++)
+        if (j + k * CP_THREADS < n) to[j + k * CP_THREADS] = x[k];
+    }
+  }
 }
 
 // planes: n_planes x (base, layers, layer stride, page stride, bytes of a page), 64-bit each; src, dst: host arrays of n_pairs pages. No page
@@ -31,11 +44,11 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
 HB_EXPORT int hb_copy_pages(const long* planes, int n_planes, const int* src, const int* dst, int n_pairs, cudaStream_t st) {
   if (n_planes <= 0 || n_pairs <= 0) return 0;
   for (int at = 0; at < n_planes; at += CP_PLANES) {
-    CopyArgs a = {};
-    const int n = n_planes - at < CP_PLANES ? n_planes - at : CP_PLANES;
+    CopyArgs a;
+    a.n_planes = n_planes - at < CP_PLANES ? n_planes - at : CP_PLANES;
     int layers = 0;
     bool wide = true;
-    for (int i = 0; i < n; i++) {
+    for (int i = 0; i < a.n_planes; i++) {
       const long* p = planes + 5 * (at + i);
       a.plane[i] = {(char*)p[0], p[2], p[3], p[4], (int)p[1]};
       layers = a.plane[i].layers > layers ? a.plane[i].layers : layers;
@@ -48,8 +61,8 @@ HB_EXPORT int hb_copy_pages(const long* planes, int n_planes, const int* src, co
         a.src[i] = src[first + i];
         a.dst[i] = dst[first + i];
       }
-      if (wide) hb_launch(copy_pages_kernel<uint4>, dim3(m, layers, n), dim3(256), 0, st, a);
-      else hb_launch(copy_pages_kernel<uint8_t>, dim3(m, layers, n), dim3(256), 0, st, a);
+      if (wide) hb_launch(copy_pages_kernel<uint4>, dim3(m, layers), dim3(CP_THREADS), 0, st, a);
+      else hb_launch(copy_pages_kernel<uint8_t>, dim3(m, layers), dim3(CP_THREADS), 0, st, a);
     }
   }
   HB_CHECK_LAUNCH("hb_copy_pages");

@@ -58,6 +58,17 @@ class Cache8:
             raise ops.KernelError(f"a cache in 8 bits of {tuple(k.shape)}")
         object.__setattr__(self, "code", CODES[k.dtype])
         object.__setattr__(self, "tensors", (k, v, self.k_scale, self.v_scale))
+        object.__setattr__(self, "mma", None)                      # see _on_tensor_cores
+        # as the binding reads it (Cache in csrc/cache8_binding.cpp); -1: not on one GPU
+        one = k.is_cuda and {t.device for t in self.tensors} == {k.device}
+        numbers = np.array([t.data_ptr() for t in self.tensors] + list(k.shape) + [self.code, k.device.index if one else -1], dtype=np.int64)
+        object.__setattr__(self, "_native", numbers)
+        object.__setattr__(self, "native", numbers.ctypes.data)
+        # as the binding reads it (Cache in csrc/cache8_binding.cpp); -1: no device
+        one = {t.device for t in self.tensors} == {k.device} and k.is_cuda
+        numbers = np.array([t.data_ptr() for t in self.tensors] + list(k.shape) + [self.code, k.device.index if one else -1], dtype=np.int64)
+        object.__setattr__(self, "_native", numbers)
+        object.__setattr__(self, "native", numbers.ctypes.data)
 
     @property
     def n_kv_heads(self) -> int:
@@ -104,6 +115,18 @@ def store_cache8(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, cache
     the largest code (127, or 448). In any other block the scale grows to that where it is larger, and the codes that are there are rounded to it once
     more: half a step each time that it grows. Numbers that are not finite do not count for a: infinities become the largest code, NaN becomes 0.
     Places of a block that no row goes to keep their codes where the scale stays or begins anew. A cache has at most 2^31 - 1 places."""
+    bound = _bound or _binding()
+    if bound is not False and k.is_cuda:
+        done = bound.store(k, v, slot_map, cache.native)
+        if done is not None:
+            _done(done, 1)
+            return cache
+    bound = _binding() if _bound is None and k.is_cuda else _bound
+    if bound and k.is_cuda:
+        done = bound.store(k, v, slot_map, cache.native)
+        if done is not None:
+            _done(done, 1)
+            return cache
     _here("store_cache8", k, v, slot_map, *cache.tensors)
     width = cache.n_kv_heads * cache.head_dim
     if k.dim() != 2 or k.shape != v.shape or k.shape[1] != width or k.dtype != v.dtype or (width > 1 and (k.stride(1) != 1 or v.stride(1) != 1)):
@@ -122,6 +145,16 @@ def store_cache8(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, cache
 def expand_cache8(cache: Cache8, pages: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The numbers of `pages` (int32 [n]) as keys and values [n, n_kv_heads, page_size, head_dim] in float32 or bfloat16; zeros for a page number
     outside of the cache."""
+    bound = _bound or _binding()
+    if bound is not False and pages.is_cuda and dtype in ops._DT:
+        done = bound.expand(pages, cache.native, ops._DT[dtype])
+        if done is not None:
+            return _done(done, 1)
+    bound = _binding() if _bound is None and pages.is_cuda else _bound
+    if bound and pages.is_cuda and dtype in ops._DT:
+        done = bound.expand(pages, cache.native, ops._DT[dtype])
+        if done is not None:
+            return _done(done, 1)
     _here("expand_cache8", pages, *cache.tensors)
     _ints("expand_cache8", "pages", pages)
     return _expand(cache, pages, None, pages.numel(), dtype)
@@ -145,84 +178,162 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     head_dim] of its type; query head h reads kv head h // (n_heads / n_kv_heads). A row at position p sees the keys j <= p (and j > p - window,
     for a window above 0) whose pages are in the block table and in the cache; one that sees none is 0. scale: 1 / sqrt(head_dim) by default. Scores,
     softmax and sums are 32-bit. Codes at places that a row of the step sees are numbers (e4m3 has a NaN; storing leaves none)."""
-    table = batch.block_tables[group]
+    table, T, D = batch.block_tables[group], batch.n_rows, cache.head_dim
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    tensor_cores = q.is_cuda and _on_tensor_cores(cache)
+    portions = tensor_cores and batch.max_q_len >= PORTION_ROWS
+    if tensor_cores and not portions:
+        bound = _binding() if _bound is None else _bound
+        if bound:
+            cut = _cut(batch, cache, n_heads, window, 0)
+            done = bound.attend(q, cache.native, table, batch.positions, cut.tiles, cut.native, scale, out)
+            if done is not None:
+                return _done(done, 1)
     _here("attention_cache8", q, table, batch.positions, batch.row_request, *cache.tensors, out)
-    T, D = batch.n_rows, cache.head_dim
-    if n_heads < 1 or n_heads % cache.n_kv_heads:
-        raise ops.KernelError(f"attention_cache8: {n_heads} heads are not a multiple of {cache.n_kv_heads} kv heads")
+    _heads(cache, n_heads, window)
     if D > 256:
         raise ops.KernelError(f"attention_cache8: heads of {D}, at most 256")
     if q.shape != (T, n_heads * D) or q.stride(1) != 1:
         raise ops.KernelError(f"attention_cache8: q {tuple(q.shape)}, strides {q.stride()}; {T} rows of {n_heads} heads of {D} are expected")
     dt = ops._dt(q)
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or table.shape[0] != batch.n_requests:
+    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.shape[0] != batch.n_requests:
         raise ops.KernelError(f"attention_cache8: block table {tuple(table.shape)} {table.dtype} of {batch.n_requests} requests")
-    if window < 0:
-        raise ops.KernelError(f"attention_cache8: window {window}")
     if out is None:
         out = torch.empty(T, n_heads * D, dtype=q.dtype, device=q.device)
     elif out.shape != (T, n_heads * D) or out.dtype != q.dtype or not out.is_contiguous():
         raise ops.KernelError(f"attention_cache8: out {tuple(out.shape)} {out.dtype}, strides {out.stride()}")
     if not T:
         return out
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    single = batch.max_q_len == 1 and T == batch.n_requests
-    if _on_tensor_cores(cache):
-        _attend_mma(q, dt, cache, batch, table, single, n_heads // cache.n_kv_heads, int(window), scale, out)
+    if not tensor_cores:
+        single = batch.max_q_len == 1 and T == batch.n_requests
+        ops._call("cache8", "hb_cache8_attention_any", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
+                  cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
+                  None if single else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
+                  out.data_ptr(), ops._stream())
         return out
-    ops._call("cache8", "hb_cache8_attention_any", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
-              cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
-              None if single else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
-              out.data_ptr(), ops._stream())
+    limit = PORTION_ROWS if portions and _flash_takes(q, cache, out, n_heads, scale) else 0
+    if limit:
+        _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit)
+    if not limit or min(batch.h_q_len) < limit:
+        cut = _cut(batch, cache, n_heads, window, limit)
+        ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
+                  cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], None, batch.positions.data_ptr(),
+                  ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), ops._stream())
     return out
+
+
+def _heads(cache: Cache8, n_heads: int, window: int) -> None:
+    if n_heads < 1 or n_heads % cache.n_kv_heads:
+        raise ops.KernelError(f"attention_cache8: {n_heads} heads are not a multiple of {cache.n_kv_heads} kv heads")
+    if window < 0:
+        raise ops.KernelError(f"attention_cache8: window {window}")
 
 
 def _on_tensor_cores(cache: Cache8) -> bool:
     """Whether the kernel on warp MMAs takes the cache's sizes and place in memory (csrc/cache8_attention_mma.cu)."""
-    return (ops.fast_kernels_on() and (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0
-            and bool(ops._fn("cache8", "hb_cache8_attention_mma_supported")(cache.n_kv_heads, cache.page_size, cache.head_dim, cache.k.shape[0])))
+    if cache.mma is None:
+        object.__setattr__(cache, "mma", (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0
+                           and bool(ops._fn("cache8", "hb_cache8_attention_mma_supported")(cache.n_kv_heads, cache.page_size, cache.head_dim, cache.k.shape[0])))
+    return cache.mma and ops.fast_kernels_on()
 
 
-def _attend_mma(q, dt, cache: Cache8, batch, table, single: bool, G: int, window: int, scale: float, out) -> None:
-    pairs = G if single else batch.max_q_len * G
-    nt = 1 if pairs <= 8 else 2 if pairs <= 16 else 4
-    tiles = None if single else _tiles(batch, G, nt)
-    n_tiles = batch.n_rows if single else tiles.shape[0]
-    keys = min(batch.max_pos + 1, window + batch.max_q_len) if window else batch.max_pos + 1
-    ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
-              cache.n_kv_heads, cache.page_size, cache.head_dim, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
-              None, batch.positions.data_ptr(), ops._ptr(tiles), n_tiles, nt,
-              _ranks(n_tiles * (-(-G // (8 * nt)) if single else 1) * cache.n_kv_heads, keys), G, window, scale, out.data_ptr(), ops._stream())
+PORTION_ROWS = 64       # requests of so many rows of bfloat16 have their pages expanded, for the flash kernel
 
 
-def _ranks(tiles: int, keys: int) -> int:
-    """Blocks that share a tile's keys."""
+def _flash_takes(q, cache: Cache8, out, n_heads: int, scale: float) -> bool:
+    return (q.dtype == torch.bfloat16 and q.is_contiguous() and scale > 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
+            and ops.fast.flash_prefill_tc_supported(n_heads, cache.n_kv_heads, cache.head_dim, cache.page_size))
+
+
+def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int) -> None:
+    """Requests of `limit` rows or more: the pages that they see as 16-bit numbers, side by side, and the flash kernel over them."""
+    index, places = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)
+    k, v = _expand(cache, table, index, index.numel(), torch.bfloat16)
+    ops.fast.flash_prefill_tc(q, k, v, places, batch.req_q_start, batch.req_q_len, batch.req_ctx_len, out, batch.max_q_len, n_heads, cache.n_kv_heads,
+                              cache.head_dim, cache.page_size, window, scale, limit)
+
+
+def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: int):
+    """For requests of `limit` rows or more: where in the block table the pages stand that their rows see (int32 [n]), and the table of the n pages
+    side by side (int32 [requests, width], -1: none)."""
+    key = ("cache8 pages", page_size, width, window, limit)
+    if key not in batch.extra:
+        index, places, n = [], np.full((batch.n_requests, width), -1, dtype=np.int32), 0
+        for r, (held, rows) in enumerate(zip(batch.h_ctx_len, batch.h_q_len)):
+            if rows < limit:
+                continue
+            first, end = max(0, held - window + 1) // page_size if window else 0, min(width, -(-(held + rows) // page_size))
+            if end > first:
+                index.append(np.arange(first, end, dtype=np.int32) + r * width)
+                places[r, first:end] = np.arange(n, n + end - first, dtype=np.int32)
+                n += end - first
+        batch.extra[key] = _to_device(np.concatenate(index + [places.ravel()]), batch)
+    both = batch.extra[key][0]
+    n = both.numel() - batch.n_requests * width
+    return both[:n], both[n:].view(batch.n_requests, width)
+
+
+def _to_device(numbers: np.ndarray, batch):
+    """(on the device, the host's copy, which stays until the other is over)"""
+    host = torch.from_numpy(numbers)
+    if batch.tokens.is_cuda:
+        host = host.pin_memory()
+    return host.to(batch.tokens.device, non_blocking=True), host
+
+
+class _Cut:
+    """How the rows of requests of fewer than `limit` rows (0: of all) are cut into tiles of 8 nt (row, query head) pairs of a kv head, whose keys
+    `ranks` blocks share. tiles: int32 [n, 4] on the device, (request, its first row, first pair, pairs of its rows); None where row t is request t's."""
+
+    def __init__(self, batch, cache: Cache8, n_heads: int, window: int, limit: int):
+        _heads(cache, n_heads, window)
+        G = n_heads // cache.n_kv_heads
+        some = [(r, a, c, n) for r, (a, c, n) in enumerate(zip(batch.h_q_start, batch.h_ctx_len, batch.h_q_len)) if n < limit or not limit]
+        most, last = max((n for *_, n in some), default=1), batch.max_pos if not limit else max(c + n - 1 for _, _, c, n in some)
+        self.nt = min(4, -(-most * G // 8))
+        self.tiles, self.n_tiles, tiles = None, batch.n_rows, batch.n_rows * -(-G // (8 * self.nt))
+        if most > 1 or len(some) < batch.n_rows:
+            counts = np.array([-(-n * G // (8 * self.nt)) for *_, n in some])
+            numbers = np.empty((int(counts.sum()), 4), dtype=np.int32)
+            for i, column in ((0, [r for r, *_ in some]), (1, [a for _, a, *_ in some]), (3, [n * G for *_, n in some])):
+                numbers[:, i] = np.repeat(np.array(column, dtype=np.int64), counts)
+            numbers[:, 2] = (np.arange(len(numbers)) - np.repeat(np.cumsum(counts) - counts, counts)) * 8 * self.nt
+            self.tiles, self._host = _to_device(numbers, batch)
+            self.n_tiles = tiles = len(numbers)
+        blocks = 4 if self.nt == 1 else 2 if cache.head_dim == 128 and self.nt > 2 else 4 if cache.head_dim == 64 and self.nt == 2 else 3      # an SM
+        self.ranks = _ranks(tiles * cache.n_kv_heads, min(last + 1, window + most) if window else last + 1, 148 * blocks)
+        # as the binding reads it (Cut in csrc/cache8_binding.cpp)
+        self._native = np.array([batch.n_rows, batch.n_requests, self.n_tiles, self.nt, self.ranks, G, window], dtype=np.int64)
+        self.native = self._native.ctypes.data
+
+
+def _cut(batch, cache: Cache8, n_heads: int, window: int, limit: int) -> _Cut:
+    key = ("cache8 cut", n_heads, cache.n_kv_heads, window, limit)
+    cut = batch.extra.get(key)
+    if cut is None:
+        cut = batch.extra[key] = _Cut(batch, cache, n_heads, window, limit)
+    return cut
+
+
+def _ranks(tiles: int, keys: int, resident: int) -> int:
+    """Blocks that share a tile's keys: 1, 2, 4 or 8, as long as all are on the GPU at once (`resident`) and have 64 keys each."""
     ranks = 1
-    while ranks < 8 and tiles * ranks < 4 * 148 and keys > 64 * ranks:
+    while ranks < 8 and 2 * ranks * tiles <= resident and keys >= 128 * ranks:
         ranks *= 2
     return ranks
-
-
-def _tiles(batch, G: int, nt: int) -> torch.Tensor:
-    """int32 [tiles, 4] on the device: (request, its first row, first (row, head) pair, pairs of its rows), pairs in tiles of 8 nt."""
-    key = ("cache8 tiles", G, nt)
-    if key not in batch.extra:
-        parts = []
-        for r, (start, n) in enumerate(zip(batch.h_q_start, batch.h_q_len)):
-            first = np.arange(0, n * G, 8 * nt, dtype=np.int32)
-            part = np.empty((len(first), 4), dtype=np.int32)
-            part[:, 0], part[:, 1], part[:, 2], part[:, 3] = r, start, first, n * G
-            parts.append(part)
-        host = torch.from_numpy(np.concatenate(parts))
-        host = host.pin_memory() if batch.tokens.is_cuda else host
-        batch.extra[key] = host.to(batch.tokens.device, non_blocking=True), host       # (the host's copy until the other is over)
-    return batch.extra[key][0]
 
 
 def copy_pages(planes: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
     """Page src[i] to page dst[i], for every i, in all layers of all `planes` ([layers, pages, ...] each, a page's numbers side by side; of any types
     and sizes). src and dst are numbers of the host: pages below 0 or outside of a plane, a page copied to twice, and one both copied from and to
     are refused. A source may be copied to several pages."""
+    there = bool(planes) and planes[0].is_cuda
+    bound = _binding() if _bound is None and there else _bound
+    if bound and there:
+        done = bound.copy(planes, src, dst)
+        if done is not None:
+            _done(done, 1)
+            return
     pairs = [np.ascontiguousarray(x, dtype=np.int64) for x in (src, dst)]
     src, dst = pairs
     if src.ndim != 1 or src.shape != dst.shape:
@@ -239,9 +350,31 @@ def copy_pages(planes: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
         if t.numel():
             e = t.element_size()
             numbers.append((t.data_ptr(), t.shape[0], t.stride(0) * e, t.stride(1) * e, inner * e))
-    if len(np.unique(dst)) != len(dst) or np.intersect1d(src, dst).size:
+    if len(set(dst.tolist())) != len(dst) or set(src.tolist()) & set(dst.tolist()):
         raise ops.KernelError("copy_pages: a page is copied to twice, or both copied from and to")
     if not len(src) or not numbers:
         return
     numbers, src, dst = np.array(numbers, dtype=np.int64), src.astype(np.int32), dst.astype(np.int32)
     ops._call("cache8", "hb_copy_pages", numbers.ctypes.data, len(numbers), src.ctypes.data, dst.ctypes.data, len(src), ops._stream())
+
+
+_bound = None
+
+
+def _binding():
+    """The binding (csrc/cache8_binding.cpp), at the addresses of the library's calls; False where it cannot be had."""
+    global _bound
+    lib, module = library.load("cache8"), library.load_binding("cache8")
+    if module is not None:
+        module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value
+                      for name in ("hb_cache8_store", "hb_cache8_expand", "hb_cache8_attention_mma", "hb_copy_pages")))
+    _bound = module or False
+    return _bound
+
+
+def _done(result, launches: int):
+    """What a call through the binding gave."""
+    if result.__class__ is int and result:
+        raise ops.KernelError(library.load("cache8").hb_last_error().decode())
+    library.launches[0] += launches
+    return result

@@ -47,7 +47,7 @@ OWN_HEADERS: Dict[str, List[str]] = {"cache8": ["cache8.cuh"]}      # headers of
 
 
 # binding name -> its source; the module is called hipinfer_b200_<name>_binding
-BINDINGS: Dict[str, str] = {"drafts": "drafts_binding.cpp"}
+BINDINGS: Dict[str, str] = {"drafts": "drafts_binding.cpp", "cache8": "cache8_binding.cpp"}
 
 
 class KernelLibraryError(RuntimeError):
