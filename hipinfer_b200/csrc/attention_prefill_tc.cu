@@ -40,7 +40,13 @@
 // tile less the bias of its nearest key bounds the tile's scores from above; that bound takes the maximum's place (any
 // reference value gives the same quotient; the caller keeps the bias's spread within a tile far from the exponent's range),
 // and a score meets its bias once, in the exponent.
+//
+// C8: the keys and values are codes of a cache in 8 bits (csrc/cache8.cuh) as 16-bit numbers, which hold them exactly, in pages of their own, and meet
+// their scales here: a key's in its scores' multiplication by the scale (the maximum is taken of each 16 keys' maxima, scaled), a value's in the
+// weight's exponent (the row's sum is taken block by block and divided by it again). With keys and values rounded to 16 bits ahead of the products a result is off by 1.6 times as much.
 #include "tc_common.cuh"
+
+#include <type_traits>
 
 constexpr int FT_BM = 128, FT_BN = 128;
 constexpr int FT_TILE = 128 * 64 * 2;  // one [128][64] bf16 tile: 16 KB; a [128][head_dim] operand is head_dim / 64 of them, 64 columns each
@@ -222,6 +228,35 @@ __device__ __forceinline__ bool ft_bring(const FtSpan& sp, const int* table, int
   }
   return true;
 }
+// C8: the scales of the keys' 16-place blocks (csrc/cache8.cuh, C8Scale): of kv head h and request r, the block of key j is
+// scale[h * ld + base[r] + j / 16]; blocks of a whole tile ahead of a request's first and two behind its last may be read, and are numbers.
+struct Ft8 {
+  const float4* scale;
+  const int* base;
+  long ld;
+};
+// The scales of a tile's blocks, tile by tile of an item, as a warp's lanes l < 8 hold them, asked for a tile ahead.
+struct FtScales {
+  const float4* from;
+  int step;
+  float4 next;
+  float k, v_log2, v_inv;      // K's scale times the softmax's, in base 2; V's as a power of two, and 1 / V's
+  uint32_t gone;               // blocks whose page is not there
+  __device__ __forceinline__ FtScales(const Ft8& c8, int request, int h, int tile, int step_)
+      : from(c8.scale + h * c8.ld + c8.base[request] + tile * 8 + (threadIdx.x & 7)), step(step_ * 8), next(*from) {}
+  __device__ __forceinline__ void advance() {          // to the next of this warp's tiles
+    k = fabsf(next.x), v_log2 = next.y, v_inv = next.z;
+    gone = __ballot_sync(0xffffffffu, next.x < 0.f) & 0xffu;
+    from += step;
+    next = *from;
+  }
+};
+struct FtNoScales {
+  float k, v_log2, v_inv;
+  uint32_t gone;
+  template <typename... A> __device__ __forceinline__ explicit FtNoScales(const A&...) {}
+  __device__ __forceinline__ void advance() {}
+};
 // The exponentials of two scores.
 template <bool EX>
 __device__ __forceinline__ void ft_exp(uint32_t s0, uint32_t s1, uint64_t scale2, uint64_t sub2, float r1, float r2, float dist, float& p0, float& p1) {
@@ -238,13 +273,15 @@ __device__ __forceinline__ void ft_exp(uint32_t s0, uint32_t s1, uint64_t scale2
 // more than FT_SLACK, so P <= 2^FT_SLACK; the sum l_run is in the same units, and O / l_run is exact whichever maxima were used.
 constexpr float FT_SLACK = 8.f;
 
-template <bool EX>
+template <bool EX, bool C8>
 __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const int* __restrict__ bt, int bt_stride, const int* __restrict__ q_start,
     const int* __restrict__ q_len, const int* __restrict__ ctx_len, __nv_bfloat16* __restrict__ out, int Hq, int Hkv,
     int page_size, int window, float scale_log2, int min_rows, int* status, const float* __restrict__ r1p,
-    const float* __restrict__ r2p, const float* __restrict__ sink, int req0, int reqs, int qt0, int qts, int most) {
+    const float* __restrict__ r2p, const float* __restrict__ sink, int req0, int reqs, int qt0, int qts, int most,
+    const Ft8 c8) {
+  static_assert(!(EX && C8), "a bias or a sink, or codes");
   constexpr int FT_D = 128, NH = FT_D / 64, OPND = NH * FT_TILE;
   // the 128-byte swizzle wants the tiles on 1 KB boundaries, and there is no room for slack: checked below
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -396,14 +433,17 @@ __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
       const float r1 = EX && r1p ? r1p[hq] : 0.f, r2 = EX && r1p ? r2p[hq] : 0.f;
       const uint32_t tmem_o = tmem + 256 + (k & 1) * 128 + lane_base;
       float m_run = -INFINITY, l_run = 0.f;
+      std::conditional_t<C8, FtScales, FtNoScales> now(c8, e.w, hq / (Hq / Hkv), sp.kt_lo + (int)((t0 ^ c) & 1), 2);
       for (int i = (t0 ^ c) & 1; i < sp.n; i += 2) {
+        now.advance();
         const uint32_t t = t0 + i, ph = (t >> 1) & 1, ph_before = ((t - 1) >> 1) & 1;     // this tile's use, and that of the tile before
         const int k_base = (sp.kt_lo + i) * FT_BN;
         const bool need_mask = k_base + FT_BN - 1 > e.z || (window > 0 && k_base < sp.p_last - window + 1);
         if (!wait(&bar->s_full[c], ph)) break;
         hb_tc_fence_after();
-        // a row of S in one read; in two with a bias (EX), whose chains are longer and want registers of their own: the second half stays, the first is read again
-        constexpr int H = EX ? 64 : 128;
+        // a row of S in one read; in two with a bias (EX) or codes (C8), whose chains are longer and want registers of their own: the second half stays, the first is read again
+        constexpr bool HALVES = EX || C8;
+        constexpr int H = HALVES ? 64 : 128;
         uint32_t sr[H];
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         const int hi_j = qp - k_base, lo_j = window > 0 ? qp - window - k_base : -1;  // key j of the tile is visible iff lo_j < j <= hi_j
@@ -415,10 +455,10 @@ __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
           for (int q = 0; q < H; q += 32) ft_ld32_fence(sr + q);
         };
         auto mask = [&](int at) {
-          if (need_mask) {
+          if (need_mask || (C8 && now.gone)) {
 #pragma unroll
             for (int j = 0; j < H; j++)
-              if (!(j + at <= hi_j && j + at > lo_j)) sr[j] = __float_as_uint(-INFINITY);
+              if (!(j + at <= hi_j && j + at > lo_j) || (C8 && (now.gone >> ((j + at) / 16) & 1))) sr[j] = __float_as_uint(-INFINITY);
           }
         };
         auto free_s = [&] {        // the scores of the warpgroup's next tile may overwrite S
@@ -429,12 +469,27 @@ __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
 #pragma unroll
         for (int at = 0; at < 128; at += H) {
           read(at);
-          if (!EX) free_s();
+          if (!HALVES) free_s();
           mask(at);
+          if (C8) {
+            float f[4];      // (the four are asked for together: one at a time, each was waited for)
+#pragma unroll
+            for (int b = 0; b < 4; b++) f[b] = __shfl_sync(0xffffffffu, now.k, at / 16 + b);
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+              float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+              for (int j = b * 16; j < b * 16 + 16; j += 4) {
+                x0 = fmaxf(fmaxf(x0, __uint_as_float(sr[j])), __uint_as_float(sr[j + 1]));
+                x1 = fmaxf(fmaxf(x1, __uint_as_float(sr[j + 2])), __uint_as_float(sr[j + 3]));
+              }
+              mx[b] = fmaxf(mx[b], fmaxf(x0, x1) * f[b]);
+            }
+          } else
 #pragma unroll
           for (int j = 0; j < H; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], __uint_as_float(sr[j])), __uint_as_float(sr[j + 1]));
         }
-        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (C8 ? 1.f : scale_log2);
         const float dist0 = (float)(qp - k_base);                     // of the tile's first key
         if (EX) m_tile -= r1 * __log2f(fmaf(r2, fmaxf(dist0 - (FT_BN - 1), 0.f), 1.f));
         if (i > 0) {       // the maximum so far, from the other warpgroup's tile
@@ -455,30 +510,54 @@ __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
         uint64_t sum2[2] = {0ull, 0ull};   // four sums of pairs, of keys 64-127 first (the order that one warpgroup with half a row in registers has)
 #pragma unroll
         for (int hh = 1; hh >= 0; hh--) {
-          if (EX && hh == 0) {
+          if (HALVES && hh == 0) {
             read(0);
             free_s();
             mask(0);
           }
-          uint32_t* x = sr + (EX ? 0 : hh * 64);
+          uint32_t* x = sr + (HALVES ? 0 : hh * 64);
+          uint64_t scale_j = scale2, sub_j = sub2, block2 = 0ull;
+          float k_of[4], v_log2_of[4], v_inv_of[4];
+          if (C8) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+              k_of[b] = __shfl_sync(0xffffffffu, now.k, hh * 4 + b);
+              v_log2_of[b] = __shfl_sync(0xffffffffu, now.v_log2, hh * 4 + b);
+              v_inv_of[b] = __shfl_sync(0xffffffffu, now.v_inv, hh * 4 + b);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {  // masked scores are -inf: 2^-inf = 0
             float p0, p1, p2, p3;
-            ft_exp<EX>(x[j], x[j + 1], scale2, sub2, r1, r2, dist0 - (float)(j + hh * 64), p0, p1);
-            ft_exp<EX>(x[j + 2], x[j + 3], scale2, sub2, r1, r2, dist0 - (float)(j + 2 + hh * 64), p2, p3);
-            sum2[(j >> 2) & 1] = ft_add2(sum2[(j >> 2) & 1], ft_pack2(__float_as_uint(p0 + p1), __float_as_uint(p2 + p3)));
+            if (C8 && j % 16 == 0) {      // the weights come times their value's scale, and a block's sum is divided by it
+              const uint32_t f = __float_as_uint(k_of[j / 16]);
+              const uint32_t d = __float_as_uint(v_log2_of[j / 16] - sub);
+              scale_j = ft_pack2(f, f), sub_j = ft_pack2(d, d);
+              block2 = 0ull;
+            }
+            ft_exp<EX>(x[j], x[j + 1], scale_j, sub_j, r1, r2, dist0 - (float)(j + hh * 64), p0, p1);
+            ft_exp<EX>(x[j + 2], x[j + 3], scale_j, sub_j, r1, r2, dist0 - (float)(j + 2 + hh * 64), p2, p3);
+            if (C8) {
+              block2 = ft_add2(block2, ft_pack2(__float_as_uint(p0 + p1), __float_as_uint(p2 + p3)));
+              if (j % 16 == 12) {
+                const uint32_t d = __float_as_uint(v_inv_of[j / 16]);
+                sum2[(j >> 4) & 1] = ft_fma2(block2, ft_pack2(d, d), sum2[(j >> 4) & 1]);
+              }
+            } else {
+              sum2[(j >> 2) & 1] = ft_add2(sum2[(j >> 2) & 1], ft_pack2(__float_as_uint(p0 + p1), __float_as_uint(p2 + p3)));
+            }
             x[j >> 1] = hb_pack_bf16(p0, p1);
             x[(j >> 1) + 1] = hb_pack_bf16(p2, p3);
           }
           // (without a bias the exponentials of the whole row come first: half by half they were 10 % slower)
-          if (EX || hh == 0) {
+          if (HALVES || hh == 0) {
             // the product of the tile two before has read P
-            if ((!EX || hh == 1) && t >= 2 && !wait(&bar->pv_done[c], ph ^ 1)) break;
+            if ((!HALVES || hh == 1) && t >= 2 && !wait(&bar->pv_done[c], ph ^ 1)) break;
             // 64 keys = eight 16-byte chunks of this row in K block hh of P
 #pragma unroll
-            for (int cc = EX ? hh * 8 : 0; cc < (EX ? hh * 8 + 8 : 16); cc++) {
+            for (int cc = HALVES ? hh * 8 : 0; cc < (HALVES ? hh * 8 + 8 : 16); cc++) {
               const uint32_t dst = hb_smem_u32(sP + (2 * c + (cc >> 3)) * FT_TILE) + r * 128 + (((cc & 7) ^ (r & 7)) << 4);
-              const uint32_t* y = sr + (EX ? 0 : (cc >> 3) * 64) + 4 * (cc & 7);
+              const uint32_t* y = sr + (HALVES ? 0 : (cc >> 3) * 64) + 4 * (cc & 7);
               asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
             }
           }
@@ -525,7 +604,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
       if (ok && wait(&bar->pv_done[cl], ph_last)) {
         hb_tc_fence_after();
         if (EX && sink) l_run += hb_exp2(fmaf(sink[hq], 1.4426950408889634f, -m_run));
-        const float inv = 1.f / l_run;
+        const float inv = C8 && l_run == 0.f ? 0.f : 1.f / l_run;
         constexpr int HC = FT_D / 2;                                 // this warpgroup's columns: c * HC ..
         uint32_t o[HC];
         hb_tmem_ld64_nowait(tmem_o + c * HC, o);
@@ -565,13 +644,15 @@ __global__ void __launch_bounds__(FT_THREADS, 1) flash_prefill_tc_kernel(
 // ---------------------------------------------------------------------------------------
 // head_dim 64: one chain, two CTAs an SM.
 // ---------------------------------------------------------------------------------------
-template <bool EX>
+template <bool EX, bool C8>
 __global__ void __launch_bounds__(256, 2) flash_prefill_tc64_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const int* __restrict__ bt, int bt_stride, const int* __restrict__ q_start,
     const int* __restrict__ q_len, const int* __restrict__ ctx_len, __nv_bfloat16* __restrict__ out, int Hq, int Hkv,
     int page_size, int window, float scale_log2, int min_rows, int* status, const float* __restrict__ r1p,
-    const float* __restrict__ r2p, const float* __restrict__ sink, int req0, int reqs, int qt0, int qts, int most) {
+    const float* __restrict__ r2p, const float* __restrict__ sink, int req0, int reqs, int qt0, int qts, int most,
+    const Ft8 c8) {
+  static_assert(!(EX && C8), "a bias or a sink, or codes");
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                 // [128][64]
   uint8_t* sP = sQ + FT_TILE;         // two K blocks of [128 rows][64 keys]
@@ -697,7 +778,9 @@ __global__ void __launch_bounds__(256, 2) flash_prefill_tc64_kernel(
       const int qp = e.z + min(r, e.y - 1);      // rows past the portion's end are computed, never stored
       const float r1 = EX && r1p ? r1p[hq] : 0.f, r2 = EX && r1p ? r2p[hq] : 0.f;
       float m_run = -INFINITY, l_run = 0.f;
+      std::conditional_t<C8, FtScales, FtNoScales> now(c8, e.w, hq / (Hq / Hkv), sp.kt_lo, 1);
       for (int i = 0; i < sp.n && ok; i++, cnt++) {
+        now.advance();
         const int k_base = (sp.kt_lo + i) * FT_BN;
         const bool need_mask = k_base + FT_BN - 1 > e.z || (window > 0 && k_base < sp.p_last - window + 1);
         const int hi_j = qp - k_base, lo_j = window > 0 ? qp - window - k_base : -1;  // key j of the tile is visible iff lo_j < j <= hi_j
@@ -710,15 +793,30 @@ __global__ void __launch_bounds__(256, 2) flash_prefill_tc64_kernel(
           hb_tmem_ld64_nowait(tmem_s + lane_base + hh * 64, sr);
           hb_tmem_ld_wait();
           hb_tmem_ld_fence64(sr);
-          if (need_mask) {
+          if (need_mask || (C8 && now.gone)) {
 #pragma unroll
             for (int j = 0; j < 64; j++)
-              if (!(j + hh * 64 <= hi_j && j + hh * 64 > lo_j)) sr[j] = __float_as_uint(-INFINITY);
+              if (!(j + hh * 64 <= hi_j && j + hh * 64 > lo_j) || (C8 && (now.gone >> (hh * 4 + j / 16) & 1))) sr[j] = __float_as_uint(-INFINITY);
           }
+          if (C8) {
+            float f[4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) f[b] = __shfl_sync(0xffffffffu, now.k, hh * 4 + b);
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+              float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+              for (int j = b * 16; j < b * 16 + 16; j += 4) {
+                x0 = fmaxf(fmaxf(x0, __uint_as_float(sr[j])), __uint_as_float(sr[j + 1]));
+                x1 = fmaxf(fmaxf(x1, __uint_as_float(sr[j + 2])), __uint_as_float(sr[j + 3]));
+              }
+              mx[b] = fmaxf(mx[b], fmaxf(x0, x1) * f[b]);
+            }
+          } else
 #pragma unroll
           for (int j = 0; j < 64; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], __uint_as_float(sr[j])), __uint_as_float(sr[j + 1]));
         }
-        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (C8 ? 1.f : scale_log2);
         const float dist0 = (float)(qp - k_base);                     // of the tile's first key
         if (EX) m_tile -= r1 * __log2f(fmaf(r2, fmaxf(dist0 - (FT_BN - 1), 0.f), 1.f));
         const bool grow = m_tile > m_run + FT_SLACK;   // also the first tile with a visible key: m_run is -inf
@@ -740,18 +838,42 @@ __global__ void __launch_bounds__(256, 2) flash_prefill_tc64_kernel(
             hb_tc_fence_before();
             __syncwarp();
             if (lane == 0) hb_mbar_arrive(&bar->s_free);  // the last read of S: the scores of the next tile may overwrite it
-            if (need_mask) {
+            if (need_mask || (C8 && now.gone)) {
 #pragma unroll
               for (int j = 0; j < 64; j++)
-                if (!(j <= hi_j && j > lo_j)) sr[j] = __float_as_uint(-INFINITY);
+                if (!(j <= hi_j && j > lo_j) || (C8 && (now.gone >> (j / 16) & 1))) sr[j] = __float_as_uint(-INFINITY);
+            }
+          }
+          uint64_t scale_j = scale2, sub_j = sub2, block2 = 0ull;
+          float k_of[4], v_log2_of[4], v_inv_of[4];
+          if (C8) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+              k_of[b] = __shfl_sync(0xffffffffu, now.k, hh * 4 + b);
+              v_log2_of[b] = __shfl_sync(0xffffffffu, now.v_log2, hh * 4 + b);
+              v_inv_of[b] = __shfl_sync(0xffffffffu, now.v_inv, hh * 4 + b);
             }
           }
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {  // masked scores are -inf: 2^-inf = 0
             float p0, p1, p2, p3;
-            ft_exp<EX>(sr[j], sr[j + 1], scale2, sub2, r1, r2, dist0 - (float)(j + hh * 64), p0, p1);
-            ft_exp<EX>(sr[j + 2], sr[j + 3], scale2, sub2, r1, r2, dist0 - (float)(j + 2 + hh * 64), p2, p3);
-            sum2[(j >> 2) & 1] = ft_add2(sum2[(j >> 2) & 1], ft_pack2(__float_as_uint(p0 + p1), __float_as_uint(p2 + p3)));
+            if (C8 && j % 16 == 0) {      // the weights come times their value's scale, and a block's sum is divided by it
+              const uint32_t f = __float_as_uint(k_of[j / 16]);
+              const uint32_t d = __float_as_uint(v_log2_of[j / 16] - sub);
+              scale_j = ft_pack2(f, f), sub_j = ft_pack2(d, d);
+              block2 = 0ull;
+            }
+            ft_exp<EX>(sr[j], sr[j + 1], scale_j, sub_j, r1, r2, dist0 - (float)(j + hh * 64), p0, p1);
+            ft_exp<EX>(sr[j + 2], sr[j + 3], scale_j, sub_j, r1, r2, dist0 - (float)(j + 2 + hh * 64), p2, p3);
+            if (C8) {
+              block2 = ft_add2(block2, ft_pack2(__float_as_uint(p0 + p1), __float_as_uint(p2 + p3)));
+              if (j % 16 == 12) {
+                const uint32_t d = __float_as_uint(v_inv_of[j / 16]);
+                sum2[(j >> 4) & 1] = ft_fma2(block2, ft_pack2(d, d), sum2[(j >> 4) & 1]);
+              }
+            } else {
+              sum2[(j >> 2) & 1] = ft_add2(sum2[(j >> 2) & 1], ft_pack2(__float_as_uint(p0 + p1), __float_as_uint(p2 + p3)));
+            }
             sr[j >> 1] = hb_pack_bf16(p0, p1);
             sr[(j >> 1) + 1] = hb_pack_bf16(p2, p3);
           }
@@ -790,7 +912,7 @@ __global__ void __launch_bounds__(256, 2) flash_prefill_tc64_kernel(
       if (ok) {
         hb_tc_fence_after();
         if (EX && sink) l_run += hb_exp2(fmaf(sink[hq], 1.4426950408889634f, -m_run));
-        const float inv = 1.f / l_run;
+        const float inv = C8 && l_run == 0.f ? 0.f : 1.f / l_run;
         uint32_t o[64];
         hb_tmem_ld64_nowait(tmem_o + lane_base, o);
         hb_tmem_ld_wait();
@@ -870,17 +992,17 @@ HB_EXPORT int hb_flash_prefill_tc_launches(int T, int R, int max_q_len, int Hq, 
 // q, out [T, Hq, D] bf16; caches [num_pages, Hkv, page_size, D] bf16 (D 64 or 128); per request q_start, q_len,
 // ctx_len and a block table row, as hb_flash_prefill. Requests with fewer than min_rows rows are
 // skipped. `status` is set to 1 if a bounded wait ran out.
-HB_EXPORT int hb_flash_prefill_tc(const void* q, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride,
-                                  const int* q_start, const int* q_len, const int* ctx_len, void* out, int T, int R,
-                                  int max_q_len, int Hq, int Hkv, int D, int page_size, int window, float scale,
-                                  int min_rows, int* status, const float* r1, const float* r2, const float* sink,
-                                  cudaStream_t st) {
+static int flash_prefill_tc(const void* q, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* q_start,
+                            const int* q_len, const int* ctx_len, void* out, int T, int R, int max_q_len, int Hq, int Hkv, int D, int page_size,
+                            int window, float scale, int min_rows, int* status, const float* r1, const float* r2, const float* sink, const Ft8* c8,
+                            cudaStream_t st) {
   if (R <= 0 || max_q_len <= 0 || T <= 0) return 0;
   if (!hb_flash_prefill_tc_supported(Hq, Hkv, D, page_size))
     HB_FAIL("hb_flash_prefill_tc: %d/%d heads of %d with pages of %d are not supported", Hq, Hkv, D, page_size);
   if (R > 65535 || max_q_len > 65535 * FT_BM) HB_FAIL("hb_flash_prefill_tc: %d requests / portions of %d rows are beyond the grid limit", R, max_q_len);
   if (!status) HB_FAIL("hb_flash_prefill_tc: no status word");
   const bool ex = r1 || sink;
+  const Ft8 codes = c8 ? *c8 : Ft8{};
   if ((r1 != nullptr) != (r2 != nullptr) || (ex && window > 0)) HB_FAIL("hb_flash_prefill_tc: a distance bias needs both of its vectors, and no window");
   CUtensorMap mq, mk, mv;
   if (hb_make_tensor_map_bf16(&mq, q, (uint64_t)T, (uint64_t)Hq * D, (uint64_t)Hq * D, FT_BM)) return -1;
@@ -900,7 +1022,7 @@ HB_EXPORT int hb_flash_prefill_tc(const void* q, const void* kc, const void* vc,
       configured = true;                                                                                                        \
     }                                                                                                                           \
     e = hb_launch(KERN, grid, THREADS, SMEM, st, mq, mk, mv, bt, bt_stride, q_start, q_len, ctx_len, (__nv_bfloat16*)out, Hq,   \
-                  Hkv, page_size, window, sl2, min_rows, status, r1, r2, sink, req0, reqs, qt0, qts, most);         \
+                  Hkv, page_size, window, sl2, min_rows, status, r1, r2, sink, req0, reqs, qt0, qts, most, codes);  \
   } while (0)
   for (int req0 = 0; req0 < R && e == cudaSuccess; req0 += c.req_step)
     for (int qt0 = 0; qt0 < c.tiles && e == cudaSuccess; qt0 += c.qt_step) {
@@ -909,13 +1031,36 @@ HB_EXPORT int hb_flash_prefill_tc(const void* q, const void* kc, const void* vc,
       const int grid = (int)(items < c.ctas ? (items > 0 ? items : 1) : c.ctas);
       const long share = (long)(D == 64 ? FT_OWN64 : FT_OWN) * grid / Hq;      // (of a smaller grid: whatever the lengths say, a CTA's items have places)
       const int most = share < c.most ? (int)share : c.most;
-      if (D == 64 && !ex) FT_LAUNCH(flash_prefill_tc64_kernel<false>, 256, FT_SMEM64);
-      else if (D == 64) FT_LAUNCH(flash_prefill_tc64_kernel<true>, 256, FT_SMEM64);
-      else if (!ex) FT_LAUNCH(flash_prefill_tc_kernel<false>, FT_THREADS, FT_SMEM);
-      else FT_LAUNCH(flash_prefill_tc_kernel<true>, FT_THREADS, FT_SMEM);
+      if (D == 64 && c8) FT_LAUNCH((flash_prefill_tc64_kernel<false, true>), 256, FT_SMEM64);
+      else if (D == 64 && !ex) FT_LAUNCH((flash_prefill_tc64_kernel<false, false>), 256, FT_SMEM64);
+      else if (D == 64) FT_LAUNCH((flash_prefill_tc64_kernel<true, false>), 256, FT_SMEM64);
+      else if (c8) FT_LAUNCH((flash_prefill_tc_kernel<false, true>), FT_THREADS, FT_SMEM);
+      else if (!ex) FT_LAUNCH((flash_prefill_tc_kernel<false, false>), FT_THREADS, FT_SMEM);
+      else FT_LAUNCH((flash_prefill_tc_kernel<true, false>), FT_THREADS, FT_SMEM);
     }
 #undef FT_LAUNCH
   if (e != cudaSuccess) HB_FAIL("hb_flash_prefill_tc: %s", cudaGetErrorString(e));
   HB_CHECK_LAUNCH("hb_flash_prefill_tc");
   return 0;
+}
+
+HB_EXPORT int hb_flash_prefill_tc(const void* q, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride,
+                                  const int* q_start, const int* q_len, const int* ctx_len, void* out, int T, int R,
+                                  int max_q_len, int Hq, int Hkv, int D, int page_size, int window, float scale,
+                                  int min_rows, int* status, const float* r1, const float* r2, const float* sink,
+                                  cudaStream_t st) {
+  return flash_prefill_tc(q, kc, vc, num_pages, bt, bt_stride, q_start, q_len, ctx_len, out, T, R, max_q_len, Hq, Hkv, D, page_size, window, scale,
+                          min_rows, status, r1, r2, sink, nullptr, st);
+}
+
+// The same over codes of a cache in 8 bits as 16-bit numbers (kc, vc, bt: pages of their own, each request's one after the other), whose scales,
+// the softmax's among them, stand as Ft8 says.
+HB_EXPORT int hb_flash_prefill_tc_cache8(const void* q, const void* kc, const void* vc, long num_pages, const int* bt, int bt_stride, const int* q_start,
+                                         const int* q_len, const int* ctx_len, void* out, int T, int R, int max_q_len, int Hq, int Hkv, int D,
+                                         int page_size, int window, int min_rows, int* status, const void* scale, const int* base, long ld_scale,
+                                         cudaStream_t st) {
+  if (page_size % 16 || ((uintptr_t)scale & 15)) HB_FAIL("hb_flash_prefill_tc_cache8: pages of %d, or scales that are not aligned", page_size);
+  const Ft8 c8 = {(const float4*)scale, base, ld_scale};
+  return flash_prefill_tc(q, kc, vc, num_pages, bt, bt_stride, q_start, q_len, ctx_len, out, T, R, max_q_len, Hq, Hkv, D, page_size, window, 1.f,
+                          min_rows, status, nullptr, nullptr, nullptr, &c8, st);
 }

@@ -27,7 +27,6 @@
 
 #include <cuda_fp16.h>
 
-#include <type_traits>
 
 constexpr int C8M_WARPS = 4, C8M_RANKS = 8;      // warps of a block; blocks of a cluster at most
 
@@ -148,6 +147,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   extern __shared__ __align__(128) uint8_t smem[];
   uint2* q_sh = (uint2*)smem;                                           // [part][nt][step][lane]
   float* o_sh = (float*)smem;                                           // [warp][pair][PITCH], over the query when it is done with
+  __shared__ float col_sh[Z::Q_REGS ? 1 : PAIRS];
   __shared__ float m_sh[C8M_WARPS][PAIRS], l_sh[C8M_WARPS][PAIRS], m_cta[PAIRS], l_cta[PAIRS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3, h = blockIdx.y;
   const int ranks = gridDim.x, rank = blockIdx.x;
@@ -207,9 +207,8 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   uint2 q_reg[Z::Q_REGS ? PARTS : 1][Z::Q_REGS ? Q_STEPS : 1];
   float col[NT][2];                                                     // of columns 2 tq, 2 tq + 1: score = product * col * the unit's scale
   int col_hi[NT][2];                                                    // their rows' positions
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-    const int pair = pair0 + nt * 8 + g;
+  if (Z::Q_REGS || warp < NT) {                                         // each warp its own, or a warp 8 pairs for all
+    const int nt = Z::Q_REGS ? 0 : warp, pair = pair0 + nt * 8 + g;
     float x[STEPS][4], most = 0.f;
     if (nt * 8 + g < n) {
       const T* q = (const T*)a.q + (t0 + pair / a.G) * a.ld_q + ((long)h * a.G + pair % a.G) * D;
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       if constexpr (Z::Q_REGS) q_reg[part][step] = v;
       else q_sh[((part * NT + nt) * Q_STEPS + step) * 32 + lane] = v;
     };
-    if (Z::Q_REGS || warp == 0) {                                       // (every warp knows `down`; one writes the query)
+    {
       if constexpr (Z::Q_INT) {
 #pragma unroll
         for (int s = 0; s < Q_STEPS; s++) {
@@ -282,14 +281,18 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
         }
       }
     }
+    if constexpr (Z::Q_REGS) col[0][0] = __shfl_sync(0xffffffffu, down, 8 * tq), col[0][1] = __shfl_sync(0xffffffffu, down, 8 * tq + 4);
+    else if (tq == 0) col_sh[nt * 8 + g] = down;
+  }
+  if constexpr (!Z::Q_REGS) __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
 #pragma unroll
     for (int c = 0; c < 2; c++) {
-      col[nt][c] = __shfl_sync(0xffffffffu, down, (2 * tq + c) * 4);
       const int i = nt * 8 + 2 * tq + c;
+      if constexpr (!Z::Q_REGS) col[nt][c] = col_sh[i];
       col_hi[nt][c] = i < n ? a.pos[t0 + (pair0 + i) / a.G] : -1;
     }
-  }
-  __syncthreads();
 
   float o[STEPS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -573,17 +576,38 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
 }
 
 template <typename CT, typename T, int D, int NT>
-static cudaError_t launch(const C8Attend& a, int tiles, int ranks, cudaStream_t st) {
-  constexpr int smem = C8Sizes<CT, T, D, NT>::SMEM;
+static cudaError_t configure() {                                        // once on each device
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && configured[dev])) return e;
+  e = cudaFuncSetAttribute(cache8_attention_mma_kernel<CT, T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C8Sizes<CT, T, D, NT>::SMEM);
+  if (e == cudaSuccess && dev < 64) configured[dev] = true;
+  return e;
+}
+
+template <typename CT, typename T, int D, int NT>
+static cudaError_t clusters(int ranks, int* n) {
+  cudaError_t e = configure<CT, T, D, NT>();
   if (e != cudaSuccess) return e;
-  if (smem > 40 * 1024 && (dev >= 64 || !configured[dev])) {
-    e = cudaFuncSetAttribute(cache8_attention_mma_kernel<CT, T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) configured[dev] = true;
-  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks, 1, 1);
+  cfg.blockDim = dim3(32 * C8M_WARPS);
+  cfg.dynamicSmemBytes = C8Sizes<CT, T, D, NT>::SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(n, cache8_attention_mma_kernel<CT, T, D, NT>, &cfg);
+}
+
+template <typename CT, typename T, int D, int NT>
+static cudaError_t launch(const C8Attend& a, int tiles, int ranks, cudaStream_t st) {
+  constexpr int smem = C8Sizes<CT, T, D, NT>::SMEM;
+  cudaError_t e = configure<CT, T, D, NT>();
+  if (e != cudaSuccess) return e;
   C8Attend b = a;
   for (int first = 0; first < tiles; first += 65535) {                  // (the grid's limit)
     b.first_tile = first;
@@ -594,9 +618,34 @@ static cudaError_t launch(const C8Attend& a, int tiles, int ranks, cudaStream_t 
   return cudaSuccess;
 }
 
+// e = what the call gives with DD and NN for the sizes d and n.
+#define C8_VARIANTS(d, n, ...)                                                                                       \
+  do {                                                                                                               \
+    if ((d) == 64) {                                                                                                 \
+      constexpr int DD = 64;                                                                                         \
+      if ((n) == 1) { constexpr int NN = 1; e = __VA_ARGS__; } else if ((n) == 2) { constexpr int NN = 2; e = __VA_ARGS__; } \
+      else if ((n) == 3) { constexpr int NN = 3; e = __VA_ARGS__; } else if ((n) == 4) { constexpr int NN = 4; e = __VA_ARGS__; } \
+    } else if ((d) == 128) {                                                                                         \
+      constexpr int DD = 128;                                                                                        \
+      if ((n) == 1) { constexpr int NN = 1; e = __VA_ARGS__; } else if ((n) == 2) { constexpr int NN = 2; e = __VA_ARGS__; } \
+      else if ((n) == 3) { constexpr int NN = 3; e = __VA_ARGS__; } else if ((n) == 4) { constexpr int NN = 4; e = __VA_ARGS__; } \
+    }                                                                                                                \
+  } while (0)
+
 HB_EXPORT int hb_cache8_attention_mma_supported(int Hkv, int page_size, int D, long n_pages) {
   return Hkv >= 1 && Hkv <= 65535 && page_size >= C8_BLOCK && page_size % C8_BLOCK == 0 && (D == 64 || D == 128) &&
          n_pages * Hkv * (page_size / C8_BLOCK) < (1L << 31);
+}
+
+// Clusters of `ranks` blocks that the current device holds at once (their blocks share a part of it, so it need not be its blocks by their number).
+HB_EXPORT int hb_cache8_attention_mma_clusters(int dt, int ct, int D, int nt, int ranks) {
+  int n = 0;
+  cudaError_t e = cudaErrorInvalidValue;
+  C8_DISPATCH(ct, "hb_cache8_attention_mma_clusters", HB_DISPATCH_1(dt, "hb_cache8_attention_mma_clusters", {
+    C8_VARIANTS(D, nt, (clusters<CT, TA, DD, NN>(ranks, &n)));
+  }));
+  if (e != cudaSuccess) HB_FAIL("hb_cache8_attention_mma_clusters: %s", cudaGetErrorString(e));
+  return n;
 }
 
 // tiles: n_tiles int4 on the device (C8Attend), pairs in tiles of 8 nt; null: n_tiles rows of one token each, whose G heads are cut into tiles of 8 nt.
@@ -615,12 +664,7 @@ HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const vo
   const int count = tiles ? n_tiles : n_tiles * a.tiles_row;
   cudaError_t e = cudaErrorInvalidValue;
   C8_DISPATCH(ct, "hb_cache8_attention_mma", HB_DISPATCH_1(dt, "hb_cache8_attention_mma", {
-    const auto go = [&](auto d) {
-      constexpr int N = decltype(d)::value;
-      return nt == 1 ? launch<CT, TA, N, 1>(a, count, ranks, st) : nt == 2 ? launch<CT, TA, N, 2>(a, count, ranks, st)
-           : nt == 3 ? launch<CT, TA, N, 3>(a, count, ranks, st) : nt == 4 ? launch<CT, TA, N, 4>(a, count, ranks, st) : cudaErrorInvalidValue;
-    };
-    e = D == 64 ? go(std::integral_constant<int, 64>()) : go(std::integral_constant<int, 128>());
+    C8_VARIANTS(D, nt, (launch<CT, TA, DD, NN>(a, count, ranks, st)));
   }));
   if (e != cudaSuccess) HB_FAIL("hb_cache8_attention_mma: %s", cudaGetErrorString(e));
   HB_CHECK_LAUNCH("hb_cache8_attention_mma");

@@ -17,7 +17,7 @@ struct Cache {
 };
 // What it makes of a step's lengths for one call: how the rows are cut into tiles.
 struct Cut {
-  int64_t rows, requests, n_tiles, nt, ranks, group, window;
+  int64_t rows, requests, n_tiles, nt, ranks, group, window, max_pos;
 };
 typedef int (*StoreFn)(const void*, const void*, long, long, int, const int*, int, int, int, int, long, int, void*, void*, float*, float*, void*);
 typedef int (*ExpandFn)(const void*, const void*, const float*, const float*, int, const int*, const int*, long, long, int, int, int, void*, void*, int, void*);
@@ -106,7 +106,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor* tiles = a[4] == Py_None ? nullptr : tensor(a[4], c->device);
   const int64_t width = c->kv_heads * cut.group * c->head_dim;
   if (!q || !table || !pos || (!tiles && a[4] != Py_None) || q->dim() != 2 || q->size(0) != cut.rows || !cut.rows || q->size(1) != width || q->stride(1) != 1 ||
-      type_code(*q) < 0 || !ints(*table, 2) || table->size(0) != cut.requests || !ints(*pos, 1) || pos->size(0) != cut.rows ||
+      type_code(*q) < 0 || !ints(*table, 2) || table->size(0) != cut.requests ||
+      table->size(1) * c->page_size <= cut.max_pos || !ints(*pos, 1) || pos->size(0) != cut.rows ||
       (tiles && (!ints(*tiles, 2) || tiles->size(0) != cut.n_tiles || tiles->size(1) != 4)))
     Py_RETURN_NONE;
   const double scale = PyFloat_AsDouble(a[6]);

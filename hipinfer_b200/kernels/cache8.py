@@ -9,6 +9,7 @@ The reference keeps its cache in the activations' type (src/api.cu:1409-1411) an
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
@@ -25,6 +26,8 @@ ops._SIGS["cache8"] = {
     "hb_cache8_attention_any": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _f, _p, _p],
     "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p],
     "hb_cache8_attention_mma_supported": [_i, _i, _i, _l],
+    "hb_cache8_attention_mma_clusters": [_i, _i, _i, _i, _i],
+    "hb_cache8_portions": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _f, _p, _p, _p, _p],
     "hb_copy_pages": [_p, _i, _p, _p, _i, _p],
 }
 BLOCK8 = 16                                                        # places of a page that share a scale
@@ -181,11 +184,11 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     table, T, D = batch.block_tables[group], batch.n_rows, cache.head_dim
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     tensor_cores = q.is_cuda and _on_tensor_cores(cache)
-    portions = tensor_cores and batch.max_q_len >= PORTION_ROWS
+    portions = tensor_cores and batch.max_q_len >= PORTION_ROWS[0]
     if tensor_cores and not portions:
         bound = _binding() if _bound is None else _bound
         if bound:
-            cut = _cut(batch, cache, n_heads, window, 0)
+            cut = _cut(batch, cache, ops._dt(q), n_heads, window, 0)
             done = bound.attend(q, cache.native, table, batch.positions, cut.tiles, cut.native, scale, out)
             if done is not None:
                 return _done(done, 1)
@@ -196,8 +199,10 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     if q.shape != (T, n_heads * D) or q.stride(1) != 1:
         raise ops.KernelError(f"attention_cache8: q {tuple(q.shape)}, strides {q.stride()}; {T} rows of {n_heads} heads of {D} are expected")
     dt = ops._dt(q)
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.shape[0] != batch.n_requests:
-        raise ops.KernelError(f"attention_cache8: block table {tuple(table.shape)} {table.dtype} of {batch.n_requests} requests")
+    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.shape[0] != batch.n_requests \
+            or table.shape[1] * cache.page_size <= batch.max_pos:
+        raise ops.KernelError(f"attention_cache8: block table {tuple(table.shape)} {table.dtype}; {batch.n_requests} requests of up to {batch.max_pos + 1} "
+                              f"tokens in pages of {cache.page_size}")
     if out is None:
         out = torch.empty(T, n_heads * D, dtype=q.dtype, device=q.device)
     elif out.shape != (T, n_heads * D) or out.dtype != q.dtype or not out.is_contiguous():
@@ -211,11 +216,11 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
                   None if single else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
                   out.data_ptr(), ops._stream())
         return out
-    limit = PORTION_ROWS if portions and _flash_takes(q, cache, out, n_heads, scale) else 0
+    limit = _portion_limit(batch, cache, n_heads, window) if portions and _flash_takes(q, cache, out, n_heads, scale) else 0
     if limit:
         _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit)
     if not limit or min(batch.h_q_len) < limit:
-        cut = _cut(batch, cache, n_heads, window, limit)
+        cut = _cut(batch, cache, dt, n_heads, window, limit)
         ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
                   cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], None, batch.positions.data_ptr(),
                   ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), ops._stream())
@@ -237,7 +242,40 @@ def _on_tensor_cores(cache: Cache8) -> bool:
     return cache.mma and ops.fast_kernels_on()
 
 
-PORTION_ROWS = 64       # requests of so many rows of bfloat16 have their pages expanded, for the flash kernel
+PORTION_ROWS = (16, 32, 64, 128)
+
+
+def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
+    """From how many rows on a request's pages are expanded for the flash kernel (one of PORTION_ROWS; 0: none are). Per (row, head) and key the
+    flash kernel takes a third of the warp MMAs' time, but works in tiles of 128 rows, walks a tile's keys one after the other and wants the keys
+    expanded; the choice is the least of the step's estimated times. Both as measured, us: 32 heads over 8 of 128, one portion of 64 rows behind 500
+    tokens 19 on warp MMAs and 17 with the flash kernel, behind 8,000 59 and 111; 256 rows behind 2,000 63 and 38, behind 24,000 533 and 346; heads of 64: 15 and
+    18, 51 and 126; 54 and 43, 485 and 439."""
+    key = ("cache8 limit", n_heads, cache.n_kv_heads, cache.head_dim, cache.code, window)
+    if key not in batch.extra:
+        rows, held = np.array(batch.h_q_len, dtype=np.float64), np.array(batch.h_ctx_len, dtype=np.float64)
+        keys = np.minimum(held, window) + rows if window else held + rows
+        best = None
+        for limit in PORTION_ROWS + (0,):
+            flash = rows >= limit if limit else rows < 0
+            if limit and not flash.any():
+                continue
+            us = 0.0
+            if flash.any():
+                n, k = rows[flash], keys[flash]
+                padded = np.ceil(n / 128) * 128 * (k - n / 2)
+                us += 10 + k.sum() * cache.n_kv_heads * cache.head_dim * 6 / 4e6 + max(0.8e-6 * n_heads * padded.sum(), 1.7 / 128 * k.max())
+            if not flash.all():
+                G, most = n_heads // cache.n_kv_heads, int(keys[~flash].max())
+                nt = min(4, -(-int(rows[~flash].max()) * G // 8))
+                tiles = int(np.ceil(rows[~flash] * G / (8 * nt)).sum()) * cache.n_kv_heads
+                clusters = functools.partial(_clusters, 1, cache.code, cache.head_dim, nt)
+                ranks = _ranks(tiles, most, clusters)
+                us += 12 + max(1.0, tiles / clusters(ranks)) * most / ranks * (0.007 + 0.004 * nt)
+            if best is None or us < best[0]:
+                best = us, limit
+        batch.extra[key] = best[1]
+    return batch.extra[key]
 
 
 def _flash_takes(q, cache: Cache8, out, n_heads: int, scale: float) -> bool:
@@ -245,32 +283,41 @@ def _flash_takes(q, cache: Cache8, out, n_heads: int, scale: float) -> bool:
             and ops.fast.flash_prefill_tc_supported(n_heads, cache.n_kv_heads, cache.head_dim, cache.page_size))
 
 
+_AHEAD = 32             # C8_AHEAD of csrc/cache8_store.cu
+
+
 def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int) -> None:
-    """Requests of `limit` rows or more: the pages that they see as 16-bit numbers, side by side, and the flash kernel over them."""
-    index, places = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)
-    k, v = _expand(cache, table, index, index.numel(), torch.bfloat16)
-    ops.fast.flash_prefill_tc(q, k, v, places, batch.req_q_start, batch.req_q_len, batch.req_ctx_len, out, batch.max_q_len, n_heads, cache.n_kv_heads,
-                              cache.head_dim, cache.page_size, window, scale, limit)
+    """Requests of `limit` rows or more: the codes of the pages that they see as 16-bit numbers, side by side, their scales beside them, and the flash
+    kernel over both."""
+    index, places, base = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)      # (one page at least: a row sees its own key)
+    n, device = index.numel(), q.device
+    k, v = (torch.empty((n,) + cache.k.shape[1:], dtype=torch.bfloat16, device=device) for _ in range(2))
+    scales = torch.empty(cache.n_kv_heads, n * cache8_blocks(cache.page_size) + 2 * _AHEAD, 4, dtype=torch.float32, device=device)
+    ops._call("cache8", "hb_cache8_portions", *(t.data_ptr() for t in cache.tensors), cache.code, table.data_ptr(), index.data_ptr(), n, cache.k.shape[0],
+              *cache.k.shape[1:], scale, k.data_ptr(), v.data_ptr(), scales.data_ptr(), ops._stream())
+    ops.fast.flash_prefill_tc_cache8(q, k, v, places, batch.req_q_start, batch.req_q_len, batch.req_ctx_len, out, batch.max_q_len, n_heads,
+                                     cache.n_kv_heads, cache.head_dim, cache.page_size, window, limit, scales, base)
 
 
 def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: int):
-    """For requests of `limit` rows or more: where in the block table the pages stand that their rows see (int32 [n]), and the table of the n pages
-    side by side (int32 [requests, width], -1: none)."""
+    """For requests of `limit` rows or more: where in the block table the pages stand that their rows see (int32 [n]), the table of the n pages side
+    by side (int32 [requests, width], -1: none), and at which of the n pages' blocks of 16 places each request's first key would stand (int32)."""
     key = ("cache8 pages", page_size, width, window, limit)
     if key not in batch.extra:
         index, places, n = [], np.full((batch.n_requests, width), -1, dtype=np.int32), 0
+        base, blocks = np.zeros(batch.n_requests, dtype=np.int32), cache8_blocks(page_size)
         for r, (held, rows) in enumerate(zip(batch.h_ctx_len, batch.h_q_len)):
             if rows < limit:
                 continue
-            first, end = max(0, held - window + 1) // page_size if window else 0, min(width, -(-(held + rows) // page_size))
-            if end > first:
-                index.append(np.arange(first, end, dtype=np.int32) + r * width)
-                places[r, first:end] = np.arange(n, n + end - first, dtype=np.int32)
-                n += end - first
-        batch.extra[key] = _to_device(np.concatenate(index + [places.ravel()]), batch)
-    both = batch.extra[key][0]
-    n = both.numel() - batch.n_requests * width
-    return both[:n], both[n:].view(batch.n_requests, width)
+            first, end = max(0, held - window + 1) // page_size if window else 0, -(-(held + rows) // page_size)
+            index.append(np.arange(first, end, dtype=np.int32) + r * width)
+            places[r, first:end] = np.arange(n, n + end - first, dtype=np.int32)
+            base[r] = (n - first) * blocks + _AHEAD
+            n += end - first
+        batch.extra[key] = _to_device(np.concatenate(index + [places.ravel(), base]), batch)
+    both, R = batch.extra[key][0], batch.n_requests
+    n = both.numel() - R * (width + 1)
+    return both[:n], both[n:n + R * width].view(R, width), both[n + R * width:]
 
 
 def _to_device(numbers: np.ndarray, batch):
@@ -285,7 +332,7 @@ class _Cut:
     """How the rows of requests of fewer than `limit` rows (0: of all) are cut into tiles of 8 nt (row, query head) pairs of a kv head, whose keys
     `ranks` blocks share. tiles: int32 [n, 4] on the device, (request, its first row, first pair, pairs of its rows); None where row t is request t's."""
 
-    def __init__(self, batch, cache: Cache8, n_heads: int, window: int, limit: int):
+    def __init__(self, batch, cache: Cache8, dt: int, n_heads: int, window: int, limit: int):
         _heads(cache, n_heads, window)
         G = n_heads // cache.n_kv_heads
         some = [(r, a, c, n) for r, (a, c, n) in enumerate(zip(batch.h_q_start, batch.h_ctx_len, batch.h_q_len)) if n < limit or not limit]
@@ -300,25 +347,36 @@ class _Cut:
             numbers[:, 2] = (np.arange(len(numbers)) - np.repeat(np.cumsum(counts) - counts, counts)) * 8 * self.nt
             self.tiles, self._host = _to_device(numbers, batch)
             self.n_tiles = tiles = len(numbers)
-        blocks = 4 if self.nt == 1 else 2 if cache.head_dim == 128 and self.nt > 2 else 4 if cache.head_dim == 64 and self.nt == 2 else 3      # an SM
-        self.ranks = _ranks(tiles * cache.n_kv_heads, min(last + 1, window + most) if window else last + 1, 148 * blocks)
+        self.ranks = _ranks(tiles * cache.n_kv_heads, min(last + 1, window + most) if window else last + 1, functools.partial(_clusters, dt, cache.code, cache.head_dim, self.nt))
         # as the binding reads it (Cut in csrc/cache8_binding.cpp)
-        self._native = np.array([batch.n_rows, batch.n_requests, self.n_tiles, self.nt, self.ranks, G, window], dtype=np.int64)
+        self._native = np.array([batch.n_rows, batch.n_requests, self.n_tiles, self.nt, self.ranks, G, window, batch.max_pos], dtype=np.int64)
         self.native = self._native.ctypes.data
 
 
-def _cut(batch, cache: Cache8, n_heads: int, window: int, limit: int) -> _Cut:
-    key = ("cache8 cut", n_heads, cache.n_kv_heads, window, limit)
+def _cut(batch, cache: Cache8, dt: int, n_heads: int, window: int, limit: int) -> _Cut:
+    key = ("cache8 cut", cache.code, cache.k.shape[1:], dt, n_heads, window, limit)
     cut = batch.extra.get(key)
     if cut is None:
-        cut = batch.extra[key] = _Cut(batch, cache, n_heads, window, limit)
+        cut = batch.extra[key] = _Cut(batch, cache, dt, n_heads, window, limit)
     return cut
 
 
-def _ranks(tiles: int, keys: int, resident: int) -> int:
-    """Blocks that share a tile's keys: 1, 2, 4 or 8, as long as all are on the GPU at once (`resident`) and have 64 keys each."""
-    ranks = 1
-    while ranks < 8 and 2 * ranks * tiles <= resident and keys >= 128 * ranks:
+@functools.lru_cache(maxsize=None)
+def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
+    """Clusters of `ranks` blocks of the kernel on warp MMAs that are on the GPU at once."""
+    n = ops._fn("cache8", "hb_cache8_attention_mma_clusters")(dt, code, head_dim, nt, ranks)
+    if n < 1:
+        raise ops.KernelError(library.load("cache8").hb_last_error().decode())
+    return n
+
+
+def _ranks(tiles: int, keys: int, clusters) -> int:
+    """Blocks (1 to 8, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 64 keys each.
+    Lengths differ, and a wave of blocks ends with its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand
+    tokens, us: 153 as one wave of one block a tile, 142 of four; of 2,000 each 49 and 60)."""
+    most = min(8, max(1, keys // 64))
+    ranks = next((r for r in range(most, 1, -1) if clusters(r) >= tiles), 1)
+    while 2 * ranks <= 8 and tiles <= 4 * clusters(2 * ranks) and keys >= 4096 * ranks:
         ranks *= 2
     return ranks
 

@@ -32,6 +32,7 @@ _SIGS = {
     "hb_flash_prefill": [_p, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p],
     "hb_flash_prefill_supported": [_i, _i, _i],
     "hb_flash_prefill_tc": [_p, _p, _p, _l, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p, _p, _p, _p, _p],
+    "hb_flash_prefill_tc_cache8": [_p, _p, _p, _l, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _l, _p],
     "hb_flash_prefill_tc_supported": [_i, _i, _i, _i],
     "hb_flash_prefill_tc_launches": [_i, _i, _i, _i, _i, _i],
     "hb_attn_diff_decode": [_p, _p, _p, _l, _p, _i, _p, _p, _p, _l, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _f, _f, _f, _i, _p, _i, _p, _p, _p],
@@ -52,7 +53,7 @@ _SIGS = {
     "hb_rows_norm_supported": [_i, _i],
 }
 _fns = {}
-_LAUNCHES = {"hb_rows_scaled_qkv_rope": 1, "hb_rows_scaled_swiglu": 1, "hb_rows_norm_qkv_rope": 1, "hb_rows_add": 1, "hb_rows_norm_swiglu": 1, "hb_gemm_tc_rope_kv": 1, "hb_slices_finish": 1, "hb_add_rmsnorm_slices": 1, "hb_rope_kv_slices": 1, "hb_gemm_tc": 1, "hb_gemm_tc_slices": 1, "hb_gemm_stream": 1, "hb_attn_decode": 1, "hb_flash_prefill": 1, "hb_flash_prefill_tc": 1, "hb_flash_diff_tc": 1, "hb_attn_diff_decode": 1, "hb_gemm_tc_grouped": 1}
+_LAUNCHES = {"hb_rows_scaled_qkv_rope": 1, "hb_rows_scaled_swiglu": 1, "hb_rows_norm_qkv_rope": 1, "hb_rows_add": 1, "hb_rows_norm_swiglu": 1, "hb_gemm_tc_rope_kv": 1, "hb_slices_finish": 1, "hb_add_rmsnorm_slices": 1, "hb_rope_kv_slices": 1, "hb_gemm_tc": 1, "hb_gemm_tc_slices": 1, "hb_gemm_stream": 1, "hb_attn_decode": 1, "hb_flash_prefill": 1, "hb_flash_prefill_tc": 1, "hb_flash_prefill_tc_cache8": 1, "hb_flash_diff_tc": 1, "hb_attn_diff_decode": 1, "hb_gemm_tc_grouped": 1}
 _status = None
 _status_address = None
 
@@ -607,6 +608,16 @@ def flash_prefill_tc(q, k_cache, v_cache, block_table, q_start, q_len, ctx_len, 
           block_table.data_ptr(), block_table.stride(0), q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(),
           out.data_ptr(), q.shape[0], q_len.numel(), int(max_q_len), n_heads, n_kv_heads, head_dim, page_size, int(window),
           float(scale), int(min_rows), _status_ptr(), *_extras(distance, sink), _stream())
+    return out
+
+
+def flash_prefill_tc_cache8(q, k_pages, v_pages, places, q_start, q_len, ctx_len, out, max_q_len, n_heads, n_kv_heads, head_dim, page_size, window,
+                            min_rows, scales, base):
+    """The same over a cache in 8 bits (ops.Cache8): k_pages, v_pages are its codes in bfloat16, in pages of their own that `places` names as a block
+    table does, scales and base what csrc/attention_prefill_tc.cu calls Ft8."""
+    _call("hb_flash_prefill_tc_cache8", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], places.data_ptr(), places.stride(0),
+          q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), out.data_ptr(), q.shape[0], q_len.numel(), int(max_q_len), n_heads, n_kv_heads, head_dim,
+          page_size, int(window), int(min_rows), _status_ptr(), scales.data_ptr(), base.data_ptr(), scales.shape[1], _stream())
     return out
 
 

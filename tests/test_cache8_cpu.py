@@ -100,6 +100,10 @@ def test_attention_refuses(calls):
                          (q, 4, dict(out=torch.zeros(3, 512)[:, ::2]))):
         with pytest.raises(ops.KernelError):
             ops.attention_cache8(x, cache, batch, 0, heads, **kw)
+    short = batch_of([5, 20], [1, 2])
+    short.block_tables[0] = short.block_tables[0][:, :1].contiguous()                     # (23 tokens in one page of 16)
+    with pytest.raises(ops.KernelError, match="up to 22 tokens"):
+        ops.attention_cache8(q, cache, short, 0, 4)
     batch.block_tables[0] = batch.block_tables[0].long()
     with pytest.raises(ops.KernelError):
         ops.attention_cache8(q, cache, batch, 0, 4)
