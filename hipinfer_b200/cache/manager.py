@@ -16,7 +16,7 @@ page a request gets is reproducible.
 
 A request may be FORKED: the new one names the whole pages that its parent has filled, and each page counts who holds it;
 it is free again when the last of them lets go. A page held twice is never written: both requests go on in pages of their
-own. A request may also be TRUNCATED, when drafted tokens that it was run with are refused.
+own. Where a fork shall begin inside a page it gets a page of its own there, to which the parent's is to be copied. A request may also be TRUNCATED, when drafted tokens that it was run with are refused.
 
 Beside the pages there are STATE SLOTS: one integer per live request, handed out at admission
 and returned at the end, which indexes tensors of fixed per-request state (a recurrent or
@@ -178,6 +178,7 @@ class RequestCache:
     length: int = 0
     tables: List[List[int]] = field(default_factory=list)  # per group: logical page -> page id or -1
     fresh_slot: bool = True  # the state slot has not been zeroed on the device yet
+    copied: List[Optional[Tuple[int, int]]] = field(default_factory=list)  # of a fork, per group: the page to be copied and where to
 
 
 class CacheManager:
@@ -222,20 +223,38 @@ class CacheManager:
         self.slots.release(rc.state_slot)
         del self.requests[request_id]
 
-    def fork(self, request_id, new_id) -> RequestCache:
+    def fork(self, request_id, new_id, length: Optional[int] = None) -> RequestCache:
         """A new request that holds the whole pages of `request_id`: its length is theirs, and the tokens behind them, if it
         shall have them too, are run again. State slots are not copied: a request whose model keeps per-request state has
         nothing to be forked from. Raises CacheError where the retention rule has given back pages that a query behind the
-        whole pages reads (at a page's end it never has)."""
+        whole pages reads (at a page's end it never has).
+
+        With `length` the new request has exactly so many tokens: the page that the last of them share with none or more of the
+        parent's is one of its own, and `copied` names, per group, the parent's page and its own (None where the length is a
+        page's end or the parent's page is gone). Raises OutOfPages (nothing changed) where a pool has no page for it."""
         rc = self.get(request_id)
-        whole = rc.length // self.page_size
-        if not self._kept(rc, whole * self.page_size):
-            raise CacheError(f"request {request_id!r} cannot be forked at {whole * self.page_size} of its {rc.length} tokens: pages "
+        if length is None:
+            length = rc.length // self.page_size * self.page_size
+        if not 0 <= length <= rc.length:
+            raise CacheError(f"request {request_id!r} holds {rc.length} tokens and cannot be forked at {length}")
+        whole, inside = divmod(length, self.page_size)
+        if not self._kept(rc, length):
+            raise CacheError(f"request {request_id!r} cannot be forked at {length} of its {rc.length} tokens: pages "
                              f"that would be read are gone")
+        if inside:
+            for g, pool in enumerate(self.pools):
+                if rc.tables[g][whole] >= 0 and not pool.free_count:
+                    raise OutOfPages(f"group {self.groups[g].name!r}: a fork of request {request_id!r} at {length} tokens needs a page, none is free")
         new = self.add_request(new_id)
-        new.length = whole * self.page_size
+        new.length = length
         for g, table in enumerate(rc.tables):
             new.tables[g] = [self.pools[g].share(p) if p >= 0 else -1 for p in table[:whole]]
+            if inside:
+                page = self.pools[g].alloc() if table[whole] >= 0 else -1
+                new.tables[g].append(page)
+                new.copied.append((table[whole], page) if page >= 0 else None)
+            else:
+                new.copied.append(None)
         return new
 
     def truncate(self, request_id, length: int) -> int:

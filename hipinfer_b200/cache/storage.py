@@ -3,7 +3,8 @@
 Per cache group and plane (keys, values, or what else the group's mixers keep per token) one
 tensor [layer cache, page, head, page_size, width] in the compute element type: a (page, head)
 pair is one contiguous run of page_size * width elements, which is what the attention kernels
-stream. Per declared state one tensor [state slot, *shape]. The pools start zeroed: a kernel
+stream. Keys and values may be kept in 8 bits instead: the same tensors hold codes, and planes "k_scale" and "v_scale"
+[layer cache, page, head, blocks of 16 places] the float32 scales (ops.Cache8). Per declared state one tensor [state slot, *shape]. The pools start zeroed: a kernel
 that loads a whole page and masks the tail must never meet a NaN pattern there.
 
 The reference allocates `[layer][slot][kv head][max_seq][head_dim]` once (src/api.cu:1409-1411).
@@ -15,6 +16,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..kernels import ops
 from .manager import CacheGroupSpec
 
 
@@ -23,6 +25,7 @@ class LayerCache:
     planes: Dict[str, torch.Tensor]      # plane name -> [page, head, page_size, width]
     group: int
     write: bool
+    cache8: object = None                # the planes as an ops.Cache8, where they are in 8 bits
 
     @property
     def k(self) -> torch.Tensor:
@@ -33,12 +36,22 @@ class LayerCache:
         return self.planes["v"]
 
 
+def _planes8(group: CacheGroupSpec, pages: int, page_size: int, dtype, device) -> Dict[str, torch.Tensor]:
+    if [name for name, _, _ in group.planes] != ["k", "v"] or group.planes[0][1:] != group.planes[1][1:]:
+        raise ValueError(f"cache group {group.name!r}: planes {group.planes} cannot be kept in 8 bits (keys and values of one shape can)")
+    (_, heads, width), n = group.planes[0], group.n_layers
+    codes = {name: torch.zeros(n, pages, heads, page_size, width, dtype=torch.uint8, device=device).view(dtype) for name in "kv"}
+    return {**codes, **{f"{name}_scale": torch.zeros(n, pages, heads, ops.cache8_blocks(page_size), dtype=torch.float32, device=device) for name in "kv"}}
+
+
 class CacheStorage:
     def __init__(self, groups: Sequence[CacheGroupSpec], num_pages: Sequence[int], page_size: int, dtype, device,
-                 state_specs: Dict[Tuple[int, str], Tuple[Tuple[int, ...], torch.dtype]], num_state_slots: int):
-        self.groups, self.page_size, self.dtype = list(groups), page_size, dtype
+                 state_specs: Dict[Tuple[int, str], Tuple[Tuple[int, ...], torch.dtype]], num_state_slots: int,
+                 cache_dtype: Optional[torch.dtype] = None):
+        self.groups, self.page_size, self.dtype, self.cache_dtype = list(groups), page_size, dtype, cache_dtype
         self.kv = [{name: torch.zeros(g.n_layers, n, heads, page_size, width, dtype=dtype, device=device)
-                    for name, heads, width in g.planes} for g, n in zip(self.groups, num_pages)]
+                    for name, heads, width in g.planes} for g, n in zip(self.groups, num_pages)] if cache_dtype is None else \
+                  [_planes8(g, n, page_size, cache_dtype, device) for g, n in zip(self.groups, num_pages)]
         self.state: Dict[Tuple[int, str], torch.Tensor] = {
             key: torch.zeros((num_state_slots,) + tuple(shape), dtype=dt, device=device)
             for key, (shape, dt) in state_specs.items()}
@@ -52,8 +65,9 @@ class CacheStorage:
             return None
         key = (plan.group, plan.slot, plan.write)
         if key not in self._layer_caches:
-            self._layer_caches[key] = LayerCache({name: t[plan.slot] for name, t in self.kv[plan.group].items()},
-                                                 plan.group, plan.write)
+            planes = {name: t[plan.slot] for name, t in self.kv[plan.group].items()}
+            self._layer_caches[key] = LayerCache(planes, plan.group, plan.write,
+                                                 None if self.cache_dtype is None else ops.Cache8(*(planes[n] for n in ("k", "v", "k_scale", "v_scale"))))
         return self._layer_caches[key]
 
     def layer_state(self, step: int) -> Dict[str, torch.Tensor]:
@@ -64,7 +78,13 @@ class CacheStorage:
         for t in self.state.values():
             t[slot].zero_()
 
+    def copy_pages(self, group: int, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Pages of a group copied to others, in all its layers and planes."""
+        ops.copy_pages(list(self.kv[group].values()), src, dst)
+
     def bytes_per_token(self) -> int:
+        if self.cache_dtype is not None:
+            return -(-sum(t[:, 0].numel() * t.element_size() for g in self.kv for t in g.values()) // self.page_size)
         return sum(g.elements_per_token() for g in self.groups) * torch.empty((), dtype=self.dtype).element_size()
 
     def nbytes(self) -> int:

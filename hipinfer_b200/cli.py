@@ -4,7 +4,7 @@ are kept, with --model for a folder of config.json and model.safetensors.
 
     python -m hipinfer_b200 generate --model DIR --tokens 1 2 3 --new 8 [--mode bf16|fp32]
                                      [--temperature T --seed S] [--max-batch --max-seq --max-prefill]
-                                     [--samples N --drafts K]
+                                     [--samples N --drafts K] [--cache-dtype int8|float8_e4m3fn]
     python -m hipinfer_b200 random-model --config config.json --out DIR --seed 0 [--std 0.02] [--dtype bfloat16]
     python -m hipinfer_b200 replay --model DIR --dtype bfloat16 --out DIR --max-tokens N   (steps on stdin)
     python -m hipinfer_b200 bench [bench.py's options]        (the measurement program beside the package)
@@ -31,6 +31,7 @@ def main(argv=None) -> int:
     g.add_argument("--max-batch", type=int, default=8)
     g.add_argument("--max-seq", type=int, default=2048)
     g.add_argument("--max-prefill", type=int, default=1024)
+    g.add_argument("--cache-dtype", default=None, choices=["int8", "float8_e4m3fn", "fp8"], help="keep keys and values in 8 bits")
     r = sub.add_parser("random-model", help="write a model folder with seeded random weights")
     r.add_argument("--config", required=True, help="a config.json of a registered architecture")
     r.add_argument("--out", required=True)
@@ -64,7 +65,7 @@ def main(argv=None) -> int:
     if a.cmd == "generate":
         from .engine.api import Engine
 
-        eng = Engine(a.model, max_batch=a.max_batch, max_seq=a.max_seq, max_prefill=a.max_prefill, dtype=a.mode)
+        eng = Engine(a.model, max_batch=a.max_batch, max_seq=a.max_seq, max_prefill=a.max_prefill, dtype=a.mode, cache_dtype=a.cache_dtype)
         print({k: getattr(eng, k) for k in ("vocab", "hidden", "inter", "layers", "heads", "kv_heads", "head_dim",
                                             "max_pos", "tied")})
         if a.samples or a.drafts:

@@ -11,6 +11,9 @@ for bad arguments (scripts/hipinfer.py:386-390). What is new beside them: `dtype
 ("bfloat16" or "float32"), temperature sampling, requests through the scheduler
 (`add_request`, `step`, `run`), many samples of one prompt (`sample_many`), random weights, and `runner` for the step function itself.
 
+`cache_dtype` ("int8" or "float8_e4m3fn"; None: `dtype`) keeps keys and values in 8 bits with a scale for each 16 tokens and head: half
+the bytes (or a quarter) for models whose layers attend to plain keys and values (the Llama decoder; others are refused).
+
 `max_batch` is the most requests live at a time, `max_seq` the longest sequence, `max_prefill`
 the token budget of a step (the reference's prefill chunk, src/api.cu:1788).
 """
@@ -34,9 +37,9 @@ class Engine:
     def __init__(self, path: Optional[str] = None, max_batch: int = 8, max_seq: int = 2048, max_prefill: int = 1024,
                  dtype: str = "bfloat16", device: str = "cuda:0", config: Union[ModelConfig, dict, None] = None,
                  random_weights: Optional[int] = None, std: float = 0.02, page_size: int = 16,
-                 num_pages: Optional[int] = None, pipeline: bool = True):
+                 num_pages: Optional[int] = None, pipeline: bool = True, cache_dtype: Optional[str] = None):
         kw = dict(dtype=dtype, device=device, page_size=page_size, num_pages=num_pages, max_model_len=max_seq,
-                  max_num_seqs=max_batch)
+                  max_num_seqs=max_batch, cache_dtype=cache_dtype)
         if path is not None:
             self.runner = ModelRunner.from_folder(path, **kw)
         elif config is not None and random_weights is not None:

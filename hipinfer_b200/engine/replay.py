@@ -37,6 +37,7 @@ def main(argv=None) -> int:
                     help="most tokens live requests hold at any time (each rounded up to 64); sizes the cache pool")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--max-requests", type=int, default=4, help="most requests live at a time")
+    ap.add_argument("--cache-dtype", default=None, choices=["int8", "float8_e4m3fn", "fp8"], help="keep keys and values in 8 bits")
     ap.add_argument("--planes", action="store_true",
                     help="also write <step>.planes.safetensors: every layer's named planes of the step's rows "
                          "(parts/planes.py), named <order index>.<plane>; such steps run eagerly")
@@ -54,7 +55,7 @@ def main(argv=None) -> int:
     num_pages = -(-a.max_tokens // 64) * (64 // a.page_size)
     # no request holds more than the pool: tables of positions and block tables are made for that length at most
     runner = ModelRunner.from_folder(a.model, dtype=a.dtype, page_size=a.page_size, num_pages=num_pages,
-                                     max_num_seqs=a.max_requests, max_model_len=num_pages * a.page_size)
+                                     max_num_seqs=a.max_requests, max_model_len=num_pages * a.page_size, cache_dtype=a.cache_dtype)
     for line in sys.stdin:
         line = line.strip()
         if not line:

@@ -24,6 +24,9 @@ from .batch import StepBatch, StepEntry, build_step_batch, shared_prefixes
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
 
 
+CACHE_DTYPES = {"int8": torch.int8, "float8_e4m3fn": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
+
+
 class StepError(ValueError):
     """A step that cannot run: a token outside the vocabulary, a request beyond the longest
     sequence, a `want` outside the entry (the reference returns -1 for such arguments,
@@ -33,7 +36,7 @@ class StepError(ValueError):
 class ModelRunner:
     def __init__(self, config: ModelConfig, tensors: Dict[str, torch.Tensor], dtype="bfloat16", device="cuda:0",
                  page_size: int = 16, num_pages: Optional[int] = None, max_model_len: Optional[int] = None,
-                 max_num_seqs: int = 8, cuda_graphs: bool = True):
+                 max_num_seqs: int = 8, cuda_graphs: bool = True, cache_dtype=None):
         if not torch.cuda.is_available():
             raise RuntimeError("hipinfer_b200 runs on a CUDA device (sm_100a); none is visible and there is no "
                                "CPU implementation")
@@ -44,15 +47,18 @@ class ModelRunner:
         self.spec = get_architecture(config.architecture).build_spec(config)
         self.max_model_len = int(min(max_model_len or self.spec.max_position, self.spec.max_position))
         self.page_size = int(page_size)
-        self.ctx = BuildContext(self.dtype, self.device, self.page_size, self.max_model_len)
+        self.cache_dtype = cache8_dtype(cache_dtype)
+        self.ctx = BuildContext(self.dtype, self.device, self.page_size, self.max_model_len, self.cache_dtype)
         self.model = DecoderModel(self.spec, self.ctx)
+        if self.cache_dtype is not None:
+            check_cache8(self.model)
         self.model.load(tensors)
         pages_per_seq = -(-self.max_model_len // self.page_size)
         n_pages = int(num_pages) if num_pages is not None else pages_per_seq * max_num_seqs
         groups = self.model.cache_groups
         self.cache = CacheManager(groups, self.page_size, [n_pages] * len(groups), max_num_seqs)
         self.storage = CacheStorage(groups, [n_pages] * len(groups), self.page_size, self.dtype, self.device,
-                                    self.model.state_specs, max_num_seqs)
+                                    self.model.state_specs, max_num_seqs, self.cache_dtype)
         self.vocab_size = self.spec.vocab_size
         self.steps_run = 0
         # decode-only steps (one token per request, every row wanted) are replayed from a CUDA
@@ -278,13 +284,18 @@ class ModelRunner:
         self._np_tables.pop(request_id, None)
         self._forked.discard(request_id)
 
-    def fork(self, request_id, new_id) -> int:
+    def fork(self, request_id, new_id, length: Optional[int] = None) -> int:
         """Request `new_id` begins with the whole pages of `request_id`, which both hold from then on (neither writes them);
-        returns how many tokens those are. Requests that stand side by side in a step and hold the same pages attend to them
-        together (ops.attention_shared). Raises StepError for a model that keeps state besides the pages."""
+        returns how many tokens those are. With `length` it begins with exactly so many tokens: a page that they end inside of is
+        copied (ops.copy_pages). Requests that stand side by side in a step and hold the same pages attend to them
+        together (ops.attention_shared). Raises StepError for a model that keeps state besides the pages, OutOfPages (nothing
+        changed) where the cache has no page for the copy."""
         if self.model.state_specs:
             raise StepError("a request of a model with per-request state cannot be forked: its state is not in the pages")
-        rc = self.cache.fork(request_id, new_id)
+        rc = self.cache.fork(request_id, new_id, length)
+        for g, pages in enumerate(rc.copied):
+            if pages is not None:
+                self.storage.copy_pages(g, [pages[0]], [pages[1]])
         self._np_tables.pop(new_id, None)
         self._forked.add(new_id)
         return rc.length
@@ -299,6 +310,24 @@ class ModelRunner:
 
     def live_requests(self):
         return list(self.cache.requests)
+
+
+def cache8_dtype(name) -> Optional[torch.dtype]:
+    """The codes of a cache in 8 bits by name ("int8", "float8_e4m3fn" or "fp8") or type; None: a cache of the compute type."""
+    if name is None:
+        return None
+    dtype = CACHE_DTYPES.get(name) if isinstance(name, str) else name
+    if dtype not in CACHE_DTYPES.values():
+        raise ValueError(f"cache type {name!r}: one of {sorted(CACHE_DTYPES)} is possible, or None")
+    return dtype
+
+
+def check_cache8(model: DecoderModel) -> None:
+    """Raises ValueError for a model with a layer whose mixer keeps what 8 bits do not hold."""
+    for i, (st, plan) in enumerate(zip(model.spec.order, model.cache_plan)):
+        mixer = model.layers[st.layer].mixer
+        if plan is not None and not mixer.takes_cache8:
+            raise ValueError(f"a cache in 8 bits is not possible: the mixer of step {i} ({type(mixer).__name__}) keeps its cache in the compute type")
 
 
 def _ignorable(spec) -> List[str]:

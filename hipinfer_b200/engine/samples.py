@@ -89,9 +89,12 @@ class Sampling:
 
     def _run_prompt(self) -> torch.Tensor:
         """The prompt as sample 0's, in portions; the others are forked from it where its last whole page ends (later, a window's
-        pages that they read may be gone) and run the rest with their first step. Returns the logits behind the prompt."""
+        pages that they read may be gone) and run the rest with their first step, or at its end, with a copy of its last page. Returns the logits behind the prompt."""
         P, at, forks = len(self.prompt), 0, self.rids[1:] if self.n_new > 1 else []
-        whole = P // self.runner.page_size * self.runner.page_size
+        # a cache in 8 bits: the forks begin behind the prompt, the page that it ends inside of copied. Run again beside other tokens, the
+        # rest would be rounded to another block's scale than the prompt's own.
+        copied = getattr(self.runner, "cache_dtype", None) is not None
+        whole = P if copied else P // self.runner.page_size * self.runner.page_size
         for end in sorted({whole if forks else P, P} - {0}):
             while at < end:
                 part = self.prompt[at:min(end, at + self.max_prefill)]
@@ -99,7 +102,7 @@ class Sampling:
                 logits = self.runner.step([StepEntry(self.rids[0], part, [len(part) - 1] if at == P else [])])
             if end == whole:
                 for rid in forks:
-                    self.runner.fork(self.rids[0], rid)
+                    self.runner.fork(self.rids[0], rid, *([P] if copied else []))
         return logits
 
     def _behind(self, i) -> int:

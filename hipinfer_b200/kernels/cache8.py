@@ -109,6 +109,17 @@ def _ints(what: str, name: str, x: torch.Tensor, n: Optional[int] = None) -> Non
         raise ops.KernelError(f"{what}: {name} {tuple(x.shape)} {x.dtype}, strides {x.stride()}; int32 [{'n' if n is None else n}] side by side is expected")
 
 
+_rows = {}
+
+
+def row_places(device, n: int) -> torch.Tensor:
+    """0 .. n - 1 (int32): the places of a step's rows in pages of one place. Older, shorter tensors are kept: a captured graph may hold their addresses."""
+    held = _rows.setdefault(device, [])
+    if not held or held[-1].numel() < n:
+        held.append(torch.arange(max(n, 4096, 2 * held[-1].numel() if held else 0), dtype=torch.int32, device=device))
+    return held[-1][:n]
+
+
 def store_cache8(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, cache: Cache8) -> Cache8:
     """Rows k, v [T, n_kv_heads * head_dim] (float32 or bfloat16; rows may be part of wider ones) stored at the places slot_map (int32 [T], page *
     page_size + place; a number outside of the cache stores nothing).

@@ -1752,4 +1752,4 @@ def output_norm(x: torch.Tensor, y, weight: torch.Tensor, bias: Optional[torch.T
 # Attention over shared prefixes and the verification of drafted tokens (kernels/drafts.py)
 from .drafts import MAX_DRAFTS, SharedPlan, attention_shared, verify_drafts  # noqa: E402,F401
 # A paged cache in 8 bits, and copying pages (kernels/cache8.py)
-from .cache8 import BLOCK8, Cache8, attention_cache8, cache8_blocks, copy_pages, expand_cache8, new_cache8, store_cache8  # noqa: E402,F401
+from .cache8 import BLOCK8, Cache8, attention_cache8, cache8_blocks, copy_pages, expand_cache8, new_cache8, row_places, store_cache8  # noqa: E402,F401

@@ -31,10 +31,11 @@ import torch
 
 @dataclass(frozen=True)
 class BuildContext:
-    dtype: torch.dtype            # compute element type of activations and the cache
+    dtype: torch.dtype            # compute element type of activations and, unless it is in 8 bits, the cache
     device: Any
     page_size: int = 16
     max_model_len: int = 2048
+    cache_dtype: Optional[torch.dtype] = None     # the codes of a cache in 8 bits (ops.Cache8); None: the cache is of `dtype`
 
     @staticmethod
     def meta() -> "BuildContext":
@@ -87,6 +88,8 @@ class Part:
 class Mixer(Part):
     # Its attention reads the pages that neighbours in a step hold together once for all of them (StepBatch.shared).
     reads_shared_pages = False
+    # It keeps keys "k" and values "v" and does so in 8 bits where the context has a cache_dtype (LayerCache.cache8).
+    takes_cache8 = False
 
     def cache_need(self) -> Optional[CacheNeed]:
         return None
