@@ -11,16 +11,27 @@ constexpr float C8_LEAST = 1e-30f;              // below it a block's largest nu
 
 __host__ __device__ constexpr int c8_blocks(int page_size) { return (page_size + C8_BLOCK - 1) / C8_BLOCK; }
 
-// A code type: its largest number, code to number, and number (already within +- the largest) to the nearest code, ties to the even one.
+// A code type: its largest number, code to number, and number (already within +- the largest) to the nearest code, ties to the even one; four of them
+// to four bytes.
 struct C8Int8 {
   static constexpr float MOST = 127.f;
   static __device__ __forceinline__ float value(uint8_t c) { return (float)(int8_t)c; }
-  static __device__ __forceinline__ uint8_t code(float x) { return (uint8_t)(int8_t)__float2int_rn(x); }
+  // (1.5 x 2^23 + x has x's nearest integer in its last bits, ties to even; conversions to integers run at an eighth of an addition's rate)
+  static __device__ __forceinline__ uint32_t code4(const float* x) {
+    const uint32_t a = __float_as_uint(__fadd_rn(x[0], 12582912.f)), b = __float_as_uint(__fadd_rn(x[1], 12582912.f));
+    const uint32_t c = __float_as_uint(__fadd_rn(x[2], 12582912.f)), d = __float_as_uint(__fadd_rn(x[3], 12582912.f));
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  }
+  static __device__ __forceinline__ uint8_t code(float x) { return (uint8_t)__float_as_uint(__fadd_rn(x, 12582912.f)); }
 };
 struct C8E4m3 {
   static constexpr float MOST = 448.f;
   static __device__ __forceinline__ float value(uint8_t c) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+  }
+  static __device__ __forceinline__ uint32_t code4(const float* x) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3) << 16;
   }
   static __device__ __forceinline__ uint8_t code(float x) { return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 };

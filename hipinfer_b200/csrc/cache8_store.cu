@@ -1,6 +1,8 @@
 // Storing rows into a cache in 8 bits, and reading pages of it back as numbers.
 #include "cache8.cuh"
 
+#include <type_traits>
+
 // Rows of K and V [T][Hkv * D] go to the places slot[t] = page * page_size + place, in any order; of several rows for one place the last
 // counts. A block (16 places of a page) is taken over by the first row of the call that goes to it: the CTAs of that row look through all
 // slots for the others (a block's places are consecutive slots), and each of their warps has one kv head of K or V: it takes the largest |x| of
@@ -8,27 +10,28 @@
 // it was, and where it grew the block's codes are rounded once more, to r(code * (old / new)); then the rows' codes, r(x * (1 / scale)),
 // overwrite theirs. Numbers that are not finite have no part in a; infinities become the largest code, NaN 0. All arithmetic is 32-bit,
 // each operation rounded by itself (no contraction), so that a block's bits are a matter of its rows and what it held alone.
-constexpr int C8S_WARPS = 8, C8S_ROWS = 16;
+constexpr int C8S_WARPS = 8, C8S_ROWS = 16, C8S_LOOK = 8;
 
-// E numbers side by side, as floats, and as codes to memory.
-template <int E> __device__ __forceinline__ void c8_load(const float* p, float* x) {
-  if constexpr (E == 4) *(float4*)x = *(const float4*)p;
-  else x[0] = *p;
-}
-template <int E> __device__ __forceinline__ void c8_load(const __nv_bfloat16* p, float* x) {
-  if constexpr (E == 8) {
-    const uint4 r = *(const uint4*)p;
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// E numbers side by side as they are in memory (16 bytes of them, or one), as floats, and as codes to memory.
+template <typename T, int E> struct C8Piece {
+  using Raw = std::conditional_t<E == 1, T, uint4>;
+  static __device__ __forceinline__ void floats(const Raw& r, float* x) {
+    if constexpr (E == 1) {
+      x[0] = hb_to_float(r);
+    } else {
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-  } else {
-    x[0] = __bfloat162float(*p);
+      for (int i = 0; i < 4; i++) {
+        if constexpr (E == 4) x[i] = __uint_as_float(w[i]);
+        else x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
   }
-}
-template <int E> __device__ __forceinline__ void c8_store(uint8_t* p, const uint8_t* c) {
-  if constexpr (E == 8) *(uint2*)p = *(const uint2*)c;
-  else if constexpr (E == 4) *(uint32_t*)p = *(const uint32_t*)c;
-  else *p = *c;
+};
+template <typename CT, int E> __device__ __forceinline__ void c8_store(uint8_t* p, const float* x) {
+  if constexpr (E == 8) *(uint2*)p = make_uint2(CT::code4(x), CT::code4(x + 4));
+  else if constexpr (E == 4) *(uint32_t*)p = CT::code4(x);
+  else *p = CT::code(*x);
 }
 
 // E numbers are loaded at a time; ITEMS > 0: a lane's numbers of a block (16 rows of D are 32 lanes x ITEMS x E) stay in registers between
@@ -44,22 +47,33 @@ __global__ void __launch_bounds__(32 * C8S_WARPS) cache8_store_kernel(const T* k
   const bool mine = h < Hkv, is_v = pair & 1;
   const T* x = (is_v ? v : k) + (long)h * D;
   const long ld = is_v ? ld_v : ld_k;
+  // rows that are stored and go to another block than the row before, of the CTA's `rows_cta` (at most 31): a lane has a row
   const int t0 = blockIdx.x * rows_cta;
-  for (int t = t0; t < min(t0 + rows_cta, n_rows); t++) {
-    const int s = slot[t];
-    if (s < 0 || s >= n_slots) continue;
-    const int page = s / page_size, first = s % page_size / C8_BLOCK * C8_BLOCK, places = min(C8_BLOCK, page_size - first);
-    const int lo = page * page_size + first;                     // the block's places are slots lo .. lo + places - 1
-    if (t > 0 && (unsigned)(slot[t - 1] - lo) < (unsigned)places) continue;
+  int lo_mine = -1;                                              // a block's places are slots lo .. lo + places - 1
+  {
+    const int row = t0 - 1 + lane, s = row >= 0 && lane <= rows_cta && row < n_rows ? slot[row] : -1;
+    if (s >= 0 && s < n_slots) lo_mine = s - s % page_size % C8_BLOCK;
+  }
+  const int lo_before = __shfl_up_sync(0xffffffffu, lo_mine, 1);
+  for (uint32_t heads = __ballot_sync(0xffffffffu, lane > 0 && lo_mine >= 0 && lo_mine != lo_before); heads; heads &= heads - 1) {
+    const int at_lane = __ffs(heads) - 1, t = t0 - 1 + at_lane, lo = __shfl_sync(0xffffffffu, lo_mine, at_lane);
+    const int page = lo / page_size, first = lo % page_size, places = min(C8_BLOCK, page_size - first);
     __syncthreads();
     if (tid < C8_BLOCK) win[tid] = -1;
     if (tid == C8_BLOCK) earlier = 0;
     __syncthreads();
-    for (int i = tid; i < n_rows; i += 32 * C8S_WARPS) {
-      const unsigned place = (unsigned)(slot[i] - lo);
-      if (place < (unsigned)places) {
-        if (i < t) earlier = 1;
-        atomicMax(&win[place], i);
+    for (int i0 = tid; i0 < n_rows; i0 += C8S_LOOK * 32 * C8S_WARPS) {      // (asked for eight at a time: one by one, 6,000 rows took 44 us)
+      int s_of[C8S_LOOK];
+#pragma unroll
+      for (int j = 0; j < C8S_LOOK; j++) s_of[j] = i0 + j * 32 * C8S_WARPS < n_rows ? slot[i0 + j * 32 * C8S_WARPS] : -1;
+#pragma unroll
+      for (int j = 0; j < C8S_LOOK; j++) {
+        const unsigned place = (unsigned)(s_of[j] - lo);
+        if (place < (unsigned)places) {
+          const int i = i0 + j * 32 * C8S_WARPS;
+          if (i < t) earlier = 1;
+          atomicMax(&win[place], i);
+        }
       }
     }
     __syncthreads();
@@ -70,53 +84,54 @@ __global__ void __launch_bounds__(32 * C8S_WARPS) cache8_store_kernel(const T* k
     const bool fresh = win[0] >= 0;
     const float old = fresh ? 0.f : *scale;
     const int pieces = D / E, items = places * pieces;           // piece i: place i / pieces, numbers i % pieces * E ..
-    float kept[ITEMS ? ITEMS : 1][E], most = 0.f;
-    const auto largest = [&](const float* y) {
+    using Piece = C8Piece<T, E>;
+    using Raw = typename Piece::Raw;
+    Raw kept[ITEMS ? ITEMS : 1];
+    float most = 0.f;
+    const auto largest = [&](const Raw& r) {
+      float y[E];
+      Piece::floats(r, y);
 #pragma unroll
       for (int e = 0; e < E; e++)
         if (fabsf(y[e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(y[e]));
     };
+    const auto load = [&](int i) { return *(const Raw*)(x + win[i / pieces] * ld + i % pieces * E); };
     if constexpr (ITEMS > 0) {
 #pragma unroll
       for (int j = 0; j < ITEMS; j++) {
-        const int i = j * 32 + lane, row = win[i / pieces];
-        if (row >= 0) c8_load<E>(x + row * ld + i % pieces * E, kept[j]);
-        else
-#pragma unroll
-          for (int e = 0; e < E; e++) kept[j][e] = 0.f;
+        kept[j] = Raw{};
+        if (win[(j * 32 + lane) / pieces] >= 0) kept[j] = load(j * 32 + lane);
       }
 #pragma unroll
       for (int j = 0; j < ITEMS; j++) largest(kept[j]);
     } else {
       for (int i = lane; i < items; i += 32)
-        if (win[i / pieces] >= 0) {
-          c8_load<E>(x + win[i / pieces] * ld + i % pieces * E, kept[0]);
-          largest(kept[0]);
-        }
+        if (win[i / pieces] >= 0) largest(load(i));
     }
     float now = __fdiv_rn(fmaxf(hb_warp_max(most), C8_LEAST), CT::MOST);
     if (!fresh && now > old) {
       const float f = __fdiv_rn(old, now);
       for (int i = lane; i < items; i += 32)
         if (win[i / pieces] < 0) {
-          uint8_t c[E];
+          float z[E];
 #pragma unroll
-          for (int e = 0; e < E; e++) c[e] = CT::code(__fmul_rn(CT::value(at[(long)i * E + e]), f));
-          c8_store<E>(at + (long)i * E, c);
+          for (int e = 0; e < E; e++) z[e] = __fmul_rn(CT::value(at[(long)i * E + e]), f);
+          c8_store<CT, E>(at + (long)i * E, z);
         }
     } else if (!fresh) {
       now = old;
     }
     if (lane == 0) *scale = now;
     const float inv = __fdiv_rn(1.f, now);
-    const auto put = [&](int i, const float* y) {
-      __align__(8) uint8_t c[E];
+    const auto put = [&](int i, const Raw& r) {
+      float y[E], z[E];
+      Piece::floats(r, y);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const float z = __fmul_rn(y[e], inv);
-        c[e] = CT::code(z != z ? 0.f : fminf(fmaxf(z, -CT::MOST), CT::MOST));
+        z[e] = __fmul_rn(y[e], inv);
+        z[e] = z[e] != z[e] ? 0.f : fminf(fmaxf(z[e], -CT::MOST), CT::MOST);
       }
-      c8_store<E>(at + (long)i * E, c);
+      c8_store<CT, E>(at + (long)i * E, z);
     };
     if constexpr (ITEMS > 0) {
 #pragma unroll
@@ -124,10 +139,7 @@ __global__ void __launch_bounds__(32 * C8S_WARPS) cache8_store_kernel(const T* k
         if (win[(j * 32 + lane) / pieces] >= 0) put(j * 32 + lane, kept[j]);
     } else {
       for (int i = lane; i < items; i += 32)
-        if (win[i / pieces] >= 0) {
-          c8_load<E>(x + win[i / pieces] * ld + i % pieces * E, kept[0]);
-          put(i, kept[0]);
-        }
+        if (win[i / pieces] >= 0) put(i, load(i));
     }
   }
 }
