@@ -18,10 +18,11 @@
 // Codes are integers (or e4m3 numbers) of at most 8 significant bits, exact in f16. The query of a pair is scaled by a power of two to below 2^10 and
 // split into f16 parts: one holds all of a bf16 query, two hold 22 bits of a 32-bit one. A bf16 query meets int8 keys as they are: it is rounded to
 // 16 bits of its pair's largest number, two int8 parts (2^-16 of that number is less than what bf16 keeps of it), whose products with the codes are
-// exact in integers; the keys' conversion was a sixth of all instructions. Weights are taken at 2^7 of a running bound of the scores that
-// is raised only when a score passes it by 8 (in base 2), so that they stay below 2^15 in f16 (two parts where the rows are 32-bit), and
-// raising it, which costs a pass over the accumulators, is rare. Scales, sums and accumulators are 32-bit: V's scale multiplies a unit's product on its way
-// into the accumulator, so blocks of very unlike scales lose nothing.
+// exact in integers; the keys' conversion was a sixth of all instructions. A weight is 2^(10 + score - bound), where the bound lies 8 (in base 2) above
+// a score that was the largest once and is raised only when one passes it, so that raising it, which costs a pass over the accumulators, is
+// rare. It goes into the product with V times its unit's scale over a reference, that of an earlier unit, which is exchanged (another pass) only
+// where the two are more than 2^5 apart: below 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing.
+// Scales, sums and accumulators are 32-bit.
 #include "cache8.cuh"
 #include "tc_common.cuh"
 
@@ -91,20 +92,27 @@ template <int PARTS> __device__ __forceinline__ void c8_split(float x, float y, 
   }
 }
 
-// Two int8 products of 32 dimensions.
+// Products of 32 int8 dimensions.
 __device__ __forceinline__ void c8_imma(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void c8_imma_zero(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
 
-// A unit in shared memory: keys' codes [16][D], then values'. Piece c (16 bytes) of key row r lies at:
+// A unit in shared memory: keys' codes [16][D], then values'. Piece c (16 bytes) of row r lies at: (K is read by ldmatrix, eight rows of a piece
+// together; V by pieces, or halves of them, of rows 2 tq.)
 template <int D> __device__ __forceinline__ uint32_t c8_at_k(int r, int c) {
-  return D == 128 ? r * 128 + ((c ^ ((r & 1) << 2)) << 4) : r * 64 + (c << 4);
+  return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : (r >> 1) * 128 + (((r & 1) * 4 + (c ^ (r >> 1 & 3))) << 4);
 }
 template <int D> __device__ __forceinline__ uint32_t c8_at_v(int r, int c) {
-  if constexpr (D == 128) return r * 128 + ((c ^ (r & 6)) << 4);
+  if constexpr (D == 128) return c8_at_k<D>(r, c);
   const int p = (r >> 1) + (r & 1) * 8;                               // the rows that a product reads together stand side by side
   return p * 64 + ((c ^ (p & 2)) << 4);
 }
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   const auto fetch = [&](int i, int base, int slot) {                   // stage i, of the BATCH from `base` on or the next
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int l = i % BATCH * U + u, x = __shfl_sync(0xffffffffu, now.at, l), y = __shfl_sync(0xffffffffu, next.at, l), at = i - base < BATCH ? x : y;
+      const int at = __shfl_sync(0xffffffffu, i - base < BATCH ? now.at : next.at, i % BATCH * U + u);
       if (i < count && at >= 0) c8_fetch<D>(ring + (slot * U + u) * Z::UNIT, a.kc, a.vc, at, lane);
     }
     hb_cp_async_commit();
@@ -214,7 +222,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       const T* q = (const T*)a.q + (t0 + pair / a.G) * a.ld_q + ((long)h * a.G + pair % a.G) * D;
 #pragma unroll
       for (int s = 0; s < STEPS; s++) {
-        const T* p = q + (s >> 2) * 64 + tq * 16 + (s & 3) * 4;
+        const T* p = q + s * 16 + tq * 4;
         if (a.q_aligned) {
           const float4 f = hb_load4(p);
           x[s][0] = f.x, x[s][1] = f.y, x[s][2] = f.z, x[s][3] = f.w;
@@ -294,57 +302,52 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       col_hi[nt][c] = i < n ? a.pos[t0 + (pair0 + i) / a.G] : -1;
     }
 
-  float o[STEPS][NT][4], m[NT][2], l[NT][2];
+  float o[STEPS][NT][4], bound[NT][2], sub[NT][2], l[NT][2];            // a weight is 2^(score - sub)
+  float v_ref = 0.f, v_inv = 0.f;                                       // V's reference scale, which o is to be multiplied with, and its inverse
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    m[nt][0] = m[nt][1] = -INFINITY;
+    bound[nt][0] = bound[nt][1] = -INFINITY;
+    sub[nt][0] = sub[nt][1] = 0.f;
     l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
   }
 
   // the scores of a unit, in 32 bits
+  const uint32_t k_lane = c8_at_k<D>((lane >> 3 & 1) * 8 + (lane & 7), lane >> 4);      // ldmatrix: rows 0-7 and 8-15 of a piece, then of the next
   const auto products = [&](uint32_t stage, float k_scale, float (&s)[NT][4]) {
     int si[2][NT][4];                                                   // two chains of products: of int8 parts, or of every second step
     float sf[2][NT][4];
+    const auto query = [&](int part, int nt, int step) {
+      if constexpr (Z::Q_REGS) return q_reg[part][step];
+      else return q_sh[((part * NT + nt) * Q_STEPS + step) * 32 + lane];
+    };
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) si[i][nt][c] = 0, sf[i][nt][c] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 64; j++) {
-      const uint4 x = c8_lds16(stage + c8_at_k<D>(g, j * 4 + tq)), y = c8_lds16(stage + c8_at_k<D>(g + 8, j * 4 + tq));
-      const uint32_t wx[4] = {x.x, x.y, x.z, x.w}, wy[4] = {y.x, y.y, y.z, y.w};
-      const auto query = [&](int part, int nt, int step) {
-        if constexpr (Z::Q_REGS) return q_reg[part][step];
-        else return q_sh[((part * NT + nt) * Q_STEPS + step) * 32 + lane];
-      };
+    for (int j = 0; j < D / 32; j++) {
+      uint32_t w[4];                                                    // four codes of keys g and g + 8, and those 16 dimensions on
+      hb_ldmatrix_x4(w, (stage + k_lane) ^ (j * 32));
       if constexpr (Z::Q_INT) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const uint32_t f[4] = {wx[2 * i], wy[2 * i], wx[2 * i + 1], wy[2 * i + 1]};
+        for (int p = 0; p < 2; p++)
 #pragma unroll
-          for (int p = 0; p < 2; p++)
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              const uint2 b = query(p, nt, j * 2 + i);
-              c8_imma(si[p][nt], f, b.x, b.y);
-            }
-        }
+          for (int nt = 0; nt < NT; nt++) {
+            const uint2 b = query(p, nt, j);
+            if (j == 0) c8_imma_zero(si[p][nt], w, b.x, b.y);
+            else c8_imma(si[p][nt], w, b.x, b.y);
+          }
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 2; i++) {
           uint32_t f[4];
-          c8_halves<CT>(wx[i], f[0], f[2]);
-          c8_halves<CT>(wy[i], f[1], f[3]);
+          c8_halves<CT>(w[2 * i], f[0], f[2]);
+          c8_halves<CT>(w[2 * i + 1], f[1], f[3]);
 #pragma unroll
           for (int p = 0; p < PARTS; p++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-              const uint2 b = query(p, nt, j * 4 + i);
-              c8_mma(sf[i & 1][nt], f, b.x, b.y);
+              const uint2 b = query(p, nt, j * 2 + i);
+              if (j == 0 && p == 0) c8_mma_zero(sf[i][nt], f, b.x, b.y);
+              else c8_mma(sf[i][nt], f, b.x, b.y);
             }
         }
       }
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) raise |= s[u][nt][c] > m[nt][c & 1] + 8.f;
+        for (int c = 0; c < 4; c++) raise |= s[u][nt][c] > bound[nt][c & 1];
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
@@ -397,34 +400,50 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          if (mx > m[nt][c] + 8.f) {
-            const float f = hb_exp2(m[nt][c] - mx);
-            m[nt][c] = mx;
+          if (mx > bound[nt][c]) {
+            const float f = hb_exp2(bound[nt][c] - (mx + 8.f));         // 0 while nothing has been summed
+            bound[nt][c] = mx + 8.f;
+            sub[nt][c] = mx - 2.f;                                      // (a weight is at most 2^10)
             l[nt][c] *= f;
 #pragma unroll
             for (int i = 0; i < STEPS; i++) o[i][nt][c] *= f, o[i][nt][c + 2] *= f;
           }
         }
     }
-    uint32_t b[U][W_PARTS][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const float b0 = (m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - 7.f, b1 = (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - 7.f;
+    for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const float w0 = hb_exp2(s[u][nt][0] - b0), w1 = hb_exp2(s[u][nt][1] - b1), w2 = hb_exp2(s[u][nt][2] - b0), w3 = hb_exp2(s[u][nt][3] - b1);
-        l[nt][0] += w0 + w2;
-        l[nt][1] += w1 + w3;
-        uint32_t x[W_PARTS], y[W_PARTS];
-        c8_split<W_PARTS>(w0, w1, x);
-        c8_split<W_PARTS>(w2, w3, y);
+      for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-        for (int p = 0; p < W_PARTS; p++) b[u][p][nt][0] = c8_transpose(x[p]), b[u][p][nt][1] = c8_transpose(y[p]);
+        for (int c = 0; c < 4; c++) s[u][nt][c] = hb_exp2(s[u][nt][c] - sub[nt][c & 1]);
+        l[nt][0] += s[u][nt][0] + s[u][nt][2];
+        l[nt][1] += s[u][nt][1] + s[u][nt][3];
       }
-    }
 #pragma unroll
     for (int u = 0; u < U; u++) {
       if (at[u] < 0) continue;
+      float ratio = v_scale[u] * v_inv;                                 // of V's scale to the reference
+      if (v_scale[u] > 1e-37f && !(ratio >= 1.f / 32 && ratio <= 32.f)) {
+        const float f = v_ref / v_scale[u];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int i = 0; i < STEPS; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[i][nt][c] *= f;
+        v_ref = v_scale[u];
+        v_inv = 1.f / v_ref;
+        ratio = 1.f;
+      }
+      uint32_t b[W_PARTS][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        uint32_t x[W_PARTS], y[W_PARTS];
+        c8_split<W_PARTS>(s[u][nt][0] * ratio, s[u][nt][1] * ratio, x);
+        c8_split<W_PARTS>(s[u][nt][2] * ratio, s[u][nt][3] * ratio, y);
+#pragma unroll
+        for (int p = 0; p < W_PARTS; p++) b[p][nt][0] = c8_transpose(x[p]), b[p][nt][1] = c8_transpose(y[p]);
+      }
       uint32_t v[4][D / 32];                                            // codes of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: dimensions g D / 8 ..
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -454,13 +473,9 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
           c8_halves<CT>(x, f[0], f[1]);
           c8_halves<CT>(y, f[2], f[3]);
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            float d[4];
-            c8_mma_zero(d, f, b[u][0][nt][0], b[u][0][nt][1]);
-            if constexpr (W_PARTS == 2) c8_mma(d, f, b[u][1][nt][0], b[u][1][nt][1]);
+          for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) o[2 * j + half][nt][c] = fmaf(v_scale[u], d[c], o[2 * j + half][nt][c]);
-          }
+            for (int p = 0; p < W_PARTS; p++) c8_mma(o[2 * j + half][nt], f, b[p][nt][0], b[p][nt][1]);
         }
       }
     }
@@ -500,7 +515,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
       if (g == 0) {
-        m_sh[warp][nt * 8 + 2 * tq + c] = m[nt][c];
+        m_sh[warp][nt * 8 + 2 * tq + c] = bound[nt][c];
         l_sh[warp][nt * 8 + 2 * tq + c] = x;
       }
     }
@@ -512,7 +527,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
     for (int i = 0; i < STEPS; i++)
 #pragma unroll
       for (int c = 0; c < 4; c++)
-        o_sh[(warp * PAIRS + nt * 8 + 2 * tq + (c & 1)) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c];
+        o_sh[(warp * PAIRS + nt * 8 + 2 * tq + (c & 1)) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c] * v_ref;
   __syncthreads();
   for (int pair = tid; pair < PAIRS; pair += 32 * C8M_WARPS) {
     float mx = -INFINITY, sum = 0.f;
