@@ -46,7 +46,7 @@ struct C8Attend {
   int first_tile, tiles_row, G, window;
   float scale_log2;
   void* out;
-  int q_aligned;
+  int q_aligned, out_aligned;
 };
 
 // D += A B, f16 operands; D = A B without an addend.
@@ -144,7 +144,8 @@ template <typename CT, typename T, int D, int NT> struct C8Sizes {
   static constexpr bool Q_REGS = NT == 1 && (Q_INT || PARTS == 1);
   static constexpr int QUERY = Q_REGS ? 0 : PARTS * NT * Q_STEPS * 32 * 8, UNIT = 2 * C8_BLOCK * D, RING = C8M_WARPS * STAGES * U * UNIT;
   static constexpr int PITCH = D + 4, JOINED = C8M_WARPS * 8 * NT * PITCH * 4;
-  static constexpr int SMEM = QUERY + RING > JOINED ? QUERY + RING : JOINED;
+  static constexpr int WORK = QUERY + RING > JOINED ? QUERY + RING : JOINED;
+  static constexpr int INBOX = 16 * (2 * NT * D + C8M_RANKS), SMEM = WORK + INBOX + INBOX / 2;     // (items of a tile, rounded up for every rank)
   static constexpr int BLOCKS = NT == 1 ? 4 : D == 64 ? (NT == 2 ? 4 : 3) : NT == 2 ? 3 : 2;      // an SM, by registers
 };
 
@@ -156,10 +157,14 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   uint2* q_sh = (uint2*)smem;                                           // [part][nt][step][lane]
   float* o_sh = (float*)smem;                                           // [warp][pair][PITCH], over the query when it is done with
   __shared__ float col_sh[Z::Q_REGS ? 1 : PAIRS];
-  __shared__ float m_sh[C8M_WARPS][PAIRS], l_sh[C8M_WARPS][PAIRS], m_cta[PAIRS], l_cta[PAIRS];
+  __shared__ float2 ml_sh[C8M_WARPS][PAIRS];                            // a warp's bounds and sums
+  float4* inbox = (float4*)(smem + Z::WORK);                            // [rank][share]: the parts that this block joins
+  float2* inbox_ml = (float2*)(smem + Z::WORK + Z::INBOX);              // and their bounds and sums
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3, h = blockIdx.y;
   const int ranks = gridDim.x, rank = blockIdx.x;
+  const auto cluster_wait = [] { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };
   hb_pdl_launch();
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   hb_pdl_wait();
   int r, t0, pair0, pairs;
   if (a.tiles) {
@@ -170,10 +175,20 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
     pair0 = (a.first_tile + blockIdx.z) % a.tiles_row * PAIRS, pairs = a.G;
     r = a.row_req ? a.row_req[t0] : t0;
   }
+  // single rows that see all of their keys: the first pages are asked for together with the positions, which say how many they are
+  constexpr int BATCH = 32 / U;
+  const int id = rank * C8M_WARPS + warp, stride = ranks * C8M_WARPS;
+  const bool early = !a.tiles && !a.row_req && a.window <= 0;
+  int early_page = -1;
+  if (early) {
+    const int i = ((id + lane / U * stride) * U + lane % U) / a.upp;
+    if (t0 < a.table_rows && i < a.table_width) early_page = a.bt[t0 * a.ld_table + i];
+  }
   const int n = min(PAIRS, pairs - pair0);                              // pairs of this tile
   const int row_first = t0 + pair0 / a.G, row_last = t0 + (pair0 + n - 1) / a.G;
   // the keys that any of its rows sees, and those that all of them see (positions of a request's rows ascend)
-  const int p_lo = a.pos[row_first], p_hi = a.pos[row_last], window = a.window > 0 ? a.window : 0x7fffffff;
+  const int window = a.window > 0 ? a.window : 0x7fffffff;
+  const int p_lo = a.pos[row_first], p_hi = a.pos[row_last];
   const int see_lo = max(0, p_lo < window ? 0 : p_lo - window + 1), all_lo = p_hi < window ? 0 : p_hi - window + 1;
   const int u_lo = see_lo / C8_BLOCK;
   const int u_hi = r >= 0 && r < a.table_rows ? (int)min((long)(p_hi < 0 ? -1 : p_hi / C8_BLOCK), (long)a.table_width * a.upp - 1) : -1;
@@ -181,15 +196,14 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
 
   const uint32_t ring = hb_smem_u32(smem) + Z::QUERY + warp * STAGES * U * Z::UNIT;
   // this warp's stages: U units each, the id-th and every (ranks * WARPS)th from there; a lane looks up one unit of 32, 32 units ahead
-  constexpr int BATCH = 32 / U;
-  const int id = rank * C8M_WARPS + warp, stride = ranks * C8M_WARPS, s_lo = u_lo / U, first = s_lo + id;
+  const int s_lo = u_lo / U, first = s_lo + id;
   const int count = u_hi < first * U ? 0 : (u_hi / U - first) / stride + 1;
   struct Units { int at; float k_scale, v_scale; };
   const auto look = [&](int i) {                                        // stages i .. i + BATCH - 1
     Units x = {-1, 0.f, 0.f};
     const int unit = (first + (i + lane / U) * stride) * U + lane % U;
     if (i + lane / U < count && unit >= u_lo && unit <= u_hi) {
-      const int page = table[unit / a.upp];
+      const int page = early && i == 0 ? early_page : table[unit / a.upp];
       if (page >= 0 && page < a.n_pages) {
         x.at = (page * a.Hkv + h) * a.upp + unit % a.upp;
         x.k_scale = a.ks[x.at];
@@ -510,84 +524,75 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   for (int nt = 0; nt < NT; nt++)
 #pragma unroll
     for (int c = 0; c < 2; c++) {
-      float x = l[nt][c];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) {
-        m_sh[warp][nt * 8 + 2 * tq + c] = bound[nt][c];
-        l_sh[warp][nt * 8 + 2 * tq + c] = x;
-      }
+      l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 4);
+      l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
+      l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
     }
-  __syncthreads();                                                      // (and the query is read no more)
-  // dimension d = g D / 8 + 2 i + e lies at 16 i + 8 e + g: the lanes of a store in different banks
+  __syncthreads();                                                      // rings and query are read no more
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-    for (int i = 0; i < STEPS; i++)
+    for (int c = 0; c < 4; c++) {
+      const int pair = nt * 8 + 2 * tq + (c & 1);
+      if (g == 0 && c < 2) ml_sh[warp][pair] = make_float2(bound[nt][c], l[nt][c]);
+      // dimension d = g D / 8 + 2 i + e lies at 16 i + 8 e + g: the lanes of a store in different banks
 #pragma unroll
-      for (int c = 0; c < 4; c++)
-        o_sh[(warp * PAIRS + nt * 8 + 2 * tq + (c & 1)) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c] * v_ref;
-  __syncthreads();
-  for (int pair = tid; pair < PAIRS; pair += 32 * C8M_WARPS) {
-    float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < C8M_WARPS; w++) mx = fmaxf(mx, m_sh[w][pair]);
-#pragma unroll
-    for (int w = 0; w < C8M_WARPS; w++) {
-      const float f = m_sh[w][pair] == mx && mx == -INFINITY ? 1.f : hb_exp2(m_sh[w][pair] - mx);
-      m_sh[w][pair] = f;                                                // from here on: what the warp's result is multiplied with
-      sum += l_sh[w][pair] * f;
+      for (int i = 0; i < STEPS; i++) o_sh[(warp * PAIRS + pair) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c] * v_ref;
     }
-    m_cta[pair] = mx;
-    l_cta[pair] = sum;
-  }
   __syncthreads();
   const auto place = [](int d) { return d % (D / 8) / 2 * 16 + d % 2 * 8 + d / (D / 8); };
+  const auto factor = [](float m, float mx) { return mx == -INFINITY ? 1.f : hb_exp2(m - mx); };      // (NaN sums without a bound count)
   T* out = (T*)a.out;
-  const auto put = [&](int pair, int d, float x, float sum) {
+  const auto put = [&](int pair, int d, const float (&x)[4], float sum) {
     const int i = pair0 + pair;
-    out[((long)(t0 + i / a.G) * a.Hkv * a.G + (long)h * a.G + i % a.G) * D + d] = hb_from_float<T>(sum == 0.f ? 0.f : x / sum);
-  };
-  for (int i = tid; i < n * D; i += 32 * C8M_WARPS) {
-    const int pair = i / D, d = i % D;
-    float x = 0.f;
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    T* to = out + ((long)(t0 + i / a.G) * a.Hkv * a.G + (long)h * a.G + i % a.G) * D + d;
+    if (a.out_aligned) {
+      hb_store4(to, make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f));
+    } else {
 #pragma unroll
-    for (int w = 0; w < C8M_WARPS; w++) x = fmaf(o_sh[(w * PAIRS + pair) * PITCH + place(d)], m_sh[w][pair], x);
-    if (ranks == 1) put(pair, d, x, l_cta[pair]);
-    else o_sh[pair * PITCH + place(d)] = x;                             // (its warp 0's number was this thread's alone)
+      for (int e = 0; e < 4; e++) to[e] = hb_from_float<T>(x[e] * f);
+    }
+  };
+  // rank r of the cluster ends the items (pair, four dimensions) r * share .. ; the others' parts come into its inbox
+  const int items = n * (D / 4), share = (items + ranks - 1) / ranks;
+  if (ranks > 1) cluster_wait();                                        // the others have started
+  for (int i = tid; i < items; i += 32 * C8M_WARPS) {
+    const int pair = i / (D / 4), d = i % (D / 4) * 4;
+    float mx = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < C8M_WARPS; w++) mx = fmaxf(mx, ml_sh[w][pair].x);
+#pragma unroll
+    for (int w = 0; w < C8M_WARPS; w++) {
+      const float2 ml = ml_sh[w][pair];
+      const float f = factor(ml.x, mx);
+      sum = fmaf(ml.y, f, sum);
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = fmaf(o_sh[(w * PAIRS + pair) * PITCH + place(d + e)], f, x[e]);
+    }
+    if (ranks == 1) {
+      put(pair, d, x, sum);
+      continue;
+    }
+    const int to = i / share, at = rank * share + i % share;
+    uint32_t box = hb_mapa(inbox + at, to), ml = hb_mapa(inbox_ml + at, to);
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]) : "memory");
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(ml), "f"(mx), "f"(sum) : "memory");
   }
   if (ranks == 1) return;
-  hb_cluster_sync();
-  const uint32_t o_at = hb_smem_u32(o_sh), m_at = hb_smem_u32(m_cta), l_at = hb_smem_u32(l_cta);
-  for (int i = rank * 32 * C8M_WARPS + tid; i < n * D; i += ranks * 32 * C8M_WARPS) {
-    const int pair = i / D, d = i % D;
-    float xs[C8M_RANKS], ms[C8M_RANKS], ls[C8M_RANKS], mx = -INFINITY, x = 0.f, sum = 0.f;
-#pragma unroll
-    for (int c = 0; c < C8M_RANKS; c++)
-      if (c < ranks) {
-        const auto far = [&](uint32_t p) {
-          uint32_t q;
-          float f;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(q) : "r"(p), "r"(c));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(q) : "memory");
-          return f;
-        };
-        xs[c] = far(o_at + (pair * PITCH + place(d)) * 4), ms[c] = far(m_at + pair * 4), ls[c] = far(l_at + pair * 4);
-      }
-#pragma unroll
-    for (int c = 0; c < C8M_RANKS; c++)
-      if (c < ranks) mx = fmaxf(mx, ms[c]);
-#pragma unroll
-    for (int c = 0; c < C8M_RANKS; c++)
-      if (c < ranks) {
-        const float f = ms[c] == mx && mx == -INFINITY ? 1.f : hb_exp2(ms[c] - mx);
-        x = fmaf(xs[c], f, x);
-        sum = fmaf(ls[c], f, sum);
-      }
-    put(pair, d, x, sum);
+  hb_cluster_sync();                                                    // (nobody's memory is touched behind it)
+  for (int i = tid; i < share && rank * share + i < items; i += 32 * C8M_WARPS) {
+    float mx = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < ranks; c++) mx = fmaxf(mx, inbox_ml[c * share + i].x);
+    for (int c = 0; c < ranks; c++) {
+      const float2 ml = inbox_ml[c * share + i];
+      const float4 y = inbox[c * share + i];
+      const float f = factor(ml.x, mx);
+      sum = fmaf(ml.y, f, sum);
+      x[0] = fmaf(y.x, f, x[0]), x[1] = fmaf(y.y, f, x[1]), x[2] = fmaf(y.z, f, x[2]), x[3] = fmaf(y.w, f, x[3]);
+    }
+    put((rank * share + i) / (D / 4), (rank * share + i) % (D / 4) * 4, x, sum);
   }
-  hb_cluster_sync();                                                    // nobody leaves while its numbers are read
 }
 
 template <typename CT, typename T, int D, int NT>
@@ -675,7 +680,7 @@ HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const vo
   const size_t size = dt == HB_F32 ? 4 : 2;
   C8Attend a = {q, ld_q, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, n_pages, Hkv, page_size / C8_BLOCK, bt, ld_table, table_rows, table_width,
                 row_req, pos, (const int4*)tiles, 0, (G + 8 * nt - 1) / (8 * nt), G, window, scale * 1.4426950408889634f, out,
-                !(((uintptr_t)q | ld_q * size) & (4 * size - 1))};
+                !(((uintptr_t)q | ld_q * size) & (4 * size - 1)), !((uintptr_t)out & (4 * size - 1))};
   const int count = tiles ? n_tiles : n_tiles * a.tiles_row;
   cudaError_t e = cudaErrorInvalidValue;
   C8_DISPATCH(ct, "hb_cache8_attention_mma", HB_DISPATCH_1(dt, "hb_cache8_attention_mma", {

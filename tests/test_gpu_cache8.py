@@ -342,3 +342,31 @@ def test_planes_that_are_part_of_wider_ones_and_many_planes():
     assert torch.equal(whole, want)
     ops.copy_pages(planes, [], [])
     assert torch.equal(whole, want)
+
+
+def test_an_output_and_queries_at_odd_addresses():
+    batch, tables, pages = step([200, 9, 70], [1, 3, 2], 16)
+    for D in (64, 128):
+        for dtype in (torch.bfloat16, torch.float32):
+            cache = on_gpu(filled(pages, 2, 16, D, torch.int8))
+            wide = torch.randn(6, 8 * D + 1, device=DEV).to(dtype)
+            q = wide[:, 1:]
+            want = ops.attention_cache8(q.contiguous(), cache, batch, 0, 8)
+            room = torch.full((6 * 8 * D + 2,), 3.0, dtype=dtype, device=DEV)
+            out = room[1:-1].view(6, 8 * D)
+            assert ops.attention_cache8(q, cache, batch, 0, 8, out=out) is out and same(out, want) and room[0] == room[-1] == 3.0
+
+
+@pytest.mark.parametrize("group", [1, 5, 8, 9, 17, 33])
+@pytest.mark.parametrize("held", [[0, 15, 16, 33], [130, 700, 1500, 64], [5000, 17, 2049, 4096]])
+def test_rows_joined_over_every_number_of_blocks(group, held, monkeypatch):
+    """Tiles whose keys 1 to 8 blocks share, with pairs that fill them in part."""
+    from hipinfer_b200.kernels import cache8
+
+    batch, tables, pages = step(held, [1] * len(held), 32)
+    cache = filled(pages, 2, 32, 64, torch.int8)
+    q = torch.randn(len(held), 2 * group * 64, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16)
+    for ranks in range(1, 9):
+        monkeypatch.setattr(cache8, "_ranks", lambda *a: ranks)
+        batch.extra.clear()
+        check(q, cache, batch, tables, 2 * group)
