@@ -29,7 +29,7 @@
 #include <cuda_fp16.h>
 
 
-constexpr int C8M_WARPS = 4, C8M_RANKS = 8;      // warps of a block; blocks of a cluster at most
+constexpr int C8M_WARPS = 4, C8M_RANKS = 16;     // warps of a block; blocks of a cluster at most
 
 struct C8Attend {
   const void* q;
@@ -163,9 +163,9 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3, h = blockIdx.y;
   const int ranks = gridDim.x, rank = blockIdx.x;
   const auto cluster_wait = [] { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };
-  hb_pdl_launch();
   if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   hb_pdl_wait();
+  hb_pdl_launch();                                                      // (behind the wait: see cache8_portions_kernel)
   int r, t0, pair0, pairs;
   if (a.tiles) {
     const int4 t = a.tiles[a.first_tile + blockIdx.z];
@@ -602,6 +602,7 @@ static cudaError_t configure() {                                        // once 
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || (dev < 64 && configured[dev])) return e;
   e = cudaFuncSetAttribute(cache8_attention_mma_kernel<CT, T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C8Sizes<CT, T, D, NT>::SMEM);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(cache8_attention_mma_kernel<CT, T, D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) configured[dev] = true;
   return e;
 }

@@ -27,7 +27,7 @@ ops._SIGS["cache8"] = {
     "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p],
     "hb_cache8_attention_mma_supported": [_i, _i, _i, _l],
     "hb_cache8_attention_mma_clusters": [_i, _i, _i, _i, _i],
-    "hb_cache8_portions": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _f, _p, _p, _p, _p],
+    "hb_cache8_portions": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _f, _p, _p, _p, _i, _p],
     "hb_copy_pages": [_p, _i, _p, _p, _i, _p],
 }
 BLOCK8 = 16                                                        # places of a page that share a scale
@@ -228,13 +228,14 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
                   out.data_ptr(), ops._stream())
         return out
     limit = _portion_limit(batch, cache, n_heads, window) if portions and _flash_takes(q, cache, out, n_heads, scale) else 0
-    if limit:
-        _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit)
-    if not limit or min(batch.h_q_len) < limit:
+    others = not limit or min(batch.h_q_len) < limit
+    if others:
         cut = _cut(batch, cache, dt, n_heads, window, limit)
         ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
                   cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], None, batch.positions.data_ptr(),
                   ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), ops._stream())
+    if limit:
+        _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit, others)
     return out
 
 
@@ -297,7 +298,7 @@ def _flash_takes(q, cache: Cache8, out, n_heads: int, scale: float) -> bool:
 _AHEAD = 32             # C8_AHEAD of csrc/cache8_store.cu
 
 
-def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int) -> None:
+def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int, beside: bool) -> None:
     """Requests of `limit` rows or more: the codes of the pages that they see as 16-bit numbers, side by side, their scales beside them, and the flash
     kernel over both."""
     index, places, base = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)      # (one page at least: a row sees its own key)
@@ -305,7 +306,7 @@ def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, 
     k, v = (torch.empty((n,) + cache.k.shape[1:], dtype=torch.bfloat16, device=device) for _ in range(2))
     scales = torch.empty(cache.n_kv_heads, n * cache8_blocks(cache.page_size) + 2 * _AHEAD, 4, dtype=torch.float32, device=device)
     ops._call("cache8", "hb_cache8_portions", *(t.data_ptr() for t in cache.tensors), cache.code, table.data_ptr(), index.data_ptr(), n, cache.k.shape[0],
-              *cache.k.shape[1:], scale, k.data_ptr(), v.data_ptr(), scales.data_ptr(), ops._stream())
+              *cache.k.shape[1:], scale, k.data_ptr(), v.data_ptr(), scales.data_ptr(), beside, ops._stream())
     ops.fast.flash_prefill_tc_cache8(q, k, v, places, batch.req_q_start, batch.req_q_len, batch.req_ctx_len, out, batch.max_q_len, n_heads,
                                      cache.n_kv_heads, cache.head_dim, cache.page_size, window, limit, scales, base)
 
@@ -382,10 +383,12 @@ def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
 
 
 def _ranks(tiles: int, keys: int, clusters) -> int:
-    """Blocks (1 to 8, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 64 keys each.
+    """Blocks (1 to 16, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 128 keys each; more than
+    8 where they have an SM each and 512 keys (one request of 24,000 tokens, heads of 64, us: 22 with 8, 16 with 16; of 500 5.5 with 4, 5.8 with 7; four of
+    2,000 7.9 with 8, 9.1 with 12).
     Lengths differ, and a wave of blocks ends with its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand
     tokens, us: 153 as one wave of one block a tile, 142 of four; of 2,000 each 49 and 60)."""
-    most = min(8, max(1, keys // 64))
+    most = max(1, min(8, keys // 128), min(16, keys // 512, 148 // tiles))
     ranks = next((r for r in range(most, 1, -1) if clusters(r) >= tiles), 1)
     while 2 * ranks <= 8 and tiles <= 4 * clusters(2 * ranks) and keys >= 4096 * ranks:
         ranks *= 2

@@ -360,13 +360,13 @@ def test_an_output_and_queries_at_odd_addresses():
 @pytest.mark.parametrize("group", [1, 5, 8, 9, 17, 33])
 @pytest.mark.parametrize("held", [[0, 15, 16, 33], [130, 700, 1500, 64], [5000, 17, 2049, 4096]])
 def test_rows_joined_over_every_number_of_blocks(group, held, monkeypatch):
-    """Tiles whose keys 1 to 8 blocks share, with pairs that fill them in part."""
+    """Tiles whose keys 1 to 16 blocks share, with pairs that fill them in part."""
     from hipinfer_b200.kernels import cache8
 
     batch, tables, pages = step(held, [1] * len(held), 32)
     cache = filled(pages, 2, 32, 64, torch.int8)
     q = torch.randn(len(held), 2 * group * 64, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16)
-    for ranks in range(1, 9):
+    for ranks in range(1, 17):
         monkeypatch.setattr(cache8, "_ranks", lambda *a: ranks)
         batch.extra.clear()
         check(q, cache, batch, tables, 2 * group)
