@@ -18,11 +18,11 @@
 // Codes are integers (or e4m3 numbers) of at most 8 significant bits, exact in f16. The query of a pair is scaled by a power of two to below 2^10 and
 // split into f16 parts: one holds all of a bf16 query, two hold 22 bits of a 32-bit one. A bf16 query meets int8 keys as they are: it is rounded to
 // 16 bits of its pair's largest number, two int8 parts (2^-16 of that number is less than what bf16 keeps of it), whose products with the codes are
-// exact in integers; the keys' conversion was a sixth of all instructions. A weight is 2^(10 + score - bound), where the bound lies 8 (in base 2) above
-// a score that was the largest once and is raised only when one passes it, so that raising it, which costs a pass over the accumulators, is
-// rare. It goes into the product with V times its unit's scale over a reference, that of an earlier unit, which is exchanged (another pass) only
-// where the two are more than 2^5 apart: below 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing.
-// Scales, sums and accumulators are 32-bit.
+// exact in integers; the keys' conversion was a sixth of all instructions. A weight is 2^(score - sub), where sub lies 2 (in base 2) below
+// a score that was the largest once and is raised only when a weight passes 2^10, so that raising it, which costs a pass over the accumulators, is
+// rare. It is made times its unit's V scale over a reference, that of an earlier unit, which is exchanged (another pass) only where the two are more
+// than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing; a unit's sum is divided
+// by that ratio again. Scales, sums and accumulators are 32-bit.
 #include "cache8.cuh"
 #include "tc_common.cuh"
 
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   // this warp's stages: U units each, the id-th and every (ranks * WARPS)th from there; a lane looks up one unit of 32, 32 units ahead
   const int s_lo = u_lo / U, first = s_lo + id;
   const int count = u_hi < first * U ? 0 : (u_hi / U - first) / stride + 1;
-  struct Units { int at; float k_scale, v_scale; };
+  struct Units { int at; float k_scale, v_log2; };                      // V's scale as a power of two
   const auto look = [&](int i) {                                        // stages i .. i + BATCH - 1
     Units x = {-1, 0.f, 0.f};
     const int unit = (first + (i + lane / U) * stride) * U + lane % U;
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       if (page >= 0 && page < a.n_pages) {
         x.at = (page * a.Hkv + h) * a.upp + unit % a.upp;
         x.k_scale = a.ks[x.at];
-        x.v_scale = a.vs[x.at];
+        x.v_log2 = __log2f(fmaxf(a.vs[x.at], 1e-37f));                  // (a block that nothing was stored to: a scale of 0)
       }
     }
     return x;
@@ -316,20 +316,20 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       col_hi[nt][c] = i < n ? a.pos[t0 + (pair0 + i) / a.G] : -1;
     }
 
-  float o[STEPS][NT][4], bound[NT][2], sub[NT][2], l[NT][2];            // a weight is 2^(score - sub)
-  float v_ref = 0.f, v_inv = 0.f;                                       // V's reference scale, which o is to be multiplied with, and its inverse
+  float o[STEPS][NT][4], sub[NT][2], most[NT][2], l[NT][2];             // most: the largest exponent of a weight, 10; -inf while there is no score yet
+  float v_ref = 0.f;                                                    // V's reference scale, which o is to be multiplied with, as a power of two
+  bool none = true;                                                     // no unit yet
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    bound[nt][0] = bound[nt][1] = -INFINITY;
-    sub[nt][0] = sub[nt][1] = 0.f;
-    l[nt][0] = l[nt][1] = 0.f;
+    sub[nt][0] = sub[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+    most[nt][0] = most[nt][1] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < STEPS; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
   }
 
-  // the scores of a unit, in 32 bits
+  // the scores of a unit over col and its scale, in 32 bits
   const uint32_t k_lane = c8_at_k<D>((lane >> 3 & 1) * 8 + (lane & 7), lane >> 4);      // ldmatrix: rows 0-7 and 8-15 of a piece, then of the next
-  const auto products = [&](uint32_t stage, float k_scale, float (&s)[NT][4]) {
+  const auto products = [&](uint32_t stage, float (&s)[NT][4]) {
     int si[2][NT][4];                                                   // two chains of products: of int8 parts, or of every second step
     float sf[2][NT][4];
     const auto query = [&](int part, int nt, int step) {
@@ -370,18 +370,22 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int c = 0; c < 4; c++)
-        s[nt][c] = (Z::Q_INT ? (float)(si[0][nt][c] * 256 + si[1][nt][c]) : sf[0][nt][c] + sf[1][nt][c]) * (col[nt][c & 1] * k_scale);
+        s[nt][c] = Z::Q_INT ? (float)(si[0][nt][c] * 256 + si[1][nt][c]) : sf[0][nt][c] + sf[1][nt][c];
   };
   // U units side by side in shared memory, whose first place is key0; at < 0: one that is not there
-  const auto compute = [&](uint32_t stage, int key0, const int (&at)[U], const float (&k_scale)[U], const float (&v_scale)[U]) {
-    float s[U][NT][4];
+  const auto compute = [&](uint32_t stage, int key0, const int (&at)[U], const float (&k_scale)[U], const float (&v_log2)[U]) {
+    float w[U][NT][4];                                                  // scores, then the weights' exponents, then the weights
 #pragma unroll
     for (int u = 0; u < U; u++) {
       if (at[u] >= 0) {
-        products(stage + u * Z::UNIT, k_scale[u], s[u]);
+        products(stage + u * Z::UNIT, w[u]);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) w[u][nt][c] = fmaf(w[u][nt][c], col[nt][c & 1] * k_scale[u], -sub[nt][c & 1]);
       } else {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = -INFINITY;
+        for (int nt = 0; nt < NT; nt++) w[u][nt][0] = w[u][nt][1] = w[u][nt][2] = w[u][nt][3] = -INFINITY;
       }
     }
     const bool whole = key0 >= all_lo && key0 + U * C8_BLOCK - 1 <= p_lo;
@@ -393,68 +397,72 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
 #pragma unroll
           for (int c = 0; c < 4; c++) {
             const int key = key0 + u * C8_BLOCK + g + (c >> 1) * 8, hi = col_hi[nt][c & 1];
-            if (key > hi || hi - key >= window) s[u][nt][c] = -INFINITY;
+            if (key > hi || hi - key >= window) w[u][nt][c] = -INFINITY;
           }
     }
     bool raise = false;
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+      for (int c = 0; c < 2; c++) {
+        float mx = fmaxf(w[0][nt][c], w[0][nt][c + 2]);
 #pragma unroll
-        for (int c = 0; c < 4; c++) raise |= s[u][nt][c] > bound[nt][c & 1];
+        for (int u = 1; u < U; u++) mx = fmaxf(mx, fmaxf(w[u][nt][c], w[u][nt][c + 2]));
+        raise |= mx > most[nt][c];
+      }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          float mx = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+          float mx = fmaxf(w[0][nt][c], w[0][nt][c + 2]);
 #pragma unroll
-          for (int u = 1; u < U; u++) mx = fmaxf(mx, fmaxf(s[u][nt][c], s[u][nt][c + 2]));
+          for (int u = 1; u < U; u++) mx = fmaxf(mx, fmaxf(w[u][nt][c], w[u][nt][c + 2]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          if (mx > bound[nt][c]) {
-            const float f = hb_exp2(bound[nt][c] - (mx + 8.f));         // 0 while nothing has been summed
-            bound[nt][c] = mx + 8.f;
-            sub[nt][c] = mx - 2.f;                                      // (a weight is at most 2^10)
+          if (mx > most[nt][c]) {
+            const float up = mx - 2.f, f = most[nt][c] == -INFINITY ? 0.f : hb_exp2(-up);      // 0 while nothing has been summed
+            most[nt][c] = 10.f;
+            sub[nt][c] += up;
             l[nt][c] *= f;
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u][nt][c] -= up, w[u][nt][c + 2] -= up;
 #pragma unroll
             for (int i = 0; i < STEPS; i++) o[i][nt][c] *= f, o[i][nt][c + 2] *= f;
           }
         }
     }
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) s[u][nt][c] = hb_exp2(s[u][nt][c] - sub[nt][c & 1]);
-        l[nt][0] += s[u][nt][0] + s[u][nt][2];
-        l[nt][1] += s[u][nt][1] + s[u][nt][3];
-      }
-#pragma unroll
     for (int u = 0; u < U; u++) {
       if (at[u] < 0) continue;
-      float ratio = v_scale[u] * v_inv;                                 // of V's scale to the reference
-      if (v_scale[u] > 1e-37f && !(ratio >= 1.f / 32 && ratio <= 32.f)) {
-        const float f = v_ref / v_scale[u];
+      float ratio = v_log2[u] - v_ref;                                  // of V's scale to the reference
+      if (none || !(fabsf(ratio) <= 5.f)) {
+        const float f = none ? 0.f : hb_exp2(-ratio);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int i = 0; i < STEPS; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++) o[i][nt][c] *= f;
-        v_ref = v_scale[u];
-        v_inv = 1.f / v_ref;
-        ratio = 1.f;
+        v_ref = v_log2[u];
+        none = false;
+        ratio = 0.f;
+      }
+      const float back = hb_exp2(-ratio);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) w[u][nt][c] = hb_exp2(w[u][nt][c] + ratio);
+        l[nt][0] = fmaf(w[u][nt][0] + w[u][nt][2], back, l[nt][0]);
+        l[nt][1] = fmaf(w[u][nt][1] + w[u][nt][3], back, l[nt][1]);
       }
       uint32_t b[W_PARTS][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         uint32_t x[W_PARTS], y[W_PARTS];
-        c8_split<W_PARTS>(s[u][nt][0] * ratio, s[u][nt][1] * ratio, x);
-        c8_split<W_PARTS>(s[u][nt][2] * ratio, s[u][nt][3] * ratio, y);
+        c8_split<W_PARTS>(w[u][nt][0], w[u][nt][1], x);
+        c8_split<W_PARTS>(w[u][nt][2], w[u][nt][3], y);
 #pragma unroll
         for (int p = 0; p < W_PARTS; p++) b[p][nt][0] = c8_transpose(x[p]), b[p][nt][1] = c8_transpose(y[p]);
       }
@@ -511,7 +519,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
     for (int u = 0; u < U; u++) {
       const int l = i % BATCH * U + u;
       at[u] = __shfl_sync(0xffffffffu, now.at, l);
-      fk[u] = __shfl_sync(0xffffffffu, now.k_scale, l), fv[u] = __shfl_sync(0xffffffffu, now.v_scale, l);
+      fk[u] = __shfl_sync(0xffffffffu, now.k_scale, l), fv[u] = __shfl_sync(0xffffffffu, now.v_log2, l);
     }
     compute(ring + slot * U * Z::UNIT, (first + i * stride) * U * C8_BLOCK, at, fk, fv);
     ahead = slot;
@@ -528,16 +536,17 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
       l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
     }
+  const float v_scale = none ? 0.f : hb_exp2(v_ref);
   __syncthreads();                                                      // rings and query are read no more
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const int pair = nt * 8 + 2 * tq + (c & 1);
-      if (g == 0 && c < 2) ml_sh[warp][pair] = make_float2(bound[nt][c], l[nt][c]);
+      if (g == 0 && c < 2) ml_sh[warp][pair] = make_float2(most[nt][c] == -INFINITY ? -INFINITY : sub[nt][c], l[nt][c]);
       // dimension d = g D / 8 + 2 i + e lies at 16 i + 8 e + g: the lanes of a store in different banks
 #pragma unroll
-      for (int i = 0; i < STEPS; i++) o_sh[(warp * PAIRS + pair) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c] * v_ref;
+      for (int i = 0; i < STEPS; i++) o_sh[(warp * PAIRS + pair) * PITCH + i * 16 + (c >> 1) * 8 + g] = o[i][nt][c] * v_scale;
     }
   __syncthreads();
   const auto place = [](int d) { return d % (D / 8) / 2 * 16 + d % 2 * 8 + d / (D / 8); };

@@ -383,13 +383,17 @@ def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
 
 
 def _ranks(tiles: int, keys: int, clusters) -> int:
-    """Blocks (1 to 16, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 128 keys each; more than
-    8 where they have an SM each and 512 keys (one request of 24,000 tokens, heads of 64, us: 22 with 8, 16 with 16; of 500 5.5 with 4, 5.8 with 7; four of
-    2,000 7.9 with 8, 9.1 with 12).
-    Lengths differ, and a wave of blocks ends with its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand
-    tokens, us: 153 as one wave of one block a tile, 142 of four; of 2,000 each 49 and 60)."""
-    most = max(1, min(8, keys // 128), min(16, keys // 512, 148 // tiles))
-    ranks = next((r for r in range(most, 1, -1) if clusters(r) >= tiles), 1)
+    """Blocks (1 to 16, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 128 keys each while
+    there are at most two on an SM, else 400, or 512 in clusters of 3, 5, 6 and 7, which fill the GPU less evenly; more than 8 where they have an SM each
+    and 512 keys. Measured, us: 4 requests of 2,000 tokens (8 kv heads of 64) 8.8 with 4, 8.2 with 8; 8 of 2,000 9.6 and 10.5; 16 of 2,000 13.1 with 2,
+    14.3 with 3, 13.0 with 4, of 8,000 34.7 with 2 and 28.7 with 4; one of 24,000 22 with 8, 16 with 16. Lengths differ, and a wave of blocks ends with
+    its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand tokens, heads of 128: 145 as one wave of one block
+    a tile, 137 and 135 as two and four; of 2,000 each 48, 51 and 58)."""
+    def fits(r):
+        least = 512 if r > 8 else 128 if tiles * r <= 2 * 148 else 400 if r in (2, 4, 8) else 512
+        return keys >= least * r and (r <= 8 or tiles * r <= 148) and clusters(r) >= tiles
+
+    ranks = next((r for r in range(16, 1, -1) if fits(r)), 1)
     while 2 * ranks <= 8 and tiles <= 4 * clusters(2 * ranks) and keys >= 4096 * ranks:
         ranks *= 2
     return ranks
