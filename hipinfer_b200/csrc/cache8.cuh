@@ -11,11 +11,17 @@ constexpr float C8_LEAST = 1e-30f;              // below it a block's largest nu
 
 __host__ __device__ constexpr int c8_blocks(int page_size) { return (page_size + C8_BLOCK - 1) / C8_BLOCK; }
 
-// A code type: its largest number, code to number, and number (already within +- the largest) to the nearest code, ties to the even one; four of them
+// A code type: its largest number, code to number (four of them from four bytes), and number (already within +- the largest) to the nearest code, ties to the even one; four of them
 // to four bytes.
 struct C8Int8 {
   static constexpr float MOST = 127.f;
   static __device__ __forceinline__ float value(uint8_t c) { return (float)(int8_t)c; }
+  // (with the sign bit turned a byte u is code + 128, and 0x4b000000 | u is 2^23 + u)
+  static __device__ __forceinline__ void values4(uint32_t w, float* x) {
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 + i)) - 8388736.f;
+  }
   // (1.5 x 2^23 + x has x's nearest integer in its last bits, ties to even; conversions to integers run at an eighth of an addition's rate)
   static __device__ __forceinline__ uint32_t code4(const float* x) {
     const uint32_t a = __float_as_uint(__fadd_rn(x[0], 12582912.f)), b = __float_as_uint(__fadd_rn(x[1], 12582912.f));
@@ -28,6 +34,11 @@ struct C8E4m3 {
   static constexpr float MOST = 448.f;
   static __device__ __forceinline__ float value(uint8_t c) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+  }
+  static __device__ __forceinline__ void values4(uint32_t w, float* x) {
+    const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)), b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3));
+    const float2 p = __half22float2(a), q = __half22float2(b);
+    x[0] = p.x, x[1] = p.y, x[2] = q.x, x[3] = q.y;
   }
   static __device__ __forceinline__ uint32_t code4(const float* x) {
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3) |

@@ -27,6 +27,19 @@ template <typename T, int E> struct C8Piece {
       }
     }
   }
+  // NaN becomes 0 and what is beyond +-most becomes that (of bf16 its first 16 bits, half a code below at the most)
+  static __device__ __forceinline__ uint32_t finite(uint32_t w, uint32_t most) {
+    const uint32_t a = w & 0x7fffffffu;
+    return a > 0x7f800000u ? 0u : (w ^ a) | min(a, most);
+  }
+  static __device__ __forceinline__ void finite(Raw& r, float most) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    const uint32_t m = __float_as_uint(most);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      w[i] = E == 4 ? finite(w[i], m) : finite(w[i] & 0xffff0000u, m) & 0xffff0000u | finite(w[i] << 16, m) >> 16;
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 };
 template <typename CT, int E> __device__ __forceinline__ void c8_store(uint8_t* p, const float* x) {
   if constexpr (E == 8) *(uint2*)p = make_uint2(CT::code4(x), CT::code4(x + 4));
@@ -88,13 +101,14 @@ __global__ void __launch_bounds__(32 * C8S_WARPS) cache8_store_kernel(const T* k
     using Raw = typename Piece::Raw;
     Raw kept[ITEMS ? ITEMS : 1];
     float most = 0.f;
-    const auto largest = [&](const Raw& r) {
+    const auto largest = [&](const Raw& r) {                     // of the finite ones
       float y[E];
       Piece::floats(r, y);
 #pragma unroll
       for (int e = 0; e < E; e++)
         if (fabsf(y[e]) <= 3.402823466e38f) most = fmaxf(most, fabsf(y[e]));
     };
+    bool odd = false;                                            // some of the numbers kept are not finite
     const auto load = [&](int i) { return *(const Raw*)(x + win[i / pieces] * ld + i % pieces * E); };
     if constexpr (ITEMS > 0) {
 #pragma unroll
@@ -102,34 +116,75 @@ __global__ void __launch_bounds__(32 * C8S_WARPS) cache8_store_kernel(const T* k
         kept[j] = Raw{};
         if (win[(j * 32 + lane) / pieces] >= 0) kept[j] = load(j * 32 + lane);
       }
+      // the largest |x| by its bits, of 16-bit numbers two at a time; only where one is not finite are they looked at one by one
+      uint32_t bits = 0;
 #pragma unroll
-      for (int j = 0; j < ITEMS; j++) largest(kept[j]);
+      for (int j = 0; j < ITEMS; j++) {
+        const uint32_t w[4] = {kept[j].x, kept[j].y, kept[j].z, kept[j].w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) bits = sizeof(T) == 4 ? max(bits, w[i] & 0x7fffffffu) : __vmaxu2(bits, w[i] & 0x7fff7fffu);
+      }
+      if (sizeof(T) == 2) bits = max(bits & 0xffff0000u, bits << 16);
+      bits = __reduce_max_sync(0xffffffffu, bits);
+      odd = bits >= 0x7f800000u;
+      most = __uint_as_float(bits);
+      if (odd) {
+        most = 0.f;
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) largest(kept[j]);
+        most = hb_warp_max(most);
+      }
     } else {
       for (int i = lane; i < items; i += 32)
         if (win[i / pieces] >= 0) largest(load(i));
+      most = hb_warp_max(most);
     }
-    float now = __fdiv_rn(fmaxf(hb_warp_max(most), C8_LEAST), CT::MOST);
+    float now = __fdiv_rn(fmaxf(most, C8_LEAST), CT::MOST);
     if (!fresh && now > old) {
       const float f = __fdiv_rn(old, now);
-      for (int i = lane; i < items; i += 32)
-        if (win[i / pieces] < 0) {
-          float z[E];
+      using Codes = std::conditional_t<E == 8, uint2, std::conditional_t<E == 4, uint32_t, uint8_t>>;
+      const auto again = [&](int i, const Codes& c) {
+        float z[E];
+        if constexpr (E == 8) CT::values4(c.x, z), CT::values4(c.y, z + 4);
+        else if constexpr (E == 4) CT::values4(c, z);
+        else z[0] = CT::value(c);
 #pragma unroll
-          for (int e = 0; e < E; e++) z[e] = __fmul_rn(CT::value(at[(long)i * E + e]), f);
-          c8_store<CT, E>(at + (long)i * E, z);
+        for (int e = 0; e < E; e++) z[e] = __fmul_rn(z[e], f);
+        c8_store<CT, E>(at + (long)i * E, z);
+      };
+      if constexpr (ITEMS > 0) {
+        constexpr int AHEAD = ITEMS < 8 ? ITEMS : 8;             // asked for before the first is used
+#pragma unroll 1
+        for (int j = 0; j < ITEMS; j += AHEAD) {
+          Codes c[AHEAD];
+#pragma unroll
+          for (int n = 0; n < AHEAD; n++) c[n] = *(const Codes*)(at + ((j + n) * 32 + lane) * E);
+#pragma unroll
+          for (int n = 0; n < AHEAD; n++)
+            if (win[((j + n) * 32 + lane) / pieces] < 0) again((j + n) * 32 + lane, c[n]);
         }
+      } else {
+        for (int i = lane; i < items; i += 32)
+          if (win[i / pieces] < 0) again(i, at[i]);
+      }
     } else if (!fresh) {
       now = old;
     }
     if (lane == 0) *scale = now;
     const float inv = __fdiv_rn(1.f, now);
+    if constexpr (ITEMS > 0)
+      if (odd) {
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) Piece::finite(kept[j], fminf(__fmul_rn(now, CT::MOST), 3.402823466e38f));
+      }
     const auto put = [&](int i, const Raw& r) {
       float y[E], z[E];
       Piece::floats(r, y);
 #pragma unroll
       for (int e = 0; e < E; e++) {
         z[e] = __fmul_rn(y[e], inv);
-        z[e] = z[e] != z[e] ? 0.f : fminf(fmaxf(z[e], -CT::MOST), CT::MOST);
+        // (numbers kept are finite by now, and no more than a rounding beyond the largest code, which they become)
+        if constexpr (ITEMS == 0) z[e] = z[e] != z[e] ? 0.f : fminf(fmaxf(z[e], -CT::MOST), CT::MOST);
       }
       c8_store<CT, E>(at + (long)i * E, z);
     };
@@ -174,6 +229,12 @@ HB_EXPORT int hb_cache8_store(const void* k, const void* v, long ld_k, long ld_v
 // Page i of the output [n][Hkv][page_size][D] is page table[index[i]] of the cache (table[i] without an index); a number outside of the
 // cache's pages gives zeros. E codes at a time: 8 of them are a load of 8 bytes and a store of 16 (bf16) or two, so that a warp's stores are
 // whole lines; a page of one plane is a block's.
+constexpr int C8E_AHEAD = 4;      // pieces that a thread asks for before it uses the first
+// CTAs that share `pieces` of 8 bytes: one piece a thread while there are few of them, all of them one CTA's when they are many.
+static int c8_split(long ctas, long pieces) {
+  const long most = (pieces + 255) / 256, room = 8L * 148 / ctas;
+  return (int)(room < 1 ? 1 : room < most ? room : most > 64 ? 64 : most);
+}
 template <typename CT, typename T, int E>
 __global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, const int* table,
                                                             const int* index, long n_pages, int Hkv, int page_size, int D, T* k, T* v) {
@@ -181,33 +242,50 @@ __global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, c
   hb_pdl_wait();
   const long i = blockIdx.x;
   const bool is_v = blockIdx.y;
-  const int pieces = Hkv * page_size * D / E, blocks = c8_blocks(page_size);
+  const int step = gridDim.z * 256;
+  const int pieces = Hkv * page_size * D / E, row_pieces = D / E, blocks = c8_blocks(page_size);
+  const bool whole = page_size % C8_BLOCK == 0;
   T* out = (is_v ? v : k) + i * pieces * E;
   const long page = table[index ? index[i] : i];
   const bool there = page >= 0 && page < n_pages;
   const uint8_t* codes = (is_v ? vc : kc) + (there ? page : 0) * pieces * E;
   const float* scales = (is_v ? vs : ks) + (there ? page : 0) * Hkv * blocks;
-#pragma unroll 4
-  for (int j = threadIdx.x; j < pieces; j += 256) {
-    const int row = j / (D / E);                    // of the page's rows, head by head
-    const float f = there ? scales[row / page_size * blocks + row % page_size / C8_BLOCK] : 0.f;
-    if constexpr (E == 8) {
-      const uint2 w = there ? *(const uint2*)(codes + (long)j * E) : make_uint2(0u, 0u);
-      float x[8];
+  for (int j0 = blockIdx.z * 256 + threadIdx.x; j0 < pieces; j0 += C8E_AHEAD * step) {
+    uint2 w[C8E_AHEAD];
+    float f[C8E_AHEAD];
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = CT::value((uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)))) * f;
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        if constexpr (sizeof(T) == 4) *(float4*)(out + (long)j * E + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    for (int k = 0; k < C8E_AHEAD; k++) {
+      const int j = j0 + k * step;
+      w[k] = make_uint2(0u, 0u), f[k] = 0.f;
+      if (there && j < pieces) {
+        if constexpr (E == 8) w[k] = *(const uint2*)(codes + (long)j * E);
+        else w[k].x = codes[j];
+        const int row = j / row_pieces;                          // of the page's rows, head by head
+        f[k] = scales[whole ? row / C8_BLOCK : row / page_size * blocks + row % page_size / C8_BLOCK];
       }
-      if constexpr (sizeof(T) == 2) {
-        __nv_bfloat162 y[4];
+    }
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        *(uint4*)(out + (long)j * E) = *(const uint4*)y;
+    for (int k = 0; k < C8E_AHEAD; k++) {
+      const int j = j0 + k * step;
+      if (j >= pieces) break;
+      if constexpr (E == 8) {
+        float x[8];
+        CT::values4(w[k].x, x);
+        CT::values4(w[k].y, x + 4);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = there ? x[e] * f[k] : 0.f;
+        if constexpr (sizeof(T) == 4) {
+          *(float4*)(out + (long)j * E) = make_float4(x[0], x[1], x[2], x[3]);
+          *(float4*)(out + (long)j * E + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+          __nv_bfloat162 y[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+          *(uint4*)(out + (long)j * E) = *(const uint4*)y;
+        }
+      } else {
+        out[j] = hb_from_float<T>(there ? CT::value((uint8_t)w[k].x) * f[k] : 0.f);
       }
-    } else {
-      out[j] = hb_from_float<T>(there ? CT::value(codes[j]) * f : 0.f);
     }
   }
 }
@@ -219,8 +297,8 @@ HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, 
     HB_FAIL("hb_cache8_expand: %ld of %ld pages of %d heads, %d places and %d", n, n_pages, Hkv, page_size, D);
   const bool wide = D % 8 == 0 && !(((uintptr_t)kc | (uintptr_t)vc) & 7) && !(((uintptr_t)k | (uintptr_t)v) & 15);
 #define C8E_LAUNCH(E)                                                                                                                                   \
-  hb_launch(cache8_expand_kernel<CT, TA, E>, dim3(n, 2), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n_pages, Hkv, \
-            page_size, D, (TA*)k, (TA*)v)
+  hb_launch(cache8_expand_kernel<CT, TA, E>, dim3(n, 2, c8_split(2 * n, (long)Hkv * page_size * D / E)), dim3(256), 0, st, (const uint8_t*)kc,            \
+            (const uint8_t*)vc, ks, vs, table, index, n_pages, Hkv, page_size, D, (TA*)k, (TA*)v)
   C8_DISPATCH(ct, "hb_cache8_expand", HB_DISPATCH_1(dt, "hb_cache8_expand", {
     if (wide) C8E_LAUNCH(8);
     else C8E_LAUNCH(1);
@@ -248,33 +326,42 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
   const long i = blockIdx.x;
   const int blocks = c8_blocks(page_size);
   const long ld = n * blocks + 2 * C8_AHEAD;
+  const int step = gridDim.y * 256;
   if (i == n) {
-    for (int j = threadIdx.x; j < Hkv * 2 * C8_AHEAD; j += 256) {
-      const int at = j % (2 * C8_AHEAD);
-      scale[j / (2 * C8_AHEAD) * ld + (at < C8_AHEAD ? at : n * blocks + at)] = make_float4(1.f, 0.f, 1.f, 0.f);
-    }
+    if (blockIdx.y == 0)
+      for (int j = threadIdx.x; j < Hkv * 2 * C8_AHEAD; j += 256) {
+        const int at = j % (2 * C8_AHEAD);
+        scale[j / (2 * C8_AHEAD) * ld + (at < C8_AHEAD ? at : n * blocks + at)] = make_float4(1.f, 0.f, 1.f, 0.f);
+      }
     if (beside) hb_pdl_wait();
     return;
   }
   const long page = table[index[i]];
   const bool there = page >= 0 && page < n_pages;
-  for (int j = threadIdx.x; j < Hkv * blocks; j += 256) {
+  const int pieces = Hkv * page_size * D / 8;
+  for (int j0 = blockIdx.y * 256 + threadIdx.x; j0 < 2 * pieces; j0 += C8E_AHEAD * step) {
+    uint2 w[C8E_AHEAD];
+#pragma unroll
+    for (int u = 0; u < C8E_AHEAD; u++) {
+      const int j = j0 + u * step;
+      w[u] = there && j < 2 * pieces ? *(const uint2*)((j >= pieces ? vc : kc) + (page * pieces + (j >= pieces ? j - pieces : j)) * 8L) : make_uint2(0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < C8E_AHEAD; u++) {
+      const int j = j0 + u * step;
+      if (j >= 2 * pieces) break;
+      float x[8];
+      CT::values4(w[u].x, x);
+      CT::values4(w[u].y, x + 4);
+      __nv_bfloat162 y[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(there ? x[2 * e] : 0.f, there ? x[2 * e + 1] : 0.f);
+      *(uint4*)((j >= pieces ? v : k) + (i * pieces + (j >= pieces ? j - pieces : j)) * 8L) = *(const uint4*)y;
+    }
+  }
+  for (int j = blockIdx.y * 256 + threadIdx.x; j < Hkv * blocks; j += step) {
     const float x = there ? fmaxf(ks[page * Hkv * blocks + j], C8_LEAST) * scale_log2 : -1.f, y = there ? fmaxf(vs[page * Hkv * blocks + j], C8_LEAST) : 1.f;
     scale[j / blocks * ld + C8_AHEAD + i * blocks + j % blocks] = make_float4(x, log2f(y), 1.f / y, 0.f);
-  }
-  const int pieces = Hkv * page_size * D / 8;
-#pragma unroll 4
-  for (int j = threadIdx.x; j < 2 * pieces; j += 256) {
-    const bool is_v = j >= pieces;
-    const long at = (is_v ? j - pieces : j) * 8L;
-    const uint2 w = there ? *(const uint2*)((is_v ? vc : kc) + page * pieces * 8 + at) : make_uint2(0u, 0u);
-    __nv_bfloat162 y[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const uint32_t pair = (e < 2 ? w.x : w.y) >> (16 * (e & 1));
-      y[e] = __floats2bfloat162_rn(CT::value((uint8_t)pair), CT::value((uint8_t)(pair >> 8)));
-    }
-    *(uint4*)((is_v ? v : k) + i * pieces * 8 + at) = *(const uint4*)y;
   }
   if (beside) hb_pdl_wait();
 }
@@ -288,7 +375,7 @@ HB_EXPORT int hb_cache8_portions(const void* kc, const void* vc, const float* ks
   if (n >= 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || D % 8 || 2L * Hkv * page_size * D > 0x7fffffffL - 256 || n_pages < 1)
     HB_FAIL("hb_cache8_portions: %ld of %ld pages of %d heads, %d places and %d", n, n_pages, Hkv, page_size, D);
   C8_DISPATCH(ct, "hb_cache8_portions",
-      hb_launch(cache8_portions_kernel<CT>, dim3(n + 1), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n, n_pages, Hkv,
+      hb_launch(cache8_portions_kernel<CT>, dim3(n + 1, beside ? 1 : c8_split(n + 1, 2L * Hkv * page_size * D / 8)), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n, n_pages, Hkv,
                 page_size, D, scale * 1.4426950408889634f, (__nv_bfloat16*)k, (__nv_bfloat16*)v, (float4*)scales, beside != 0));
   HB_CHECK_LAUNCH("hb_cache8_portions");
   return 0;
