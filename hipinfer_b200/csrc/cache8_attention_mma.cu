@@ -41,8 +41,8 @@ struct C8Attend {
   const int* bt;
   long ld_table;
   int table_rows, table_width;
-  const int *row_req, *pos;    // row_req null: row t is request t's
-  const int4* tiles;           // (request, its first row, first pair, pairs of its rows); null: single rows, tiles_row tiles each
+  const int* pos;
+  const int4* tiles;           // (request, its first row, first pair, pairs of its rows); null: row t is request t's, tiles_row tiles each
   int first_tile, tiles_row, G, window;
   float scale_log2;
   void* out;
@@ -173,12 +173,12 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   } else {
     t0 = (a.first_tile + blockIdx.z) / a.tiles_row;
     pair0 = (a.first_tile + blockIdx.z) % a.tiles_row * PAIRS, pairs = a.G;
-    r = a.row_req ? a.row_req[t0] : t0;
+    r = t0;
   }
   // single rows that see all of their keys: the first pages are asked for together with the positions, which say how many they are
   constexpr int BATCH = 32 / U;
   const int id = rank * C8M_WARPS + warp, stride = ranks * C8M_WARPS;
-  const bool early = !a.tiles && !a.row_req && a.window <= 0;
+  const bool early = !a.tiles && a.window <= 0;
   int early_page = -1;
   if (early) {
     const int i = ((id + lane / U * stride) * U + lane % U) / a.upp;
@@ -682,14 +682,14 @@ HB_EXPORT int hb_cache8_attention_mma_clusters(int dt, int ct, int D, int nt, in
 // kc and vc are 16-byte aligned.
 HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const void* kc, const void* vc, const float* ks, const float* vs, int ct,
                                       long n_pages, int Hkv, int page_size, int D, const int* bt, long ld_table, int table_rows, int table_width,
-                                      const int* row_req, const int* pos, const int* tiles, int n_tiles, int nt, int ranks, int G, int window,
+                                      const int* pos, const int* tiles, int n_tiles, int nt, int ranks, int G, int window,
                                       float scale, void* out, cudaStream_t st) {
   if (n_tiles <= 0) return 0;
-  if (!hb_cache8_attention_mma_supported(Hkv, page_size, D, n_pages) || G < 1 || ranks < 1 || ranks > C8M_RANKS || (((uintptr_t)kc | (uintptr_t)vc) & 15))
+  if (!hb_cache8_attention_mma_supported(Hkv, page_size, D, n_pages) || G < 1 || nt < 1 || nt > 4 || ranks < 1 || ranks > C8M_RANKS || (((uintptr_t)kc | (uintptr_t)vc) & 15))
     HB_FAIL("hb_cache8_attention_mma: %d kv heads of %d for %d heads each, pages of %d, %d ranks", Hkv, D, G, page_size, ranks);
   const size_t size = dt == HB_F32 ? 4 : 2;
   C8Attend a = {q, ld_q, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, n_pages, Hkv, page_size / C8_BLOCK, bt, ld_table, table_rows, table_width,
-                row_req, pos, (const int4*)tiles, 0, (G + 8 * nt - 1) / (8 * nt), G, window, scale * 1.4426950408889634f, out,
+                pos, (const int4*)tiles, 0, (G + 8 * nt - 1) / (8 * nt), G, window, scale * 1.4426950408889634f, out,
                 !(((uintptr_t)q | ld_q * size) & (4 * size - 1)), !((uintptr_t)out & (4 * size - 1))};
   const int count = tiles ? n_tiles : n_tiles * a.tiles_row;
   cudaError_t e = cudaErrorInvalidValue;

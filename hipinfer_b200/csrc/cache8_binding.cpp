@@ -20,9 +20,9 @@ struct Cut {
   int64_t rows, requests, n_tiles, nt, ranks, group, window, max_pos;
 };
 typedef int (*StoreFn)(const void*, const void*, long, long, int, const int*, int, int, int, int, long, int, void*, void*, float*, float*, void*);
-typedef int (*ExpandFn)(const void*, const void*, const float*, const float*, int, const int*, const int*, long, long, int, int, int, void*, void*, int, void*);
+typedef int (*ExpandFn)(const void*, const void*, const float*, const float*, int, const int*, long, long, int, int, int, void*, void*, int, void*);
 typedef int (*AttendFn)(const void*, int, long, const void*, const void*, const float*, const float*, int, long, int, int, int, const int*, long, int, int,
-                        const int*, const int*, const int*, int, int, int, int, int, float, void*, void*);
+                        const int*, const int*, int, int, int, int, int, float, void*, void*);
 typedef int (*CopyFn)(const long*, int, const int*, const int*, int, void*);
 StoreFn store_fn;
 ExpandFn expand_fn;
@@ -72,7 +72,7 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (pages, address of a Cache, an empty tensor of the results' type): keys and values; or as above
+// (pages, address of a Cache, the results' type as type_code has it): keys and values; or as above
 PyObject* expand(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 3) return PyErr_Format(PyExc_TypeError, "three arguments are expected");
@@ -84,7 +84,7 @@ PyObject* expand(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t count = pages->size(0);
   at::Tensor k = empty({count, c->kv_heads, c->page_size, c->head_dim}, type, *pages), v = empty(k.sizes(), type, *pages);
   const int r = expand_fn((const void*)c->k, (const void*)c->v, (const float*)c->k_scale, (const float*)c->v_scale, (int)c->code,
-                          (const int*)pages->const_data_ptr(), nullptr, (long)count, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim,
+                          (const int*)pages->const_data_ptr(), (long)count, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim,
                           k.mutable_data_ptr(), v.mutable_data_ptr(), type_code(k), stream());
   if (r) return PyLong_FromLong(r);
   PyObject* out = PyTuple_New(2);
@@ -122,7 +122,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const int r = attend_fn(q->const_data_ptr(), type_code(*q), (long)q->stride(0), (const void*)c->k, (const void*)c->v, (const float*)c->k_scale,
                           (const float*)c->v_scale, (int)c->code, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim,
-                          (const int*)table->const_data_ptr(), (long)table->size(1), (int)cut.requests, (int)table->size(1), nullptr,
+                          (const int*)table->const_data_ptr(), (long)table->size(1), (int)cut.requests, (int)table->size(1),
                           (const int*)pos->const_data_ptr(), tiles ? (const int*)tiles->const_data_ptr() : nullptr, (int)cut.n_tiles, (int)cut.nt,
                           (int)cut.ranks, (int)cut.group, (int)cut.window, (float)scale, out.mutable_data_ptr(), stream());
   if (r) return PyLong_FromLong(r);

@@ -27,17 +27,18 @@ template <typename T, int E> struct C8Piece {
       }
     }
   }
-  // NaN becomes 0 and what is beyond +-most becomes that (of bf16 its first 16 bits, half a code below at the most)
+  // NaN becomes 0 and what is beyond +-most becomes that; of bf16 the number nearest to it, which is off by 2^-8 of it at most, less than half the
+  // step to the code below (1 of 127, or 32 of 448) or above
   static __device__ __forceinline__ uint32_t finite(uint32_t w, uint32_t most) {
     const uint32_t a = w & 0x7fffffffu;
     return a > 0x7f800000u ? 0u : (w ^ a) | min(a, most);
   }
   static __device__ __forceinline__ void finite(Raw& r, float most) {
     uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    const uint32_t m = __float_as_uint(most);
+    const uint32_t m = E == 4 ? __float_as_uint(most) : min((__float_as_uint(most) + 0x8000u) & 0xffff0000u, 0x7f7f0000u);
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      w[i] = E == 4 ? finite(w[i], m) : finite(w[i] & 0xffff0000u, m) & 0xffff0000u | finite(w[i] << 16, m) >> 16;
+      w[i] = E == 4 ? finite(w[i], m) : finite(w[i] & 0xffff0000u, m) | finite(w[i] << 16, m) >> 16;
     r = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
@@ -226,18 +227,20 @@ HB_EXPORT int hb_cache8_store(const void* k, const void* v, long ld_k, long ld_v
   return 0;
 }
 
-// Page i of the output [n][Hkv][page_size][D] is page table[index[i]] of the cache (table[i] without an index); a number outside of the
+// Page i of the output [n][Hkv][page_size][D] is page table[i] of the cache; a number outside of the
 // cache's pages gives zeros. E codes at a time: 8 of them are a load of 8 bytes and a store of 16 (bf16) or two, so that a warp's stores are
 // whole lines; a page of one plane is a block's.
 constexpr int C8E_AHEAD = 4;      // pieces that a thread asks for before it uses the first
-// CTAs that share `pieces` of 8 bytes: one piece a thread while there are few of them, all of them one CTA's when they are many.
+// CTAs that share `pieces` of 8 bytes: one piece a thread while there are few of them, all of them one CTA's when they are many (64 pages of 8 heads of
+// 128 3.1 us, with one CTA a page and plane 4.6; 4,000 pages 66 us either way). A thread's numbers of pieces end less than C8E_BEYOND behind the last.
+constexpr int C8E_SPLIT = 64, C8E_BEYOND = C8E_SPLIT * 256 * (C8E_AHEAD + 1);
 static int c8_split(long ctas, long pieces) {
   const long most = (pieces + 255) / 256, room = 8L * 148 / ctas;
-  return (int)(room < 1 ? 1 : room < most ? room : most > 64 ? 64 : most);
+  return (int)(room < 1 ? 1 : room < most ? (room < C8E_SPLIT ? room : C8E_SPLIT) : most < C8E_SPLIT ? most : C8E_SPLIT);
 }
 template <typename CT, typename T, int E>
 __global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, const int* table,
-                                                            const int* index, long n_pages, int Hkv, int page_size, int D, T* k, T* v) {
+                                                            long n_pages, int Hkv, int page_size, int D, T* k, T* v) {
   hb_pdl_launch();
   hb_pdl_wait();
   const long i = blockIdx.x;
@@ -246,7 +249,7 @@ __global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, c
   const int pieces = Hkv * page_size * D / E, row_pieces = D / E, blocks = c8_blocks(page_size);
   const bool whole = page_size % C8_BLOCK == 0;
   T* out = (is_v ? v : k) + i * pieces * E;
-  const long page = table[index ? index[i] : i];
+  const long page = table[i];
   const bool there = page >= 0 && page < n_pages;
   const uint8_t* codes = (is_v ? vc : kc) + (there ? page : 0) * pieces * E;
   const float* scales = (is_v ? vs : ks) + (there ? page : 0) * Hkv * blocks;
@@ -290,15 +293,15 @@ __global__ void __launch_bounds__(256) cache8_expand_kernel(const uint8_t* kc, c
   }
 }
 
-HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, const float* vs, int ct, const int* table, const int* index, long n,
-                               long n_pages, int Hkv, int page_size, int D, void* k, void* v, int dt, cudaStream_t st) {
+HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, const float* vs, int ct, const int* table, long n, long n_pages,
+                               int Hkv, int page_size, int D, void* k, void* v, int dt, cudaStream_t st) {
   if (n <= 0) return 0;
-  if (n > 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || (long)Hkv * page_size * D > 0x7fffffffL - 256 || n_pages < 1)
+  if (n > 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || (long)Hkv * page_size * D > 0x7fffffffL - C8E_BEYOND || n_pages < 1)
     HB_FAIL("hb_cache8_expand: %ld of %ld pages of %d heads, %d places and %d", n, n_pages, Hkv, page_size, D);
   const bool wide = D % 8 == 0 && !(((uintptr_t)kc | (uintptr_t)vc) & 7) && !(((uintptr_t)k | (uintptr_t)v) & 15);
 #define C8E_LAUNCH(E)                                                                                                                                   \
   hb_launch(cache8_expand_kernel<CT, TA, E>, dim3(n, 2, c8_split(2 * n, (long)Hkv * page_size * D / E)), dim3(256), 0, st, (const uint8_t*)kc,            \
-            (const uint8_t*)vc, ks, vs, table, index, n_pages, Hkv, page_size, D, (TA*)k, (TA*)v)
+            (const uint8_t*)vc, ks, vs, table, n_pages, Hkv, page_size, D, (TA*)k, (TA*)v)
   C8_DISPATCH(ct, "hb_cache8_expand", HB_DISPATCH_1(dt, "hb_cache8_expand", {
     if (wide) C8E_LAUNCH(8);
     else C8E_LAUNCH(1);
@@ -310,7 +313,8 @@ HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, 
 
 // What the flash kernel for portions wants of a cache: the codes of pages table[index[i]] as bf16, which holds them exactly, and the scales of
 // their blocks, scale[h][C8_AHEAD + i * blocks + block] of n * blocks and C8_AHEAD on either side: {K's times `scale_log2`, log2 of V's, 1 / V's, 0}, K's negative where
-// the page is not there. No scale is less than 1e-30 (a block that nothing was stored to; 0 times a masked score is not a number), and what
+// the page is not there. No scale is less than 1e-30 (a block that nothing was stored to; 0 times a masked score is not a number), places that nothing was stored to may hold anything, and
+// so codes and scales that are not numbers become 0 and 1e-30, and what
 // lies on either side, for tiles that reach over a request's ends, are ones.
 //
 // `beside`: the kernel ahead is cache8_attention_mma_kernel for a step's other rows, which lets this one start when it has itself waited for what came
@@ -355,12 +359,15 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
       CT::values4(w[u].y, x + 4);
       __nv_bfloat162 y[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(there ? x[2 * e] : 0.f, there ? x[2 * e + 1] : 0.f);
+      for (int e = 0; e < 8; e++) x[e] = there && x[e] == x[e] ? x[e] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
       *(uint4*)((j >= pieces ? v : k) + (i * pieces + (j >= pieces ? j - pieces : j)) * 8L) = *(const uint4*)y;
     }
   }
   for (int j = blockIdx.y * 256 + threadIdx.x; j < Hkv * blocks; j += step) {
-    const float x = there ? fmaxf(ks[page * Hkv * blocks + j], C8_LEAST) * scale_log2 : -1.f, y = there ? fmaxf(vs[page * Hkv * blocks + j], C8_LEAST) : 1.f;
+    const auto number = [](float s) { return s <= 3.402823466e38f ? fmaxf(s, C8_LEAST) : C8_LEAST; };
+    const float x = there ? number(ks[page * Hkv * blocks + j]) * scale_log2 : -1.f, y = there ? number(vs[page * Hkv * blocks + j]) : 1.f;
     scale[j / blocks * ld + C8_AHEAD + i * blocks + j % blocks] = make_float4(x, log2f(y), 1.f / y, 0.f);
   }
   if (beside) hb_pdl_wait();
@@ -372,7 +379,7 @@ HB_EXPORT int hb_cache8_portions(const void* kc, const void* vc, const float* ks
                                  long n_pages, int Hkv, int page_size, int D, float scale, void* k, void* v, void* scales, int beside,
                                  cudaStream_t st) {
   if (n <= 0) return 0;
-  if (n >= 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || D % 8 || 2L * Hkv * page_size * D > 0x7fffffffL - 256 || n_pages < 1)
+  if (n >= 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || D % 8 || 2L * Hkv * page_size * D > 0x7fffffffL - C8E_BEYOND || n_pages < 1)
     HB_FAIL("hb_cache8_portions: %ld of %ld pages of %d heads, %d places and %d", n, n_pages, Hkv, page_size, D);
   C8_DISPATCH(ct, "hb_cache8_portions",
       hb_launch(cache8_portions_kernel<CT>, dim3(n + 1, beside ? 1 : c8_split(n + 1, 2L * Hkv * page_size * D / 8)), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n, n_pages, Hkv,

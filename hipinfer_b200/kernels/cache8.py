@@ -1,6 +1,8 @@
 """Operators of a paged cache in 8 bits: storing a step's keys and values, reading pages back, attention over it; and copying pages of a cache
 of any type, as forks inside a page need it. Reached as `ops.Cache8`, `ops.new_cache8`, `ops.store_cache8`, `ops.expand_cache8`, `ops.attention_cache8`
-and `ops.copy_pages` (csrc/cache8_store.cu, cache8_attention.cu, copy_pages.cu).
+and `ops.copy_pages` (csrc/cache8_store.cu: storing and reading back; cache8_attention_mma.cu: attention of single rows and short portions on
+warp MMAs; attention_prefill_tc.cu: of longer portions; cache8_attention.cu: of any other sizes; copy_pages.cu; cache8_binding.cpp: calls without
+the interpreter).
 
 A cache holds, for keys and for values, codes [page, kv head, page_size, head_dim] (int8, or e4m3) and scales float32 [page, kv head, blocks], one
 for each block of 16 places of a page (the last block of a page may have fewer); a place's numbers are code * scale.
@@ -22,9 +24,9 @@ from . import library, ops
 _p, _i, _l, _f = C.c_void_p, C.c_int, C.c_long, C.c_float
 ops._SIGS["cache8"] = {
     "hb_cache8_store": [_p, _p, _l, _l, _i, _p, _i, _i, _i, _i, _l, _i, _p, _p, _p, _p, _p],
-    "hb_cache8_expand": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _p, _p, _i, _p],
+    "hb_cache8_expand": [_p, _p, _p, _p, _i, _p, _l, _l, _i, _i, _i, _p, _p, _i, _p],
     "hb_cache8_attention_any": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _f, _p, _p],
-    "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p],
+    "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p],
     "hb_cache8_attention_mma_supported": [_i, _i, _i, _l],
     "hb_cache8_attention_mma_clusters": [_i, _i, _i, _i, _i],
     "hb_cache8_portions": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _f, _p, _p, _p, _i, _p],
@@ -39,7 +41,7 @@ def cache8_blocks(page_size: int) -> int:
     return -(-page_size // BLOCK8)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Cache8:
     """A layer's cache in 8 bits: codes k, v [pages, n_kv_heads, page_size, head_dim], scales k_scale, v_scale [pages, n_kv_heads, blocks]."""
 
@@ -67,11 +69,9 @@ class Cache8:
         numbers = np.array([t.data_ptr() for t in self.tensors] + list(k.shape) + [self.code, k.device.index if one else -1], dtype=np.int64)
         object.__setattr__(self, "_native", numbers)
         object.__setattr__(self, "native", numbers.ctypes.data)
-        # as the binding reads it (Cache in csrc/cache8_binding.cpp); -1: no device
-        one = {t.device for t in self.tensors} == {k.device} and k.is_cuda
-        numbers = np.array([t.data_ptr() for t in self.tensors] + list(k.shape) + [self.code, k.device.index if one else -1], dtype=np.int64)
-        object.__setattr__(self, "_native", numbers)
-        object.__setattr__(self, "native", numbers.ctypes.data)
+
+    def __reduce__(self):                                          # (a copy has addresses of its own)
+        return Cache8, self.tensors
 
     @property
     def n_kv_heads(self) -> int:
@@ -113,10 +113,14 @@ _rows = {}
 
 
 def row_places(device, n: int) -> torch.Tensor:
-    """0 .. n - 1 (int32): the places of a step's rows in pages of one place. Older, shorter tensors are kept: a captured graph may hold their addresses."""
+    """0 .. n - 1 (int32): the places of a step's rows in pages of one place. Older, shorter tensors are kept: a captured graph may hold their addresses.
+    Not made while a graph is captured."""
     held = _rows.setdefault(device, [])
     if not held or held[-1].numel() < n:
-        held.append(torch.arange(max(n, 4096, 2 * held[-1].numel() if held else 0), dtype=torch.int32, device=device))
+        if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise ops.KernelError(f"row_places: {n} rows are more than before; run the step once before it is captured")
+        # (copied from the host, which waits: streams other than the current one may read it)
+        held.append(torch.arange(max(n, 4096, 2 * held[-1].numel() if held else 0), dtype=torch.int32).to(device))
     return held[-1][:n]
 
 
@@ -129,12 +133,6 @@ def store_cache8(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, cache
     the largest code (127, or 448). In any other block the scale grows to that where it is larger, and the codes that are there are rounded to it once
     more: half a step each time that it grows. Numbers that are not finite do not count for a: infinities become the largest code, NaN becomes 0.
     Places of a block that no row goes to keep their codes where the scale stays or begins anew. A cache has at most 2^31 - 1 places."""
-    bound = _bound or _binding()
-    if bound is not False and k.is_cuda:
-        done = bound.store(k, v, slot_map, cache.native)
-        if done is not None:
-            _done(done, 1)
-            return cache
     bound = _binding() if _bound is None and k.is_cuda else _bound
     if bound and k.is_cuda:
         done = bound.store(k, v, slot_map, cache.native)
@@ -159,11 +157,6 @@ def store_cache8(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, cache
 def expand_cache8(cache: Cache8, pages: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The numbers of `pages` (int32 [n]) as keys and values [n, n_kv_heads, page_size, head_dim] in float32 or bfloat16; zeros for a page number
     outside of the cache."""
-    bound = _bound or _binding()
-    if bound is not False and pages.is_cuda and dtype in ops._DT:
-        done = bound.expand(pages, cache.native, ops._DT[dtype])
-        if done is not None:
-            return _done(done, 1)
     bound = _binding() if _bound is None and pages.is_cuda else _bound
     if bound and pages.is_cuda and dtype in ops._DT:
         done = bound.expand(pages, cache.native, ops._DT[dtype])
@@ -171,16 +164,13 @@ def expand_cache8(cache: Cache8, pages: torch.Tensor, dtype: torch.dtype = torch
             return _done(done, 1)
     _here("expand_cache8", pages, *cache.tensors)
     _ints("expand_cache8", "pages", pages)
-    return _expand(cache, pages, None, pages.numel(), dtype)
-
-
-def _expand(cache: Cache8, table: torch.Tensor, index: Optional[torch.Tensor], n: int, dtype: torch.dtype):
-    """Page i of the result is page table[i], or table.flatten()[index[i]], of the cache."""
     if dtype not in ops._DT:
         raise ops.KernelError(f"expand_cache8: element type {dtype} is not supported (float32 and bfloat16 are)")
-    k, v = (torch.empty((n,) + cache.k.shape[1:], dtype=dtype, device=cache.k.device) for _ in range(2))
-    if n and k.numel():
-        ops._call("cache8", "hb_cache8_expand", *(t.data_ptr() for t in cache.tensors), cache.code, table.data_ptr(), ops._ptr(index), n, cache.k.shape[0],
+    k, v = (torch.empty((pages.numel(),) + cache.k.shape[1:], dtype=dtype, device=cache.k.device) for _ in range(2))
+    if k.numel() and not cache.k.numel():
+        return k.zero_(), v.zero_()
+    if k.numel():
+        ops._call("cache8", "hb_cache8_expand", *(t.data_ptr() for t in cache.tensors), cache.code, pages.data_ptr(), pages.numel(), cache.k.shape[0],
                   *cache.k.shape[1:], k.data_ptr(), v.data_ptr(), ops._DT[dtype], ops._stream())
     return k, v
 
@@ -191,12 +181,16 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     the step's own among them, are in `cache`. q [T, n_heads * head_dim] (bfloat16 or float32; rows may be part of wider ones), out [T, n_heads *
     head_dim] of its type; query head h reads kv head h // (n_heads / n_kv_heads). A row at position p sees the keys j <= p (and j > p - window,
     for a window above 0) whose pages are in the block table and in the cache; one that sees none is 0. scale: 1 / sqrt(head_dim) by default. Scores,
-    softmax and sums are 32-bit. Codes at places that a row of the step sees are numbers (e4m3 has a NaN; storing leaves none)."""
+    softmax and sums are 32-bit. Codes at places that a row of the step sees are numbers (e4m3 has a NaN; storing leaves none).
+
+    A graph that a call is captured into wants the batch, with its tensors, to live as long as itself. A step in which a request brings several rows is
+    laid out by the host at the batch's first call, from the lengths that the batch was built with: it has to have run once before it is captured, and is
+    replayed for those lengths; a step of one row a request follows positions and tables that are written over the batch's."""
     table, T, D = batch.block_tables[group], batch.n_rows, cache.head_dim
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     tensor_cores = q.is_cuda and _on_tensor_cores(cache)
     portions = tensor_cores and batch.max_q_len >= PORTION_ROWS[0]
-    if tensor_cores and not portions:
+    if tensor_cores and not portions and T:
         bound = _binding() if _bound is None else _bound
         if bound:
             cut = _cut(batch, cache, ops._dt(q), n_heads, window, 0)
@@ -221,18 +215,17 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     if not T:
         return out
     if not tensor_cores:
-        single = batch.max_q_len == 1 and T == batch.n_requests
         ops._call("cache8", "hb_cache8_attention_any", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
                   cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
-                  None if single else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
+                  None if _single_rows(batch) else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
                   out.data_ptr(), ops._stream())
         return out
     limit = _portion_limit(batch, cache, n_heads, window) if portions and _flash_takes(q, cache, out, n_heads, scale) else 0
-    others = not limit or min(batch.h_q_len) < limit
+    others = not limit or any(0 < n < limit for n in batch.h_q_len)
     if others:
         cut = _cut(batch, cache, dt, n_heads, window, limit)
         ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
-                  cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], None, batch.positions.data_ptr(),
+                  cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], batch.positions.data_ptr(),
                   ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), ops._stream())
     if limit:
         _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit, others)
@@ -277,7 +270,7 @@ def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
                 n, k = rows[flash], keys[flash]
                 padded = np.ceil(n / 128) * 128 * (k - n / 2)
                 us += 10 + k.sum() * cache.n_kv_heads * cache.head_dim * 6 / 4e6 + max(0.8e-6 * n_heads * padded.sum(), 1.7 / 128 * k.max())
-            if not flash.all():
+            if rows[~flash].any():
                 G, most = n_heads // cache.n_kv_heads, int(keys[~flash].max())
                 nt = min(4, -(-int(rows[~flash].max()) * G // 8))
                 tiles = int(np.ceil(rows[~flash] * G / (8 * nt)).sum()) * cache.n_kv_heads
@@ -314,8 +307,7 @@ def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, 
 def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: int):
     """For requests of `limit` rows or more: where in the block table the pages stand that their rows see (int32 [n]), the table of the n pages side
     by side (int32 [requests, width], -1: none), and at which of the n pages' blocks of 16 places each request's first key would stand (int32)."""
-    key = ("cache8 pages", page_size, width, window, limit)
-    if key not in batch.extra:
+    def pages():
         index, places, n = [], np.full((batch.n_requests, width), -1, dtype=np.int32), 0
         base, blocks = np.zeros(batch.n_requests, dtype=np.int32), cache8_blocks(page_size)
         for r, (held, rows) in enumerate(zip(batch.h_ctx_len, batch.h_q_len)):
@@ -326,10 +318,25 @@ def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: in
             places[r, first:end] = np.arange(n, n + end - first, dtype=np.int32)
             base[r] = (n - first) * blocks + _AHEAD
             n += end - first
-        batch.extra[key] = _to_device(np.concatenate(index + [places.ravel(), base]), batch)
-    both, R = batch.extra[key][0], batch.n_requests
+        return np.concatenate(index + [places.ravel(), base])
+
+    both, R = _on_stream(batch, ("cache8 pages", page_size, width, window, limit), lambda: _to_device(pages(), batch))[0], batch.n_requests
     n = both.numel() - R * (width + 1)
     return both[:n], both[n:n + R * width].view(R, width), both[n + R * width:]
+
+
+def _on_stream(batch, key, make):
+    """What `make` lays out on the device for the batch, kept with it: a stream has its own, since another one need not wait for it. A stream that is
+    being captured makes none (it would be there only when the graph is replayed) and takes what there is, which capturing begins behind."""
+    stream = ops._stream() if batch.tokens.is_cuda else None
+    kept = batch.extra.setdefault(key, {})
+    if stream not in kept:
+        if stream is not None and torch.cuda.is_current_stream_capturing():
+            if not kept:
+                raise ops.KernelError("attention_cache8: a step in which a request brings several rows has to have run once before it is captured")
+            return next(iter(kept.values()))
+        kept[stream] = make()
+    return kept[stream]
 
 
 def _to_device(numbers: np.ndarray, batch):
@@ -348,10 +355,10 @@ class _Cut:
         _heads(cache, n_heads, window)
         G = n_heads // cache.n_kv_heads
         some = [(r, a, c, n) for r, (a, c, n) in enumerate(zip(batch.h_q_start, batch.h_ctx_len, batch.h_q_len)) if n < limit or not limit]
-        most, last = max((n for *_, n in some), default=1), batch.max_pos if not limit else max(c + n - 1 for _, _, c, n in some)
+        most, last = max([1] + [n for *_, n in some]), batch.max_pos if not limit else max(c + n - 1 for _, _, c, n in some)
         self.nt = min(4, -(-most * G // 8))
         self.tiles, self.n_tiles, tiles = None, batch.n_rows, batch.n_rows * -(-G // (8 * self.nt))
-        if most > 1 or len(some) < batch.n_rows:
+        if not _single_rows(batch):
             counts = np.array([-(-n * G // (8 * self.nt)) for *_, n in some])
             numbers = np.empty((int(counts.sum()), 4), dtype=np.int32)
             for i, column in ((0, [r for r, *_ in some]), (1, [a for _, a, *_ in some]), (3, [n * G for *_, n in some])):
@@ -367,10 +374,17 @@ class _Cut:
 
 def _cut(batch, cache: Cache8, dt: int, n_heads: int, window: int, limit: int) -> _Cut:
     key = ("cache8 cut", cache.code, cache.k.shape[1:], dt, n_heads, window, limit)
-    cut = batch.extra.get(key)
-    if cut is None:
-        cut = batch.extra[key] = _Cut(batch, cache, dt, n_heads, window, limit)
-    return cut
+    if _single_rows(batch):                                        # (nothing of it is on the device)
+        cut = batch.extra.get(key)
+        if cut is None:
+            cut = batch.extra[key] = _Cut(batch, cache, dt, n_heads, window, limit)
+        return cut
+    return _on_stream(batch, key, lambda: _Cut(batch, cache, dt, n_heads, window, limit))
+
+
+def _single_rows(batch) -> bool:
+    """Whether row t is request t's, for all rows."""
+    return batch.max_q_len == 1 and batch.n_rows == batch.n_requests
 
 
 @functools.lru_cache(maxsize=None)

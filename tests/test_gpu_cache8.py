@@ -11,7 +11,7 @@ import torch
 
 import plain_cache8 as plain
 from hipinfer_b200.engine.batch import StepEntry, build_step_batch
-from hipinfer_b200.kernels import ops
+from hipinfer_b200.kernels import cache8, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -370,3 +370,138 @@ def test_rows_joined_over_every_number_of_blocks(group, held, monkeypatch):
         monkeypatch.setattr(cache8, "_ranks", lambda *a: ranks)
         batch.extra.clear()
         check(q, cache, batch, tables, 2 * group)
+
+
+# ------------------------------------------------------------------------------------------ calls that differ from an engine's
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [0, 50])
+def test_places_that_no_row_of_a_portion_sees_do_not_count(D, window):
+    """NaN codes and scales behind a portion's last token and, with a window, ahead of its first key."""
+    held, rows, ps = [70, 300, 0], [45, 1, 133], 16
+    batch, tables, pages = step(held, rows, ps)
+    cache = filled(pages, 2, ps, D, torch.float8_e4m3fn)
+    q = torch.randn(sum(rows), 8 * D, generator=torch.Generator().manual_seed(12)).to(torch.bfloat16)
+    clean = ops.attention_cache8(q.to(DEV), on_gpu(cache), batch, 0, 8, window)
+    seen = {(t[j // ps], j % ps) for t, h, n in zip(tables, held, rows) for j in range(max(0, h - window + 1) if window else 0, h + n)}
+    blocks = {p for p, i in seen}
+    for p in range(pages):
+        for i in range(ps):
+            if (p, i) not in seen:
+                cache[0].view(torch.uint8)[p, :, i] = 0x7f
+                cache[1].view(torch.uint8)[p, :, i] = 0xff
+        if p not in blocks:
+            cache[2][p, ::2], cache[3][p, ::2], cache[2][p, 1::2], cache[3][p, 1::2] = float("nan"), float("inf"), float("inf"), float("nan")
+    assert same(ops.attention_cache8(q.to(DEV), on_gpu(cache), batch, 0, 8, window), clean)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_portion_s_rows_with_infinities_and_nan_stay_alone(D):
+    batch, tables, pages = step([100, 20], [70, 1], 16)
+    q = torch.randn(71, 4 * D, generator=torch.Generator().manual_seed(13)).to(torch.bfloat16)
+    cache = on_gpu(filled(pages, 2, 16, D, torch.int8))
+    want = ops.attention_cache8(q.to(DEV), cache, batch, 0, 4)
+    q[3, 5], q[40, D + 1], q[70, 3 * D] = float("nan"), float("inf"), float("-inf")
+    got = ops.attention_cache8(q.to(DEV), cache, batch, 0, 4)
+    bad = torch.zeros(71, 4, dtype=torch.bool)
+    bad[3, 0] = bad[40, 1] = bad[70, 3] = True
+    assert torch.equal(got.view(71, 4, D).isnan().all(-1).cpu(), bad) and same(got.view(71, 4, D)[~bad.to(DEV)], want.view(71, 4, D)[~bad.to(DEV)])
+
+
+@pytest.mark.parametrize("rows", [[1, 0, 1], [0, 1, 1], [0, 0, 0], [0, 3, 0, 1], [0, 40, 1], [40, 0, 0], [17] + [0] * 16])
+@pytest.mark.parametrize("D", [64, 128, 72])
+def test_requests_without_a_row(rows, D):
+    held = [37 + 5 * i for i in range(len(rows))]
+    batch, tables, pages = step(held, rows, 16)
+    q = torch.randn(sum(rows), 8 * D, generator=torch.Generator().manual_seed(14)).to(torch.bfloat16)
+    cache = filled(pages, 2, 16, D, torch.int8)
+    if sum(rows):
+        check(q, cache, batch, tables, 8)
+    else:
+        assert ops.attention_cache8(q.to(DEV), on_gpu(cache), batch, 0, 8).shape == (0, 8 * D)
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1], [2, 1, 5], [1, 90, 3]])
+def test_a_batch_on_several_streams_at_once(rows):
+    batch, tables, pages = step([400, 21, 1300], rows, 16)
+    cache = on_gpu(filled(pages, 2, 16, 64, torch.int8))
+    q = torch.randn(sum(rows), 512, device=DEV).to(torch.bfloat16)
+    want = ops.attention_cache8(q, cache, step([400, 21, 1300], rows, 16)[0], 0, 8)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams:                                            # none waits for another
+        with torch.cuda.stream(s):
+            got += [ops.attention_cache8(q, cache, batch, 0, 8) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(same(x, want) for x in got)
+
+
+@pytest.mark.parametrize("rows", [[2, 1, 5], [1, 90, 3], [64, 64, 200]])
+def test_a_step_of_several_rows_is_captured_after_a_run(rows):
+    batch, tables, pages = step([400, 21, 1300], rows, 16)
+    cache = on_gpu(filled(pages, 2, 16, 64, torch.int8))
+    q = torch.randn(sum(rows), 512, device=DEV).to(torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="once before it is captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.attention_cache8(q, cache, batch, 0, 8)
+    ops.attention_cache8(q, cache, batch, 0, 8)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, ops.attention_cache8(q, cache, batch, 0, 8)))
+    fresh = torch.randn_like(q)
+    q.copy_(fresh)
+    want = ops.attention_cache8(fresh, cache, step([400, 21, 1300], rows, 16)[0], 0, 8)
+    for graph, out in graphs + graphs:
+        graph.replay()
+        assert same(out, want)
+        out.zero_()
+
+
+def test_a_copy_of_a_cache_has_its_own_memory():
+    import copy
+    cache = on_gpu(filled(5, 2, 16, 64, torch.int8))
+    other = copy.deepcopy(cache)
+    before = [t.clone() for t in cache.tensors]
+    x = torch.randn(1, 128, device=DEV)
+    ops.store_cache8(x, x, torch.tensor([16], dtype=torch.int32, device=DEV), other)
+    torch.cuda.synchronize()
+    assert all(same(a, b) for a, b in zip(cache.tensors, before)) and not same(other.k, cache.k)
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(copy.copy(cache).tensors, cache.tensors))
+
+
+def test_pages_of_an_empty_cache_are_zeros():
+    cache = on_gpu(filled(0, 2, 16, 64, torch.int8))
+    k, v = ops.expand_cache8(cache, torch.tensor([0, -1, 3], dtype=torch.int32, device=DEV))
+    assert k.shape == v.shape == (3, 2, 16, 64) and not k.any() and not v.any()
+
+
+def test_places_of_rows_are_not_made_while_a_graph_is_captured():
+    ops.row_places(DEV, 1)
+    n = max(t.numel() for t in cache8._rows[DEV]) + 1
+    with pytest.raises(ops.KernelError, match="before it is captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.row_places(DEV, n)
+    assert ops.row_places(DEV, n).tolist() == list(range(n))
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 33])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=ids)
+@pytest.mark.parametrize("codes", CODES, ids=ids)
+def test_blocks_with_numbers_that_are_not_finite_among_others(rows, dtype, codes):
+    """Infinities, NaN and the type's largest numbers in rows at odd places, over blocks that hold larger numbers already."""
+    heads, ps, D, pages = 2, 32, 128, 3
+    cache = filled(pages, heads, ps, D, codes)
+    g = torch.Generator().manual_seed(rows)
+    k, v = (torch.randn(rows, heads * D, generator=g).to(dtype) for _ in range(2))
+    for t, x in ((k, float("inf")), (v, float("-inf")), (k, float("nan")), (v, float("nan"))):
+        t.view(-1)[torch.randperm(t.numel(), generator=g)[:9]] = x
+    if rows > 16:
+        v[16, 3:9] = torch.finfo(dtype).max
+    slots = [(7 + i) % (pages * ps) for i in range(rows)]
+    got = on_gpu(cache)
+    ops.store_cache8(k.to(DEV), v.to(DEV), torch.tensor(slots, dtype=torch.int32, device=DEV), got)
+    for x, c, s, gc, gs in ((k, cache[0], cache[2], got.k, got.k_scale), (v, cache[1], cache[3], got.v, got.v_scale)):
+        wc, ws = plain.store(x, slots, c, s)
+        assert same(gs, ws) and same(gc, wc)
