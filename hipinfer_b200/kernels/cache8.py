@@ -208,6 +208,8 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
             or table.shape[1] * cache.page_size <= batch.max_pos:
         raise ops.KernelError(f"attention_cache8: block table {tuple(table.shape)} {table.dtype}; {batch.n_requests} requests of up to {batch.max_pos + 1} "
                               f"tokens in pages of {cache.page_size}")
+    for name in ("positions", "row_request"):
+        _ints("attention_cache8", name, getattr(batch, name), T)
     if out is None:
         out = torch.empty(T, n_heads * D, dtype=q.dtype, device=q.device)
     elif out.shape != (T, n_heads * D) or out.dtype != q.dtype or not out.is_contiguous():
@@ -235,7 +237,7 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
 def _heads(cache: Cache8, n_heads: int, window: int) -> None:
     if n_heads < 1 or n_heads % cache.n_kv_heads:
         raise ops.KernelError(f"attention_cache8: {n_heads} heads are not a multiple of {cache.n_kv_heads} kv heads")
-    if window < 0:
+    if not 0 <= window < 2 ** 31:
         raise ops.KernelError(f"attention_cache8: window {window}")
 
 

@@ -140,3 +140,40 @@ def test_a_run_of_the_plain_storing_is_what_its_words_say():
     codes, scales = plain.store(torch.tensor([[254.0, 3.0]]), [18], codes, scales)
     assert scales[1].tolist() == [[2.0]] and codes[1, 0, :3].tolist() == [[0, -64], [32, 1], [127, 2]]
     assert np.isfinite(plain.numbers(codes, scales)).all()
+
+
+@pytest.mark.parametrize("change", [dict(positions=torch.zeros(3, dtype=torch.int64)), dict(positions=torch.zeros(2, dtype=torch.int32)),
+                                    dict(row_request=torch.zeros(3, 1, dtype=torch.int32)), dict(positions=torch.zeros(6, dtype=torch.int32)[::2])])
+def test_attention_refuses_rows_places_of_another_form(calls, change):
+    cache, batch = ops.new_cache8(**CACHE), batch_of([5, 20], [1, 2])
+    for name, x in change.items():
+        setattr(batch, name, x)
+    with pytest.raises(ops.KernelError, match=next(iter(change))):
+        ops.attention_cache8(torch.zeros(3, 256), cache, batch, 0, 4)
+    assert not calls
+
+
+@pytest.mark.parametrize("window", [-1, 2 ** 31, 2 ** 32 + 5])
+def test_attention_refuses_windows_of_more_than_31_bits(calls, window):
+    with pytest.raises(ops.KernelError, match="window"):
+        ops.attention_cache8(torch.zeros(3, 256), ops.new_cache8(**CACHE), batch_of([5, 20], [1, 2]), 0, 4, window)
+    assert not calls
+
+
+def test_a_copy_of_a_cache_names_its_own_tensors():
+    import copy
+    import pickle
+
+    cache = ops.new_cache8(**CACHE)
+    for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert [int(x) for x in other._native[:4]] == [t.data_ptr() for t in other.tensors] and other.native != cache.native
+        assert all(a.data_ptr() != b.data_ptr() for a, b in zip(other.tensors, cache.tensors))
+
+
+@pytest.mark.parametrize("rows", [[0, 20, 1], [0, 0, 17, 300], [16]])
+def test_pages_of_portions_pass_requests_without_rows_over(rows):
+    batch = batch_of([40] * len(rows), rows)
+    index, places, base = cache8._pages_of_portions(batch, 16, batch.block_tables[0].shape[1], 0, 16)
+    assert index.numel() == sum(-(-(40 + n) // 16) for n in rows if n >= 16)
+    for r, n in enumerate(rows):
+        assert int((places[r] >= 0).sum()) == (-(-(40 + n) // 16) if n >= 16 else 0)
