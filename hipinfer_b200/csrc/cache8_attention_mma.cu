@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   // this warp's stages: U units each, the id-th and every (ranks * WARPS)th from there; a lane looks up one unit of 32, 32 units ahead
   const int s_lo = u_lo / U, first = s_lo + id;
   const int count = u_hi < first * U ? 0 : (u_hi / U - first) / stride + 1;
-  struct Units { int at; float k_scale, v_log2; };                      // V's scale as a power of two
+  struct Units { int at; float k_scale, v_scale; };
   const auto look = [&](int i) {                                        // stages i .. i + BATCH - 1
     Units x = {-1, 0.f, 0.f};
     const int unit = (first + (i + lane / U) * stride) * U + lane % U;
@@ -207,11 +207,13 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
       if (page >= 0 && page < a.n_pages) {
         x.at = (page * a.Hkv + h) * a.upp + unit % a.upp;
         x.k_scale = a.ks[x.at];
-        x.v_log2 = __log2f(fmaxf(a.vs[x.at], 1e-37f));                  // (a block that nothing was stored to: a scale of 0)
+        x.v_scale = a.vs[x.at];
       }
     }
     return x;
   };
+  // (V's scales as powers of two only where they are used: nothing waits for them ahead of the units' fetches; of a block that nothing was stored to: 0)
+  const auto v_power = [](float s) { return __log2f(fmaxf(s, 1e-37f)); };
   Units now = look(0), next = {-1, 0.f, 0.f};
   if (count > BATCH) next = look(BATCH);
   const auto fetch = [&](int i, int base, int slot) {                   // stage i, of the BATCH from `base` on or the next
@@ -503,11 +505,13 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
     }
   };
 
+  now.v_scale = v_power(now.v_scale);
 #pragma unroll 1
   for (int i = 0, base = 0, slot = 0, ahead = STAGES - 1; i < count; i++) {      // (not unrolled: three times the code was 12 % slower)
     if (i - base == BATCH) {
       base = i;
       now = next;
+      now.v_scale = v_power(now.v_scale);
       next = look(base + BATCH);
     }
     hb_cp_async_wait<STAGES - 2>();
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
     for (int u = 0; u < U; u++) {
       const int l = i % BATCH * U + u;
       at[u] = __shfl_sync(0xffffffffu, now.at, l);
-      fk[u] = __shfl_sync(0xffffffffu, now.k_scale, l), fv[u] = __shfl_sync(0xffffffffu, now.v_log2, l);
+      fk[u] = __shfl_sync(0xffffffffu, now.k_scale, l), fv[u] = __shfl_sync(0xffffffffu, now.v_scale, l);
     }
     compute(ring + slot * U * Z::UNIT, (first + i * stride) * U * C8_BLOCK, at, fk, fv);
     ahead = slot;
