@@ -351,7 +351,7 @@ def _to_device(numbers: np.ndarray, batch):
 
 class _Cut:
     """How the rows of requests of fewer than `limit` rows (0: of all) are cut into tiles of 8 nt (row, query head) pairs of a kv head, whose keys
-    `ranks` blocks share. tiles: int32 [n, 4] on the device, (request, its first row, first pair, pairs of its rows); None where row t is request t's."""
+    `ranks` blocks share. tiles: int32 [n, 4] on the device, (request, row and query head, of its kv head's, of the first pair, pairs); None where row t is request t's."""
 
     def __init__(self, batch, cache: Cache8, dt: int, n_heads: int, window: int, limit: int):
         _heads(cache, n_heads, window)
@@ -363,9 +363,10 @@ class _Cut:
         if not _single_rows(batch):
             counts = np.array([-(-n * G // (8 * self.nt)) for *_, n in some])
             numbers = np.empty((int(counts.sum()), 4), dtype=np.int32)
-            for i, column in ((0, [r for r, *_ in some]), (1, [a for _, a, *_ in some]), (3, [n * G for *_, n in some])):
-                numbers[:, i] = np.repeat(np.array(column, dtype=np.int64), counts)
-            numbers[:, 2] = (np.arange(len(numbers)) - np.repeat(np.cumsum(counts) - counts, counts)) * 8 * self.nt
+            request, row, pairs = (np.repeat(np.array(x, dtype=np.int64), counts) for x in ([r for r, *_ in some], [a for _, a, *_ in some], [n * G for *_, n in some]))
+            pair = (np.arange(len(numbers)) - np.repeat(np.cumsum(counts) - counts, counts)) * 8 * self.nt
+            for i, column in enumerate((request, row + pair // G, pair % G, np.minimum(8 * self.nt, pairs - pair))):
+                numbers[:, i] = column
             self.tiles, self._host = _to_device(numbers, batch)
             self.n_tiles = tiles = len(numbers)
         self.ranks = _ranks(tiles * cache.n_kv_heads, min(last + 1, window + most) if window else last + 1, functools.partial(_clusters, dt, cache.code, cache.head_dim, self.nt))
