@@ -7,12 +7,12 @@
 //
 // Scores are S^T = K Q^T and results O^T = V^T P^T, so that the 16 rows of an MMA are keys (or dimensions) and its 8 columns the pairs: eight
 // query heads fill it, where Q as the rows would leave half of it empty. The order of the dimensions within a product is free, and so K's
-// operand is what a thread has loaded: 16 bytes of key g and of key g + 8, four codes a step. V's needs two keys' codes of one dimension side by side:
+// operand is what ldmatrix gives of bytes: four codes of key g and of key g + 8 a register. V's needs two keys' codes of one dimension side by side:
 // bytes of four loads are interleaved.
 //
 // A warp's units come by cp.async through a ring of its own in shared memory, two or three units ahead, so that nothing waits for another warp and the
 // registers are left to the products: with the units ahead in registers (166 of them, 12 warps an SM) every second stall was for a result of the
-// warp's own, and 64 requests of 8,000 tokens (128) took 208 us. 16-byte pieces are exchanged within a unit so that the reads of a product's operand
+// warp's own, and 64 requests of 8,000 tokens (128) took 208 us, 165 now. 16-byte pieces are exchanged within a unit so that the reads of a product's operand
 // touch every bank once.
 //
 // Codes are integers (or e4m3 numbers) of at most 8 significant bits, exact in f16. The query of a pair is scaled by a power of two to below 2^10 and
@@ -23,6 +23,10 @@
 // rare. It is made times its unit's V scale over a reference, that of an earlier unit, which is exchanged (another pass) only where the two are more
 // than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing; a unit's sum is divided
 // by that ratio again. Scales, sums and accumulators are 32-bit.
+//
+// What bounds it: with many long requests the copy bandwidth (64 of 8,000 tokens, 8 kv heads of 128: 165 us, 6.4 TB/s, 97 % of a copy's; heads of 64 94 us,
+// 85 %, with half the issue slots used); with few the chain from the positions to the join (one of 700, heads of 64: 5.4 us; 8 of 2,000: 8.1);
+// with several rows a request the warps' own products and softmax (16 of 2,300 with 5 rows each, heads of 64: 17.9 us for 38 MB).
 #include "cache8.cuh"
 #include "tc_common.cuh"
 
@@ -48,6 +52,7 @@ struct C8Attend {
   float scale_log2;
   void* out;
   int q_aligned, out_aligned;
+  int beside;                  // the kernel behind this one is cache8_portions_kernel, which does not wait: it may start when this one has waited
 };
 
 // D += A B, f16 operands; D = A B without an addend.
@@ -166,7 +171,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   const auto cluster_wait = [] { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };
   if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   hb_pdl_wait();
-  hb_pdl_launch();                                                      // (behind the wait: see cache8_portions_kernel)
+  if (a.beside) hb_pdl_launch();
   int r, t0, head0, n;                                                  // n pairs, from head0 of row t0 on
   if (a.tiles) {
     const int4 t = a.tiles[a.first_tile + blockIdx.z];
@@ -545,6 +550,9 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   }
   hb_cp_async_wait<0>();
 
+  // What comes next may start on the SMs that are done and load its weights; sooner, its blocks are in this one's way: a decode step of 8 requests of 2,048
+  // tokens (16 layers, heads of 64) 0.84 to 0.88 ms, 0.92 with the launch ahead of the wait, 0.88 behind it.
+  if (!a.beside) hb_pdl_launch();
   // the warps' results, then the blocks'
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
@@ -702,7 +710,7 @@ HB_EXPORT int hb_cache8_attention_mma_clusters(int dt, int ct, int D, int nt, in
 HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const void* kc, const void* vc, const float* ks, const float* vs, int ct,
                                       long n_pages, int Hkv, int page_size, int D, const int* bt, long ld_table, int table_rows, int table_width,
                                       const int* pos, const int* tiles, int n_tiles, int nt, int ranks, int G, int window,
-                                      float scale, void* out, cudaStream_t st) {
+                                      float scale, void* out, int beside, cudaStream_t st) {
   if (n_tiles <= 0) return 0;
   if (!hb_cache8_attention_mma_supported(Hkv, page_size, D, n_pages) || G < 1 || G > 32767 || nt < 1 || nt > 4 || ranks < 1 || ranks > C8M_RANKS || (((uintptr_t)kc | (uintptr_t)vc) & 15))
     HB_FAIL("hb_cache8_attention_mma: %d kv heads of %d for %d heads each, pages of %d, %d ranks", Hkv, D, G, page_size, ranks);
@@ -710,7 +718,7 @@ HB_EXPORT int hb_cache8_attention_mma(const void* q, int dt, long ld_q, const vo
   const int upp = page_size / C8_BLOCK;
   C8Attend a = {q, ld_q, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, n_pages, Hkv, upp, upp & (upp - 1) ? -1 : __builtin_ctz(upp), bt, ld_table, table_rows,
                 table_width, pos, (const int4*)tiles, 0, (G + 8 * nt - 1) / (8 * nt), G, window, (uint32_t)(((1L << 32) + G - 1) / G), scale * 1.4426950408889634f, out,
-                !(((uintptr_t)q | ld_q * size) & (4 * size - 1)), !((uintptr_t)out & (4 * size - 1))};
+                !(((uintptr_t)q | ld_q * size) & (4 * size - 1)), !((uintptr_t)out & (4 * size - 1)), beside};
   const int count = tiles ? n_tiles : n_tiles * a.tiles_row;
   cudaError_t e = cudaErrorInvalidValue;
   C8_DISPATCH(ct, "hb_cache8_attention_mma", HB_DISPATCH_1(dt, "hb_cache8_attention_mma", {

@@ -22,7 +22,7 @@ struct Cut {
 typedef int (*StoreFn)(const void*, const void*, long, long, int, const int*, int, int, int, int, long, int, void*, void*, float*, float*, void*);
 typedef int (*ExpandFn)(const void*, const void*, const float*, const float*, int, const int*, long, long, int, int, int, void*, void*, int, void*);
 typedef int (*AttendFn)(const void*, int, long, const void*, const void*, const float*, const float*, int, long, int, int, int, const int*, long, int, int,
-                        const int*, const int*, int, int, int, int, int, float, void*, void*);
+                        const int*, const int*, int, int, int, int, int, float, void*, int, void*);
 typedef int (*CopyFn)(const long*, int, const int*, const int*, int, void*);
 StoreFn store_fn;
 ExpandFn expand_fn;
@@ -124,7 +124,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           (const float*)c->v_scale, (int)c->code, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim,
                           (const int*)table->const_data_ptr(), (long)table->size(1), (int)cut.requests, (int)table->size(1),
                           (const int*)pos->const_data_ptr(), tiles ? (const int*)tiles->const_data_ptr() : nullptr, (int)cut.n_tiles, (int)cut.nt,
-                          (int)cut.ranks, (int)cut.group, (int)cut.window, (float)scale, out.mutable_data_ptr(), stream());
+                          (int)cut.ranks, (int)cut.group, (int)cut.window, (float)scale, out.mutable_data_ptr(), 0, stream());
   if (r) return PyLong_FromLong(r);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

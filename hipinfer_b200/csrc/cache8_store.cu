@@ -10,6 +10,9 @@
 // it was, and where it grew the block's codes are rounded once more, to r(code * (old / new)); then the rows' codes, r(x * (1 / scale)),
 // overwrite theirs. Numbers that are not finite have no part in a; infinities become the largest code, NaN 0. All arithmetic is 32-bit,
 // each operation rounded by itself (no contraction), so that a block's bits are a matter of its rows and what it held alone.
+//
+// What bounds it: few rows, a chain of a few loads (one row, 8 heads of 128, 2.8 us; 64 rows of 64 requests 3.6); many, issue slots (6,000 rows of a prompt 10.9 us,
+// 5.6 by bandwidth, 58 % of the slots used). The maximum is taken of the numbers' bits, two of 16 bits at a time, and a block's rows stay in registers.
 constexpr int C8S_WARPS = 8, C8S_ROWS = 16, C8S_LOOK = 8;
 
 // E numbers side by side as they are in memory (16 bytes of them, or one), as floats, and as codes to memory.
@@ -229,7 +232,8 @@ HB_EXPORT int hb_cache8_store(const void* k, const void* v, long ld_k, long ld_v
 
 // Page i of the output [n][Hkv][page_size][D] is page table[i] of the cache; a number outside of the
 // cache's pages gives zeros. E codes at a time: 8 of them are a load of 8 bytes and a store of 16 (bf16) or two, so that a warp's stores are
-// whole lines; a page of one plane is a block's.
+// whole lines; a page of one plane is a block's, or a few blocks' where pages are few. Bound by
+// bandwidth where pages are many (4,000 pages of 8 heads of 128 66 us, 60 by a copy's; 380 8.2, of 5.7), else by one round of loads (64 pages 3.1 us).
 constexpr int C8E_AHEAD = 4;      // pieces that a thread asks for before it uses the first
 // CTAs that share `pieces` of 8 bytes: one piece a thread while there are few of them, all of them one CTA's when they are many (64 pages of 8 heads of
 // 128 3.1 us, with one CTA a page and plane 4.6; 4,000 pages 66 us either way). A thread's numbers of pieces end less than C8E_BEYOND behind the last.
@@ -318,7 +322,8 @@ HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, 
 // lies on either side, for tiles that reach over a request's ends, are ones.
 //
 // `beside`: the kernel ahead is cache8_attention_mma_kernel for a step's other rows, which lets this one start when it has itself waited for what came
-// before it: the cache is as this kernel wants it, and the two run side by side (a step of two portions and four single rows 7 us of 119). This
+// before it: the cache is as this kernel wants it, and the two run side by side (a step of two portions and four single rows 7 us of 119). Its 380 pages of 8 heads of
+// 128 take 8 us; with a page's work shared by blocks it took the single rows' blocks their place (104 us the step, 108). This
 // kernel still does not end before that one has.
 constexpr int C8_AHEAD = 32;
 template <typename CT>

@@ -26,7 +26,7 @@ ops._SIGS["cache8"] = {
     "hb_cache8_store": [_p, _p, _l, _l, _i, _p, _i, _i, _i, _i, _l, _i, _p, _p, _p, _p, _p],
     "hb_cache8_expand": [_p, _p, _p, _p, _i, _p, _l, _l, _i, _i, _i, _p, _p, _i, _p],
     "hb_cache8_attention_any": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _f, _p, _p],
-    "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p, _p],
+    "hb_cache8_attention_mma": [_p, _i, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _l, _i, _i, _p, _p, _i, _i, _i, _i, _i, _f, _p, _i, _p],
     "hb_cache8_attention_mma_supported": [_i, _i, _i, _l],
     "hb_cache8_attention_mma_clusters": [_i, _i, _i, _i, _i],
     "hb_cache8_portions": [_p, _p, _p, _p, _i, _p, _p, _l, _l, _i, _i, _i, _f, _p, _p, _p, _i, _p],
@@ -228,7 +228,7 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
         cut = _cut(batch, cache, dt, n_heads, window, limit)
         ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
                   cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], batch.positions.data_ptr(),
-                  ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), ops._stream())
+                  ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), bool(limit), ops._stream())
     if limit:
         _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit, others)
     return out
@@ -256,8 +256,8 @@ def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
     """From how many rows on a request's pages are expanded for the flash kernel (one of PORTION_ROWS; 0: none are). Per (row, head) and key the
     flash kernel takes a third of the warp MMAs' time, but works in tiles of 128 rows, walks a tile's keys one after the other and wants the keys
     expanded; the choice is the least of the step's estimated times. Both as measured, us: 32 heads over 8 of 128, one portion of 64 rows behind 500
-    tokens 19 on warp MMAs and 17 with the flash kernel, behind 8,000 59 and 111; 256 rows behind 2,000 63 and 38, behind 24,000 533 and 346; heads of 64: 15 and
-    18, 51 and 126; 54 and 43, 485 and 439."""
+    tokens 12.8 on warp MMAs and 15.5 with the flash kernel, behind 8,000 46.8 and 101; 256 rows behind 2,000 49.7 and 35.8, behind 24,000 474 and 290;
+    heads of 64: 11.3 and 18.7, 33.0 and 122; 42.4 and 41.5, 329 and 343. The estimates are off by a sixth at most where the times are not alike."""
     key = ("cache8 limit", n_heads, cache.n_kv_heads, cache.head_dim, cache.code, window)
     if key not in batch.extra:
         rows, held = np.array(batch.h_q_len, dtype=np.float64), np.array(batch.h_ctx_len, dtype=np.float64)
@@ -267,18 +267,20 @@ def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
             flash = rows >= limit if limit else rows < 0
             if limit and not flash.any():
                 continue
-            us = 0.0
+            us, wide = 0.0, cache.head_dim == 128
             if flash.any():
                 n, k = rows[flash], keys[flash]
-                padded = np.ceil(n / 128) * 128 * (k - n / 2)
-                us += 10 + k.sum() * cache.n_kv_heads * cache.head_dim * 6 / 4e6 + max(0.8e-6 * n_heads * padded.sum(), 1.7 / 128 * k.max())
+                padded = np.ceil(n / 128) * 128 * (k - n / 2)                 # (row, key) pairs of whole tiles; or one tile's keys in their order
+                us += 8 + k.sum() * cache.n_kv_heads * cache.head_dim * 6 / 5.5e6 + max((0.8e-6 if wide else 0.45e-6) * n_heads * padded.sum(),
+                                                                                   (1.35 if wide else 1.72) / 128 * k.max())
             if rows[~flash].any():
-                G, most = n_heads // cache.n_kv_heads, int(keys[~flash].max())
-                nt = min(4, -(-int(rows[~flash].max()) * G // 8))
-                tiles = int(np.ceil(rows[~flash] * G / (8 * nt)).sum()) * cache.n_kv_heads
-                clusters = functools.partial(_clusters, 1, cache.code, cache.head_dim, nt)
-                ranks = _ranks(tiles, most, clusters)
-                us += 12 + max(1.0, tiles / clusters(ranks)) * most / ranks * (0.007 + 0.004 * nt)
+                n, k = rows[~flash], keys[~flash]
+                G, most = n_heads // cache.n_kv_heads, int(k.max())
+                nt = min(4, -(-int(n.max()) * G // 8))
+                tiles = np.ceil(n * G / (8 * nt)) * cache.n_kv_heads
+                ranks = _ranks(int(tiles.sum()), most, functools.partial(_clusters, 1, cache.code, cache.head_dim, nt))
+                one = 0.0027 + 0.0021 * nt if wide else 0.0016 + 0.0014 * nt  # a key of a tile on a full SM; by itself a block takes 1.7 times as long
+                us += 6.5 + max((tiles * (k - n / 2)).sum() / 148 * one, most / ranks * 1.7 * one, k.sum() * cache.n_kv_heads * cache.head_dim * 2 / 6e6)
             if best is None or us < best[0]:
                 best = us, limit
         batch.extra[key] = best[1]
@@ -402,10 +404,10 @@ def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
 def _ranks(tiles: int, keys: int, clusters) -> int:
     """Blocks (1 to 16, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 128 keys each while
     there are at most two on an SM, else 400, or 512 in clusters of 3, 5, 6 and 7, which fill the GPU less evenly; more than 8 where they have an SM each
-    and 512 keys. Measured, us: 4 requests of 2,000 tokens (8 kv heads of 64) 8.8 with 4, 8.2 with 8; 8 of 2,000 9.6 and 10.5; 16 of 2,000 13.1 with 2,
-    14.3 with 3, 13.0 with 4, of 8,000 34.7 with 2 and 28.7 with 4; one of 24,000 22 with 8, 16 with 16. Lengths differ, and a wave of blocks ends with
-    its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand tokens, heads of 128: 145 as one wave of one block
-    a tile, 137 and 135 as two and four; of 2,000 each 48, 51 and 58)."""
+    and 512 keys. Measured, us: 4 requests of 2,000 tokens (8 kv heads of 64) 7.1 with 4, 6.4 with 8; 8 of 2,000 8.0 and 8.2; 16 of 2,000 11.4 with 2,
+    10.9 with 4, 15.0 with 8, of 8,000 32.0 with 2 and 27.5 with 4; one of 8,000 9.6 with 8, 8.4 with 15. Lengths differ, and a wave of blocks ends with
+    its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand tokens, heads of 128: 146 as one wave of one block
+    a tile, 134 as two; of 8,000 each 173 and 162; of 2,000 each 46 and 48)."""
     def fits(r):
         least = 512 if r > 8 else 128 if tiles * r <= 2 * 148 else 400 if r in (2, 4, 8) else 512
         return keys >= least * r and (r <= 8 or tiles * r <= 148) and clusters(r) >= tiles
