@@ -146,7 +146,9 @@ template <typename CT, typename T, int D, int NT> struct C8Sizes {
   static constexpr bool Q_INT = sizeof(T) == 2 && CT::MOST == C8Int8::MOST;                       // the query in int8 parts
   static constexpr int PARTS = sizeof(T) == 4 || Q_INT ? 2 : 1, W_PARTS = sizeof(T) == 4 ? 2 : 1;  // of the query, of the weights
   static constexpr int STEPS = D / 16, Q_STEPS = Q_INT ? D / 32 : D / 16;
-  static constexpr int U = D == 128 ? 1 : 2, STAGES = 3;                                          // units of a stage (4 KB), stages of a ring
+  // units of a stage, stages of a ring. 4 KB a stage; one unit of 2 KB at 32 pairs, whose registers two do not fit in (16 requests of 2,300 tokens with 8 rows
+  // each, heads of 64: 23.7 us with two, 22.8 with one; at 24 pairs 17.9 and 17.7, and 64 such requests with 5 rows 58 and 64)
+  static constexpr int U = D == 128 || NT == 4 ? 1 : 2, STAGES = 3;
   static constexpr bool Q_REGS = NT == 1 && (Q_INT || PARTS == 1);
   static constexpr int QUERY = Q_REGS ? 0 : PARTS * NT * Q_STEPS * 32 * 8, UNIT = 2 * C8_BLOCK * D, RING = C8M_WARPS * STAGES * U * UNIT;
   static constexpr int PITCH = D + 4, JOINED = C8M_WARPS * 8 * NT * PITCH * 4;
