@@ -21,7 +21,7 @@
 // exact in integers; the keys' conversion was a sixth of all instructions. A weight is 2^(score - sub), where sub lies 2 (in base 2) below
 // a score that was the largest once and is raised only when a weight passes 2^10, so that raising it, which costs a pass over the accumulators, is
 // rare. It is made times its unit's V scale over a reference, that of an earlier unit, which is exchanged (another pass) only where the two are more
-// than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing; a unit's sum is divided
+// than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing that counts; a unit's sum is divided
 // by that ratio again. Scales, sums and accumulators are 32-bit.
 //
 // What bounds it: with many long requests the copy bandwidth (64 of 8,000 tokens, 8 kv heads of 128: 165 us, 6.4 TB/s, 97 % of a copy's; heads of 64 94 us,
@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
   }
 
   float o[STEPS][NT][4], sub[NT][2], most[NT][2], l[NT][2];             // most: the largest exponent of a weight, 10; -inf while there is no score yet
+  float v_top = -INFINITY;                                              // the largest of V's scales so far
   float v_ref = 0.f;                                                    // V's reference scale, which o is to be multiplied with, as a power of two
   bool none = true;                                                     // no unit yet
 #pragma unroll
@@ -459,7 +460,11 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
 #pragma unroll
     for (int u = 0; u < U; u++) {
       if (at[u] < 0) continue;
-      float ratio = v_log2[u] - v_ref;                                  // of V's scale to the reference
+      // A scale of less than 2^-60 of the largest counts as that: what it multiplies is then off by 2^-53 of the largest value at most, and o, which is
+      // divided by the reference, stays below 2^100 (blocks of zeros have a scale of 1e-30 / M, those that nothing was stored to 0).
+      const float v_now = fmaxf(v_log2[u], v_top - 60.f);
+      v_top = fmaxf(v_top, v_now);
+      float ratio = v_now - v_ref;                                       // of V's scale to the reference
       if (none || !(fabsf(ratio) <= 5.f)) {
         const float f = none ? 0.f : hb_exp2(-ratio);
 #pragma unroll
@@ -468,7 +473,7 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
           for (int i = 0; i < STEPS; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++) o[i][nt][c] *= f;
-        v_ref = v_log2[u];
+        v_ref = v_now;
         none = false;
         ratio = 0.f;
       }

@@ -378,8 +378,7 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
   if (beside) hb_pdl_wait();
 }
 
-// scale: 4 floats x Hkv x hb_cache8_portions_scales(n, page_size), 16-byte aligned as k and v are; kc, vc 8-byte aligned; D a multiple of 8.
-HB_EXPORT long hb_cache8_portions_scales(long n, int page_size) { return n * c8_blocks(page_size) + 2 * C8_AHEAD; }
+// scale: 4 floats x Hkv x (n * blocks of a page + 2 C8_AHEAD), 16-byte aligned as k and v are; kc, vc 8-byte aligned; D a multiple of 8.
 HB_EXPORT int hb_cache8_portions(const void* kc, const void* vc, const float* ks, const float* vs, int ct, const int* table, const int* index, long n,
                                  long n_pages, int Hkv, int page_size, int D, float scale, void* k, void* v, void* scales, int beside,
                                  cudaStream_t st) {

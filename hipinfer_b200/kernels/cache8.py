@@ -43,7 +43,8 @@ def cache8_blocks(page_size: int) -> int:
 
 @dataclass(frozen=True, eq=False)
 class Cache8:
-    """A layer's cache in 8 bits: codes k, v [pages, n_kv_heads, page_size, head_dim], scales k_scale, v_scale [pages, n_kv_heads, blocks]."""
+    """A layer's cache in 8 bits: codes k, v [pages, n_kv_heads, page_size, head_dim], scales k_scale, v_scale [pages, n_kv_heads, blocks], none of them
+    negative."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -189,7 +190,7 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     table, T, D = batch.block_tables[group], batch.n_rows, cache.head_dim
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     tensor_cores = q.is_cuda and _on_tensor_cores(cache)
-    portions = tensor_cores and batch.max_q_len >= PORTION_ROWS[0]
+    portions = tensor_cores and batch.max_q_len >= PORTION_ROWS[0] and cache.k.shape[0] > 0
     if tensor_cores and not portions and T:
         bound = _binding() if _bound is None else _bound
         if bound:

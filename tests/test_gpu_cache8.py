@@ -505,3 +505,28 @@ def test_blocks_with_numbers_that_are_not_finite_among_others(rows, dtype, codes
     for x, c, s, gc, gs in ((k, cache[0], cache[2], got.k, got.k_scale), (v, cache[1], cache[3], got.v, got.v_scale)):
         wc, ws = plain.store(x, slots, c, s)
         assert same(gs, ws) and same(gc, wc)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [3, 1], [40, 1], [600, 1]])
+@pytest.mark.parametrize("D", [64, 128, 80])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=ids)
+def test_blocks_of_zeros_among_others(rows, D, dtype):
+    """Values of all-zero blocks as storing leaves them (scale 1e-30 / M), blocks that nothing was stored to (scale 0), and tiny ones, in turn."""
+    batch, tables, pages = step([900, 333], rows, 16)
+    k, v, ks, vs = filled(pages, 2, 16, D, torch.int8)
+    for at, scale in ((0, 1e-30 / 127), (2, 0.0), (3, 1e-20), (5, 1e-12)):
+        vs[at::7] = scale
+    v[0::7] = v[2::7] = 0
+    q = torch.randn(sum(rows), 8 * D, generator=torch.Generator().manual_seed(15)).to(dtype)
+    check(q, (k, v, ks, vs), batch, tables, 8)
+    vs *= 1e-9
+    check(q, (k, v, ks, vs), batch, tables, 8)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [3, 1], [40, 1]])
+@pytest.mark.parametrize("D", [64, 80])
+def test_an_empty_cache_gives_zeros(rows, D):
+    batch, _, _ = step([900, 333], rows, 16)
+    q = torch.randn(sum(rows), 8 * D, device=DEV).to(torch.bfloat16)
+    out = torch.ones_like(q)
+    assert not ops.attention_cache8(q, on_gpu(filled(0, 2, 16, D, torch.int8)), batch, 0, 8, out=out).any()
