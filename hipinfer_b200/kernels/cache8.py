@@ -263,13 +263,15 @@ def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
     if key not in batch.extra:
         rows, held = np.array(batch.h_q_len, dtype=np.float64), np.array(batch.h_ctx_len, dtype=np.float64)
         keys = np.minimum(held, window) + rows if window else held + rows
-        best = None
+        best, before = None, 0
         for limit in PORTION_ROWS + (0,):
             flash = rows >= limit if limit else rows < 0
-            if limit and not flash.any():
+            count = np.count_nonzero(flash)
+            if limit and count in (0, before):                                # none, or the same as with the limit before
                 continue
+            before = count
             us, wide = 0.0, cache.head_dim == 128
-            if flash.any():
+            if count:
                 n, k = rows[flash], keys[flash]
                 padded = np.ceil(n / 128) * 128 * (k - n / 2)                 # (row, key) pairs of whole tiles; or one tile's keys in their order
                 us += 8 + k.sum() * cache.n_kv_heads * cache.head_dim * 6 / 5.5e6 + max((0.8e-6 if wide else 0.45e-6) * n_heads * padded.sum(),
