@@ -281,7 +281,7 @@ def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
                 G, most = n_heads // cache.n_kv_heads, int(k.max())
                 nt = min(4, -(-int(n.max()) * G // 8))
                 tiles = np.ceil(n * G / (8 * nt)) * cache.n_kv_heads
-                ranks = _ranks(int(tiles.sum()), most, functools.partial(_clusters, 1, cache.code, cache.head_dim, nt))
+                ranks = _ranks(int(tiles.sum()), most, float(k.mean()), functools.partial(_clusters, 1, cache.code, cache.head_dim, nt))
                 one = 0.0027 + 0.0021 * nt if wide else 0.0016 + 0.0014 * nt  # a key of a tile on a full SM; by itself a block takes 1.7 times as long
                 us += 6.5 + max((tiles * (k - n / 2)).sum() / 148 * one, most / ranks * 1.7 * one, k.sum() * cache.n_kv_heads * cache.head_dim * 2 / 6e6)
             if best is None or us < best[0]:
@@ -374,7 +374,9 @@ class _Cut:
                 numbers[:, i] = column
             self.tiles, self._host = _to_device(numbers, batch)
             self.n_tiles = tiles = len(numbers)
-        self.ranks = _ranks(tiles * cache.n_kv_heads, min(last + 1, window + most) if window else last + 1, functools.partial(_clusters, dt, cache.code, cache.head_dim, self.nt))
+        seen = min(last + 1, window + most) if window else last + 1
+        mean = sum(min(c + n, seen) for _, _, c, n in some) / max(1, len(some))
+        self.ranks = _ranks(tiles * cache.n_kv_heads, seen, mean, functools.partial(_clusters, dt, cache.code, cache.head_dim, self.nt))
         # as the binding reads it (Cut in csrc/cache8_binding.cpp)
         self._native = np.array([batch.n_rows, batch.n_requests, self.n_tiles, self.nt, self.ranks, G, window, batch.max_pos], dtype=np.int64)
         self.native = self._native.ctypes.data
@@ -404,19 +406,27 @@ def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
     return n
 
 
-def _ranks(tiles: int, keys: int, clusters) -> int:
-    """Blocks (1 to 16, a cluster) that share a tile's keys: as many as are on the GPU at once (`clusters`: of so many blocks), with 128 keys each while
-    there are at most two on an SM, else 400, or 512 in clusters of 3, 5, 6 and 7, which fill the GPU less evenly; more than 8 where they have an SM each
-    and 512 keys. Measured, us: 4 requests of 2,000 tokens (8 kv heads of 64) 7.1 with 4, 6.4 with 8; 8 of 2,000 8.0 and 8.2; 16 of 2,000 11.4 with 2,
-    10.9 with 4, 15.0 with 8, of 8,000 32.0 with 2 and 27.5 with 4; one of 8,000 9.6 with 8, 8.4 with 15. Lengths differ, and a wave of blocks ends with
-    its longest: where a block still has 2,048 keys, up to four waves (64 requests of 4 to 8 thousand tokens, heads of 128: 146 as one wave of one block
-    a tile, 134 as two; of 8,000 each 173 and 162; of 2,000 each 46 and 48)."""
+def _ranks(tiles: int, keys: int, mean: float, clusters) -> int:
+    """Blocks (1 to 16, a cluster) that share a tile's keys (`keys` the longest's, `mean` of all): as many as are on the GPU at once (`clusters`: of so
+    many blocks), with 64 keys each while there is one on an SM, or two and clusters of 2, 4 and 8; else 270, or 512 in clusters of 3, 5, 6 and 7, which fill the
+    GPU less evenly; more than 8 where they have an SM each, 16 with 128 keys each, 9 to 15 with 512. Measured, us: one request of 700 tokens (8 kv heads of 64)
+    5.9 with 2, 5.1 with 4, 4.6 with 8, of 2,000 5.4 with 8, 5.0 with 16, of 8,000 9.6 and 8.2; 5 of 900 5.6 with 4, 6.3 with 7; 4 of 2,000 7.1 with 4, 6.4 with 8; 8 of
+    2,000 8.0 and 8.2; 16 of 1,500 11.0 with 2, 9.7 with 4, 14.3 with 8; 32 of 500 7.4 with 1 and 8.2 with 2, of 700 10.1 and 9.6; 24 of 1,300 12.2 with 2 and 15.0
+    with 3. Where lengths differ a wave of blocks ends with its longest: while a block still has 2,048 keys of a
+    tile, or 1,450 of lengths that differ much, up to four waves (heads of 128: 64 requests of 8,000 tokens 173 as one wave of one block a tile, 162 as two, 167
+    with four blocks; 64 of 4 to 8 thousand 140, 137 and 133; 48 of 3 to 6 thousand 79, 82 and 76; 96 of 2 to 4 thousand 111 and 102; 64 of 2,000 46 and 48)."""
     def fits(r):
-        least = 512 if r > 8 else 128 if tiles * r <= 2 * 148 else 400 if r in (2, 4, 8) else 512
+        even = r in (2, 4, 8)
+        if r > 8:
+            least = 128 if r == 16 else 512
+        elif tiles * r <= (2 * 148 if even else 148):
+            least = 64
+        else:
+            least = 270 if even else 512
         return keys >= least * r and (r <= 8 or tiles * r <= 148) and clusters(r) >= tiles
 
     ranks = next((r for r in range(16, 1, -1) if fits(r)), 1)
-    while 2 * ranks <= 8 and tiles <= 4 * clusters(2 * ranks) and keys >= 4096 * ranks:
+    while 2 * ranks <= 8 and tiles <= 4 * clusters(2 * ranks) and keys >= (4096 if mean > 0.85 * keys else 2900) * ranks:
         ranks *= 2
     return ranks
 
