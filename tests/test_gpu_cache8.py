@@ -530,3 +530,32 @@ def test_an_empty_cache_gives_zeros(rows, D):
     q = torch.randn(sum(rows), 8 * D, device=DEV).to(torch.bfloat16)
     out = torch.ones_like(q)
     assert not ops.attention_cache8(q, on_gpu(filled(0, 2, 16, D, torch.int8)), batch, 0, 8, out=out).any()
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [5, 2], [300, 1]])
+@pytest.mark.parametrize("D, ps", [(128, 16), (96, 16)])
+def test_pages_beyond_32_bits_of_bytes(rows, D, ps):
+    """The same pages at the end of a cache whose codes take more than 2^32 bytes: the same bits."""
+    heads, dtype = 8, torch.int8
+    batch, tables, pages = step([200, 41], rows, ps)
+    small = on_gpu(filled(pages, heads, ps, D, dtype))
+    n = 2 ** 32 // (heads * ps * D) + pages + 3
+    big = ops.new_cache8(n, heads, ps, D, dtype, DEV)
+    for a, b in zip(big.tensors, small.tensors):
+        a[n - pages:].copy_(b)
+    q = torch.randn(sum(rows), 32 * D, device=DEV).to(torch.bfloat16)
+    want = ops.attention_cache8(q, small, batch, 0, 32)
+    x = torch.randn(7, heads * D, device=DEV).to(torch.bfloat16)
+    slots = torch.arange(3 * ps + 11, 3 * ps + 18, dtype=torch.int32, device=DEV) % (pages * ps)
+    ops.store_cache8(x, x, slots, small)
+    after = ops.attention_cache8(q, small, batch, 0, 32)
+    high = step([200, 41], rows, ps)[0]
+    high.block_tables[0] += (high.block_tables[0] >= 0) * (n - pages)
+    assert same(ops.attention_cache8(q, big, high, 0, 32), want)
+    ops.store_cache8(x, x, slots + (n - pages) * ps, big)
+    assert same(ops.attention_cache8(q, big, high, 0, 32), after)
+    which = torch.arange(pages, dtype=torch.int32, device=DEV)
+    for a, b in zip(ops.expand_cache8(big, which + (n - pages)), ops.expand_cache8(small, which)):
+        assert same(a, b)
+    ops.copy_pages([t[None] for t in big.tensors], list(range(n - pages, n)), list(range(1, pages + 1)))
+    assert all(same(a[1:pages + 1], b) for a, b in zip(big.tensors, small.tensors))
