@@ -1,6 +1,6 @@
 // The operators of a cache in 8 bits, and copying pages, for arguments that are as they should be: checks, allocations and the library's calls
 // without the interpreter (kernels/cache8.py calls these first; where they answer None, its own checks say what is wrong). A decode step's calls
-// are bounded by their host time: the attention's is 17 us through the interpreter, copying 500 pages 200.
+// are bounded by their host time: the attention's is 4 us, 17 through the interpreter, 20 and 60 with portions; copying 500 pages took 200.
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -19,14 +19,25 @@ struct Cache {
 struct Cut {
   int64_t rows, requests, n_tiles, nt, ranks, group, window, max_pos;
 };
+// And how a step's portions go through the flash kernel: their pages (`pages` of the block table's places, of `scales` blocks), the portions' lengths, on the
+// device, and the kernel's status word.
+struct Portions {
+  int64_t rows, requests, width, pages, scales, limit, max_q_len, group, window, max_pos, index, places, base, q_start, q_len, ctx_len, status;
+};
 typedef int (*StoreFn)(const void*, const void*, long, long, int, const int*, int, int, int, int, long, int, void*, void*, float*, float*, void*);
 typedef int (*ExpandFn)(const void*, const void*, const float*, const float*, int, const int*, long, long, int, int, int, void*, void*, int, void*);
 typedef int (*AttendFn)(const void*, int, long, const void*, const void*, const float*, const float*, int, long, int, int, int, const int*, long, int, int,
                         const int*, const int*, int, int, int, int, int, float, void*, int, void*);
+typedef int (*PortionsFn)(const void*, const void*, const float*, const float*, int, const int*, const int*, long, long, int, int, int, float, void*, void*,
+                          void*, int, void*);
+typedef int (*FlashFn)(const void*, const void*, const void*, long, const int*, int, const int*, const int*, const int*, void*, int, int, int, int, int, int, int,
+                       int, int, int*, const void*, const int*, long, void*);
 typedef int (*CopyFn)(const long*, int, const int*, const int*, int, void*);
 StoreFn store_fn;
 ExpandFn expand_fn;
 AttendFn attend_fn;
+PortionsFn portions_fn;
+FlashFn flash_fn;
 CopyFn copy_fn;
 
 const at::Tensor* tensor(PyObject* x, int64_t device) {          // a strided one on that GPU
@@ -46,11 +57,13 @@ at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& li
 }
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 4) return PyErr_Format(PyExc_TypeError, "four addresses are expected");
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "six addresses are expected");
   store_fn = (StoreFn)PyLong_AsVoidPtr(a[0]);
   expand_fn = (ExpandFn)PyLong_AsVoidPtr(a[1]);
   attend_fn = (AttendFn)PyLong_AsVoidPtr(a[2]);
   copy_fn = (CopyFn)PyLong_AsVoidPtr(a[3]);
+  portions_fn = (PortionsFn)PyLong_AsVoidPtr(a[4]);
+  flash_fn = (FlashFn)PyLong_AsVoidPtr(a[5]);
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -95,13 +108,17 @@ PyObject* expand(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, address of a Cache, block table, positions, tiles or None, address of a Cut, scale, out or None): the output; or as above
+// (q, address of a Cache, block table, positions, tiles or None, address of a Cut, scale, out or None, address of Portions or 0): the output; or as above.
+// With portions the Cut is of the other rows, 0 where there are none; a code below 0 is one of the flash kernel's.
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 8) return PyErr_Format(PyExc_TypeError, "eight arguments are expected");
+  if (n != 9) return PyErr_Format(PyExc_TypeError, "nine arguments are expected");
   const Cache* c = cache(a[1]);
   if (!c) Py_RETURN_NONE;
-  const Cut& cut = *(const Cut*)PyLong_AsVoidPtr(a[5]);
+  const Portions* flash = (const Portions*)PyLong_AsVoidPtr(a[8]);
+  const Cut* others = (const Cut*)PyLong_AsVoidPtr(a[5]);
+  if (!flash && !others) Py_RETURN_NONE;
+  const Cut cut = others ? *others : Cut{flash->rows, flash->requests, 0, 1, 1, flash->group, flash->window, flash->max_pos};
   const at::Tensor *q = tensor(a[0], c->device), *table = tensor(a[2], c->device), *pos = tensor(a[3], c->device);
   const at::Tensor* tiles = a[4] == Py_None ? nullptr : tensor(a[4], c->device);
   const int64_t width = c->kv_heads * cut.group * c->head_dim;
@@ -110,6 +127,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       table->size(1) * c->page_size <= cut.max_pos || !ints(*pos, 1) || pos->size(0) != cut.rows ||
       (tiles && (!ints(*tiles, 2) || tiles->size(0) != cut.n_tiles || tiles->size(1) != 4)))
     Py_RETURN_NONE;
+  if (flash && (!q->is_contiguous() || q->scalar_type() != at::kBFloat16 || ((uintptr_t)q->const_data_ptr() & 15) || table->size(1) != flash->width)) Py_RETURN_NONE;
   const double scale = PyFloat_AsDouble(a[6]);
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   at::Tensor out;
@@ -119,12 +137,27 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* given = tensor(a[7], c->device);
     if (!given || given->sizes() != q->sizes() || given->scalar_type() != q->scalar_type() || !given->is_contiguous()) Py_RETURN_NONE;
     out = *given;
+    if (flash && ((uintptr_t)out.const_data_ptr() & 15)) Py_RETURN_NONE;
   }
-  const int r = attend_fn(q->const_data_ptr(), type_code(*q), (long)q->stride(0), (const void*)c->k, (const void*)c->v, (const float*)c->k_scale,
+  int r = !others ? 0 : attend_fn(q->const_data_ptr(), type_code(*q), (long)q->stride(0), (const void*)c->k, (const void*)c->v, (const float*)c->k_scale,
                           (const float*)c->v_scale, (int)c->code, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim,
                           (const int*)table->const_data_ptr(), (long)table->size(1), (int)cut.requests, (int)table->size(1),
                           (const int*)pos->const_data_ptr(), tiles ? (const int*)tiles->const_data_ptr() : nullptr, (int)cut.n_tiles, (int)cut.nt,
-                          (int)cut.ranks, (int)cut.group, (int)cut.window, (float)scale, out.mutable_data_ptr(), 0, stream());
+                          (int)cut.ranks, (int)cut.group, (int)cut.window, (float)scale, out.mutable_data_ptr(), flash ? 1 : 0, stream());
+  if (!r && flash) {
+    at::Tensor k = empty({flash->pages, c->kv_heads, c->page_size, c->head_dim}, at::kBFloat16, *q), v = empty(k.sizes(), at::kBFloat16, *q);
+    at::Tensor scales = empty({c->kv_heads, flash->scales, 4}, at::kFloat, *q);
+    r = portions_fn((const void*)c->k, (const void*)c->v, (const float*)c->k_scale, (const float*)c->v_scale, (int)c->code, (const int*)table->const_data_ptr(),
+                    (const int*)flash->index, (long)flash->pages, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim, (float)scale,
+                    k.mutable_data_ptr(), v.mutable_data_ptr(), scales.mutable_data_ptr(), others ? 1 : 0, stream());
+    if (!r) {
+      r = flash_fn(q->const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), (long)flash->pages, (const int*)flash->places, (int)flash->width,
+                   (const int*)flash->q_start, (const int*)flash->q_len, (const int*)flash->ctx_len, out.mutable_data_ptr(), (int)cut.rows, (int)cut.requests,
+                   (int)flash->max_q_len, (int)(c->kv_heads * cut.group), (int)c->kv_heads, (int)c->head_dim, (int)c->page_size, (int)cut.window,
+                   (int)flash->limit, (int*)flash->status, scales.const_data_ptr(), (const int*)flash->base, (long)flash->scales, stream());
+      if (r) return PyLong_FromLong(-1);
+    }
+  }
   if (r) return PyLong_FromLong(r);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

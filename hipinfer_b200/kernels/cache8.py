@@ -190,14 +190,18 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     table, T, D = batch.block_tables[group], batch.n_rows, cache.head_dim
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     tensor_cores = q.is_cuda and _on_tensor_cores(cache)
-    portions = tensor_cores and batch.max_q_len >= PORTION_ROWS[0] and cache.k.shape[0] > 0
-    if tensor_cores and not portions and T:
+    limit = 0
+    if tensor_cores and batch.max_q_len >= PORTION_ROWS[0] and cache.k.shape[0] and _flash_takes(q, cache, out, n_heads, scale):
+        limit = _portion_limit(batch, cache, n_heads, window)
+    others = tensor_cores and T and (not limit or any(0 < n < limit for n in batch.h_q_len))
+    if tensor_cores and T:
         bound = _binding() if _bound is None else _bound
         if bound:
-            cut = _cut(batch, cache, ops._dt(q), n_heads, window, 0)
-            done = bound.attend(q, cache.native, table, batch.positions, cut.tiles, cut.native, scale, out)
+            cut = _cut(batch, cache, ops._dt(q), n_heads, window, limit) if others else None
+            flash = _portions(batch, cache, table, n_heads, window, limit) if limit else None
+            done = bound.attend(q, cache.native, table, batch.positions, cut and cut.tiles, cut.native if cut else 0, scale, out, flash.native if limit else 0)
             if done is not None:
-                return _done(done, 1)
+                return _done(done, bool(others) + 2 * bool(limit))
     _here("attention_cache8", q, table, batch.positions, batch.row_request, *cache.tensors, out)
     _heads(cache, n_heads, window)
     if D > 256:
@@ -223,8 +227,6 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
                   None if _single_rows(batch) else batch.row_request.data_ptr(), batch.positions.data_ptr(), T, n_heads // cache.n_kv_heads, int(window), scale,
                   out.data_ptr(), ops._stream())
         return out
-    limit = _portion_limit(batch, cache, n_heads, window) if portions and _flash_takes(q, cache, out, n_heads, scale) else 0
-    others = not limit or any(0 < n < limit for n in batch.h_q_len)
     if others:
         cut = _cut(batch, cache, dt, n_heads, window, limit)
         ops._call("cache8", "hb_cache8_attention_mma", q.data_ptr(), dt, q.stride(0), *(t.data_ptr() for t in cache.tensors), cache.code, cache.k.shape[0],
@@ -291,24 +293,49 @@ def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:
 
 
 def _flash_takes(q, cache: Cache8, out, n_heads: int, scale: float) -> bool:
-    return (q.dtype == torch.bfloat16 and q.is_contiguous() and scale > 0 and (q.data_ptr() | out.data_ptr()) % 16 == 0
-            and ops.fast.flash_prefill_tc_supported(n_heads, cache.n_kv_heads, cache.head_dim, cache.page_size))
+    return (q.dtype == torch.bfloat16 and q.is_contiguous() and scale > 0 and (q.data_ptr() | (0 if out is None else out.data_ptr())) % 16 == 0
+            and _flash_sizes(n_heads, cache.n_kv_heads, cache.head_dim, cache.page_size))
+
+
+@functools.lru_cache(maxsize=None)
+def _flash_sizes(n_heads: int, n_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    return n_heads > 0 and n_heads % n_kv_heads == 0 and ops.fast.flash_prefill_tc_supported(n_heads, n_kv_heads, head_dim, page_size)
 
 
 _AHEAD = 32             # C8_AHEAD of csrc/cache8_store.cu
 
 
+class _Portions:
+    """A step's portions of `limit` rows or more as the binding reads them (Portions in csrc/cache8_binding.cpp)."""
+
+    def __init__(self, batch, cache: Cache8, table, n_heads: int, window: int, limit: int):
+        _heads(cache, n_heads, window)
+        self.index, self.places, self.base = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)
+        self.lengths = batch.req_q_start, batch.req_q_len, batch.req_ctx_len
+        n = self.index.numel()
+        self.scales = n * cache8_blocks(cache.page_size) + 2 * _AHEAD
+        self._native = np.array([batch.n_rows, batch.n_requests, table.shape[1], n, self.scales, limit, batch.max_q_len, n_heads // cache.n_kv_heads, window,
+                                 batch.max_pos] + [t.data_ptr() for t in (self.index, self.places, self.base) + self.lengths] + [ops.fast._status_ptr()],
+                                dtype=np.int64)
+        self.native = self._native.ctypes.data
+
+
+def _portions(batch, cache: Cache8, table, n_heads: int, window: int, limit: int) -> _Portions:
+    key = ("cache8 portions", cache.k.shape[1:], table.shape[1], n_heads, window, limit)
+    return _on_stream(batch, key, lambda: _Portions(batch, cache, table, n_heads, window, limit))
+
+
 def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int, beside: bool) -> None:
     """Requests of `limit` rows or more: the codes of the pages that they see as 16-bit numbers, side by side, their scales beside them, and the flash
     kernel over both."""
-    index, places, base = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)      # (one page at least: a row sees its own key)
-    n, device = index.numel(), q.device
+    p = _portions(batch, cache, table, n_heads, window, limit)      # (one page at least: a row sees its own key)
+    n, device = p.index.numel(), q.device
     k, v = (torch.empty((n,) + cache.k.shape[1:], dtype=torch.bfloat16, device=device) for _ in range(2))
-    scales = torch.empty(cache.n_kv_heads, n * cache8_blocks(cache.page_size) + 2 * _AHEAD, 4, dtype=torch.float32, device=device)
-    ops._call("cache8", "hb_cache8_portions", *(t.data_ptr() for t in cache.tensors), cache.code, table.data_ptr(), index.data_ptr(), n, cache.k.shape[0],
+    scales = torch.empty(cache.n_kv_heads, p.scales, 4, dtype=torch.float32, device=device)
+    ops._call("cache8", "hb_cache8_portions", *(t.data_ptr() for t in cache.tensors), cache.code, table.data_ptr(), p.index.data_ptr(), n, cache.k.shape[0],
               *cache.k.shape[1:], scale, k.data_ptr(), v.data_ptr(), scales.data_ptr(), beside, ops._stream())
-    ops.fast.flash_prefill_tc_cache8(q, k, v, places, batch.req_q_start, batch.req_q_len, batch.req_ctx_len, out, batch.max_q_len, n_heads,
-                                     cache.n_kv_heads, cache.head_dim, cache.page_size, window, limit, scales, base)
+    ops.fast.flash_prefill_tc_cache8(q, k, v, p.places, *p.lengths, out, batch.max_q_len, n_heads, cache.n_kv_heads, cache.head_dim, cache.page_size, window,
+                                     limit, scales, p.base)
 
 
 def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: int):
@@ -475,7 +502,8 @@ def _binding():
     lib, module = library.load("cache8"), library.load_binding("cache8")
     if module is not None:
         module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value
-                      for name in ("hb_cache8_store", "hb_cache8_expand", "hb_cache8_attention_mma", "hb_copy_pages")))
+                      for name in ("hb_cache8_store", "hb_cache8_expand", "hb_cache8_attention_mma", "hb_copy_pages", "hb_cache8_portions")),
+                    C.cast(library.load("fast").hb_flash_prefill_tc_cache8, C.c_void_p).value)
     _bound = module or False
     return _bound
 
@@ -483,6 +511,6 @@ def _binding():
 def _done(result, launches: int):
     """What a call through the binding gave."""
     if result.__class__ is int and result:
-        raise ops.KernelError(library.load("cache8").hb_last_error().decode())
+        raise ops.KernelError(library.load("cache8" if result > 0 else "fast").hb_last_error().decode())
     library.launches[0] += launches
     return result

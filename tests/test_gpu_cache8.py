@@ -559,3 +559,48 @@ def test_pages_beyond_32_bits_of_bytes(rows, D, ps):
         assert same(a, b)
     ops.copy_pages([t[None] for t in big.tensors], list(range(n - pages, n)), list(range(1, pages + 1)))
     assert all(same(a[1:pages + 1], b) for a, b in zip(big.tensors, small.tensors))
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [5, 2], [300, 1], [300, 200]])
+@pytest.mark.parametrize("window", [0, 100])
+def test_calls_through_the_interpreter_give_the_same_bits(rows, window, monkeypatch):
+    """Without the binding in C++: every operator, the same launches."""
+    from hipinfer_b200.kernels import library
+
+    batch, tables, pages = step([200, 41], rows, 16, window)
+    start = filled(pages, 2, 16, 128, torch.int8)
+    g = torch.Generator().manual_seed(16)
+    q, k = torch.randn(sum(rows), 8 * 128, generator=g).to(torch.bfloat16).to(DEV), torch.randn(9, 256, generator=g).to(torch.bfloat16).to(DEV)
+    slots = torch.arange(18, 27, dtype=torch.int32, device=DEV)
+
+    def run():
+        cache, before = on_gpu(start), library.launches[0]
+        attended = ops.attention_cache8(q, cache, batch, 0, 8, window)
+        ops.store_cache8(k, k, slots, cache)
+        read = ops.expand_cache8(cache, torch.arange(pages, dtype=torch.int32, device=DEV))
+        ops.copy_pages([t[None] for t in cache.tensors], [0], [1])
+        return [attended, *read, *cache.tensors], library.launches[0] - before
+
+    bound, launches = run()
+    monkeypatch.setattr(cache8, "_bound", False)
+    plainly, as_many = run()
+    assert all(same(a, b) for a, b in zip(bound, plainly)) and launches == as_many
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_portions_of_wider_rows_and_at_odd_addresses(D):
+    rows, held = [300, 1, 40], [50, 100, 7]
+    batch, tables, pages = step(held, rows, 16)
+    cache = filled(pages, 2, 16, D, torch.int8)
+    q = torch.randn(sum(rows), 8 * D, generator=torch.Generator().manual_seed(17)).to(torch.bfloat16)
+    want = check(q, cache, batch, tables, 8)
+    wide = torch.zeros(sum(rows), 8 * D + 3, dtype=torch.bfloat16, device=DEV)
+    wide[:, 2:-1] = q.to(DEV)
+    odd = torch.empty(q.numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view(q.shape).copy_(q)
+    room = torch.full((q.numel() + 2,), 3.0, dtype=torch.bfloat16, device=DEV)
+    out = room[1:-1].view(q.shape)
+    for x, to in ((wide[:, 2:-1], None), (odd, None), (q.to(DEV), out)):
+        got = ops.attention_cache8(x, on_gpu(cache), batch, 0, 8, out=to)
+        V = float(np.abs(plain.numbers(cache[1], cache[3])).max())
+        assert (got.float() - want.float()).abs().max() <= V * 2.0 ** -7 * 8        # (each within 2^-8 (2 + A) V of the exact one, A below 6)
+    assert room[0] == room[-1] == 3.0
