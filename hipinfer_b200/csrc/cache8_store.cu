@@ -317,15 +317,24 @@ HB_EXPORT int hb_cache8_expand(const void* kc, const void* vc, const float* ks, 
 
 // What the flash kernel for portions wants of a cache: the codes of pages table[index[i]] as bf16, which holds them exactly, and the scales of
 // their blocks, scale[h][C8_AHEAD + i * blocks + block] of n * blocks and C8_AHEAD on either side: {K's times `scale_log2`, log2 of V's, 1 / V's, 0}, K's negative where
-// the page is not there. No scale is less than 1e-30 (a block that nothing was stored to; 0 times a masked score is not a number), places that nothing was stored to may hold anything, and
-// so codes and scales that are not numbers become 0 and 1e-30, and what
-// lies on either side, for tiles that reach over a request's ends, are ones.
+// the page is not there. A weight is made times its value's scale and in bf16, so that a scale near the least (a block of zeros has 1e-30 / M) would lose all weights
+// but the largest, and one near the greatest would leave the type: outside of 2^-60 .. 2^60 a scale comes times 2^60 or 2^-60 and the block's codes the other way,
+// exactly. Where a scale is 0 (a block that nothing was stored to) or not a number it is 1 and the codes are 0 (0 times a masked score is not a number); places that nothing
+// was stored to may hold anything, and so codes that are not numbers become 0; what lies on either side, for tiles that reach over a request's ends, are ones.
 //
 // `beside`: the kernel ahead is cache8_attention_mma_kernel for a step's other rows, which lets this one start when it has itself waited for what came
 // before it: the cache is as this kernel wants it, and the two run side by side (a step of two portions and four single rows 7 us of 119). Its 380 pages of 8 heads of
 // 128 take 8 us; with a page's work shared by blocks it took the single rows' blocks their place (104 us the step, 108). This
 // kernel still does not end before that one has.
 constexpr int C8_AHEAD = 32;
+struct C8Shifted {
+  float scale, codes;          // what a block's scale and its codes are multiplied with
+};
+__device__ __forceinline__ C8Shifted c8_shifted(float s) {
+  constexpr float UP = 1.152921504606846976e18f;                 // 2^60
+  if (!(s > 0.f && s <= 3.402823466e38f)) return {0.f, 0.f};
+  return s < 1.f / UP ? C8Shifted{UP, 1.f / UP} : s > UP ? C8Shifted{1.f / UP, UP} : C8Shifted{1.f, 1.f};
+}
 template <typename CT>
 __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, const int* table,
                                                               const int* index, long n, long n_pages, int Hkv, int page_size, int D, float scale_log2,
@@ -347,13 +356,20 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
   }
   const long page = table[index[i]];
   const bool there = page >= 0 && page < n_pages;
-  const int pieces = Hkv * page_size * D / 8;
+  const int pieces = Hkv * page_size * D / 8, row_pieces = D / 8;
+  const bool whole = page_size % C8_BLOCK == 0;
   for (int j0 = blockIdx.y * 256 + threadIdx.x; j0 < 2 * pieces; j0 += C8E_AHEAD * step) {
     uint2 w[C8E_AHEAD];
+    float f[C8E_AHEAD];
 #pragma unroll
     for (int u = 0; u < C8E_AHEAD; u++) {
-      const int j = j0 + u * step;
-      w[u] = there && j < 2 * pieces ? *(const uint2*)((j >= pieces ? vc : kc) + (page * pieces + (j >= pieces ? j - pieces : j)) * 8L) : make_uint2(0u, 0u);
+      const int j = j0 + u * step, at = j >= pieces ? j - pieces : j;
+      w[u] = make_uint2(0u, 0u), f[u] = 0.f;
+      if (there && j < 2 * pieces) {
+        w[u] = *(const uint2*)((j >= pieces ? vc : kc) + (page * pieces + at) * 8L);
+        const int row = at / row_pieces;
+        f[u] = (j >= pieces ? vs : ks)[page * Hkv * blocks + (whole ? row / C8_BLOCK : row / page_size * blocks + row % page_size / C8_BLOCK)];
+      }
     }
 #pragma unroll
     for (int u = 0; u < C8E_AHEAD; u++) {
@@ -363,16 +379,21 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
       CT::values4(w[u].x, x);
       CT::values4(w[u].y, x + 4);
       __nv_bfloat162 y[4];
+      const float times = c8_shifted(f[u]).codes;
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = there && x[e] == x[e] ? x[e] : 0.f;
+      for (int e = 0; e < 8; e++) x[e] = x[e] == x[e] ? x[e] * times : 0.f;
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
       *(uint4*)((j >= pieces ? v : k) + (i * pieces + (j >= pieces ? j - pieces : j)) * 8L) = *(const uint4*)y;
     }
   }
   for (int j = blockIdx.y * 256 + threadIdx.x; j < Hkv * blocks; j += step) {
-    const auto number = [](float s) { return s <= 3.402823466e38f ? fmaxf(s, C8_LEAST) : C8_LEAST; };
-    const float x = there ? number(ks[page * Hkv * blocks + j]) * scale_log2 : -1.f, y = there ? number(vs[page * Hkv * blocks + j]) : 1.f;
+    const auto number = [](float s) {
+      const C8Shifted f = c8_shifted(s);
+      return f.scale == 0.f ? 1.f : s * f.scale;
+    };
+    // (K's stays above 0 whatever the softmax's scale: it multiplies masked scores, which are infinite)
+    const float x = there ? fmaxf(number(ks[page * Hkv * blocks + j]) * scale_log2, 1.17549435e-38f) : -1.f, y = there ? number(vs[page * Hkv * blocks + j]) : 1.f;
     scale[j / blocks * ld + C8_AHEAD + i * blocks + j % blocks] = make_float4(x, log2f(y), 1.f / y, 0.f);
   }
   if (beside) hb_pdl_wait();
