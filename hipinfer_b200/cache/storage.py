@@ -47,11 +47,12 @@ def _planes8(group: CacheGroupSpec, pages: int, page_size: int, dtype, device) -
 class CacheStorage:
     def __init__(self, groups: Sequence[CacheGroupSpec], num_pages: Sequence[int], page_size: int, dtype, device,
                  state_specs: Dict[Tuple[int, str], Tuple[Tuple[int, ...], torch.dtype]], num_state_slots: int,
-                 cache_dtype: Optional[torch.dtype] = None):
+                 cache_dtype: Optional[torch.dtype] = None, spare_pages: int = 0):
+        """`spare_pages` of each group lie behind those that the cache manager hands out (a cache in 8 bits alone)."""
         self.groups, self.page_size, self.dtype, self.cache_dtype = list(groups), page_size, dtype, cache_dtype
         self.kv = [{name: torch.zeros(g.n_layers, n, heads, page_size, width, dtype=dtype, device=device)
                     for name, heads, width in g.planes} for g, n in zip(self.groups, num_pages)] if cache_dtype is None else \
-                  [_planes8(g, n, page_size, cache_dtype, device) for g, n in zip(self.groups, num_pages)]
+                  [_planes8(g, n + spare_pages, page_size, cache_dtype, device) for g, n in zip(self.groups, num_pages)]
         self.state: Dict[Tuple[int, str], torch.Tensor] = {
             key: torch.zeros((num_state_slots,) + tuple(shape), dtype=dt, device=device)
             for key, (shape, dt) in state_specs.items()}

@@ -232,7 +232,7 @@ class Engine:
                     stop_token_ids: Sequence[int] = (), ignore_eos: bool = True, logprobs: bool = False):
         """n continuations of one prompt, each of n_new tokens or up to a stop token. The prompt is run and kept once; with n_draft
         a step runs up to that many tokens more per sample, looked up in its own text, and keeps those that the model would have
-        drawn; all samples' tokens and drafts together are at most max_prefill a step (fewer drafts, and then more steps, where they
+        drawn (of a cache in 8 bits: with the rounding that the drafts beside them give it, engine/samples.py); all samples' tokens and drafts together are at most max_prefill a step (fewer drafts, and then more steps, where they
         would be more). Returns the n lists of tokens; with `logprobs` also the n lists of their logarithms of probability (at temperature
         1 for greedy samples). Temperature draws come from a generator seeded with `seed`, one after the other: they repeat for
         equal arguments, and are other draws than generate()'s."""

@@ -52,6 +52,7 @@ class StepBatch:
     short_list: Optional[torch.Tensor] = None  # int32: rows of requests with fewer than SHORT_ROWS rows, in a step with longer ones
     shared: Sequence[list] = ()   # per cache group: (first request, requests, tokens) that hold the same pages (shared_prefixes), for
                                   # groups with layers of Mixer.reads_shared_pages
+    kept_rows: Optional[list] = None  # (layer cache, keys, values) of each layer whose cache is in 8 bits, where a list is put here (runner.step)
     dump: Optional[dict] = None   # debug: planes of the step are recorded here, keyed (order index, name) (parts/planes.py)
     dump_step: int = -1           # the order index the decoder is at
 

@@ -16,6 +16,7 @@ import torch
 
 from ..cache import CacheManager, CacheStorage, OutOfPages
 from ..config import ModelConfig, get_architecture, load_config
+from ..kernels import ops
 from ..models.decoder import DecoderModel
 from ..parts.registry import BuildContext
 from ..weights import load_weights, random_weights
@@ -58,7 +59,7 @@ class ModelRunner:
         groups = self.model.cache_groups
         self.cache = CacheManager(groups, self.page_size, [n_pages] * len(groups), max_num_seqs)
         self.storage = CacheStorage(groups, [n_pages] * len(groups), self.page_size, self.dtype, self.device,
-                                    self.model.state_specs, max_num_seqs, self.cache_dtype)
+                                    self.model.state_specs, max_num_seqs, self.cache_dtype, max_num_seqs)
         self.vocab_size = self.spec.vocab_size
         self.steps_run = 0
         # decode-only steps (one token per request, every row wanted) are replayed from a CUDA
@@ -69,6 +70,7 @@ class ModelRunner:
         self._table_widths = [pages_per_seq] * len(groups)
         self._np_tables: Dict[object, list] = {}
         self._forked: set = set()              # requests that began with another's pages
+        self._kept: Optional[_KeptStep] = None # what the last step's refused drafts leave behind is undone with (store_accepted)
 
     # ---------------------------------------------------------------- construction helpers
     @classmethod
@@ -124,7 +126,7 @@ class ModelRunner:
         return arrays
 
     def step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None,
-             token_map: Optional[Sequence[int]] = None, dump: Optional[dict] = None) -> torch.Tensor:
+             token_map: Optional[Sequence[int]] = None, dump: Optional[dict] = None, drafts: bool = False) -> torch.Tensor:
         """Run one batch; float32 logits [number of wanted places, vocab] on the device.
         Raises OutOfPages (nothing changed) when the cache cannot hold the new tokens.
         `device_tokens` (int32 [rows], on the device) replaces the entries' token values, which
@@ -132,8 +134,10 @@ class ModelRunner:
         the host (the reference keeps token and position on the device for the same reason,
         README.md:510-512). With `token_map` (one int per row) only rows with an entry >= 0 take
         their token from device_tokens[entry]; the others keep the value the entry gives.
-        `dump` (a dict): the step runs eagerly and leaves named planes of every layer in it (parts/planes.py)."""
+        `dump` (a dict): the step runs eagerly and leaves named planes of every layer in it (parts/planes.py).
+        `drafts`: some of the step's tokens may be taken back (truncate) before the next one; `store_accepted` then belongs between."""
         entries = list(entries)
+        self._kept = None
         token_arrays = self.check_entries(entries)
         if not entries:
             return torch.empty(0, self.vocab_size, dtype=torch.float32, device=self.device)
@@ -162,7 +166,8 @@ class ModelRunner:
             slot_maps.append(self.cache.append(e.request_id, len(e.tokens), as_arrays=True))
             tables.append(self._table_rows(rc))
         shared = self._shared_prefixes(tables, ctx_lens) if len(entries) > 1 else ()
-        graph = dump is None and self.cuda_graphs and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries)
+        keep = drafts and self.cache_dtype is not None
+        graph = dump is None and not keep and self.cuda_graphs and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries)
         if graph and any(shared) and self._saved_bytes(shared) >= self.SHARED_STEP_BYTES * len(self.spec.order):
             graph = False
         if graph:
@@ -172,6 +177,12 @@ class ModelRunner:
                                      token_map=token_map, token_arrays=token_arrays)
             self._feed(batch.tokens, batch.token_map, device_tokens, token_map)
             batch.dump, batch.shared = dump, shared
+            if keep:
+                batch.kept_rows = []
+                self._kept = _KeptStep(entries, ctx_lens, tables, slot_maps, self.page_size, [p.num_pages for p in self.cache.pools], batch.kept_rows)
+                for g, (src, dst) in enumerate(self._kept.copies()):
+                    if src:
+                        self.storage.copy_pages(g, src, dst)
             logits = self.model.forward(batch, self.storage)
         for e in entries:
             if self.cache.release_behind_window(e.request_id):
@@ -288,7 +299,8 @@ class ModelRunner:
         """Request `new_id` begins with the whole pages of `request_id`, which both hold from then on (neither writes them);
         returns how many tokens those are. With `length` it begins with exactly so many tokens: a page that they end inside of is
         copied (ops.copy_pages). Requests that stand side by side in a step and hold the same pages attend to them
-        together (ops.attention_shared). Raises StepError for a model that keeps state besides the pages, OutOfPages (nothing
+        together (ops.attention_shared). In a cache in 8 bits the copy has the parent's codes, in whose scale the parent's tokens behind
+        `length` in that block have had part. Raises StepError for a model that keeps state besides the pages, OutOfPages (nothing
         changed) where the cache has no page for the copy."""
         if self.model.state_specs:
             raise StepError("a request of a model with per-request state cannot be forked: its state is not in the pages")
@@ -301,15 +313,64 @@ class ModelRunner:
         return rc.length
 
     def truncate(self, request_id, length: int) -> None:
-        """The request's tokens from position `length` on are taken back (drafts that were refused)."""
+        """The request's tokens from position `length` on are taken back (drafts that were refused). In a cache in 8 bits the block that the
+        others end inside of keeps the scale and the roundings that the tokens taken back gave it, but for the last step's (store_accepted)."""
         if self.model.state_specs:
             raise StepError("a request of a model with per-request state cannot be cut: its state has run on")
         self.cache.truncate(request_id, length)
         for kept, table in zip(self._np_tables.get(request_id, ()), self.cache.get(request_id).tables):
             kept[1] = min(kept[1], len(table))             # (the pages that come next replace those that went)
 
+    def store_accepted(self) -> None:
+        """After a step with `drafts` and its truncations: a cache in 8 bits holds what it would if the step had brought the tokens that were kept alone
+        (a block's scale is that of the largest of the rows stored with it: a draft that stands out, refused, would leave its block's other tokens
+        coarser for good). The blocks that the step began inside of are put back, and the kept rows stored into them again: a launch a layer."""
+        kept, self._kept = self._kept, None
+        if kept is None:
+            return
+        lengths = [self.length(rid) for rid in kept.ids]
+        if not kept.damaged(lengths):
+            return
+        for g, (dst, src) in enumerate(kept.copies(lengths)):
+            if src:
+                self.storage.copy_pages(g, src, dst)
+        slots = [torch.from_numpy(s).pin_memory().to(self.device, non_blocking=True) for s in kept.accepted(lengths)]
+        for cache, k, v in kept.rows:
+            ops.store_cache8(k, v, slots[cache.group], cache.cache8)
+
     def live_requests(self):
         return list(self.cache.requests)
+
+
+class _KeptStep:
+    """A step over a cache in 8 bits, some of whose tokens may be taken back: which requests brought how many rows to which places, the page that each
+    began inside of (and a spare page of its group, behind the `pages` that are handed out, for what it held), and every layer's rows."""
+
+    def __init__(self, entries, ctx_lens, tables, slot_maps, page_size: int, pages: Sequence[int], rows: list):
+        self.ids, self.held, self.n = [e.request_id for e in entries], list(ctx_lens), [len(e.tokens) for e in entries]
+        self.page_size, self.pages, self.slot_maps, self.rows = page_size, list(pages), slot_maps, rows
+        self.begun = [[int(t[h // page_size]) if self._inside(h) else -1 for t in groups] for groups, h in zip(tables, self.held)]
+
+    def _inside(self, length: int) -> int:
+        """How many places of its block lie ahead of a token at that place."""
+        return length % self.page_size % ops.BLOCK8
+
+    def damaged(self, lengths: Sequence[int]) -> List[int]:
+        """The requests (by their places) of which tokens are kept that share a block with the step's that were taken back, from their lengths now."""
+        return [r for r, (length, h, n) in enumerate(zip(lengths, self.held, self.n)) if length < h + n and length > max(h, length) - self._inside(max(h, length))]
+
+    def copies(self, lengths: Optional[Sequence[int]] = None):
+        """Per group, the pages that the step's requests began inside of and the spare pages of what they held; of the damaged ones, with `lengths`."""
+        which = range(len(self.ids)) if lengths is None else self.damaged(lengths)
+        for g, pages in enumerate(self.pages):
+            there = [r for r in which if self.begun[r][g] >= 0]
+            yield [self.begun[r][g] for r in there], [pages + r for r in there]
+
+    def accepted(self, lengths: Sequence[int]) -> List[np.ndarray]:
+        """Per group, the step's rows' places: of the damaged requests' kept rows; -1 for all others."""
+        damaged = set(self.damaged(lengths))
+        return [np.concatenate([np.where(np.arange(n) < (lengths[r] - h if r in damaged else 0), np.asarray(self.slot_maps[r][g], dtype=np.int64), -1)
+                                for r, (h, n) in enumerate(zip(self.held, self.n))]).astype(np.int32) for g in range(len(self.pages))]
 
 
 def cache8_dtype(name) -> Optional[torch.dtype]:

@@ -2,7 +2,9 @@
 reads their keys and values once for all samples (ops.attention_shared) where a layer's attention does that
 (Mixer.reads_shared_pages: attention without a window; others share the memory alone). A sample brings its newest token and, after it, tokens drafted by
 looking up what followed the same tokens earlier in its own text; the step's logits accept or refuse them (ops.verify_drafts), and the
-cache gives back what was refused. What is drawn is distributed as if each token had been drawn alone.
+cache gives back what was refused. What is drawn is distributed as if each token had been drawn alone; over a cache in 8 bits (cache_dtype)
+up to that cache's rounding, in which a step's drafts have part: the block of 16 tokens that they share with the newest ones is rounded to the scale of its largest,
+a draft among them. A refused draft has none in later steps (ModelRunner.store_accepted).
 
 The reference copies a prompt into every batch slot (src/api.cu:1409-1411) and keeps drafts for a caller of its `verify_step` (2029-2060).
 """
@@ -142,10 +144,13 @@ class Sampling:
             starts.append(row)
             drafts.append(d)
             row += len(d) + 1
-        logits = self.runner.step(entries)
+        keep = any(drafts) and getattr(self.runner, "cache_dtype", None) is not None
+        logits = self.runner.step(entries, drafts=True) if keep else self.runner.step(entries)
         self._take(logits, starts, drafts, live)
         for i in live:
             self.runner.truncate(self.rids[i], len(self.texts[i].tokens) - 1)      # all but the token that is still to be run
+        if keep:
+            self.runner.store_accepted()
         self.steps += 1
 
     def _take(self, logits, starts, drafts, live) -> None:

@@ -174,7 +174,8 @@ def _done(result, launches: int):
 
 def verify_drafts(logits: torch.Tensor, start: torch.Tensor, n_drafts: torch.Tensor, drafts: torch.Tensor, temperature: torch.Tensor,
                   uniform: torch.Tensor, noise: torch.Tensor, draft_probs: Optional[torch.Tensor] = None):
-    """Accepts or refuses drafted tokens so that what is produced is distributed as if the target alone had drawn it.
+    """Accepts or refuses drafted tokens so that what is produced is distributed as if the target, whose logits are given, alone had drawn it. (Where
+    logits behind a cache in 8 bits are computed with drafts in the cache, the drafts have part in its rounding.)
 
     Request r has n_drafts[r] drafts in row r of `drafts` (int32 [R, K]) and n_drafts[r] + 1 rows of logits ([T, V], float32 or bfloat16) from row
     start[r] on; p_i is the softmax of the i-th over `temperature[r]` (float32 [R]; 0 or less: greedy, a point mass on the lowest index of the largest

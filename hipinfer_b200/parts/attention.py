@@ -101,6 +101,8 @@ class AttentionMixer(Mixer):
         if cache.cache8 is not None:
             if cache.write:
                 ops.store_cache8(k_rows.view(T, Hkv * D), v_rows.view(T, Hkv * D), batch.slot_maps[cache.group], cache.cache8)
+                if batch.kept_rows is not None:
+                    batch.kept_rows.append((cache, k_rows.view(T, Hkv * D), v_rows.view(T, Hkv * D)))
             ops.attention_cache8(q, cache.cache8, batch, cache.group, Hq, self.window, self.scale, att)
         else:
             ops.attention(q, cache.k, cache.v, batch, cache.group, att, Hq, Hkv, D, self.ctx.page_size, self.window,
