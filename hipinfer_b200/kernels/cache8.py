@@ -458,6 +458,9 @@ def _ranks(tiles: int, keys: int, mean: float, clusters) -> int:
     return ranks
 
 
+COPY_PLANES, COPY_PAIRS = 8, 960                                   # CP_PLANES, CP_PAIRS of csrc/copy_pages.cu: of one launch
+
+
 def copy_pages(planes: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
     """Page src[i] to page dst[i], for every i, in all layers of all `planes` ([layers, pages, ...] each, a page's numbers side by side; of any types
     and sizes). src and dst are numbers of the host: pages below 0 or outside of a plane, a page copied to twice, and one both copied from and to
@@ -467,7 +470,7 @@ def copy_pages(planes: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     if bound and there:
         done = bound.copy(planes, src, dst)
         if done is not None:
-            _done(done, 1)
+            _done(done, _copies(len(planes), len(src)))
             return
     pairs = [np.ascontiguousarray(x, dtype=np.int64) for x in (src, dst)]
     src, dst = pairs
@@ -490,7 +493,13 @@ def copy_pages(planes: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     if not len(src) or not numbers:
         return
     numbers, src, dst = np.array(numbers, dtype=np.int64), src.astype(np.int32), dst.astype(np.int32)
+    library.launches[0] += _copies(len(numbers), len(src)) - 1      # (and the one that every call counts)
     ops._call("cache8", "hb_copy_pages", numbers.ctypes.data, len(numbers), src.ctypes.data, dst.ctypes.data, len(src), ops._stream())
+
+
+def _copies(planes: int, pairs: int) -> int:
+    """Launches that copying so many pairs of pages in so many planes takes."""
+    return -(-planes // COPY_PLANES) * -(-pairs // COPY_PAIRS)
 
 
 _bound = None

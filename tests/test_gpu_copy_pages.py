@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from hipinfer_b200.kernels import ops
+from hipinfer_b200.kernels import cache8, library, ops
 from test_gpu_cache8 import DEV, same
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +72,13 @@ def test_narrow_scales_do_not_hold_the_codes_back():
 
     codes, both = least(planes[:2]), least(planes)
     assert both <= 1.75 * codes, (codes, both)
+
+
+@pytest.mark.parametrize("planes, pairs, launches", [(1, 1, 1), (8, 960, 1), (9, 1, 2), (4, 961, 2), (17, 2000, 9)])
+def test_launches_are_counted(planes, pairs, launches, monkeypatch):
+    planes = [torch.zeros(1, 2 * pairs, 4, dtype=torch.uint8, device=DEV) for _ in range(planes)]
+    for bound in (None, False):
+        monkeypatch.setattr(cache8, "_bound", bound)
+        before = library.launches[0]
+        ops.copy_pages(planes, list(range(pairs)), list(range(pairs, 2 * pairs)))
+        assert library.launches[0] - before == launches
