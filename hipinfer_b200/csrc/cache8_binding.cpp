@@ -51,6 +51,8 @@ const Cache* cache(PyObject* address) {                          // null for one
   const Cache* c = (const Cache*)PyLong_AsVoidPtr(address);
   return c && c->device == (int64_t)c10::cuda::current_device() ? c : nullptr;
 }
+// What a call of the cache8 library gave, to the interpreter: 0, or 1 where it failed (the library's own is -1, which here says that the flash kernel's did).
+PyObject* code(int r) { return PyLong_FromLong(r ? 1 : 0); }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
   return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);
@@ -68,7 +70,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// (keys, values, slot map, address of a Cache): the code of the call; None for arguments that this does not take
+// (keys, values, slot map, address of a Cache): 0, or 1 for a call that failed; None for arguments that this does not take
 PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 4) return PyErr_Format(PyExc_TypeError, "four arguments are expected");
@@ -79,7 +81,7 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
       type_code(*k) != type_code(*v) || k->stride(1) != 1 || v->stride(1) != 1 || !ints(*slots, 1) || slots->size(0) != k->size(0) || k->size(0) > 0x7fffffff ||
       !k->size(0) || !c->pages)
     Py_RETURN_NONE;
-  return PyLong_FromLong(store_fn(k->const_data_ptr(), v->const_data_ptr(), (long)k->stride(0), (long)v->stride(0), type_code(*k),
+  return code(store_fn(k->const_data_ptr(), v->const_data_ptr(), (long)k->stride(0), (long)v->stride(0), type_code(*k),
                                   (const int*)slots->const_data_ptr(), (int)k->size(0), (int)c->kv_heads, (int)c->page_size, (int)c->head_dim, (long)c->pages,
                                   (int)c->code, (void*)c->k, (void*)c->v, (float*)c->k_scale, (float*)c->v_scale, stream()));
   END_HANDLE_TH_ERRORS
@@ -99,7 +101,7 @@ PyObject* expand(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int r = expand_fn((const void*)c->k, (const void*)c->v, (const float*)c->k_scale, (const float*)c->v_scale, (int)c->code,
                           (const int*)pages->const_data_ptr(), (long)count, (long)c->pages, (int)c->kv_heads, (int)c->page_size, (int)c->head_dim,
                           k.mutable_data_ptr(), v.mutable_data_ptr(), type_code(k), stream());
-  if (r) return PyLong_FromLong(r);
+  if (r) return code(r);
   PyObject* out = PyTuple_New(2);
   if (!out) return nullptr;
   PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(k)));
@@ -109,7 +111,7 @@ PyObject* expand(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (q, address of a Cache, block table, positions, tiles or None, address of a Cut, scale, out or None, address of Portions or 0): the output; or as above.
-// With portions the Cut is of the other rows, 0 where there are none; a code below 0 is one of the flash kernel's.
+// With portions the Cut is of the other rows, 0 where there are none; -1: the flash kernel's call failed.
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 9) return PyErr_Format(PyExc_TypeError, "nine arguments are expected");
@@ -158,7 +160,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (r) return PyLong_FromLong(-1);
     }
   }
-  if (r) return PyLong_FromLong(r);
+  if (r) return code(r);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -177,7 +179,7 @@ bool numbers(PyObject* list, int64_t end, std::vector<int>& out) {      // pages
   return true;
 }
 
-// (planes, sources, targets), each a list or tuple: the code of the call; None for arguments that this does not take
+// (planes, sources, targets), each a list or tuple: 0, or 1 for a call that failed; None for arguments that this does not take
 PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 3) return PyErr_Format(PyExc_TypeError, "three arguments are expected");
@@ -205,7 +207,7 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   for (int p : src)
     if (target[p]) Py_RETURN_NONE;
-  return PyLong_FromLong(copy_fn(plane.data(), (int)planes, src.data(), dst.data(), (int)pairs, stream()));
+  return code(copy_fn(plane.data(), (int)planes, src.data(), dst.data(), (int)pairs, stream()));
   END_HANDLE_TH_ERRORS
 }
 

@@ -518,7 +518,7 @@ def _binding():
 
 
 def _done(result, launches: int):
-    """What a call through the binding gave."""
+    """What a call through the binding gave; an int other than 0: which library's call failed (above 0 cache8's, below the flash kernel's), whose words say why."""
     if result.__class__ is int and result:
         raise ops.KernelError(library.load("cache8" if result > 0 else "fast").hb_last_error().decode())
     library.launches[0] += launches
