@@ -426,9 +426,9 @@ def _single_rows(batch) -> bool:
 
 @functools.lru_cache(maxsize=None)
 def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
-    """Clusters of `ranks` blocks of the kernel on warp MMAs that are on the GPU at once."""
+    """Clusters of `ranks` blocks of the kernel on warp MMAs that are on the GPU at once; 0 where it has no room for one (16 are more than every GPU need take)."""
     n = ops._fn("cache8", "hb_cache8_attention_mma_clusters")(dt, code, head_dim, nt, ranks)
-    if n < 1:
+    if n < 0:
         raise ops.KernelError(library.load("cache8").hb_last_error().decode())
     return n
 
