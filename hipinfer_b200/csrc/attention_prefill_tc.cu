@@ -1016,12 +1016,14 @@ static int flash_prefill_tc(const void* q, const void* kc, const void* vc, long 
   if (c.most < 1) HB_FAIL("hb_flash_prefill_tc: %d heads are beyond the list of items", Hq);
 #define FT_LAUNCH(KERN, THREADS, SMEM)                                                                                           \
   do {                                                                                                                          \
-    static bool configured = false;                                                                                             \
-    if (!configured) {                                                                                                          \
+    static bool configured[64] = {}; /* the attribute belongs to a device: set once on each */                                  \
+    int dev = 0;                                                                                                                \
+    e = cudaGetDevice(&dev);                                                                                                    \
+    if (e == cudaSuccess && (dev >= 64 || !configured[dev])) {                                                                  \
       e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);                                        \
-      if (e != cudaSuccess) HB_FAIL("hb_flash_prefill_tc: %s", cudaGetErrorString(e));                                          \
-      configured = true;                                                                                                        \
+      if (e == cudaSuccess && dev < 64) configured[dev] = true;                                                                 \
     }                                                                                                                           \
+    if (e != cudaSuccess) HB_FAIL("hb_flash_prefill_tc: %s", cudaGetErrorString(e));                                            \
     e = hb_launch(KERN, grid, THREADS, SMEM, st, mq, mk, mv, bt, bt_stride, q_start, q_len, ctx_len, (__nv_bfloat16*)out, Hq,   \
                   Hkv, page_size, window, sl2, min_rows, status, r1, r2, sink, req0, reqs, qt0, qts, most, codes);  \
   } while (0)
