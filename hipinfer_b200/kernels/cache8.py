@@ -198,10 +198,16 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
         bound = _binding() if _bound is None else _bound
         if bound:
             cut = _cut(batch, cache, ops._dt(q), n_heads, window, limit) if others else None
-            flash = _portions(batch, cache, table, n_heads, window, limit) if limit else None
-            done = bound.attend(q, cache.native, table, batch.positions, cut and cut.tiles, cut.native if cut else 0, scale, out, flash.native if limit else 0)
-            if done is not None:
-                return _done(done, bool(others) + 2 * bool(limit))
+            groups = [_portions(batch, cache, table, n_heads, window, limit, g) for g in _portion_groups(batch, cache, window, limit)] if limit else [None]
+            to = out
+            for flash in groups:
+                done = bound.attend(q, cache.native, table, batch.positions, cut and cut.tiles, cut.native if cut else 0, scale, to, flash.native if flash else 0)
+                if done is None:
+                    break
+                to = _done(done, bool(cut) + 2 * bool(flash))
+                cut = None                                         # (the other rows are done with the first group)
+            else:
+                return to
     _here("attention_cache8", q, table, batch.positions, batch.row_request, *cache.tensors, out)
     _heads(cache, n_heads, window)
     if D > 256:
@@ -233,7 +239,9 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
                   cache.n_kv_heads, cache.page_size, D, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], batch.positions.data_ptr(),
                   ops._ptr(cut.tiles), cut.n_tiles, cut.nt, cut.ranks, n_heads // cache.n_kv_heads, int(window), scale, out.data_ptr(), bool(limit), ops._stream())
     if limit:
-        _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit, others)
+        for group in _portion_groups(batch, cache, window, limit):
+            _attend_portions(q, cache, batch, table, n_heads, int(window), scale, out, limit, group, others)
+            others = False
     return out
 
 
@@ -305,13 +313,40 @@ def _flash_sizes(n_heads: int, n_kv_heads: int, head_dim: int, page_size: int) -
 _AHEAD = 32             # C8_AHEAD of csrc/cache8_store.cu
 
 
-class _Portions:
-    """A step's portions of `limit` rows or more as the binding reads them (Portions in csrc/cache8_binding.cpp)."""
+# The pages that a step's portions see are expanded for some of its requests at a time, so that their codes in 16 bits take no more than this (but for a single request's, which
+# are one flash call's keys): 260,000 tokens of 8 heads of 128. Eight portions behind 100,000 tokens would be 3.3 GB at once beside a cache that was given the GPU's memory.
+PORTION_BYTES = 1 << 30
 
-    def __init__(self, batch, cache: Cache8, table, n_heads: int, window: int, limit: int):
+
+def _portion_groups(batch, cache: Cache8, window: int, limit: int) -> list:
+    """(first, end) of neighbouring requests whose portions of `limit` rows or more are expanded together."""
+    key = ("cache8 groups", cache.k.shape[1:], window, limit, PORTION_BYTES)
+    if key not in batch.extra:
+        groups, first, held, page = [], 0, 0, 4 * cache.k[0].numel()
+        for r, n in _portion_pages(batch, cache.page_size, window, limit):
+            if held and (held + n) * page > PORTION_BYTES:
+                groups.append((first, r))
+                first, held = r, 0
+            held += n
+        batch.extra[key] = groups + [(first, batch.n_requests)]
+    return batch.extra[key]
+
+
+def _portion_pages(batch, page_size: int, window: int, limit: int):
+    """(request, how many pages its rows see) of the portions of `limit` rows or more."""
+    for r, (held, rows) in enumerate(zip(batch.h_ctx_len, batch.h_q_len)):
+        if rows >= limit:
+            yield r, -(-(held + rows) // page_size) - (max(0, held - window + 1) // page_size if window else 0)
+
+
+class _Portions:
+    """A step's portions of `limit` rows or more, of the requests `group` (first, end), as the binding reads them (Portions in csrc/cache8_binding.cpp)."""
+
+    def __init__(self, batch, cache: Cache8, table, n_heads: int, window: int, limit: int, group: tuple):
         _heads(cache, n_heads, window)
-        self.index, self.places, self.base = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit)
-        self.lengths = batch.req_q_start, batch.req_q_len, batch.req_ctx_len
+        self.index, self.places, self.base = _pages_of_portions(batch, cache.page_size, table.shape[1], window, limit, group)
+        q_len = batch.req_q_len if group == (0, batch.n_requests) else _rows_of_group(batch, group)
+        self.lengths = batch.req_q_start, q_len, batch.req_ctx_len
         n = self.index.numel()
         self.scales = n * cache8_blocks(cache.page_size) + 2 * _AHEAD
         self._native = np.array([batch.n_rows, batch.n_requests, table.shape[1], n, self.scales, limit, batch.max_q_len, n_heads // cache.n_kv_heads, window,
@@ -320,15 +355,21 @@ class _Portions:
         self.native = self._native.ctypes.data
 
 
-def _portions(batch, cache: Cache8, table, n_heads: int, window: int, limit: int) -> _Portions:
-    key = ("cache8 portions", cache.k.shape[1:], table.shape[1], n_heads, window, limit)
-    return _on_stream(batch, key, lambda: _Portions(batch, cache, table, n_heads, window, limit))
+def _portions(batch, cache: Cache8, table, n_heads: int, window: int, limit: int, group: tuple) -> _Portions:
+    key = ("cache8 portions", cache.k.shape[1:], table.shape[1], n_heads, window, limit, group)
+    return _on_stream(batch, key, lambda: _Portions(batch, cache, table, n_heads, window, limit, group))
 
 
-def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int, beside: bool) -> None:
+def _rows_of_group(batch, group: tuple) -> torch.Tensor:
+    """The requests' numbers of rows (int32 on the device), 0 for those outside of the group: the flash kernel passes them over."""
+    lengths = lambda: np.array([n if group[0] <= r < group[1] else 0 for r, n in enumerate(batch.h_q_len)], dtype=np.int32)
+    return _on_stream(batch, ("cache8 rows", group), lambda: _to_device(lengths(), batch))[0]
+
+
+def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, scale: float, out, limit: int, group: tuple, beside: bool) -> None:
     """Requests of `limit` rows or more: the codes of the pages that they see as 16-bit numbers, side by side, their scales beside them, and the flash
     kernel over both."""
-    p = _portions(batch, cache, table, n_heads, window, limit)      # (one page at least: a row sees its own key)
+    p = _portions(batch, cache, table, n_heads, window, limit, group)      # (one page at least: a row sees its own key)
     n, device = p.index.numel(), q.device
     k, v = (torch.empty((n,) + cache.k.shape[1:], dtype=torch.bfloat16, device=device) for _ in range(2))
     scales = torch.empty(cache.n_kv_heads, p.scales, 4, dtype=torch.float32, device=device)
@@ -338,14 +379,16 @@ def _attend_portions(q, cache: Cache8, batch, table, n_heads: int, window: int, 
                                      limit, scales, p.base)
 
 
-def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: int):
-    """For requests of `limit` rows or more: where in the block table the pages stand that their rows see (int32 [n]), the table of the n pages side
+def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: int, group: Optional[tuple] = None):
+    """For requests of `limit` rows or more (of those from group[0] to group[1] - 1): where in the block table the pages stand that their rows see (int32 [n]), the table of the n pages side
     by side (int32 [requests, width], -1: none), and at which of the n pages' blocks of 16 places each request's first key would stand (int32)."""
+    group = group or (0, batch.n_requests)
+
     def pages():
         index, places, n = [], np.full((batch.n_requests, width), -1, dtype=np.int32), 0
         base, blocks = np.zeros(batch.n_requests, dtype=np.int32), cache8_blocks(page_size)
         for r, (held, rows) in enumerate(zip(batch.h_ctx_len, batch.h_q_len)):
-            if rows < limit:
+            if rows < limit or not group[0] <= r < group[1]:
                 continue
             first, end = max(0, held - window + 1) // page_size if window else 0, -(-(held + rows) // page_size)
             index.append(np.arange(first, end, dtype=np.int32) + r * width)
@@ -354,7 +397,7 @@ def _pages_of_portions(batch, page_size: int, width: int, window: int, limit: in
             n += end - first
         return np.concatenate(index + [places.ravel(), base])
 
-    both, R = _on_stream(batch, ("cache8 pages", page_size, width, window, limit), lambda: _to_device(pages(), batch))[0], batch.n_requests
+    both, R = _on_stream(batch, ("cache8 pages", page_size, width, window, limit, group), lambda: _to_device(pages(), batch))[0], batch.n_requests
     n = both.numel() - R * (width + 1)
     return both[:n], both[n:n + R * width].view(R, width), both[n + R * width:]
 

@@ -37,3 +37,32 @@ def test_a_gpu_without_room_for_large_clusters_takes_smaller_ones(monkeypatch):
             clusters(2)
     finally:
         cache8._clusters.cache_clear()
+
+
+def batch_of(held, rows, ps=16):
+    from hipinfer_b200.engine.batch import StepEntry, build_step_batch
+
+    tables = [[list(range(-(-(h + n) // ps)))] for h, n in zip(held, rows)]
+    return build_step_batch([StepEntry(i, [0] * n) for i, n in enumerate(rows)], held, list(range(len(rows))), tables, [[[0] * n] for n in rows], 1, "cpu")
+
+
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("most", [1, 20, 40, 10 ** 6])
+def test_portions_are_expanded_within_a_bound(monkeypatch, window, most):
+    """Groups of neighbours of at most `most` pages, a single request's aside; every portion is in one group, whose tables name its pages alone."""
+    cache = ops.new_cache8(4, 2, 16, 64, device="cpu")
+    monkeypatch.setattr(cache8, "PORTION_BYTES", most * 4 * 2 * 16 * 64)
+    held, rows = [0, 300, 40, 0, 7, 100, 160], [16, 30, 1, 333, 0, 20, 15]
+    batch = batch_of(held, rows)
+    groups, width = cache8._portion_groups(batch, cache, window, 16), batch.block_tables[0].shape[1]
+    assert [g[0] for g in groups] == [0] + [g[1] for g in groups[:-1]] and groups[-1][1] == len(rows)
+    seen = []
+    for first, end in groups:
+        index, places, base = cache8._pages_of_portions(batch, 16, width, window, 16, (first, end))
+        there = [r for r in range(first, end) if rows[r] >= 16]
+        assert there and (index.numel() <= most or len(there) == 1) and index.numel() == int((places >= 0).sum())
+        assert [r for r in range(len(rows)) if (places[r] >= 0).any()] == there
+        assert index.tolist() == [r * width + i for r in there for i in range(width) if places[r, i] >= 0]
+        assert cache8._rows_of_group(batch, (first, end)).tolist() == [n if first <= r < end else 0 for r, n in enumerate(rows)]
+        seen += index.tolist()
+    assert sorted(seen) == sorted(cache8._pages_of_portions(batch, 16, width, window, 16)[0].tolist()) and (len(groups) == 1) == (len(seen) <= most)

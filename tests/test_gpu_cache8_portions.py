@@ -284,3 +284,48 @@ def test_portions_over_pages_beyond_32_bits_of_bytes(D, portions):
     high = step([200, 41], [300, 17], ps)[0]
     high.block_tables[0] += (high.block_tables[0] >= 0) * (n - pages)
     assert same(portions(q, big, high, 32), portions(q, small, batch, 32))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [0, 100])
+def test_portions_that_are_expanded_some_at_a_time(D, window, monkeypatch):
+    """The same bits, whatever part of them is expanded together, with the binding and without, captured too; memory for one part."""
+    monkeypatch.setattr(cache8, "_portion_limit", lambda *a: 16)
+    held, rows, heads = [0, 300, 40, 1000, 7, 100, 160], [16, 30, 1, 333, 0, 20, 15], 8
+    batch, tables, pages = step(held, rows, 16, window)
+    cache = on_gpu(filled(pages, 2, 16, D, torch.int8))
+    q = queries(sum(rows) * heads * D, 20).view(-1, heads * D).to(torch.bfloat16).to(DEV)
+    want = ops.attention_cache8(q, cache, batch, 0, heads, window=window)
+    for most, groups in ((1, 4), (25, 3), (100, 1 if window else 2)):
+        monkeypatch.setattr(cache8, "PORTION_BYTES", most * 4 * 2 * 16 * D)
+        assert len(cache8._portion_groups(batch, cache, window, 16)) == groups
+        for bound in (cache8._bound, False):
+            with monkeypatch.context() as m:
+                m.setattr(cache8, "_bound", bound)
+                before, out = library.launches[0], torch.full_like(want, 7.0)
+                assert same(ops.attention_cache8(q, cache, batch, 0, heads, window=window), want) and library.launches[0] - before == 1 + 2 * groups
+                assert ops.attention_cache8(q, cache, batch, 0, heads, window=window, out=out) is out and same(out, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.attention_cache8(q, cache, batch, 0, heads, window=window)
+        out.zero_()
+        graph.replay()
+        assert same(out, want)
+
+
+def test_the_memory_of_many_long_portions(monkeypatch):
+    """Six portions behind 20,000 tokens: no more than the bound and one request's beside the output."""
+    monkeypatch.setattr(cache8, "_portion_limit", lambda *a: 16)
+    monkeypatch.setattr(cache8, "PORTION_BYTES", 1 << 24)
+    held, rows, D = [20000] * 6, [16] * 6, 128
+    batch, tables, pages = step(held, rows, 16)
+    cache = on_gpu(filled(pages, 1, 16, D, torch.int8))
+    q = queries(96 * 2 * D, 21).view(-1, 2 * D).to(torch.bfloat16).to(DEV)
+    ops.attention_cache8(q, cache, batch, 0, 2)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.attention_cache8(q, cache, batch, 0, 2)
+    one = 20016 * D * 4                                            # keys and values of a request in 16 bits; scales are a 32nd
+    assert one < torch.cuda.max_memory_allocated() - before < (1 << 24) * 1.1 + (1 << 21)
