@@ -356,20 +356,18 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
   }
   const long page = table[index[i]];
   const bool there = page >= 0 && page < n_pages;
-  const int pieces = Hkv * page_size * D / 8, row_pieces = D / 8;
-  const bool whole = page_size % C8_BLOCK == 0;
+  const int pieces = Hkv * page_size * D / 8, block_log2 = D == 64 ? 7 : 8;      // 2^block_log2 pieces of a block, 2 D
+  // whether some block of the page has a scale that comes times something: looked up once for all (asked for with every piece a step took 4 us more, of 102)
+  bool odd = false;
+  for (int j = threadIdx.x; there && j < 2 * Hkv * blocks; j += 256)
+    odd |= c8_shifted((j >= Hkv * blocks ? vs : ks)[page * Hkv * blocks + (j >= Hkv * blocks ? j - Hkv * blocks : j)]).codes != 1.f;
+  odd = __syncthreads_or(odd);
   for (int j0 = blockIdx.y * 256 + threadIdx.x; j0 < 2 * pieces; j0 += C8E_AHEAD * step) {
     uint2 w[C8E_AHEAD];
-    float f[C8E_AHEAD];
 #pragma unroll
     for (int u = 0; u < C8E_AHEAD; u++) {
-      const int j = j0 + u * step, at = j >= pieces ? j - pieces : j;
-      w[u] = make_uint2(0u, 0u), f[u] = 0.f;
-      if (there && j < 2 * pieces) {
-        w[u] = *(const uint2*)((j >= pieces ? vc : kc) + (page * pieces + at) * 8L);
-        const int row = at / row_pieces;
-        f[u] = (j >= pieces ? vs : ks)[page * Hkv * blocks + (whole ? row / C8_BLOCK : row / page_size * blocks + row % page_size / C8_BLOCK)];
-      }
+      const int j = j0 + u * step;
+      w[u] = there && j < 2 * pieces ? *(const uint2*)((j >= pieces ? vc : kc) + (page * pieces + (j >= pieces ? j - pieces : j)) * 8L) : make_uint2(0u, 0u);
     }
 #pragma unroll
     for (int u = 0; u < C8E_AHEAD; u++) {
@@ -379,9 +377,13 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
       CT::values4(w[u].x, x);
       CT::values4(w[u].y, x + 4);
       __nv_bfloat162 y[4];
-      const float times = c8_shifted(f[u]).codes;
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = x[e] == x[e] ? x[e] * times : 0.f;
+      for (int e = 0; e < 8; e++) x[e] = there && x[e] == x[e] ? x[e] : 0.f;
+      if (odd) {
+        const float times = c8_shifted((j >= pieces ? vs : ks)[page * Hkv * blocks + ((j >= pieces ? j - pieces : j) >> block_log2)]).codes;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= times;
+      }
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
       *(uint4*)((j >= pieces ? v : k) + (i * pieces + (j >= pieces ? j - pieces : j)) * 8L) = *(const uint4*)y;
@@ -399,12 +401,13 @@ __global__ void __launch_bounds__(256) cache8_portions_kernel(const uint8_t* kc,
   if (beside) hb_pdl_wait();
 }
 
-// scale: 4 floats x Hkv x (n * blocks of a page + 2 C8_AHEAD), 16-byte aligned as k and v are; kc, vc 8-byte aligned; D a multiple of 8.
+// scale: 4 floats x Hkv x (n * blocks of a page + 2 C8_AHEAD), 16-byte aligned as k and v are; kc, vc 8-byte aligned; D 64 or 128, pages of whole
+// blocks, as the flash kernel takes them.
 HB_EXPORT int hb_cache8_portions(const void* kc, const void* vc, const float* ks, const float* vs, int ct, const int* table, const int* index, long n,
                                  long n_pages, int Hkv, int page_size, int D, float scale, void* k, void* v, void* scales, int beside,
                                  cudaStream_t st) {
   if (n <= 0) return 0;
-  if (n >= 0x7fffffffL || Hkv < 1 || page_size < 1 || D < 1 || D % 8 || 2L * Hkv * page_size * D > 0x7fffffffL - C8E_BEYOND || n_pages < 1)
+  if (n >= 0x7fffffffL || Hkv < 1 || page_size < 1 || page_size % C8_BLOCK || (D != 64 && D != 128) || 2L * Hkv * page_size * D > 0x7fffffffL - C8E_BEYOND || n_pages < 1)
     HB_FAIL("hb_cache8_portions: %ld of %ld pages of %d heads, %d places and %d", n, n_pages, Hkv, page_size, D);
   C8_DISPATCH(ct, "hb_cache8_portions",
       hb_launch(cache8_portions_kernel<CT>, dim3(n + 1, beside ? 1 : c8_split(n + 1, 2L * Hkv * page_size * D / 8)), dim3(256), 0, st, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, table, index, n, n_pages, Hkv,
