@@ -122,7 +122,7 @@ class ClockSampler:
                     reasons=reasons, samples=len(sm))
 
 
-def build_engine(layers: int, max_batch: int, total_steps: int):
+def build_engine(layers: int, max_batch: int, total_steps: int, cache_dtype=None):
     import torch  # noqa: F401
     from hipinfer_b200 import Engine
 
@@ -130,7 +130,7 @@ def build_engine(layers: int, max_batch: int, total_steps: int):
     pages_per_seq = -(-(PROMPT_LEN + total_steps + 2 * max_batch + 4 * PAGE) // PAGE)
     num_pages = max(max_batch * pages_per_seq, -(-PREFILL_TOKENS // PAGE)) + 8
     return Engine(config=cfg, random_weights=0, std=0.02, dtype="bfloat16", max_batch=max_batch, max_seq=CONTEXT_LEN,
-                  max_prefill=max(PREFILL_TOKENS, PROMPT_LEN), page_size=PAGE, num_pages=num_pages)
+                  max_prefill=max(PREFILL_TOKENS, PROMPT_LEN), page_size=PAGE, num_pages=num_pages, cache_dtype=cache_dtype)
 
 
 def prompts(n, seed, length=None):
@@ -787,6 +787,7 @@ def main() -> int:
     ap.add_argument("--new", type=int, default=128, help="mixed: tokens generated per request")
     ap.add_argument("--max-prefill", type=int, default=512, help="mixed: token budget of a step")
     ap.add_argument("--pool-fraction", type=float, default=1.0, help="mixed: fraction of the pages all requests would need (< 1: preemptions)")
+    ap.add_argument("--cache-dtype", default=None, choices=["int8", "float8_e4m3fn"], help="decode: keep keys and values in 8 bits (the default run: bf16)")
     ap.add_argument("--no-points", action="store_true", help="skip the batch-1 and batch-64 decode points")
     ap.add_argument("--breakdown", action="store_true", help="print per-kernel times of a decode step and exit")
     ap.add_argument("--prefill", action="store_true", help="with --breakdown: the prefill step instead of a decode step")
@@ -820,7 +821,7 @@ def main() -> int:
     pk = peaks()
     point_batches = [] if a.no_points else [b for b in (1, 64) if b != a.batch]
     max_batch = max([a.batch] + point_batches)
-    eng = build_engine(a.layers, max_batch, a.steps + a.warmup + 8)
+    eng = build_engine(a.layers, max_batch, a.steps + a.warmup + 8, a.cache_dtype)
     clocks = ClockSampler().start()
     ms, mean_ctx, launches = decode_device(eng, a.batch, a.steps, a.warmup, clocks)
     value = a.batch / ms * 1e3
@@ -847,7 +848,8 @@ def main() -> int:
         "ms_per_step": round(ms, 4), "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
         "dtype": "bf16", "data": "synthetic: uniform-random token ids, random N(0, 0.02) bf16 weights",
         "impl": "ours",
-        "config": bench_config(a.batch, a.layers, f"inputs larger than L2: {eng.weight_bytes / 1e9:.2f} GB of weights read per step"),
+        "config": bench_config(a.batch, a.layers, f"inputs larger than L2: {eng.weight_bytes / 1e9:.2f} GB of weights read per step",
+                               a.cache_dtype or "bf16"),
         "clocks": clocks.summary(),
         "e2e": {"value": round(a.batch / e2e_ms * 1e3, 1), "unit": "tok/s", "ms_per_step": round(e2e_ms, 4),
                 "h2d_bytes_per_step": h2d, "d2h_bytes_per_step": d2h},
