@@ -191,7 +191,8 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     tensor_cores = q.is_cuda and _on_tensor_cores(cache)
     limit = 0
-    if tensor_cores and batch.max_q_len >= PORTION_ROWS[0] and cache.k.shape[0] and _flash_takes(q, cache, out, n_heads, scale):
+    if tensor_cores and batch.max_q_len >= PORTION_ROWS[0] and batch.n_requests <= FLASH_REQUESTS and cache.k.shape[0] \
+            and _flash_takes(q, cache, out, n_heads, scale):
         limit = _portion_limit(batch, cache, n_heads, window)
     others = tensor_cores and T and (not limit or any(0 < n < limit for n in batch.h_q_len))
     if tensor_cores and T:
@@ -261,6 +262,7 @@ def _on_tensor_cores(cache: Cache8) -> bool:
 
 
 PORTION_ROWS = (16, 32, 64, 128)
+FLASH_REQUESTS = 65535                                             # of a step that the flash kernel takes
 
 
 def _portion_limit(batch, cache: Cache8, n_heads: int, window: int) -> int:

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import cache8_bounds as bounds
+from hipinfer_b200.engine.batch import StepEntry, build_step_batch
 from hipinfer_b200.kernels import cache8, library, ops
 from test_gpu_cache8 import CODES, DEV, filled, ids, on_gpu, same, step
 
@@ -329,3 +330,28 @@ def test_the_memory_of_many_long_portions(monkeypatch):
     ops.attention_cache8(q, cache, batch, 0, 2)
     one = 20016 * D * 4                                            # keys and values of a request in 16 bits; scales are a 32nd
     assert one < torch.cuda.max_memory_allocated() - before < (1 << 24) * 1.1 + (1 << 21)
+
+
+def test_more_requests_than_a_flash_launch_has(monkeypatch):
+    """65,540 requests of a token each and a portion among them: the portion stays with the others' kernel, whose tiles are more than a launch has."""
+    monkeypatch.setattr(cache8, "_portion_limit", lambda *a: 16)
+    R, D, at = 65540, 64, 65537
+    rows = [1] * R
+    rows[at] = 40
+    tables = [[[r]] for r in range(R)]
+    tables[at] = [[at, R, R + 1]]
+    batch = build_step_batch([StepEntry(r, [0] * n) for r, n in enumerate(rows)], [0] * R, [0] * R, tables, [[[0] * n] for n in rows], 1, DEV)
+    g = torch.Generator().manual_seed(0)
+    codes = torch.randint(-127, 128, (2, R + 2, 1, 16, D), dtype=torch.int8, generator=g)
+    scales = torch.rand(2, R + 2, 1, 1, generator=g) * 0.02 + 0.01
+    cache = (codes[0], codes[1], scales[0], scales[1])
+    q = queries(batch.n_rows * D, 22).view(-1, D).to(torch.bfloat16)
+    before = library.launches[0]
+    got = ops.attention_cache8(q.to(DEV), on_gpu(cache), batch, 0, 1).cpu()
+    assert library.launches[0] - before == 1
+    single = torch.cat([got[:at], got[at + 40:]]).double()
+    want = (codes[1].double() * scales[1].double()[..., None])[:R, 0, 0]
+    want = torch.cat([want[:at], want[at + 1:]])
+    assert ((single - want).abs() <= want.abs() * 2.0 ** -7).all()              # (2^-8 for the result, less for the weight)
+    portion, bound = bounds.attend(q[at:at + 40], cache, [tables[at][0]], [0], [40], 1)
+    assert bounds.beyond(got[at:at + 40], portion, bound) <= 1
