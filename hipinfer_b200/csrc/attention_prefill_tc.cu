@@ -43,7 +43,9 @@
 //
 // C8: the keys and values are codes of a cache in 8 bits (csrc/cache8.cuh) as 16-bit numbers, which hold them exactly, in pages of their own, and meet
 // their scales here: a key's in its scores' multiplication by the scale (the maximum is taken of each 16 keys' maxima, scaled), a value's in the
-// weight's exponent (the row's sum is taken block by block and divided by it again). With keys and values rounded to 16 bits ahead of the products a result is off by 1.6 times as much.
+// weight's exponent (the row's sum is taken block by block and divided by it again). Weights go to the second product in bf16, as they do without codes:
+// times a value's scale they span what f16 does not; the row's sum is of the weights before that rounding. Results are off by 2.3e-3 of themselves (f16 weights over
+// a reference scale, as single rows have them: 1.7e-3). With keys and values rounded to 16 bits ahead of the products a result is off by 1.6 times as much.
 // Two portions of 887 and 1,332 rows (the second behind 1,379 tokens), 32 heads over 8 of 128: 86 us, with keys and values as they are 82.
 #include "tc_common.cuh"
 

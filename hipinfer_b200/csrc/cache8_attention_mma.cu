@@ -12,7 +12,7 @@
 //
 // A warp's units come by cp.async through a ring of its own in shared memory, two or three units ahead, so that nothing waits for another warp and the
 // registers are left to the products: with the units ahead in registers (166 of them, 12 warps an SM) every second stall was for a result of the
-// warp's own, and 64 requests of 8,000 tokens (128) took 208 us, 165 now. 16-byte pieces are exchanged within a unit so that the reads of a product's operand
+// warp's own, and 64 requests of 8,000 tokens (128) took 208 us, 163 now. 16-byte pieces are exchanged within a unit so that the reads of a product's operand
 // touch every bank once.
 //
 // Codes are integers (or e4m3 numbers) of at most 8 significant bits, exact in f16. The query of a pair is scaled by a power of two to below 2^10 and
@@ -24,9 +24,9 @@
 // than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing that counts; a unit's sum is divided
 // by that ratio again. Scales, sums and accumulators are 32-bit.
 //
-// What bounds it: with many long requests the copy bandwidth (64 of 8,000 tokens, 8 kv heads of 128: 165 us, 6.4 TB/s, 97 % of a copy's; heads of 64 94 us,
-// 85 %, with half the issue slots used); with few the chain from the positions to the join (one of 700, heads of 64: 5.4 us; 8 of 2,000: 8.1);
-// with several rows a request the warps' own products and softmax (16 of 2,300 with 5 rows each, heads of 64: 17.9 us for 38 MB).
+// What bounds it: with many long requests the copy bandwidth (64 of 8,000 tokens, 8 kv heads of 128: 163 us, 6.4 TB/s, 98 % of a copy's; heads of 64 96 us,
+// 84 %, with half the issue slots used); with few the chain from the positions to the join (one of 700, heads of 64: 4.4 us within a graph, 5.4 launched by itself; 8 of 2,000: 8.5);
+// with several rows a request the warps' own products and softmax (16 of 2,300 with 5 rows each, heads of 64: 18.3 us for 38 MB).
 #include "cache8.cuh"
 #include "tc_common.cuh"
 

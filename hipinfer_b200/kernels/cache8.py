@@ -182,7 +182,9 @@ def attention_cache8(q: torch.Tensor, cache: Cache8, batch, group: int, n_heads:
     the step's own among them, are in `cache`. q [T, n_heads * head_dim] (bfloat16 or float32; rows may be part of wider ones), out [T, n_heads *
     head_dim] of its type; query head h reads kv head h // (n_heads / n_kv_heads). A row at position p sees the keys j <= p (and j > p - window,
     for a window above 0) whose pages are in the block table and in the cache; one that sees none is 0. scale: 1 / sqrt(head_dim) by default. Scores,
-    softmax and sums are 32-bit. Codes at places that a row of the step sees are numbers (e4m3 has a NaN; storing leaves none).
+    softmax and sums are 32-bit. On their way into the second product weights are rounded: to float16 for rows of the kernel on warp MMAs (for
+    float32 rows to two of them), to bfloat16 for portions on the flash kernel, whose results are off by 2.3e-3 of themselves where the others are by 1.7e-3, most of it the result's own
+    rounding. Which of the two a bfloat16 request of 16 to 127 rows goes through is a matter of the whole step (_portion_limit), and so are its last bits. Codes at places that a row of the step sees are numbers (e4m3 has a NaN; storing leaves none).
 
     A graph that a call is captured into wants the batch, with its tensors, to live as long as itself. A step in which a request brings several rows is
     laid out by the host at the batch's first call, from the lengths that the batch was built with: it has to have run once before it is captured, and is
@@ -481,11 +483,11 @@ def _clusters(dt: int, code: int, head_dim: int, nt: int, ranks: int) -> int:
 def _ranks(tiles: int, keys: int, mean: float, clusters) -> int:
     """Blocks (1 to 16, a cluster) that share a tile's keys (`keys` the longest's, `mean` of all): as many as are on the GPU at once (`clusters`: of so
     many blocks), with 64 keys each while there is one on an SM, or two and clusters of 2, 4 and 8; else 270, or 512 in clusters of 3, 5, 6 and 7, which fill the
-    GPU less evenly; more than 8 where they have an SM each, 16 with 128 keys each, 9 to 15 with 512. Measured, us: one request of 700 tokens (8 kv heads of 64)
-    5.9 with 2, 5.1 with 4, 4.6 with 8, of 2,000 5.4 with 8, 5.0 with 16, of 8,000 9.6 and 8.2; 5 of 900 5.6 with 4, 6.3 with 7; 4 of 2,000 7.1 with 4, 6.4 with 8; 8 of
-    2,000 8.0 and 8.2; 16 of 1,500 11.0 with 2, 9.7 with 4, 14.3 with 8; 32 of 500 7.4 with 1 and 8.2 with 2, of 700 10.1 and 9.6; 24 of 1,300 12.2 with 2 and 15.0
+    GPU less evenly; more than 8 where they have an SM each, 16 with 128 keys each, 9 to 15 with 512. Measured, us within a graph: one request of 700 tokens (8 kv heads of 64)
+    5.8 with 2, 4.9 with 4, 4.4 with 8, of 2,000 5.2 with 8, 5.0 with 16, of 8,000 9.4 and 7.5; 5 of 900 5.6 with 4, 6.3 with 7; 4 of 2,000 7.1 with 4, 6.4 with 8; 8 of
+    2,000 8.5 with 4 and 7.7 to 8.1 with 8 (where the rule takes 4); 16 of 1,500 11.0 with 2, 9.7 with 4, 14.3 with 8; 32 of 500 7.4 with 1 and 8.2 with 2, of 700 10.1 and 9.6; 24 of 1,300 12.2 with 2 and 15.0
     with 3. Where lengths differ a wave of blocks ends with its longest: while a block still has 2,048 keys of a
-    tile, or 1,450 of lengths that differ much, up to four waves (heads of 128: 64 requests of 8,000 tokens 173 as one wave of one block a tile, 162 as two, 167
+    tile, or 1,450 of lengths that differ much, up to four waves (heads of 128: 64 requests of 8,000 tokens 169 as one wave of one block a tile, 163 as two, 167
     with four blocks; 64 of 4 to 8 thousand 140, 137 and 133; 48 of 3 to 6 thousand 79, 82 and 76; 96 of 2 to 4 thousand 111 and 102; 64 of 2,000 46 and 48)."""
     def fits(r):
         even = r in (2, 4, 8)
