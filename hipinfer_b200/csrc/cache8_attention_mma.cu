@@ -21,7 +21,8 @@
 // exact in integers; the keys' conversion was a sixth of all instructions. A weight is 2^(score - sub), where sub lies 2 (in base 2) below
 // a score that was the largest once and is raised only when a weight passes 2^10, so that raising it, which costs a pass over the accumulators, is
 // rare. It is made times its unit's V scale over a reference, that of an earlier unit, which is exchanged (another pass) only where the two are more
-// than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit), and blocks of very unlike scales lose nothing that counts; a unit's sum is divided
+// than 2^5 apart: at most 2^15 in f16 (two parts where the rows are 32-bit, the second times 2^12). A weight keeps its bits down to 2^-16 of the largest that its
+// warp has seen (2^-28 in two parts); what is less is off by 2^-27 (2^-39) of that one, which counts where nearly all weight is on keys whose values are all but nothing beside the others'. A unit's sum is divided
 // by that ratio again. Scales, sums and accumulators are 32-bit.
 //
 // What bounds it: with many long requests the copy bandwidth (64 of 8,000 tokens, 8 kv heads of 128: 163 us, 6.4 TB/s, 98 % of a copy's; heads of 64 96 us,
@@ -87,16 +88,18 @@ template <> __device__ __forceinline__ void c8_halves<C8E4m3>(uint32_t w, uint32
   asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
-// PARTS numbers of f16 whose sum is x, two x at a time.
-template <int PARTS> __device__ __forceinline__ void c8_split(float x, float y, uint32_t* part) {
+// PARTS numbers of f16 whose sum, the second over TIMES, is x, two x at a time. The second part of a weight comes times 2^12 (and meets its codes over 2^12, exactly): by itself
+// it would end where f16 does, and of a weight of 2^-22 of the row's largest neither part kept more than two bits.
+template <int PARTS, int TIMES = 1> __device__ __forceinline__ void c8_split(float x, float y, uint32_t* part) {
   __half2 h = __floats2half2_rn(x, y);
   part[0] = *(const uint32_t*)&h;
   if constexpr (PARTS == 2) {
     const float2 f = __half22float2(h);
-    h = __floats2half2_rn(x - f.x, y - f.y);
+    h = __floats2half2_rn((x - f.x) * TIMES, (y - f.y) * TIMES);
     part[1] = *(const uint32_t*)&h;
   }
 }
+constexpr int C8M_TIMES = 4096;
 
 // Products of 32 int8 dimensions.
 __device__ __forceinline__ void c8_imma(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -489,8 +492,8 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         uint32_t x[W_PARTS], y[W_PARTS];
-        c8_split<W_PARTS>(w[u][nt][0], w[u][nt][1], x);
-        c8_split<W_PARTS>(w[u][nt][2], w[u][nt][3], y);
+        c8_split<W_PARTS, C8M_TIMES>(w[u][nt][0], w[u][nt][1], x);
+        c8_split<W_PARTS, C8M_TIMES>(w[u][nt][2], w[u][nt][3], y);
 #pragma unroll
         for (int p = 0; p < W_PARTS; p++) b[p][nt][0] = c8_transpose(x[p]), b[p][nt][1] = c8_transpose(y[p]);
       }
@@ -523,9 +526,16 @@ __global__ void __launch_bounds__(32 * C8M_WARPS, C8Sizes<CT, T, D, NT>::BLOCKS)
           c8_halves<CT>(x, f[0], f[1]);
           c8_halves<CT>(y, f[2], f[3]);
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++)
+          for (int nt = 0; nt < NT; nt++) c8_mma(o[2 * j + half][nt], f, b[0][nt][0], b[0][nt][1]);
+          if constexpr (W_PARTS == 2) {
 #pragma unroll
-            for (int p = 0; p < W_PARTS; p++) c8_mma(o[2 * j + half][nt], f, b[p][nt][0], b[p][nt][1]);
+            for (int i = 0; i < 4; i++) {
+              const __half2 z = __hmul2(*(const __half2*)&f[i], __float2half2_rn(1.f / C8M_TIMES));
+              f[i] = *(const uint32_t*)&z;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) c8_mma(o[2 * j + half][nt], f, b[1][nt][0], b[1][nt][1]);
+          }
         }
       }
     }

@@ -16,15 +16,15 @@ import torch
 import plain_cache8 as plain
 
 
-def attend(q, cache, tables, held, rows, heads, window=0, scale=None, weights=None):
+def attend(q, cache, tables, held, rows, heads, window=0, scale=None, weights=None, sums=False):
     """(results, bounds): [T, heads, D] and [T, heads] in 64 bits, for requests that hold `held` tokens and bring `rows` rows; `weights`: a type that weights are
-    rounded to when their sum has been taken."""
+    rounded to when their sum has been taken. With `sums` also sum_j p_j rms(v_j), [T, heads]."""
     k, v, ks, vs = cache
     K, V = (torch.from_numpy(plain.numbers(*plane)) for plane in ((k, ks), (v, vs)))
     pages, Hkv, ps, D = k.shape
     scale = D ** -0.5 if scale is None else scale
     G, x, at = heads // Hkv, q.double().cpu().view(-1, Hkv, heads // Hkv, D), 0
-    out, bound = [], []
+    out, bound, total = [], [], []
     for table, h, n in zip(tables, held, rows):
         if not n:
             continue
@@ -44,10 +44,11 @@ def attend(q, cache, tables, held, rows, heads, window=0, scale=None, weights=No
             w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
             o = torch.einsum("thgn,nhd->thgd", w if weights is None else w.to(weights).double(), vj)
             spread = torch.einsum("thgn,nh->thg", w * w, vj.square().mean(-1)).sqrt()
+            total.append(torch.einsum("thgn,nh->thg", w, vj.square().mean(-1).sqrt()).reshape(len(p), heads))
             out.append(o.reshape(len(p), heads, D))
             bound.append((2.0 ** -8 * (2 * o.square().mean(-1).sqrt() + 2 * spread)).reshape(len(p), heads))
         at += n
-    return torch.cat(out), torch.cat(bound)
+    return (torch.cat(out), torch.cat(bound)) + ((torch.cat(total),) if sums else ())
 
 
 def beyond(got, want, bound):
