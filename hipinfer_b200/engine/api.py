@@ -13,6 +13,8 @@ for bad arguments (scripts/hipinfer.py:386-390). What is new beside them: `dtype
 
 `cache_dtype` ("int8" or "float8_e4m3fn"; None: `dtype`) keeps keys and values in 8 bits with a scale for each 16 tokens and head: half
 the bytes (or a quarter) for models whose layers attend to plain keys and values (the Llama decoder; others are refused).
+A block's codes are rounded to the largest of its 16 tokens, so that logits depend, by that rounding, on how a text was cut into steps: prompts in portions of
+other lengths, requests that were preempted, drafts beside a newest token.
 
 `max_batch` is the most requests live at a time, `max_seq` the longest sequence, `max_prefill`
 the token budget of a step (the reference's prefill chunk, src/api.cu:1788).
