@@ -180,6 +180,7 @@ class ModelRunner:
             if keep:
                 batch.kept_rows = []
                 self._kept = _KeptStep(entries, ctx_lens, tables, slot_maps, self.page_size, [p.num_pages for p in self.cache.pools], batch.kept_rows)
+                self._kept.requests = [self.cache.get(e.request_id) for e in entries]
                 for g, (src, dst) in enumerate(self._kept.copies()):
                     if src:
                         self.storage.copy_pages(g, src, dst)
@@ -328,7 +329,8 @@ class ModelRunner:
         kept, self._kept = self._kept, None
         if kept is None:
             return
-        lengths = [self.length(rid) for rid in kept.ids]
+        # (one that has ended meanwhile, its name perhaps another's by now, has nothing to be put back)
+        lengths = [rc.length if self.cache.requests.get(rid) is rc else 0 for rid, rc in zip(kept.ids, kept.requests)]
         if not kept.damaged(lengths):
             return
         for g, (dst, src) in enumerate(kept.copies(lengths)):

@@ -86,3 +86,20 @@ def test_a_refused_draft_that_stands_out_leaves_nothing_behind(folders, codes):
             worst = max(worst, float((a - b).abs().max() / b.abs().max()))
         far.append(worst)
     assert far[0] <= TOL["float32"] and far[1] > 2 * far[0], far
+
+
+def test_requests_that_end_before_the_kept_rows_are_stored_touch_nothing(folders):
+    """Their pages are free, or another request's of the same name."""
+    from hipinfer_b200.engine import StepEntry
+
+    folder, cfg, _ = folders["c"]
+    runner = runner_of(folder, "bfloat16", "int8")
+    text = tiny.random_tokens(60, cfg["vocab_size"], 9)
+    runner.step([StepEntry("a", text[:37], []), StepEntry("b", text[:45], []), StepEntry("c", text[:50], [])])
+    runner.step([StepEntry("a", text[37:41], range(4)), StepEntry("b", text[45:49], range(4))], drafts=True)
+    for r in ("a", "b"):
+        runner.end(r)
+    assert runner.fork("c", "a", 39) == 39                          # (its copy lies where one of them ended)
+    before = planes(runner)
+    runner.store_accepted()
+    assert same(before, planes(runner))
